@@ -1,0 +1,285 @@
+// Writing rows into a paged key-value cache, as they are or as 8-bit codes, and reading them back.
+//
+// One group of lanes has a row: head_dim values of one head of one token, 16 bytes of them a lane.  Both
+// kernels only move rows, so they are bound by memory; what decides is that every access is a whole vector
+// and that enough of them are in flight.
+//
+// 8 bits: scale = max(max |x| / 127, 2^-126), code = x / scale to the nearest, ties to even.  The quotient is
+// never formed: c = rint(x * (1 / scale)) is off by at most one, and then only next to a half; the remainder
+// x - c scale is exact (one fused multiply-add whose result fits 24 bits) and its place against scale / 2
+// puts c right.  The code is so a function of x and scale alone.
+#include <algorithm>
+
+#include "wc_paged.h"
+
+namespace wc {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T v[V];
+};
+
+__device__ __forceinline__ int8_t code8(float x, float scale, float inv) {
+  float c = rintf(x * inv);
+  const float r = fmaf(-c, scale, x), half = 0.5f * scale;
+  const bool odd = static_cast<int>(c) & 1;
+  if (r > half || (r == half && odd))
+    c += 1.f;
+  else if (r < -half || (r == -half && odd))
+    c -= 1.f;
+  return static_cast<int8_t>(static_cast<int>(c));
+}
+
+struct Write {
+  PagedTable t;
+  const char *src[2];
+  char* pages[2];
+  float* scales[2];
+  int64_t stride[2][4];
+  const int32_t *start, *count;
+  int32_t steps, dh, row, lanes_log2;
+  FastDiv by_b, by_tiles;      // sequences per model; workgroups per sequence
+};
+
+// V: values a lane loads at once; NC: of those per lane
+template <typename T, bool Q8, int V, int NC>
+__global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
+  const int tid = threadIdx.x, kv = blockIdx.y;
+  const int lanes = 1 << a.lanes_log2, lane = tid & (lanes - 1);
+  const uint32_t seq = fdiv(blockIdx.x, a.by_tiles), tile = blockIdx.x - seq * a.by_tiles.d;
+  const int64_t r = static_cast<int64_t>(tile) * (kThreads >> a.lanes_log2) + (tid >> a.lanes_log2);
+  const uint32_t step = static_cast<uint32_t>(r / a.t.heads), h = static_cast<uint32_t>(r - static_cast<int64_t>(step) * a.t.heads);
+  int n = a.count ? a.count[seq] : a.steps;
+  if (n > a.steps) {
+    n = a.steps;
+    paged_fault(a.t);
+  }
+  const int start = a.start[seq];
+  if (r >= static_cast<int64_t>(a.steps) * a.t.heads || static_cast<int>(step) >= n || start < 0) return;
+  const int64_t tok = static_cast<int64_t>(start) + step;
+  const int32_t row = tok > INT32_MAX ? -1 : paged_row(a.t, seq, static_cast<uint32_t>(tok), h);
+  if (row < 0) {
+    paged_fault(a.t);
+    return;
+  }
+  const uint32_t model = fdiv(seq, a.by_b), b = seq - model * a.by_b.d;
+  const int64_t* st = a.stride[kv];
+  const T* src = reinterpret_cast<const T*>(a.src[kv]) + model * st[0] + b * st[1] + step * st[2] + h * st[3];
+  Vec<T, V> x[NC];
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int d = (lane + c * lanes) * V;
+    if (d < a.dh) x[c] = *reinterpret_cast<const Vec<T, V>*>(src + d);
+  }
+  if constexpr (!Q8) {
+    T* dst = reinterpret_cast<T*>(a.pages[kv]) + static_cast<int64_t>(row) * a.row;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int d = (lane + c * lanes) * V;
+      if (d < a.dh) *reinterpret_cast<Vec<T, V>*>(dst + d) = x[c];
+    }
+    for (int d = a.dh + lane; d < a.row; d += lanes) dst[d] = static_cast<T>(0.f);
+  } else {
+    // the largest magnitude by its bits, under which an infinity or NaN is larger than any finite value
+    uint32_t top = 0;
+    float f[NC][V];
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        f[c][e] = (lane + c * lanes) * V < a.dh ? to_f32(x[c].v[e]) : 0.f;
+        top = max(top, __builtin_bit_cast(uint32_t, f[c][e]) & 0x7fffffffu);
+      }
+    for (int off = lanes >> 1; off; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 64)));
+    const bool finite = top < 0x7f800000u;
+    const float scale = finite ? fmaxf(__builtin_bit_cast(float, top) / 127.f, 0x1p-126f) : __builtin_nanf("");
+    const float inv = 1.f / scale;
+    int8_t* dst = reinterpret_cast<int8_t*>(a.pages[kv]) + static_cast<int64_t>(row) * a.row;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int d = (lane + c * lanes) * V;
+      Vec<int8_t, V> o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) o.v[e] = finite ? code8(f[c][e], scale, inv) : static_cast<int8_t>(0);
+      if (d < a.dh) *reinterpret_cast<Vec<int8_t, V>*>(dst + d) = o;
+    }
+    for (int d = a.dh + lane; d < a.row; d += lanes) dst[d] = 0;
+    if (lane == 0) a.scales[kv][row] = scale;
+  }
+}
+
+struct Read {
+  PagedTable t;
+  const char* pages[2];
+  const float* scales[2];
+  char* out[2];
+  const int32_t* lengths;
+  int32_t most, dh, row, lanes_log2;
+  FastDiv by_tiles;
+};
+
+template <typename T, bool Q8, int V, int NC>
+__global__ __launch_bounds__(kThreads) void cache_read_kernel(Read a) {
+  typedef typename std::conditional<Q8, int8_t, T>::type S;
+  const int tid = threadIdx.x, kv = blockIdx.y;
+  const int lanes = 1 << a.lanes_log2, lane = tid & (lanes - 1);
+  const uint32_t seq = fdiv(blockIdx.x, a.by_tiles), tile = blockIdx.x - seq * a.by_tiles.d;
+  const int64_t rows = static_cast<int64_t>(a.most) * a.t.heads;
+  const int64_t r = static_cast<int64_t>(tile) * (kThreads >> a.lanes_log2) + (tid >> a.lanes_log2);
+  if (r >= rows) return;
+  const uint32_t tok = static_cast<uint32_t>(r / a.t.heads), h = static_cast<uint32_t>(r - static_cast<int64_t>(tok) * a.t.heads);
+  const int32_t length = a.lengths[seq];
+  int32_t row = -1;
+  if (static_cast<int32_t>(tok) < length) {
+    row = paged_row(a.t, seq, tok, h);
+    if (row < 0) paged_fault(a.t);
+  }
+  if (length > a.most) paged_fault(a.t);
+  const float scale = Q8 && row >= 0 ? a.scales[kv][row] : 1.f;
+  const S* src = reinterpret_cast<const S*>(a.pages[kv]) + static_cast<int64_t>(row) * a.row;
+  T* out = reinterpret_cast<T*>(a.out[kv]) + (static_cast<int64_t>(seq) * rows + r) * a.dh;
+#pragma unroll
+  for (int c = 0; c < NC; ++c) {
+    const int d = (lane + c * lanes) * V;
+    if (d >= a.dh) continue;
+    Vec<T, V> o;
+    if (row < 0) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) o.v[e] = static_cast<T>(0.f);
+    } else {
+      const Vec<S, V> x = *reinterpret_cast<const Vec<S, V>*>(src + d);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if constexpr (Q8)
+          o.v[e] = from_f32<T>(static_cast<float>(x.v[e]) * scale);
+        else
+          o.v[e] = x.v[e];
+      }
+    }
+    *reinterpret_cast<Vec<T, V>*>(out + d) = o;
+  }
+}
+
+int log2_lanes(int64_t need) {
+  int l = 0;
+  while ((1 << l) < need && l < 6) ++l;
+  return l;
+}
+
+// Runs F<T, Q8, V, NC>: whole 16-byte vectors of T (a row of at most 256 values fits 64 lanes), else single values
+template <template <typename, bool, int, int> class F, typename A>
+void dispatch(int dtype, int bits, bool vec, const A& a, dim3 grid, hipStream_t s) {
+  auto go = [&](auto t) {
+    typedef decltype(t) T;
+    constexpr int V = 16 / sizeof(T);
+    if (bits == 8)
+      vec ? F<T, true, V, 1>::run(a, grid, s) : F<T, true, 1, 4>::run(a, grid, s);
+    else
+      vec ? F<T, false, V, 1>::run(a, grid, s) : F<T, false, 1, 4>::run(a, grid, s);
+  };
+  if (dtype == WC_F32)
+    go(float());
+  else if (dtype == WC_BF16)
+    go(bf16());
+  else
+    go(f16());
+}
+template <typename T, bool Q8, int V, int NC>
+struct RunWrite {
+  static void run(const Write& a, dim3 grid, hipStream_t s) { cache_write_kernel<T, Q8, V, NC><<<grid, kThreads, 0, s>>>(a); }
+};
+template <typename T, bool Q8, int V, int NC>
+struct RunRead {
+  static void run(const Read& a, dim3 grid, hipStream_t s) { cache_read_kernel<T, Q8, V, NC><<<grid, kThreads, 0, s>>>(a); }
+};
+
+}  // namespace
+}  // namespace wc
+
+extern "C" int32_t wc_cache_write(const wc_cache_write_args* args, void* stream) {
+  using namespace wc;
+  clear_error();
+  const char* what = "wc_cache_write";
+  WC_REQUIRE(args, WC_ERR_NULL, "%s: null args", what);
+  const wc_cache_write_args& p = *args;
+  const wc_paged_cache& c = p.cache;
+  if (int32_t rc = paged_check(c, what)) return rc;
+  const int es = dtype_size(c.dtype);
+  WC_REQUIRE(p.t >= 0, WC_ERR_SHAPE, "%s: negative size", what);
+  WC_REQUIRE(mul_sat({p.t, c.heads}) < (1ll << 31), WC_ERR_LIMIT, "%s: more than 2^31 rows per sequence", what);
+  const int64_t seqs = c.n * c.b;
+  if (seqs == 0 || p.t == 0 || c.heads == 0) return WC_OK;
+  if (int32_t rc = paged_check_pointers(c, what)) return rc;
+  WC_REQUIRE(p.k && p.v && p.start, WC_ERR_NULL, "%s: null pointer", what);
+  WC_REQUIRE(aligned(p.k, es) && aligned(p.v, es) && aligned(p.start, 4) && aligned(p.count, 4), WC_ERR_ALIGN,
+             "%s: pointers must be aligned to their elements", what);
+  Write a;
+  a.t = paged_table(c);
+  a.src[0] = static_cast<const char*>(p.k);
+  a.src[1] = static_cast<const char*>(p.v);
+  a.pages[0] = static_cast<char*>(c.k_pages);
+  a.pages[1] = static_cast<char*>(c.v_pages);
+  a.scales[0] = c.k_scales;
+  a.scales[1] = c.v_scales;
+  const int64_t st[2][4] = {{p.k_stride_n, p.k_stride_b, p.k_stride_t, p.k_stride_h},
+                            {p.v_stride_n, p.v_stride_b, p.v_stride_t, p.v_stride_h}};
+  bool vec = c.head_dim * es % 16 == 0 && aligned(p.k, 16) && aligned(p.v, 16);
+  for (int i = 0; i < 2; ++i)
+    for (int j = 0; j < 4; ++j) {
+      a.stride[i][j] = st[i][j];
+      vec = vec && ubytes(st[i][j], es) % 16 == 0;
+    }
+  a.start = p.start;
+  a.count = p.count;
+  a.steps = static_cast<int32_t>(p.t);
+  a.dh = static_cast<int32_t>(c.head_dim);
+  a.row = static_cast<int32_t>(c.row);
+  a.lanes_log2 = log2_lanes(vec ? cdiv(c.head_dim * es, 16) : c.head_dim);
+  const int64_t tiles = cdiv(p.t * c.heads, kThreads >> a.lanes_log2);
+  WC_REQUIRE(mul_sat({tiles, seqs}) < (1ll << 32) / kThreads, WC_ERR_LIMIT, "%s: too many rows for one launch", what);
+  a.by_b = make_fastdiv(static_cast<uint32_t>(c.b));
+  a.by_tiles = make_fastdiv(static_cast<uint32_t>(tiles));
+  dispatch<RunWrite>(c.dtype, c.bits, vec, a, dim3(static_cast<uint32_t>(tiles * seqs), 2), as_stream(stream));
+  return check_launch(what);
+}
+
+extern "C" int32_t wc_cache_read(const wc_cache_read_args* args, void* stream) {
+  using namespace wc;
+  clear_error();
+  const char* what = "wc_cache_read";
+  WC_REQUIRE(args, WC_ERR_NULL, "%s: null args", what);
+  const wc_cache_read_args& p = *args;
+  const wc_paged_cache& c = p.cache;
+  if (int32_t rc = paged_check(c, what)) return rc;
+  const int es = dtype_size(c.dtype);
+  WC_REQUIRE(p.max_length >= 0, WC_ERR_SHAPE, "%s: negative size", what);
+  WC_REQUIRE(mul_sat({p.max_length, c.heads}) < (1ll << 31), WC_ERR_LIMIT, "%s: more than 2^31 rows per sequence", what);
+  const int64_t seqs = c.n * c.b;
+  if (seqs == 0 || p.max_length == 0 || c.heads == 0) return WC_OK;
+  if (int32_t rc = paged_check_pointers(c, what)) return rc;
+  WC_REQUIRE(p.k && p.v && p.lengths, WC_ERR_NULL, "%s: null pointer", what);
+  WC_REQUIRE(aligned(p.k, es) && aligned(p.v, es) && aligned(p.lengths, 4), WC_ERR_ALIGN,
+             "%s: pointers must be aligned to their elements", what);
+  Read a;
+  a.t = paged_table(c);
+  a.pages[0] = static_cast<const char*>(c.k_pages);
+  a.pages[1] = static_cast<const char*>(c.v_pages);
+  a.scales[0] = c.k_scales;
+  a.scales[1] = c.v_scales;
+  a.out[0] = static_cast<char*>(p.k);
+  a.out[1] = static_cast<char*>(p.v);
+  a.lengths = p.lengths;
+  a.most = static_cast<int32_t>(p.max_length);
+  a.dh = static_cast<int32_t>(c.head_dim);
+  a.row = static_cast<int32_t>(c.row);
+  const bool vec = c.head_dim * es % 16 == 0 && aligned(p.k, 16) && aligned(p.v, 16);
+  a.lanes_log2 = log2_lanes(vec ? cdiv(c.head_dim * es, 16) : c.head_dim);
+  const int64_t tiles = cdiv(p.max_length * c.heads, kThreads >> a.lanes_log2);
+  WC_REQUIRE(mul_sat({tiles, seqs}) < (1ll << 32) / kThreads, WC_ERR_LIMIT, "%s: too many rows for one launch", what);
+  a.by_tiles = make_fastdiv(static_cast<uint32_t>(tiles));
+  dispatch<RunRead>(c.dtype, c.bits, vec, a, dim3(static_cast<uint32_t>(tiles * seqs), 2), as_stream(stream));
+  return check_launch(what);
+}

@@ -16,8 +16,10 @@ from .core.traced_wide import BinaryOp, FunctionalOp, TracedWideModel, print_tra
 from .core.ensemble_util import pack_inputs, unpack_outputs
 from .core.primitives import (
     WideAttention, WideBatchNorm1d, WideBatchNorm2d, WideConv1d, WideConv2d, WideConv3d, WideEmbedding,
-    WideGRU, WideGroupNorm, WideInstanceNorm1d, WideInstanceNorm2d, WideLayerNorm, WideLinear, WideLSTM,
+    WideGRU, WideGroupNorm, WideHeadNormRotary, WideInstanceNorm1d, WideInstanceNorm2d, WideLayerNorm, WideLinear,
+    WideLinear4bit, WideLSTM,
 )
+from .core.paged_cache import WidePagedCache
 from .api import benchmark_custom, benchmark_primitive
 
 # the reference's optional benchmark harness is not part of this build
@@ -36,7 +38,7 @@ __all__ = [
     "TracedWideModel", "FunctionalOp", "BinaryOp", "print_trace", "pack_inputs", "unpack_outputs",
     "WideLinear", "WideConv1d", "WideConv2d", "WideConv3d", "WideBatchNorm1d", "WideBatchNorm2d",
     "WideLayerNorm", "WideGroupNorm", "WideInstanceNorm1d", "WideInstanceNorm2d", "WideEmbedding",
-    "WideAttention", "WideGRU", "WideLSTM",
+    "WideAttention", "WideGRU", "WideLSTM", "WideHeadNormRotary", "WideLinear4bit", "WidePagedCache",
     "benchmark_primitive", "benchmark_multi", "benchmark_all", "benchmark_custom",
     "list_benchmark_primitives", "BenchmarkResult", "SweepParams",
 ]

@@ -1,0 +1,186 @@
+"""
+WidePagedCache: the keys and values of many sequences of N models, in pages of one pool.
+
+    cache.write(k, v, block_table, start, count)      new tokens into the pages
+    cache.read(block_table, lengths, max_length)      back to dense [N, B, max_length, Hkv, Dh]
+    cache.attend(q, block_table, lengths)             one new token of every sequence over its pages
+
+Token i of sequence (n, b) stands in slot i % page_size of page block_table[n, b, i // page_size] of
+the pool (int32 [N, B, M]; entries behind a sequence's last page are not followed and may hold
+anything, -1 for example).  Which page is whose is the caller's: pages may be handed out in any
+order, and a prefix that several sequences read may be one set of pages.  No two rows of one write
+may go to the same slot.  Pools stand as
+
+    k_pages, v_pages     [P, Hkv, page_size, row]      row: head_dim, and zeros up to whole 16 bytes
+    k_scales, v_scales   [P, Hkv, page_size]           8-bit caches only
+
+With ``quantized=True`` a row (one head of one token) is 8-bit codes and one fp32 scale: scale =
+max(max |x| / 127, 2^-126), code = x / scale to the nearest, ties to even; a row with an infinity
+or NaN reads back as NaN.
+
+A block-table entry outside the pool, a token past the table's end or a count or length beyond the
+call's is never followed: nothing is written there, it reads as zeros, takes no part in the
+attention and raises a device-side flag, which ``index_error()`` (synchronises) turns into an
+IndexError.  Nothing here allocates pages or advances lengths, and every call reads its tables on
+the GPU, so a captured graph replays with whatever they hold then.  The reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+from torch import Tensor
+
+from .. import _hip, _serve
+
+
+class WidePagedCache:
+    def __init__(self, num_pages: int, page_size: int, n_kv_heads: int, head_dim: int,
+                 dtype: torch.dtype = torch.bfloat16, quantized: bool = False,
+                 device: Union[str, torch.device] = "cuda"):
+        _hip.dtype_code(dtype, "WidePagedCache")
+        stored = torch.int8 if quantized else dtype
+        es = torch.empty((), dtype=stored).element_size()
+        row = -(-head_dim * es // 16) * 16 // es
+        shape = (num_pages, n_kv_heads, page_size)
+        pages = lambda: torch.zeros((*shape, row), dtype=stored, device=device)     # noqa: E731
+        scales = lambda: torch.zeros(shape, dtype=torch.float32, device=device) if quantized else None  # noqa: E731
+        self._adopt(pages(), pages(), scales(), scales(), head_dim, dtype)
+
+    @classmethod
+    def from_pages(cls, k_pages: Tensor, v_pages: Tensor, k_scales: Optional[Tensor] = None,
+                   v_scales: Optional[Tensor] = None, head_dim: Optional[int] = None,
+                   dtype: Optional[torch.dtype] = None) -> "WidePagedCache":
+        """A cache over pools that exist (not copied): int8 pages with their scales, of a cache for ``dtype``, or pages
+        of a floating dtype.  Rows are whole 16 bytes; columns from ``head_dim`` on hold zeros."""
+        self = cls.__new__(cls)
+        self._adopt(k_pages, v_pages, k_scales, v_scales, k_pages.shape[-1] if head_dim is None else head_dim,
+                    k_pages.dtype if dtype is None else dtype)
+        return self
+
+    def _adopt(self, k_pages, v_pages, k_scales, v_scales, head_dim, dtype) -> None:
+        what = "WidePagedCache"
+        code = _hip.dtype_code(dtype, what)
+        quantized = k_pages.dtype == torch.int8
+        _hip.require_device(what, k_pages, v_pages, k_scales, v_scales)
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+            raise ValueError(f"{what}: k and v pages must be two [P, Hkv, page_size, row] tensors of one dtype")
+        if not quantized and k_pages.dtype != dtype:
+            raise ValueError(f"{what}: pages of {k_pages.dtype} in a cache for {dtype}")
+        pages, heads, page_size, row = k_pages.shape
+        if (k_scales is None) == quantized or (v_scales is None) == quantized:
+            raise ValueError(f"{what}: 8-bit pages, and only they, come with k and v scales")
+        for t in (k_scales, v_scales):
+            if t is not None and (t.dtype != torch.float32 or t.shape != k_pages.shape[:3]):
+                raise ValueError(f"{what}: scales must be float32 [P, Hkv, page_size]")
+        if not all(t is None or t.is_contiguous() for t in (k_pages, v_pages, k_scales, v_scales)):
+            raise ValueError(f"{what}: pools must be contiguous")
+        _serve.same_device(what, k_pages, v_pages, k_scales, v_scales)
+        if not 0 < head_dim <= min(row, 256):
+            raise ValueError(f"{what}: head_dim {head_dim} must be within [1, {min(row, 256)}]")
+        if page_size < 1 or row * k_pages.element_size() % 16 or row > 512:
+            raise ValueError(f"{what}: pages of at least one token, rows of whole 16 bytes and at most 512 elements, "
+                             f"got {page_size} and {row}")
+        self.k_pages, self.v_pages, self.k_scales, self.v_scales = k_pages, v_pages, k_scales, v_scales
+        self.num_pages, self.n_kv_heads, self.page_size, self.head_dim = pages, heads, page_size, head_dim
+        self.dtype, self.quantized, self.device = dtype, quantized, k_pages.device
+        self._err = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._sizes = (code, 8 if quantized else 0, pages, page_size, heads, head_dim, row)
+
+    def _table(self, what: str, table: Tensor, n: int, b: int) -> Tensor:
+        if table.dim() != 3 or table.dtype != torch.int32 or table.shape[0] != n or table.shape[1] != b:
+            raise RuntimeError(f"{what}: block_table must be int32 [N={n}, B={b}, M], got {table.dtype} {list(table.shape)}")
+        return table if table.is_contiguous() else table.contiguous()
+
+    @staticmethod
+    def _per_sequence(what: str, name: str, t: Tensor, n: int, b: int) -> Tensor:
+        if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != n or t.shape[1] != b:
+            raise RuntimeError(f"{what}: {name} must be int32 [N={n}, B={b}], got {t.dtype} {list(t.shape)}")
+        return t if t.is_contiguous() else t.contiguous()
+
+    def write(self, k: Tensor, v: Tensor, block_table: Tensor, start: Tensor, count: Optional[Tensor] = None) -> None:
+        """Rows [0, count[n, b]) of k, v [N, B, T, Hkv, Dh] become tokens start[n, b] + 0, 1, ... of their
+        sequences (count None: all T).  Rows from count on are padding, and a sequence of negative start takes part in
+        nothing: neither is written."""
+        what = "WidePagedCache.write"
+        _hip.require_device(what, k, v, block_table, start, count)
+        _hip.require_forward_only(what, k, v)
+        if k.dim() != 5 or k.shape != v.shape or k.shape[3] != self.n_kv_heads or k.shape[4] != self.head_dim:
+            raise RuntimeError(f"{what}: k and v must be [N, B, T, {self.n_kv_heads}, {self.head_dim}], got "
+                               f"{list(k.shape)} and {list(v.shape)}")
+        if k.dtype != self.dtype or v.dtype != self.dtype:
+            raise RuntimeError(f"{what}: k {k.dtype} and v {v.dtype} in a cache for {self.dtype}")
+        n, b = k.shape[:2]
+        table = self._table(what, block_table, n, b)
+        start = self._per_sequence(what, "start", start, n, b)
+        if count is not None:
+            count = self._per_sequence(what, "count", count, n, b)
+        _serve.same_device(what, self.k_pages, k, v, table, start, count)
+        k = k if k.stride(4) == 1 else k.contiguous()
+        v = v if v.stride(4) == 1 else v.contiguous()
+        _serve.cache_write(self, k, v, table, start, count)
+
+    def read(self, block_table: Tensor, lengths: Tensor, max_length: int) -> Tuple[Tensor, Tensor]:
+        """K and V of tokens [0, lengths[n, b]) as [N, B, max_length, Hkv, Dh]; zeros from a sequence's length on."""
+        what = "WidePagedCache.read"
+        _hip.require_device(what, block_table, lengths)
+        if max_length < 0:
+            raise RuntimeError(f"{what}: max_length must not be negative, got {max_length}")
+        n, b = block_table.shape[:2]
+        table = self._table(what, block_table, n, b)
+        lengths = self._per_sequence(what, "lengths", lengths, n, b)
+        _serve.same_device(what, self.k_pages, table, lengths)
+        shape = (n, b, max_length, self.n_kv_heads, self.head_dim)
+        k = torch.empty(shape, dtype=self.dtype, device=self.device)
+        v = torch.empty(shape, dtype=self.dtype, device=self.device)
+        if k.numel():
+            _serve.cache_read(self, table, lengths, max_length, k, v)
+        return k, v
+
+    def attend(self, q: Tensor, block_table: Tensor, lengths: Tensor, first: Optional[Tensor] = None,
+               scale: Optional[float] = None, max_length: Optional[int] = None) -> Tensor:
+        """softmax(scale q k^T) v of one new token per sequence, q [N, B, Hq, Dh], over cached tokens
+        [first[n, b], lengths[n, b]) (first None: from 0; a window of w tokens is first = lengths - w).  Query
+        head h reads key head h // (Hq // Hkv); scale defaults to Dh ** -0.5.  A sequence without tokens gets
+        zeros.  ``max_length`` bounds the lengths (default: what the block table can name); a tight bound splits
+        short sequences less."""
+        what = "WidePagedCache.attend"
+        _hip.require_device(what, q, block_table, lengths, first)
+        _hip.require_forward_only(what, q)
+        if q.dim() != 4 or q.shape[3] != self.head_dim or q.shape[2] % self.n_kv_heads:
+            raise RuntimeError(f"{what}: q must be [N, B, a multiple of {self.n_kv_heads} heads, {self.head_dim}], got "
+                               f"{list(q.shape)}")
+        if q.dtype != self.dtype:
+            raise RuntimeError(f"{what}: q {q.dtype} over a cache for {self.dtype}")
+        n, b = q.shape[:2]
+        table = self._table(what, block_table, n, b)
+        lengths = self._per_sequence(what, "lengths", lengths, n, b)
+        if first is not None:
+            first = self._per_sequence(what, "first", first, n, b)
+        _serve.same_device(what, self.k_pages, q, table, lengths, first)
+        most = table.shape[2] * self.page_size
+        if max_length is None:
+            max_length = min(most, 2 ** 31 - 65)
+        elif max_length < 0:
+            raise RuntimeError(f"{what}: max_length must not be negative, got {max_length}")
+        q = q if q.stride(3) == 1 else q.contiguous()
+        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if o.numel():
+            _serve.paged_attention(self, q, o, table, lengths, first, self.head_dim ** -0.5 if scale is None else scale,
+                                   max_length, lambda need: torch.empty(need, dtype=torch.uint8, device=q.device))
+        return o
+
+    def index_error(self) -> None:
+        """Raise IndexError if any call since the last check met a page outside the pool, or a token, count or length
+        past its bounds."""
+        if int(self._err.item()) != 0:
+            self._err.zero_()
+            raise IndexError("WidePagedCache: a block-table entry, token, count or length was out of range")
+
+    def __repr__(self) -> str:
+        return (f"WidePagedCache({self.num_pages} pages of {self.page_size}, heads={self.n_kv_heads}, "
+                f"head_dim={self.head_dim}, {'int8 for ' if self.quantized else ''}{self.dtype})")
+
+
+__all__ = ["WidePagedCache"]

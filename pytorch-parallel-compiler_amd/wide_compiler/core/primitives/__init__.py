@@ -13,9 +13,11 @@ from .wide_conv2d import (
 )
 from .wide_conv3d import WideConv3d, Conv3dStrategy
 from .wide_linear import WideLinear, WideMLP2, LinearStrategy, select_linear_strategy, LINEAR_THRESHOLDS
+from .wide_linear4bit import WideLinear4bit
 from .wide_batchnorm_1d import WideBatchNorm1d
 from .wide_batchnorm_2d import WideBatchNorm2d
 from .wide_layernorm import WideLayerNorm
+from .wide_headnorm import WideHeadNormRotary
 from .wide_groupnorm import WideGroupNorm, GroupNormStrategy
 from .wide_instancenorm import WideInstanceNorm1d, WideInstanceNorm2d, InstanceNormStrategy
 from .wide_embedding import WideEmbedding, EmbeddingStrategy
@@ -30,5 +32,5 @@ __all__ = [
     "WideBatchNorm1d", "WideBatchNorm2d", "WideLayerNorm", "WideGroupNorm", "GroupNormStrategy",
     "WideInstanceNorm1d", "WideInstanceNorm2d", "InstanceNormStrategy",
     "WideEmbedding", "EmbeddingStrategy", "WideAttention", "AttentionStrategy",
-    "WideGRU", "GRUStrategy", "WideLSTM", "LSTMStrategy",
+    "WideGRU", "GRUStrategy", "WideLSTM", "LSTMStrategy", "WideHeadNormRotary", "WideLinear4bit",
 ]

@@ -19,6 +19,10 @@ dropout in training mode raises.  ``attn_mask`` follows scaled_dot_product_atten
 [N*B, heads, Tq, Tkv] scores (wide_attention.py:222-228): boolean (True = attend) or additive,
 broadcastable to that shape, not together with ``is_causal``; a query whose keys are all masked
 gets zeros, as torch's SDPA gives.
+
+Token by token: ``prompt`` runs causal self-attention and leaves the keys and values in the pages of a
+WidePagedCache, ``step`` attends one new token of every sequence over them; both take a
+WideHeadNormRotary for norms and rotation of queries and keys.  The reference has no counterpart.
 """
 
 from __future__ import annotations
@@ -111,6 +115,23 @@ class WideAttention(nn.Module):
                           c_sn=m * width, c_so=0, c_si=width, c_rows_inner=max(m, 1), bias=bias, bias_sn=b_sn)
         return out
 
+    def _qkv(self, x: Tensor, qw: Tensor, kvw: Tensor) -> Tensor:
+        """Self-attention's projections of x [N, B, T, D]: one launch writes Q (columns [0, D)) and K|V into one
+        [N, B, T, 3D] = Q | K | V buffer, which is read in place; the parameters are read as they are on every call
+        (no concatenated copy to go stale)."""
+        d, kvb = self.d_model, self.kv_bias
+        qkv = torch.empty((*x.shape[:3], 3 * d), dtype=x.dtype, device=x.device)
+        xr, r = rows_or_contiguous(x)
+        c = lambda t: None if t is None else (t if t.is_contiguous() else t.contiguous())  # noqa: E731
+        if self.q_bias is not None and kvb is not None and self.q_bias.dtype != kvb.dtype:
+            self._project(x, qw, d * d, self.q_bias, d, d, out=qkv, col0=0)
+            self._project(x, kvw, 2 * d * d, kvb, 2 * d, 2 * d, out=qkv, col0=d)
+        else:
+            _hip.grouped_gemm_pair(n=self.n, m=r.rows, k=d, o1=d, o2=2 * d, a=xr, a_sn=r.stride_n,
+                                   a_so=r.stride_outer, a_si=r.stride_inner, a_rows_inner=r.rows_inner,
+                                   w1=qw, bias1=c(self.q_bias), w2=kvw, bias2=c(kvb), c=qkv)
+        return qkv
+
     @staticmethod
     def _mask(attn_mask: Tensor, is_causal: bool, nb: int, hh: int, tq: int, tkv: int, dev) -> Tensor:
         """attn_mask (SDPA semantics over [N*B, heads, Tq, Tkv]) as the kernel's additive fp32 view:
@@ -167,19 +188,7 @@ class WideAttention(nn.Module):
                                 heads=hh, scale=dh ** -0.5, causal=is_causal)
             return self._project(attn, ow, d * d, self.out_bias, d, d)
         if query is key and key is value:
-            # self-attention: one launch writes the Q (columns [0, D)) and K|V projections into one
-            # [N, B, T, 3D] = Q | K | V buffer, which the attention kernel reads in place; the
-            # parameters are read as they are on every call (no concatenated copy to go stale)
-            qkv = torch.empty((n, b, tq, 3 * d), dtype=query.dtype, device=query.device)
-            qr, r = rows_or_contiguous(query)
-            c = lambda t: None if t is None else (t if t.is_contiguous() else t.contiguous())  # noqa: E731
-            if self.q_bias is not None and kvb is not None and self.q_bias.dtype != kvb.dtype:
-                self._project(query, qw, d * d, self.q_bias, d, d, out=qkv, col0=0)
-                self._project(query, kvw, 2 * d * d, kvb, 2 * d, 2 * d, out=qkv, col0=d)
-            else:
-                _hip.grouped_gemm_pair(n=n, m=r.rows, k=d, o1=d, o2=2 * d, a=qr, a_sn=r.stride_n,
-                                       a_so=r.stride_outer, a_si=r.stride_inner, a_rows_inner=r.rows_inner,
-                                       w1=qw, bias1=c(self.q_bias), w2=kvw, bias2=c(kvb), c=qkv)
+            qkv = self._qkv(query, qw, kvw)
             q, k_t, v_t = qkv, qkv[..., d:], qkv[..., 2 * d:]
             q_strides = k_strides = v_strides = (tq * 3 * d, 3 * d)
             attn = torch.empty((n, b, tq, d), dtype=query.dtype, device=query.device)
@@ -205,6 +214,66 @@ class WideAttention(nn.Module):
                            q_strides=(tq * d, d), k_strides=k_strides, v_strides=v_strides, o_strides=(tq * d, d),
                            scale=dh ** -0.5, causal=is_causal, mask=mask)
         return self._project(attn, ow, d * d, self.out_bias, d, d)
+
+    def _cached_heads(self, what: str, x: Tensor, cache: "WidePagedCache", positions: Tensor, head_norm):
+        """The heads of x [N, B, T, D], queries, keys and values [N, B, T, heads, Dh], for a call with a cache."""
+        params = (self.q_weight, self.kv_weight, self.out_weight, self.q_bias, self.kv_bias, self.out_bias)
+        _hip.require_device(what, x, positions, *params)
+        _hip.require_forward_only(what, x, *params)
+        if self.training and self.dropout > 0:
+            raise RuntimeError(f"{what}: attention dropout in training mode is not supported (forward-only "
+                               "inference kernels); call .eval()")
+        if x.dtype != self.q_weight.dtype:
+            raise RuntimeError(f"{what}: input dtype {x.dtype} != weight dtype {self.q_weight.dtype}")
+        if (cache.n_kv_heads, cache.head_dim, cache.dtype) != (self.n_heads, self.d_head, x.dtype):
+            raise RuntimeError(f"{what}: {cache} does not hold {self.n_heads} heads of {self.d_head} in {x.dtype}")
+        if head_norm is not None and (head_norm.n, head_norm.head_dim) != (self.n, self.d_head):
+            raise RuntimeError(f"{what}: {head_norm} does not match {self}")
+        qw, kvw = (w if w.is_contiguous() else w.contiguous() for w in (self.q_weight, self.kv_weight))
+        qkv = self._qkv(x, qw, kvw).unflatten(-1, (3, self.n_heads, self.d_head))
+        q, k, v = qkv.unbind(3)
+        if head_norm is not None:
+            q, k = head_norm(q, k, positions)
+        return q, k, v
+
+    def _project_out(self, attn: Tensor) -> Tensor:
+        d = self.d_model
+        ow = self.out_weight if self.out_weight.is_contiguous() else self.out_weight.contiguous()
+        return self._project(attn, ow, d * d, self.out_bias, d, d)
+
+    def prompt(self, x: Tensor, cache: "WidePagedCache", block_table: Tensor, lengths: Tensor,
+               head_norm: Optional["WideHeadNormRotary"] = None) -> Tensor:
+        """Causal self-attention over prompts x [N, B, T, D] whose keys and values go to the pages of ``cache`` as
+        tokens 0, 1, ...: lengths[n, b] (int32) of the T rows of each sequence are its prompt, the others padding,
+        whose outputs mean nothing.  ``head_norm`` norms and turns queries and keys first."""
+        what = "WideAttention.prompt"
+        n, d, hh, dh = self.n, self.d_model, self.n_heads, self.d_head
+        if x.dim() != 4 or x.shape[0] != n or x.shape[3] != d:
+            raise RuntimeError(f"{what}: x must be [N={n}, B, T, {d}], got {list(x.shape)}")
+        b, t = x.shape[1:3]
+        q, k, v = self._cached_heads(what, x, cache, torch.arange(t, device=x.device), head_norm)
+        cache.write(k, v, block_table, torch.zeros_like(lengths), lengths)
+        attn = torch.empty((n, b, t, d), dtype=x.dtype, device=x.device)
+        if attn.numel():
+            strides = lambda y: (t * y.stride(2), y.stride(2))  # noqa: E731 - [N, B, T] are dense
+            _hip.attention(q=q, k=k, v=v, o=attn, nb=n * b, heads=hh, sq=t, skv=t, head_dim=dh, q_strides=strides(q),
+                           k_strides=strides(k), v_strides=strides(v), o_strides=(t * d, d), scale=dh ** -0.5,
+                           causal=True)
+        return self._project_out(attn)
+
+    def step(self, x: Tensor, cache: "WidePagedCache", block_table: Tensor, lengths: Tensor,
+             head_norm: Optional["WideHeadNormRotary"] = None) -> Tensor:
+        """Self-attention of one new token of every sequence, x [N, B, D]: its keys and values go to the pages of
+        ``cache`` as token lengths[n, b] - 1 (int32; the new token counted), and its queries attend over all
+        lengths[n, b] tokens.  A sequence of length 0 takes part in nothing.  ``head_norm`` norms and turns queries
+        and keys first, at that position."""
+        what = "WideAttention.step"
+        if x.dim() != 3 or x.shape[0] != self.n or x.shape[2] != self.d_model:
+            raise RuntimeError(f"{what}: x must be [N={self.n}, B, {self.d_model}], got {list(x.shape)}")
+        start = lengths - 1
+        q, k, v = self._cached_heads(what, x[:, :, None], cache, start[..., None], head_norm)
+        cache.write(k, v, block_table, start)
+        return self._project_out(cache.attend(q[:, :, 0], block_table, lengths).flatten(-2))
 
     def _fusable(self, x: Tensor, mask: Optional[Tensor], params) -> bool:
         """The conditions of wc_self_attention: bf16, head dim 32, 1 <= S <= 512, D <= 768, no

@@ -1,0 +1,146 @@
+"""
+WideLinear4bit: N independent linear layers with weights of 4 bits, for few rows.
+
+    x [N, *batch, I]  ->  y [N, *batch, O],   y[i] = x[i] @ W[i].T + bias[i]
+    W[i, o, k] = scale[i, o, k // group] * (code[i, o, k] - zero[i, o, k // group])
+
+with codes of 0 to 15, groups of 32, 64 or 128 columns and whole-number zero points (8 where there
+are none).  The forward (wc_linear4) reads every weight once for up to 64 rows, so that a token's
+products cost what reading half a byte a weight costs; more rows go 64 at a time.  Sums are fp32;
+the scale multiplies each group's sum.
+
+The buffers hold the weights as the kernel reads them (``packed`` [N, O / 16, I / 128, 64, 4] int32,
+``scales`` and ``zeros`` [N, O / 16, groups, 16], sizes rounded up); ``from_codes`` packs them from
+rows and ``from_modules`` quantises WideLinear's modules; ``dequantize()`` gives the weights they
+stand for.  The reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+from typing import List, Optional
+
+import torch
+from torch import Tensor, nn
+
+from ... import _hip, _serve
+from .._layout import rows_or_contiguous
+
+# column e of a lane's 8 stands in this nibble of its word
+_NIBBLE = (0, 4, 1, 5, 2, 6, 3, 7)
+
+
+class WideLinear4bit(nn.Module):
+    def __init__(self, n: int, in_features: int, out_features: int, group_size: int = 128, bias: bool = True,
+                 zeros: bool = True, dtype: torch.dtype = torch.float32):
+        super().__init__()
+        if group_size not in (32, 64, 128):
+            raise ValueError(f"WideLinear4bit: group_size must be 32, 64 or 128, got {group_size}")
+        if in_features < 1:
+            raise ValueError("WideLinear4bit: in_features must be positive")
+        _hip.dtype_code(dtype, "WideLinear4bit")
+        self.n = n
+        self.in_features = in_features
+        self.out_features = out_features
+        self.group_size = group_size
+        rt, kt = -(-out_features // 16), -(-in_features // 128)
+        meta = (n, rt, kt * (128 // group_size), 16)
+        self.register_buffer("packed", torch.zeros((n, rt, kt, 64, 4), dtype=torch.int32))
+        self.register_buffer("scales", torch.zeros(meta, dtype=dtype))
+        self.register_buffer("zeros", torch.zeros(meta, dtype=torch.uint8) if zeros else None)
+        self.register_buffer("bias", torch.zeros((n, out_features), dtype=dtype) if bias else None)
+
+    def forward(self, x: Tensor) -> Tensor:
+        what = "WideLinear4bit"
+        if x.dim() < 2 or x.shape[0] != self.n or x.shape[-1] != self.in_features:
+            raise RuntimeError(f"{what}: expected input [N={self.n}, ..., {self.in_features}], got {list(x.shape)}")
+        bufs = self._buffers
+        packed, scales, zeros, bias = bufs["packed"], bufs["scales"], bufs["zeros"], bufs["bias"]
+        _hip.require_device(what, x, packed)
+        _hip.require_forward_only(what, x)
+        if x.dtype != scales.dtype or (bias is not None and bias.dtype != x.dtype):
+            raise RuntimeError(f"{what}: input dtype {x.dtype} != {scales.dtype} of scales and bias")
+        _serve.same_device(what, x, packed, scales, zeros, bias)
+        x, r = rows_or_contiguous(x)
+        y = torch.empty((*x.shape[:-1], self.out_features), dtype=x.dtype, device=x.device)
+        if y.numel():
+            _serve.linear4(n=self.n, m=r.rows, o=self.out_features, k=self.in_features, group=self.group_size, x=x,
+                           rows=r, codes=packed, scales=scales, zeros=zeros, bias=bias, y=y)
+        return y
+
+    def _pack(self, codes: Tensor, scales: Tensor, zeros: Optional[Tensor]) -> None:
+        """codes [N, O, I] uint8 of 0-15, scales and zeros [N, O, ceil(I / group)] into the buffers."""
+        n, rt, kt = self.packed.shape[:3]
+        full = torch.zeros((n, rt * 16, kt * 128), dtype=torch.uint8, device=codes.device)
+        full[:, :self.out_features, :self.in_features] = codes
+        # [n, row tile, row, column tile, word, lane group, column] -> [.., lane group, row, word, column]
+        c = full.view(n, rt, 16, kt, 4, 4, 8).permute(0, 1, 3, 5, 2, 4, 6)
+        half = torch.empty((*c.shape[:-1], 8), dtype=torch.uint8, device=codes.device)
+        half[..., list(_NIBBLE)] = c
+        words = half[..., 0::2] | (half[..., 1::2] << 4)                 # bytes, the low nibble first
+        self.packed.copy_(words.contiguous().view(torch.int32).view(self.packed.shape))
+        for dst, src in ((self.scales, scales), (self.zeros, zeros)):
+            if dst is not None:
+                rows = torch.zeros((n, rt * 16, dst.shape[2]), dtype=dst.dtype, device=codes.device)
+                rows[:, :self.out_features, :src.shape[2]] = src
+                dst.copy_(rows.view(n, rt, 16, -1).transpose(2, 3))
+
+    @classmethod
+    def from_codes(cls, codes: Tensor, scales: Tensor, *, in_features: int, group_size: int = 128,
+                   zeros: Optional[Tensor] = None, bias: Optional[Tensor] = None) -> "WideLinear4bit":
+        """codes [N, O, ceil(I / 2)] uint8, two to a byte, the even column in the low half; scales
+        [N, O, ceil(I / group)] of the dtype of the inputs; zeros the same of uint8 (0 to 15) or None; bias [N, O]."""
+        what = "WideLinear4bit.from_codes"
+        if codes.dim() != 3 or codes.dtype != torch.uint8 or codes.shape[2] != (in_features + 1) // 2:
+            raise ValueError(f"{what}: codes must be uint8 [N, O, {(in_features + 1) // 2}], got {codes.dtype} {list(codes.shape)}")
+        meta = (*codes.shape[:2], -(-in_features // group_size))
+        if tuple(scales.shape) != meta or (zeros is not None and (tuple(zeros.shape) != meta or zeros.dtype != torch.uint8)):
+            raise ValueError(f"{what}: scales and uint8 zeros must be {list(meta)}")
+        if bias is not None and tuple(bias.shape) != tuple(codes.shape[:2]):
+            raise ValueError(f"{what}: bias must be {list(codes.shape[:2])}, got {list(bias.shape)}")
+        if zeros is not None and zeros.numel() and int(zeros.max()) > 15:
+            raise ValueError(f"{what}: zero points must be within [0, 15]")
+        wide = cls(codes.shape[0], in_features, codes.shape[1], group_size, bias=bias is not None,
+                   zeros=zeros is not None, dtype=scales.dtype).to(codes.device)
+        rows = torch.stack((codes & 15, codes >> 4), -1).flatten(-2)[..., :in_features]
+        with torch.no_grad():
+            wide._pack(rows, scales, zeros)
+            if bias is not None:
+                wide.bias.copy_(bias)
+        return wide
+
+    @classmethod
+    def from_modules(cls, modules: List[nn.Linear], group_size: int = 128) -> "WideLinear4bit":
+        """Quantises N nn.Linear: each group's codes span its values and zero, code = round(w / scale) + zero."""
+        t = modules[0]
+        n, o, i = len(modules), t.out_features, t.in_features
+        wide = cls(n, i, o, group_size, bias=t.bias is not None, dtype=t.weight.dtype).to(t.weight.device)
+        groups = -(-i // group_size)
+        with torch.no_grad():
+            w = torch.stack([m.weight for m in modules]).float()
+            pad = torch.nn.functional.pad(w, (0, groups * group_size - i)).view(n, o, groups, group_size)
+            lo, hi = pad.amin(-1).clamp_max(0), pad.amax(-1).clamp_min(0)
+            scales = ((hi - lo) / 15).clamp_min(torch.finfo(t.weight.dtype).tiny).to(t.weight.dtype)
+            s = scales.float()
+            zeros = torch.round(-lo / s).clamp(0, 15)
+            codes = (torch.round(pad / s[..., None]) + zeros[..., None]).clamp(0, 15)
+            wide._pack(codes.to(torch.uint8).flatten(-2)[..., :i], scales, zeros.to(torch.uint8))
+            if t.bias is not None:
+                wide.bias.copy_(torch.stack([m.bias for m in modules]))
+        return wide
+
+    def dequantize(self) -> Tensor:
+        """The weights the codes stand for, float32 [N, O, I]."""
+        n, rt, kt = self.packed.shape[:3]
+        b = self.packed.contiguous().view(torch.uint8).view(n, rt, kt, 4, 16, 4, 4)
+        half = torch.stack((b & 15, b >> 4), -1).flatten(-2)             # nibbles in order
+        c = half[..., list(_NIBBLE)].permute(0, 1, 4, 2, 5, 3, 6).reshape(n, rt * 16, kt * 128)
+        rows = lambda t: t.transpose(2, 3).reshape(n, rt * 16, -1).float().repeat_interleave(self.group_size, -1)  # noqa: E731
+        w = (c.float() - (8.0 if self.zeros is None else rows(self.zeros))) * rows(self.scales)
+        return w[:, :self.out_features, :self.in_features]
+
+    def __repr__(self) -> str:
+        return (f"WideLinear4bit({self.n}x[{self.in_features}->{self.out_features}], group={self.group_size}"
+                f"{'' if self.zeros is None else ', zero points'})")
+
+
+__all__ = ["WideLinear4bit"]

@@ -1,0 +1,237 @@
+"""WidePagedCache.attend (GPU) against 64 bits: types, stored types, head dims, groups, pages that end inside a tile,
+lengths around a tile, windows, empty sequences, strides, values that aren't finite, tables out of range, graphs.
+
+Tolerance: half a rounding step of the result, and what attend_slack derives for the sums in fp32."""
+
+import pytest
+import torch
+
+from tests._serve import HALF, attend, attend_slack, dense, make_table, quantise, within
+from tests._util import gen
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def _setup(n, b, hq, hkv, d, page, lens, dtype, quantized, seed, spread=1.0):
+    import wide_compiler as wc
+    g = gen(seed)
+    lens = torch.as_tensor(lens, dtype=torch.int32).view(n, b)
+    table, pages = make_table(lens, page, g)
+    cache = wc.WidePagedCache(pages, page, hkv, d, dtype=dtype, quantized=quantized)
+    most = max(int(lens.max()), 1)
+    k, v = (spread * torch.randn(n, b, most, hkv, d, generator=g).to(DEV) for _ in range(2))
+    k, v = k.to(dtype), v.to(dtype)
+    q = torch.randn(n, b, hq, d, generator=g).to(DEV, dtype)
+    # what no token has must never count: pools start as NaN
+    if quantized:
+        cache.k_scales.fill_(float("nan")), cache.v_scales.fill_(float("nan"))
+    else:
+        cache.k_pages[..., :d] = float("nan")
+        cache.v_pages[..., :d] = float("nan")
+    table, lens = table.to(DEV), lens.to(DEV)
+    cache.write(k, v, table, torch.zeros_like(lens), lens)
+    if quantized:
+        k, v = quantise(k), quantise(v)
+    return cache, q, k, v, table, lens
+
+
+def _check(got, q, k, v, lens, first=None, scale=None):
+    ref, big = attend(q, k, v, lens, first, scale)
+    vmax = v.double().nan_to_num(0, 0, 0).abs().amax().item()
+    within(got, ref, HALF[got.dtype], attend_slack(got.dtype, big, q.shape[-1], k.shape[2], vmax))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("hq,hkv,d,page", [
+    (1, 1, 64, 16), (8, 8, 64, 24), (4, 1, 128, 16), (32, 8, 128, 32), (6, 2, 80, 8), (14, 2, 96, 64), (16, 1, 256, 16),
+    (17, 1, 64, 7), (40, 2, 32, 128), (2, 2, 20, 1), (3, 1, 1, 5), (4, 2, 250, 33)])
+def test_attend_layouts(hq, hkv, d, page, quantized, dtype):
+    lens = [1, 31, 33, 100, 257, 0]
+    cache, q, k, v, table, lens = _setup(2, 3, hq, hkv, d, page, lens, dtype, quantized, hq * 100 + d)
+    got = cache.attend(q, table, lens)
+    _check(got, q, k, v, lens)
+    assert (got[1, 2] == 0).all()
+    cache.index_error()
+
+
+@pytest.mark.parametrize("dtype,quantized", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float32, False),
+                                             (torch.float32, True), (torch.float16, False), (torch.float16, True)])
+@pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 32, 63, 64, 127, 128, 129, 511, 1000, 4099])
+def test_attend_lengths(length, dtype, quantized):
+    cache, q, k, v, table, lens = _setup(1, 2, 8, 2, 128, 16, [length, max(length // 3, 1)], dtype, quantized, length)
+    _check(cache.attend(q, table, lens), q, k, v, lens)
+    _check(cache.attend(q, table, lens, max_length=length, scale=0.3), q, k, v, lens, scale=0.3)
+
+
+@pytest.mark.parametrize("first", [[0, 0, 0, 0], [1, 31, 32, 33], [200, 5, 64, 300], [-7, 299, 150, 260]])
+@pytest.mark.parametrize("dtype,quantized", [(torch.bfloat16, False), (torch.float32, True)])
+def test_attend_windows(first, dtype, quantized):
+    """From any first token on; a window that starts at or behind the end is empty."""
+    cache, q, k, v, table, lens = _setup(2, 2, 4, 2, 64, 16, [200, 300, 64, 260], dtype, quantized, 5)
+    first = torch.tensor(first, dtype=torch.int32, device=DEV).view(2, 2)
+    got = cache.attend(q, table, lens, first=first)
+    _check(got, q, k, v, lens, first)
+    assert (got[(first >= lens)] == 0).all()
+
+
+def test_attend_strided_queries_and_tables():
+    cache, q, k, v, table, lens = _setup(2, 3, 8, 2, 64, 16, [40, 7, 100, 64, 33, 1], torch.bfloat16, False, 9)
+    wide = torch.full((2, 3, 8, 3 * 64 + 1), float("nan"), device=DEV, dtype=q.dtype)
+    wide[..., 65:129] = q
+    expect = cache.attend(q, table, lens)
+    assert torch.equal(cache.attend(wide[..., 65:129], table, lens), expect)
+    assert torch.equal(cache.attend(q.transpose(2, 3).contiguous().transpose(2, 3), table, lens), expect)
+    padded = torch.full((2, 3, table.shape[2] + 5), 1 << 30, device=DEV, dtype=torch.int32)   # longer: not followed
+    padded[..., :table.shape[2]] = table
+    assert torch.equal(cache.attend(q, padded[..., :table.shape[2]], lens), expect)
+    _check(cache.attend(q, padded, lens), q, k, v, lens)
+    cache.index_error()
+
+
+def test_attend_shared_prefix_pages():
+    """Two sequences over the same pages."""
+    cache, q, k, v, table, lens = _setup(1, 2, 4, 2, 64, 16, [80, 80], torch.bfloat16, False, 11)
+    table[0, 1] = table[0, 0]
+    lens[0, 1] = 50
+    k[0, 1], v[0, 1] = k[0, 0], v[0, 0]
+    _check(cache.attend(q, table, lens), q, k, v, lens)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_attend_values_far_apart(dtype):
+    """One token takes nearly all the weight, ten thousand small ones share the rest; scores far from 0."""
+    length, d = 10000, 64
+    cache, q, k, v, table, lens = _setup(1, 1, 2, 1, d, 16, [length], dtype, False, 13)
+    k = torch.zeros_like(k)
+    q = torch.ones_like(q)
+    k[..., 0] = -70.0
+    k[:, :, 4321, :, 0] = 22.0
+    v = v.abs()
+    v[:, :, 4321] = 0
+    zero = torch.zeros_like(lens)
+    cache.write(k, v, table, zero)
+    got = cache.attend(q, table, lens)
+    ref, big = attend(q, k, v, lens)
+    # the result is 10^4 exp(-11.5) of mean |v|: against itself, not the largest value (P's planes count relatively)
+    rel = HALF[dtype] + attend_slack(dtype, big, d, length, 1.0)
+    within(got, ref, rel, 0.0)
+
+
+@pytest.mark.parametrize("dtype,quantized", [(torch.bfloat16, False), (torch.float32, False), (torch.float16, True)])
+def test_attend_not_finite(dtype, quantized):
+    """A key or value that isn't finite shows as in the formula, in its own sequence only; what stands past a
+    sequence's end in its last page does not."""
+    n, b = 1, 4
+    cache, q, k, v, table, lens = _setup(n, b, 4, 2, 64, 16, [70, 70, 70, 70], dtype, quantized, 17)
+    k[0, 1, 33, 0] = float("nan")
+    v[0, 2, 69, 1, 5] = float("inf")
+    if quantized:
+        v[0, 2, 69, 1] = float("nan")
+    cache.write(k.to(dtype), v.to(dtype), table, torch.zeros_like(lens))
+    _check(cache.attend(q, table, lens), q, k, v, lens)
+    short = lens - 1                                        # the infinity is one past the end now
+    ref, _ = attend(q, k, v, short)
+    got = cache.attend(q, table, short)
+    assert torch.isfinite(got[0, 2]).all() and torch.isfinite(ref[0, 2]).all()
+    assert torch.isnan(got[0, 1, :2]).all() and torch.isfinite(got[0, 1, 2:]).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_attend_scores_of_minus_infinity(dtype):
+    """Keys of score -infinity weigh nothing; where all are, the formula has no value (NaN)."""
+    cache, q, k, v, table, lens = _setup(1, 2, 2, 1, 64, 16, [300, 40], dtype, False, 19)
+    q = q.abs() + 0.1
+    k[0, 0, :130, 0] = -float("inf")
+    k[0, 1, :, 0] = -float("inf")
+    cache.write(k, v, table, torch.zeros_like(lens), lens)
+    got = cache.attend(q, table, lens)
+    assert torch.isnan(got[0, 1]).all()
+    ref, _ = attend(q[:, :1], k[:, :1, 130:], v[:, :1, 130:], lens[:, :1] - 130)
+    big = 64.0
+    within(got[:, :1], ref, HALF[dtype], attend_slack(dtype, big, 64, 300, v.double().abs().amax().item()))
+
+
+def test_attend_tables_out_of_range_are_reported():
+    cache, q, k, v, table, lens = _setup(1, 2, 4, 2, 64, 16, [100, 64], torch.bfloat16, False, 23)
+    bad = table.clone()
+    bad[0, 0, 2] = cache.num_pages
+    bad[0, 1, 1] = -1
+    got = cache.attend(q, bad, lens)
+    with pytest.raises(IndexError):
+        cache.index_error()
+    cache.index_error()                                     # reported once
+    # tokens of those pages take no part
+    for i, lo in ((0, 32), (1, 16)):
+        keep = [t for t in range(int(lens[0, i])) if not lo <= t < lo + 16]
+        part = torch.tensor([[len(keep)]], dtype=torch.int32, device=DEV)
+        ref, big = attend(q[:, i:i + 1], k[:, i:i + 1, keep], v[:, i:i + 1, keep], part)
+        within(got[:, i:i + 1], ref, HALF[q.dtype], attend_slack(q.dtype, big, 64, 100, v.double().abs().amax().item()))
+    # a length beyond the table, and beyond max_length
+    got = cache.attend(q, table, lens + 1000)
+    with pytest.raises(IndexError):
+        cache.index_error()
+    ref = cache.attend(q, table, torch.full_like(lens, 48))
+    assert torch.equal(cache.attend(q, table, lens, max_length=48), ref)
+    with pytest.raises(IndexError):
+        cache.index_error()
+
+
+def test_attend_no_pages_and_no_sequences():
+    import wide_compiler as wc
+    cache = wc.WidePagedCache(0, 16, 2, 64)
+    q = torch.randn(1, 2, 4, 64, device=DEV, dtype=torch.bfloat16)
+    lens = torch.tensor([[0, 5]], dtype=torch.int32, device=DEV)
+    assert (cache.attend(q, torch.zeros(1, 2, 1, dtype=torch.int32, device=DEV), lens) == 0).all()
+    assert (cache.attend(q, torch.zeros(1, 2, 0, dtype=torch.int32, device=DEV), lens) == 0).all()
+    assert cache.attend(q[:, :0], torch.zeros(1, 0, 1, dtype=torch.int32, device=DEV), lens[:, :0]).shape == (1, 0, 4, 64)
+
+
+def test_attend_graph_replays_follow_the_tables():
+    """A captured call reads lengths, tables and pages as they are at each replay."""
+    cache, q, k, v, table, lens = _setup(2, 2, 8, 2, 128, 16, [500, 300, 17, 64], torch.bfloat16, False, 29)
+    cache.attend(q, table, lens)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = cache.attend(q, table, lens)
+    for step in range(4):
+        lens.sub_(5 * step)
+        if step == 2:
+            table[0, 0, :2] = table[0, 0, :2].flip(0)
+        graph.replay()
+        eager = cache.attend(q, table, lens)
+        torch.cuda.synchronize()
+        same = torch.equal(out, eager)
+        assert same, step
+    cache.index_error()
+
+
+def test_attend_on_another_stream():
+    cache, q, k, v, table, lens = _setup(1, 4, 8, 2, 128, 16, [900, 300, 17, 64], torch.bfloat16, True, 31)
+    expect = cache.attend(q, table, lens)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = cache.attend(q, table, lens)
+    other = cache.attend(q, table, lens)                    # both at once: each call has its own workspace
+    torch.cuda.synchronize()
+    assert torch.equal(got, expect) and torch.equal(other, expect)
+
+
+def test_attend_rows_beyond_four_gigabytes():
+    """Pages whose byte offsets pass 32 bits."""
+    import wide_compiler as wc
+    page, d = 128, 256
+    pages = (5 << 30) // (page * d * 2)
+    cache = wc.WidePagedCache(pages, page, 1, d)
+    g = gen(37)
+    table = torch.tensor([[[pages - 1, 3, pages - 2]]], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([[300]], dtype=torch.int32, device=DEV)
+    k, v = (torch.randn(1, 1, 300, 1, d, generator=g).to(DEV, torch.bfloat16) for _ in range(2))
+    q = torch.randn(1, 1, 2, d, generator=g).to(DEV, torch.bfloat16)
+    cache.write(k, v, table, torch.zeros_like(lens))
+    _check(cache.attend(q, table, lens), q, k, v, lens)
+    rk, rv = cache.read(table, lens, 300)
+    assert torch.equal(rk, k) and torch.equal(rv, v)

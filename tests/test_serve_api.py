@@ -1,0 +1,279 @@
+"""The decode-step operators without a GPU: their header and binding agree, the library refuses bad arguments before any
+launch, the modules refuse tensors they do not take, 4-bit weights pack and unpack exactly."""
+
+import ctypes
+import hashlib
+import os
+import re
+import subprocess
+import sys
+
+import pytest
+import torch
+
+from tests.conftest import PKG, ROOT
+from tests._util import gen
+
+HEADER = os.path.join(ROOT, "include", "wc_serve_abi.h")
+SAN_LIB = os.path.join(PKG, "wide_compiler", "libwide_hip_san.so")
+
+
+@pytest.fixture(scope="module")
+def serve():
+    from wide_compiler import _serve
+    _serve.lib()
+    return _serve
+
+
+def _text():
+    return re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+
+
+def test_binding_declares_what_the_header_does(serve):
+    declared = sorted(set(re.findall(r"\b(wc_[a-z0-9_]+)\s*\(", _text())))
+    assert sorted(serve.SIGNATURES) == declared
+    assert serve.lib().wc_serve_abi_version() == serve.ABI_VERSION
+    # the fields of every struct, in order
+    for cls, name in ((serve._HeadNormArgs, "wc_head_norm_args"), (serve._PagedCache, "wc_paged_cache"),
+                      (serve._CacheWriteArgs, "wc_cache_write_args"), (serve._CacheReadArgs, "wc_cache_read_args"),
+                      (serve._PagedAttnArgs, "wc_paged_attn_args"), (serve._Linear4Args, "wc_linear4_args")):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), _text(), flags=re.S).group(1)
+        fields = []
+        for decl in body.split(";"):
+            words = decl.replace("const", " ").replace("*", " ").split()
+            if not words:
+                continue
+            if words[0] == "wc_paged_cache":
+                fields += [f for f, _ in serve._PagedCache._fields_]
+            else:
+                fields += " ".join(words[1:]).replace(" ", "").split(",")
+        assert [f for f, _ in cls._fields_] == fields, name
+
+
+# a digest of include/wc_serve_abi.h without comments, per version
+DECLARATIONS = {1: "e232a00a8c9af035227bbb304ee734af623bbc473e96d70fae216a89ac4b4811"}
+
+
+def test_every_change_of_the_header_has_a_version_of_its_own(serve):
+    assert DECLARATIONS.get(serve.ABI_VERSION) == hashlib.sha256(" ".join(_text().split()).encode()).hexdigest()
+
+
+def _cache(a, **kw):
+    for f, v in dict(dtype=1, bits=0, n=1, b=2, pages=4, page_size=16, heads=2, head_dim=64, row=64, k_pages=4096,
+                     v_pages=4096, table=4096, table_len=3, table_stride=3, **kw).items():
+        setattr(a, f, v)
+    return a
+
+
+def test_library_refuses_bad_arguments(serve):
+    lib, big = serve.lib(), (1 << 63) - 1
+    error = lambda: lib.wc_last_error().decode()  # noqa: E731
+    for name, (_, args) in serve.SIGNATURES.items():
+        if len(args) == 2:
+            assert getattr(lib, name)(None, None) == -1, name
+    assert lib.wc_paged_attention_workspace_bytes(None) == -1
+
+    def norm(**kw):
+        a = serve._HeadNormArgs()
+        for f, v in dict(dtype=1, param_dtype=1, position_bytes=8, n=2, b=3, t=4, q_heads=4, k_heads=2, head_dim=64,
+                         rotary_dim=64, q=4096, k=4096, q_out=4096, k_out=4096, q_weight=4096, k_weight=4096, freq=4096,
+                         positions=4096, eps=1e-6, **{}).items():
+            setattr(a, f, v)
+        for f, v in kw.items():
+            setattr(a, f, v)
+        return lib.wc_head_norm_rotary(ctypes.byref(a), None)
+    assert norm(dtype=5) == -3 and norm(position_bytes=2) == -3
+    assert norm(head_dim=63) == -2 and norm(rotary_dim=66) == -2 and norm(rotary_dim=-2) == -2 and norm(b=-1) == -2
+    assert norm(head_dim=258, rotary_dim=0) == -5 and norm(t=1 << 40) == -5 and norm(n=70000) == -5 and norm(q_heads=big) == -5
+    assert norm(q=None) == -1 and norm(freq=None) == -1 and norm(q=4097) == -4 and norm(positions=4100) == -4
+    assert norm(n=0) == 0 and norm(t=0) == 0
+
+    def write(**kw):
+        a = _cache(serve._CacheWriteArgs())
+        a.t, a.k, a.v, a.start = 5, 4096, 4096, 4096
+        for f, v in kw.items():
+            setattr(a, f, v)
+        return lib.wc_cache_write(ctypes.byref(a), None)
+    assert write(dtype=9) == -3 and write(bits=4) == -3 and write(page_size=0) == -2 and write(row=60) == -2
+    assert write(head_dim=300, row=512) == -5 and write(row=68) == -4 and write(pages=1 << 31) == -5 and write(b=big) == -5
+    assert write(pages=1 << 20, page_size=1 << 12) == -5 and "2^31 rows" in error()
+    assert write(k_pages=4104) == -4 and write(k_pages=None) == -1 and write(start=None) == -1 and write(k=4097) == -4
+    assert write(bits=8) == -1 and write(t=big) == -5 and write(t=-1) == -2 and write(t=0) == 0 and write(b=0) == 0
+
+    def read(**kw):
+        a = _cache(serve._CacheReadArgs())
+        a.lengths, a.max_length, a.k, a.v = 4096, 5, 4096, 4096
+        for f, v in kw.items():
+            setattr(a, f, v)
+        return lib.wc_cache_read(ctypes.byref(a), None)
+    assert read(max_length=-1) == -2 and read(max_length=big) == -5 and read(lengths=None) == -1 and read(v=4097) == -4
+    assert read(max_length=0) == 0
+
+    def attend(**kw):
+        a = _cache(serve._PagedAttnArgs())
+        a.q_heads, a.max_length, a.q, a.o, a.lengths, a.scale = 8, 4000, 4096, 4096, 4096, 0.1
+        for f, v in kw.items():
+            setattr(a, f, v)
+        need = int(lib.wc_paged_attention_workspace_bytes(ctypes.byref(a)))
+        return lib.wc_paged_attention(ctypes.byref(a), None), need
+    assert attend(q_heads=3) == (-2, -1) and attend(q_heads=-2) == (-2, -1) and attend(max_length=-1) == (-2, -1)
+    assert attend(max_length=big) == (-5, -1) and attend(q_heads=1 << 20) == (-5, -1) and attend(row=512, dtype=0) == (-5, -1)
+    assert attend(q=None)[0] == -1 and attend(o=4097)[0] == -4 and attend(b=0) == (0, 0)
+    # 4 key heads' worth of sequences split over their length need a workspace
+    rc, need = attend(table_len=1000, max_length=16000)
+    assert rc == -6 and need > 0 and "workspace" in error()
+    assert attend(table_len=1000, max_length=16000, workspace=4100, workspace_bytes=need)[0] == -4
+    assert attend(table_len=1000, max_length=16000, workspace=4096, workspace_bytes=need - 1)[0] == -6
+
+    def linear(**kw):
+        a = serve._Linear4Args()
+        for f, v in dict(dtype=1, group=64, n=2, m=3, o=40, k=100, x=4096, x_rows_inner=3, codes=4096, scales=4096,
+                         y=4096).items():
+            setattr(a, f, v)
+        for f, v in kw.items():
+            setattr(a, f, v)
+        return lib.wc_linear4(ctypes.byref(a), None)
+    assert linear(dtype=3) == -3 and linear(group=48) == -6 and linear(k=-1) == -2 and linear(k=0) == -2
+    assert linear(o=big) == -5 and linear(k=big) == -5 and linear(x_rows_inner=1 << 32) == -5 and linear(x_rows_inner=0) == -6
+    assert linear(codes=4100) == -4 and linear(scales=4104) == -4 and linear(x=4097) == -4 and linear(zeros=4097) == -4
+    assert linear(y=None) == -1 and linear(m=0) == 0 and linear(o=0) == 0
+
+
+def test_cpu_tensors_are_refused():
+    import wide_compiler as wc
+    for call in (lambda: wc.WideHeadNormRotary(1, 64)(torch.zeros(1, 1, 1, 2, 64), torch.zeros(1, 1, 1, 2, 64), torch.zeros(1).long()),
+                 lambda: wc.WideLinear4bit(1, 64, 16)(torch.zeros(1, 2, 64)),
+                 lambda: wc.WidePagedCache(2, 16, 2, 64, device="cpu"),
+                 lambda: wc.WidePagedCache.from_pages(torch.zeros(2, 2, 16, 64), torch.zeros(2, 2, 16, 64))):
+        with pytest.raises(RuntimeError, match="ROCm device tensors only"):
+            call()
+
+
+@pytest.fixture
+def anywhere(monkeypatch):
+    """Lets CPU tensors through the modules' checks, up to the launch, which must not be reached."""
+    from wide_compiler import _hip, _serve
+
+    def reached(*args, **kw):
+        raise AssertionError("launched")
+    monkeypatch.setattr(_hip, "require_device", lambda *a: None)
+    for name in ("head_norm_rotary", "cache_write", "cache_read", "paged_attention", "linear4"):
+        monkeypatch.setattr(_serve, name, reached)
+
+
+def test_head_norm_refusals(anywhere):
+    import wide_compiler as wc
+    for kw in (dict(head_dim=63), dict(head_dim=258), dict(head_dim=64, rotary_dim=66), dict(head_dim=64, rotary_dim=5), dict(head_dim=0)):
+        with pytest.raises(ValueError):
+            wc.WideHeadNormRotary(2, **kw)
+    with pytest.raises(ValueError):
+        wc.WideHeadNormRotary.from_modules([torch.nn.RMSNorm(64)], [torch.nn.RMSNorm(64), torch.nn.RMSNorm(64)])
+    with pytest.raises(ValueError):
+        wc.WideHeadNormRotary.from_modules([torch.nn.RMSNorm(64)], [torch.nn.RMSNorm(32)])
+    mod = wc.WideHeadNormRotary(2, 64).requires_grad_(False)
+    q, k, pos = torch.zeros(2, 3, 4, 6, 64), torch.zeros(2, 3, 4, 2, 64), torch.zeros(4, dtype=torch.int64)
+    with pytest.raises(AssertionError, match="launched"):
+        mod(q, k, pos)
+    for args in ((q[:1], k, pos), (q[..., :32], k, pos), (q, k[:, :2], pos), (q, k.half(), pos), (q, k, pos.float()),
+                 (q, k, torch.zeros(5, dtype=torch.int64)), (q[0], k, pos), (q, k, torch.zeros(1, 2, 3, 4, dtype=torch.int64)),
+                 (q.double(), k.double(), pos)):
+        with pytest.raises((RuntimeError, TypeError)):
+            if args[0].dtype == torch.float64:
+                from wide_compiler import _hip
+                _hip.dtype_code(args[0].dtype, "head_norm")
+            mod(*args)
+    with pytest.raises(RuntimeError, match="forward-only"):
+        mod(q.requires_grad_(), k, pos)
+
+
+def test_cache_refusals(anywhere):
+    import wide_compiler as wc
+    pages = torch.zeros(5, 2, 16, 64, dtype=torch.bfloat16)
+    i8, scales = torch.zeros(5, 2, 16, 64, dtype=torch.int8), torch.zeros(5, 2, 16)
+    f = wc.WidePagedCache.from_pages
+    for args, kw in (((pages, pages[:4]), {}), ((pages, pages.half()), {}), ((pages, pages), dict(dtype=torch.float16)),
+                     ((pages, pages, scales, scales), {}), ((i8, i8), dict(dtype=torch.bfloat16)),
+                     ((i8, i8, scales, scales.half()), dict(dtype=torch.bfloat16)),
+                     ((i8, i8, scales, scales[:4]), dict(dtype=torch.bfloat16)),
+                     ((pages, pages), dict(head_dim=65)), ((pages, pages), dict(head_dim=0)),
+                     ((pages[..., :60].contiguous(), pages[..., :60].contiguous()), {}),
+                     ((pages.transpose(1, 2), pages.transpose(1, 2)), {}), ((pages[:, :, :0], pages[:, :, :0]), {}),
+                     ((i8, i8, scales, None), dict(dtype=torch.bfloat16))):
+        with pytest.raises(ValueError):
+            f(*args, **kw)
+    with pytest.raises(TypeError):
+        f(pages.double(), pages.double())
+    with pytest.raises(TypeError):
+        f(i8, i8, scales, scales)                            # of which dtype?
+    with pytest.raises(ValueError):
+        wc.WidePagedCache(2, 16, 2, 300, device="cpu")
+    cache = f(pages, pages)
+    k = torch.zeros(1, 3, 7, 2, 64, dtype=torch.bfloat16)
+    q = torch.zeros(1, 3, 4, 64, dtype=torch.bfloat16)
+    table, n = torch.zeros(1, 3, 4, dtype=torch.int32), torch.zeros(1, 3, dtype=torch.int32)
+    for call in (lambda: cache.write(k, k, table, n), lambda: cache.read(table, n, 9), lambda: cache.attend(q, table, n)):
+        with pytest.raises(AssertionError, match="launched"):
+            call()
+    for call in (lambda: cache.write(k[..., :32], k[..., :32], table, n), lambda: cache.write(k, k[:, :, :6], table, n),
+                 lambda: cache.write(k.half(), k.half(), table, n), lambda: cache.write(k, k, table.long(), n),
+                 lambda: cache.write(k, k, table[:, :2], n), lambda: cache.write(k, k, table, n.long()),
+                 lambda: cache.write(k, k, table, n[:, :2]), lambda: cache.write(k, k, table, n, n.float()),
+                 lambda: cache.write(k[:, :, :, :1], k[:, :, :, :1], table, n), lambda: cache.read(table[0], n, 9),
+                 lambda: cache.read(table, n, -1), lambda: cache.read(table, n[0], 9),
+                 lambda: cache.attend(q[..., :32], table, n), lambda: cache.attend(q[:, :, :3], table, n),
+                 lambda: cache.attend(q.half(), table, n), lambda: cache.attend(q, table, n, first=n[:, :1]),
+                 lambda: cache.attend(q, table, n, max_length=-1), lambda: cache.attend(q[None], table, n)):
+        with pytest.raises(RuntimeError):
+            call()
+
+
+def test_linear4_refusals(anywhere):
+    import wide_compiler as wc
+    for args, kw in (((1, 64, 16), dict(group_size=48)), ((1, 0, 16), {})):
+        with pytest.raises(ValueError):
+            wc.WideLinear4bit(*args, **kw)
+    with pytest.raises(TypeError):
+        wc.WideLinear4bit(1, 64, 16, dtype=torch.float64)
+    codes, scales = torch.zeros(2, 16, 32, dtype=torch.uint8), torch.ones(2, 16, 1)
+    zeros = torch.zeros(2, 16, 1, dtype=torch.uint8)
+    f = wc.WideLinear4bit.from_codes
+    for kw in (dict(codes=codes.int()), dict(codes=codes[0]), dict(in_features=66), dict(scales=scales[:, :8]),
+               dict(zeros=zeros + 16), dict(zeros=zeros.int()), dict(bias=torch.zeros(2, 15)), dict(group_size=32)):
+        kw = dict(codes=codes, scales=scales, in_features=64, group_size=64, zeros=zeros) | kw
+        with pytest.raises(ValueError):
+            f(kw.pop("codes"), kw.pop("scales"), **kw)
+    mod = f(codes, scales, in_features=64, group_size=64, zeros=zeros)
+    with pytest.raises(AssertionError, match="launched"):
+        mod(torch.zeros(2, 3, 64))
+    for x in (torch.zeros(2, 3, 32), torch.zeros(1, 3, 64), torch.zeros(2, 3, 64).half(), torch.zeros(64)):
+        with pytest.raises(RuntimeError):
+            mod(x)
+
+
+@pytest.mark.parametrize("n,o,k,group,zeros", [(2, 500, 1000, 32, True), (1, 16, 128, 128, False), (3, 5, 37, 64, True),
+                                               (1, 33, 129, 32, False), (2, 1, 1, 128, True)])
+def test_linear4_codes_pack_and_unpack_exactly(n, o, k, group, zeros):
+    import wide_compiler as wc
+    g = gen(k)
+    codes = torch.randint(0, 256, (n, o, (k + 1) // 2), generator=g, dtype=torch.uint8)
+    groups = -(-k // group)
+    scales = torch.rand(n, o, groups, generator=g)
+    z = torch.randint(0, 16, (n, o, groups), generator=g, dtype=torch.uint8) if zeros else None
+    mod = wc.WideLinear4bit.from_codes(codes, scales, in_features=k, group_size=group, zeros=z)
+    c = torch.stack((codes & 15, codes >> 4), -1).flatten(-2)[..., :k].float()
+    at = torch.arange(k) // group
+    assert torch.equal(mod.dequantize(), (c - (z.float()[..., at] if zeros else 8.0)) * scales[..., at])
+
+
+def test_serve_host_side_clean_under_sanitizers():
+    from tests.test_abi_sanitized import _asan_runtime
+    if not os.path.exists(SAN_LIB) or _asan_runtime() is None:
+        pytest.skip("the sanitizer-built library or its runtime is not there")
+    env = dict(os.environ)
+    env.update(LD_PRELOAD=_asan_runtime(), ASAN_OPTIONS="detect_leaks=0:abort_on_error=1:halt_on_error=1",
+               UBSAN_OPTIONS="halt_on_error=1:print_stacktrace=1")
+    probe = os.path.join(ROOT, "tests", "san_serve_probe.py")
+    r = subprocess.run([sys.executable, probe, SAN_LIB, HEADER, "400", PKG], env=env, capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stderr[-6000:]
+    assert "runtime error" not in r.stderr and "AddressSanitizer" not in r.stderr, r.stderr[-6000:]
+    assert "no sanitizer report" in r.stdout
