@@ -27,129 +27,95 @@ struct Linear4 {
   const uint8_t *codes, *zeros;
   char* y;
   int64_t xn, xo, xi;
-  int32_t m, o, k, otiles, ktiles, steps_log2, m0;    // steps: 32-column products per group
+  int32_t m, o, k, otiles, ktiles, m0;                // m0: first row of x of a launch
+  int32_t vec;                                        // rows of x are whole 16-byte vectors
   FastDiv by_rows, by_wg;                             // rows_inner; workgroups per model
 };
 
-template <typename T>
-struct alignas(16) Eight {
-  T v[8];
-};
 template <typename T>
 struct alignas(4 * sizeof(T)) Four {
   T v[4];
 };
 
-// 8 codes as 16-bit numbers with 128 (bf16) or 1024 (fp16) added, or exact bf16 (fp32)
+// 8 codes as 16-bit numbers with 128 (bf16) or 1024 (fp16) added, or exact bf16 (fp32); `over` holds the bits above a
+// nibble in a register, so that mask and bits are one instruction
 template <typename T>
-__device__ __forceinline__ u32x4 numbers(uint32_t w) {
+__device__ __forceinline__ u32x4 numbers(uint32_t w, uint32_t over) {
   u32x4 r;
-  if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+  for (int e = 0; e < 4; ++e)
+    if constexpr (sizeof(T) == 4)
       r[e] = pack_bf16x2(static_cast<float>((w >> (4 * e)) & 15u), static_cast<float>((w >> (4 * e + 16)) & 15u));
-  } else {
-    constexpr uint32_t kOver = std::is_same<T, bf16>::value ? 0x43004300u : 0x64006400u;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r[e] = ((w >> (4 * e)) & 0x000f000fu) | kOver;
-  }
+    else
+      r[e] = ((w >> (4 * e)) & 0x000f000fu) | over;
   return r;
 }
+template <typename T>
+__device__ __forceinline__ uint32_t bits_over() {
+  uint32_t v = 0;
+  if constexpr (std::is_same<T, bf16>::value) asm("v_mov_b32 %0, 0x43004300" : "=v"(v));
+  if constexpr (std::is_same<T, f16>::value) asm("v_mov_b32 %0, 0x64006400" : "=v"(v));
+  return v;
+}
 
-// MT, RT: tiles of 16 rows of x and of 16 output rows; AL: rows of x are whole 16-byte vectors
-template <typename T, int MT, int RT, int NW, bool AL>
-__global__ __launch_bounds__(NW * 64) void linear4_kernel(Linear4 a) {
+// A tile of weights in a lane's registers: codes, and for each of the GP groups of its 128 columns the scales of rows
+// 4 g + 0..3 and the zero points of the same rows (fp16: of row j, which is where they are taken off)
+template <typename T, int GP>
+struct Tile {
+  u32x4 w;
+  Four<T> scale[GP];
+  uint32_t zero[GP];
+};
+template <typename T, int GP>
+struct TileSource {
+  const u32x4* codes;
+  const T* scales;
+  const uint8_t* zeros;
+  int last;
+  __device__ __forceinline__ TileSource(const Linear4& a, uint32_t model, int ot, int lane) {
+    const int64_t t = static_cast<int64_t>(model) * a.otiles + std::min(ot, a.otiles - 1);
+    codes = reinterpret_cast<const u32x4*>(a.codes) + t * a.ktiles * 64 + lane;
+    scales = reinterpret_cast<const T*>(a.scales) + t * a.ktiles * (GP * 16) + (lane >> 4) * 4;
+    zeros = a.zeros + t * a.ktiles * (GP * 16) + (std::is_same<T, f16>::value ? lane & 15 : (lane >> 4) * 4);
+    last = a.ktiles - 1;
+  }
+  __device__ __forceinline__ void load(Tile<T, GP>& t, int kt) const {      // past the last: the last again
+    const int k = std::min(kt, last);
+    t.w = codes[k * 64];
+#pragma unroll
+    for (int s = 0; s < GP; ++s) {
+      const int64_t m = static_cast<int64_t>(k) * GP * 16 + s * 16;
+      t.scale[s] = *reinterpret_cast<const Four<T>*>(scales + m);
+      if constexpr (std::is_same<T, f16>::value)
+        t.zero[s] = zeros[m];
+      else
+        t.zero[s] = *reinterpret_cast<const uint32_t*>(zeros + m);
+    }
+  }
+};
+
+// acc += RT tiles of weights times MT * 16 rows of x; x(q, xf): the planes of all rows of columns 32 q.., sum(q, t): the
+// sum of rows t over those columns (bf16, fp32)
+template <typename T, int GP, int RT, int MT, typename X, typename S>
+__device__ __forceinline__ void multiply(const Tile<T, GP> (&tile)[RT], uint32_t over, X x, S sum, f32x4 (&acc)[RT][MT]) {
   constexpr bool kF32 = sizeof(T) == 4, kF16 = std::is_same<T, f16>::value;
-  constexpr int NX = kF32 ? 3 : 1;                     // planes of x
-  typedef typename std::conditional<kF16, f16, bf16>::type NT;
-  extern __shared__ float lds[];                       // [NW][RT * 16][MT * 16]
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
-  const uint32_t model = fdiv(blockIdx.x, a.by_wg), ot0 = (blockIdx.x - model * a.by_wg.d) * RT;
-  const int row0 = a.m0 + blockIdx.y * MT * 16;
-  const int groups = a.ktiles << (2 - a.steps_log2);   // stored groups of a row
-
-  const T* x[MT];
+  constexpr int NX = kF32 ? 3 : 1, STEPS = 4 / GP;
+  typedef typename std::conditional<kF16, f16, bf16>::type MM;
 #pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const uint32_t r = std::min(row0 + t * 16 + j, a.m - 1);      // rows past the last only fill their own columns
-    const uint32_t outer = fdiv(r, a.by_rows);
-    x[t] = reinterpret_cast<const T*>(a.x) + model * a.xn + outer * a.xo + (r - outer * a.by_rows.d) * a.xi;
-  }
-  const u32x4* codes[RT];
-  int64_t meta[RT];
+  for (int s = 0; s < GP; ++s) {
+    f32x4 part[RT][MT] = {};
+    float total[MT] = {};
 #pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    const int64_t ot = static_cast<int64_t>(model) * a.otiles + std::min<int>(ot0 + t, a.otiles - 1);
-    codes[t] = reinterpret_cast<const u32x4*>(a.codes) + ot * a.ktiles * 64 + lane;
-    meta[t] = ot * groups * 16;
-  }
-
-  f32x4 acc[RT][MT] = {};
-  f32x4 part[RT][MT] = {};
-  f32x4 ones[MT] = {};
-  const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-
-  u32x4 next[RT];
-  if (wave < a.ktiles)
-#pragma unroll
-    for (int t = 0; t < RT; ++t) next[t] = codes[t][wave * 64];
-  for (int kt = wave; kt < a.ktiles; kt += NW) {
-    u32x4 w[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) w[t] = next[t];
-    if (kt + NW < a.ktiles)
-#pragma unroll
-      for (int t = 0; t < RT; ++t) next[t] = codes[t][(kt + NW) * 64];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int k0 = kt * 128 + q * 32 + g * 8;
-      const int grp = (kt * 4 + q) >> a.steps_log2;
-      const bool last = ((q + 1) & ((1 << a.steps_log2) - 1)) == 0;
+    for (int q = s * STEPS; q < (s + 1) * STEPS; ++q) {
       u32x4 xf[MT][NX];
-#pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        if constexpr (!kF32) {
-          u32x4 v = {};
-          if constexpr (AL) {
-            if (k0 < a.k) v = *reinterpret_cast<const u32x4*>(x[t] + k0);
-          } else {
-            Eight<T> s;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s.v[e] = k0 + e < a.k ? x[t][k0 + e] : static_cast<T>(0.f);
-            v = __builtin_bit_cast(u32x4, s);
-          }
-          xf[t][0] = v;
-        } else {
-          float s[8];
-          if constexpr (AL) {
-            f32x4 lo = {}, hi = {};
-            if (k0 < a.k) lo = *reinterpret_cast<const f32x4*>(x[t] + k0);
-            if (k0 + 4 < a.k) hi = *reinterpret_cast<const f32x4*>(x[t] + k0 + 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[e] = lo[e], s[4 + e] = hi[e];
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) s[e] = k0 + e < a.k ? x[t][k0 + e] : 0.f;
-          }
-          uint4 pl[3];
-          split_planes(s, pl);
-#pragma unroll
-          for (int n = 0; n < 3; ++n) xf[t][n] = __builtin_bit_cast(u32x4, pl[n]);
-        }
-      }
-      if constexpr (!kF16)
-#pragma unroll
-        for (int t = 0; t < MT; ++t)
-#pragma unroll
-          for (int n = NX - 1; n >= 0; --n)
-            ones[t] = mma16<bf16>(__builtin_bit_cast(bf16x8, one), __builtin_bit_cast(bf16x8, xf[t][n]), ones[t]);
+      x(q, xf);
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        u32x4 c = numbers<T>(w[r][q]);
+        u32x4 c = numbers<T>(tile[r].w[q], over);
         if constexpr (kF16) {
           typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-          const f16 z = static_cast<f16>(1024.f + (a.zeros ? a.zeros[meta[r] + grp * 16 + j] : 8));
-          const h2 zz = {z, z};
+          const f16 zero = static_cast<f16>(static_cast<float>(tile[r].zero[s] + 1024u));
+          const h2 zz = {zero, zero};
 #pragma unroll
           for (int e = 0; e < 4; ++e) c[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, static_cast<uint32_t>(c[e])) - zz);
         }
@@ -157,80 +123,360 @@ __global__ __launch_bounds__(NW * 64) void linear4_kernel(Linear4 a) {
         for (int t = 0; t < MT; ++t)
 #pragma unroll
           for (int n = NX - 1; n >= 0; --n)
-            part[r][t] = mma16<NT>(__builtin_bit_cast(bf16x8, c), __builtin_bit_cast(bf16x8, xf[t][n]), part[r][t]);
+            part[r][t] = mma16<MM>(__builtin_bit_cast(bf16x8, c), __builtin_bit_cast(bf16x8, xf[t][n]), part[r][t]);
       }
-      if (last) {
+      if constexpr (!kF16)
 #pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const int64_t at = meta[r] + grp * 16 + g * 4;
-          const Four<T> sc = *reinterpret_cast<const Four<T>*>(reinterpret_cast<const T*>(a.scales) + at);
-          float z[4] = {8.f, 8.f, 8.f, 8.f};
-          if (!kF16 && a.zeros) {
-            const uint32_t zw = *reinterpret_cast<const uint32_t*>(a.zeros + at);
+        for (int t = 0; t < MT; ++t) total[t] += sum(q, t);
+    }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) z[e] = static_cast<float>((zw >> (8 * e)) & 255u);
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float scale = to_f32(tile[r].scale[s].v[e]);
+        const float zero = static_cast<float>((tile[r].zero[s] >> (8 * e)) & 255u) + (kF32 ? 0.f : 128.f);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[r][t][e] += scale * (kF16 ? part[r][t][e] : part[r][t][e] - zero * total[t]);
+      }
+  }
+}
+
+__device__ __forceinline__ bool aligned_device(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+template <typename T>
+__device__ __forceinline__ const T* x_row(const Linear4& a, uint32_t model, int row) {
+  const uint32_t r = std::min(row, a.m - 1), outer = fdiv(r, a.by_rows);    // past the last: the last again
+  return reinterpret_cast<const T*>(a.x) + model * a.xn + outer * a.xo + (r - outer * a.by_rows.d) * a.xi;
+}
+
+// 16 bytes of a row of x at column k, and its values from the row's end on as zeros: apart, because what looks at a
+// loaded value waits for it
+template <typename T, bool AL>
+__device__ __forceinline__ u32x4 x_load(const T* x, int k, int end) {
+  if constexpr (AL) {
+    return *reinterpret_cast<const u32x4*>(x + (k < end ? k : 0));
+  } else {
+    constexpr int E = 16 / sizeof(T);
+    struct alignas(16) {
+      T v[E];
+    } s;
+#pragma unroll
+    for (int e = 0; e < E; ++e) s.v[e] = x[k + e < end ? k + e : 0];
+    return __builtin_bit_cast(u32x4, s);
+  }
+}
+template <typename T, bool AL>
+__device__ __forceinline__ u32x4 x_keep(u32x4 v, int k, int end) {
+  if constexpr (AL) {
+    return k < end ? v : u32x4{};
+  } else {
+    constexpr int E = 16 / sizeof(T);
+    struct alignas(16) {
+      T v[E];
+    } s = __builtin_bit_cast(decltype(s), v);
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (k + e >= end) s.v[e] = static_cast<T>(0.f);
+    return __builtin_bit_cast(u32x4, s);
+  }
+}
+
+// outputs o..o + 3 of a row of y, those it has
+template <typename T>
+__device__ __forceinline__ void store4(T* y, int o, int end, const T* bias, f32x4 s) {
+  Four<T> r;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (bias && o + e < end) s[e] += to_f32(bias[o + e]);
+    r.v[e] = from_f32<T>(s[e]);
+  }
+  if (o + 4 <= end && aligned_device(y + o, sizeof(r)))
+    *reinterpret_cast<Four<T>*>(y + o) = r;
+  else
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (o + e < end) y[o + e] = r.v[e];
+}
+
+// Up to 16 rows of x, straight from memory: a workgroup has one tile of output rows, its waves every NW-th tile of
+// columns.  Weights come D tiles ahead of their use, x (which all workgroups share, in L2) one.
+template <typename T, int GP, int RT, int NW, bool AL>
+__global__ __launch_bounds__(NW * 64) void linear4_few_kernel(Linear4 a) {
+  constexpr bool kF32 = sizeof(T) == 4, kF16 = std::is_same<T, f16>::value;
+  constexpr int NX = kF32 ? 3 : 1, D = RT * GP > 4 || (kF32 && RT > 1) ? 2 : 4, E = 16 / sizeof(T), P = 8 / E;
+  __shared__ float lds[NW * 16 * RT * 16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
+  const uint32_t model = fdiv(blockIdx.x, a.by_wg);
+  const int ot = (blockIdx.x - model * a.by_wg.d) * RT;
+  const int row0 = a.m0 + blockIdx.y * 16;
+  const T* x = x_row<T>(a, model, row0 + j);
+  const uint32_t over = bits_over<T>();
+  const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+
+  struct Columns {
+    u32x4 v[4][P];                       // 8 columns of each 32
+  };
+  auto bring = [&](Columns& c, int kt) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int h = 0; h < P; ++h) c.v[q][h] = x_load<T, AL>(x, kt * 128 + q * 32 + g * 8 + h * E, a.k);
+  };
+
+  f32x4 acc[RT][1] = {};
+  Tile<T, GP> tile[D][RT];
+  auto fetch = [&](int slot, int kt) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) TileSource<T, GP>(a, model, ot + t, lane).load(tile[slot][t], kt);
+  };
+  Columns cols[2];
+#pragma unroll
+  for (int i = 0; i < D; ++i) fetch(i, wave + i * NW);
+  bring(cols[0], wave);
+  for (int kt0 = wave; kt0 < a.ktiles; kt0 += D * NW) {
+#pragma unroll
+    for (int i = 0; i < D; ++i) {
+      const int kt = kt0 + i * NW;
+      if (kt < a.ktiles) {
+        bring(cols[(i + 1) & 1], kt + NW);
+        u32x4 xf[4][NX];
+        float sums[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          u32x4 v[P];
+#pragma unroll
+          for (int h = 0; h < P; ++h) v[h] = x_keep<T, AL>(cols[i & 1].v[q][h], kt * 128 + q * 32 + g * 8 + h * E, a.k);
+          if constexpr (kF32) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = __builtin_bit_cast(f32x4, v[e / 4])[e % 4];
+            uint4 pl[3];
+            split_planes(f, pl);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) xf[q][n] = __builtin_bit_cast(u32x4, pl[n]);
+          } else {
+            xf[q][0] = v[0];
           }
+          if constexpr (!kF16) {
+            f32x4 s = {};
 #pragma unroll
-          for (int t = 0; t < MT; ++t) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              float s = part[r][t][e];
-              if constexpr (!kF16) s -= (z[e] + (kF32 ? 0.f : 128.f)) * ones[t][e];
-              acc[r][t][e] += to_f32(sc.v[e]) * s;
-            }
-            part[r][t] = f32x4{};
+            for (int n = NX - 1; n >= 0; --n)
+              s = mma16<bf16>(__builtin_bit_cast(bf16x8, one), __builtin_bit_cast(bf16x8, xf[q][n]), s);
+            sums[q] = s[0];
           }
         }
+        multiply<T, GP, RT, 1>(tile[i], over,
+                               [&](int q, u32x4(&f)[1][NX]) {
 #pragma unroll
-        for (int t = 0; t < MT; ++t) ones[t] = f32x4{};
+                                 for (int n = 0; n < NX; ++n) f[0][n] = xf[q][n];
+                               },
+                               [&](int q, int) { return sums[q]; }, acc);
+        fetch(i, kt + D * NW);
+      }
+    }
+  }
+  constexpr int N = RT * 16;
+#pragma unroll
+  for (int t = 0; t < RT; ++t) *reinterpret_cast<f32x4*>(lds + (wave * 16 + j) * N + t * 16 + g * 4) = acc[t][0];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * N; i += NW * 64) {
+    const int row = row0 + i / N, o = ot * 16 + i % N;
+    if (row >= a.m || o >= a.o) continue;
+    float s = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) s += lds[w * 16 * N + i];
+    if (a.bias) s += to_f32(reinterpret_cast<const T*>(a.bias)[static_cast<int64_t>(model) * a.o + o]);
+    reinterpret_cast<T*>(a.y)[(static_cast<int64_t>(model) * a.m + row) * a.o + o] = from_f32<T>(s);
+  }
+}
+
+// More rows, through LDS: a workgroup of 8 waves, WR of them over output rows (RT tiles each) and WK over columns,
+// brings CK tiles of 128 columns of x at a time, split into planes (fp32) and with the sums over 32 columns that the
+// zero points want, once for all its output rows.  Weights come straight into registers, D tiles ahead of their use.
+constexpr int kPad = 136;          // 16-bit values in a staged row: 128, and 8 that move the rows to other banks
+
+template <typename T, int GP, int MT, int RT, int WR, int WK, int CK, bool AL>
+__global__ __launch_bounds__(WR * WK * 64) void linear4_rows_kernel(Linear4 a) {
+  constexpr bool kF32 = sizeof(T) == 4, kF16 = std::is_same<T, f16>::value;
+  constexpr int NX = kF32 ? 3 : 1, M = MT * 16, NT = WR * WK * 64;
+  static_assert(CK % WK == 0, "every wave has whole tiles of a chunk");
+  constexpr int PER = CK / WK, D = PER < 2 ? PER : 2;                   // tiles of a wave in a chunk; in flight
+  constexpr int PC = CK * M * 16 / NT, E = 16 / sizeof(T), P = 8 / E;   // pieces of 8 columns of a row each thread brings
+  static_assert(PER % D == 0 && CK * M * 16 % NT == 0, "slots repeat with the chunk, pieces with the threads");
+  extern __shared__ float lds[];
+  uint16_t* xs = reinterpret_cast<uint16_t*>(lds);                      // [CK][NX][M][kPad]
+  float* sums = lds + CK * NX * M * kPad / 2;                           // [CK][4][M]
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, j = lane & 15, g = lane >> 4;
+  const int wr = wave / WK, wk = wave % WK;
+  const uint32_t model = fdiv(blockIdx.x, a.by_wg);
+  const int ot0 = (blockIdx.x - model * a.by_wg.d) * (WR * RT) + wr * RT;
+  const int row0 = a.m0 + blockIdx.y * M;
+  const uint32_t over = bits_over<T>();
+
+  // piece i of a thread: row r % M of tile r / M, r = tid / 16 + i NT / 16, columns 8 (tid % 16)
+  u32x4 xr[PC][P];
+  const T* src[PC];
+#pragma unroll
+  for (int i = 0; i < PC; ++i) src[i] = x_row<T>(a, model, row0 + (tid / 16 + i * (NT / 16)) % M);
+  auto bring = [&](int kt0) {
+#pragma unroll
+    for (int i = 0; i < PC; ++i)
+#pragma unroll
+      for (int h = 0; h < P; ++h)
+        xr[i][h] = x_load<T, AL>(src[i], (kt0 + (tid / 16 + i * (NT / 16)) / M) * 128 + (tid % 16) * 8 + h * E, a.k);
+  };
+  auto stage = [&](int kt0) {
+#pragma unroll
+    for (int i = 0; i < PC; ++i) {
+      const int p = tid / 16 + i * (NT / 16), r = p % M, k = p / M, c = tid % 16;
+      uint16_t* dst = xs + (k * NX * M + r) * kPad + c * 8;
+      float f[8];
+      u32x4 v[P];
+#pragma unroll
+      for (int h = 0; h < P; ++h) v[h] = x_keep<T, AL>(xr[i][h], (kt0 + k) * 128 + c * 8 + h * E, a.k);
+      if constexpr (kF32) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = __builtin_bit_cast(f32x4, v[e / 4])[e % 4];
+        uint4 pl[3];
+        split_planes(f, pl);
+#pragma unroll
+        for (int n = 0; n < 3; ++n) *reinterpret_cast<uint4*>(dst + n * M * kPad) = pl[n];
+      } else {
+        *reinterpret_cast<u32x4*>(dst) = v[0];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[2 * e] = bf16_lo(v[0][e]), f[2 * e + 1] = bf16_hi(v[0][e]);
+      }
+      if constexpr (!kF16) {
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += f[e];
+        sum += __shfl_xor(sum, 1, 64);
+        sum += __shfl_xor(sum, 2, 64);
+        if ((c & 3) == 0) sums[(k * 4 + c / 4) * M + r] = sum;
+      }
+    }
+  };
+
+  f32x4 acc[RT][MT] = {};
+  Tile<T, GP> tile[D][RT];
+  auto fetch = [&](int slot, int kt) {
+#pragma unroll
+    for (int t = 0; t < RT; ++t) TileSource<T, GP>(a, model, ot0 + t, lane).load(tile[slot][t], kt);
+  };
+  bring(0);
+#pragma unroll
+  for (int i = 0; i < D; ++i) fetch(i, i * WK + wk);
+  for (int kt0 = 0; kt0 < a.ktiles; kt0 += CK) {
+    if (kt0) __syncthreads();
+    stage(kt0);
+    __syncthreads();
+    if (kt0 + CK < a.ktiles) bring(kt0 + CK);
+    // not unrolled further than the slots ask: code that runs once is fetched from memory as it runs
+#pragma unroll 1
+    for (int i0 = 0; i0 < PER; i0 += D) {
+#pragma unroll
+      for (int d = 0; d < D; ++d) {
+        const int i = i0 + d, ct = i * WK + wk;            // tile of the chunk
+        if (kt0 + ct < a.ktiles) {
+          const uint16_t* x = xs + ct * NX * M * kPad + j * kPad + g * 8;
+          const float* sum = sums + ct * 4 * M + j;
+          multiply<T, GP, RT, MT>(tile[d], over,
+                                  [&](int q, u32x4(&f)[MT][NX]) {
+#pragma unroll
+                                    for (int t = 0; t < MT; ++t)
+#pragma unroll
+                                      for (int n = 0; n < NX; ++n)
+                                        f[t][n] = *reinterpret_cast<const u32x4*>(x + (n * M + t * 16) * kPad + q * 32);
+                                  },
+                                  [&](int q, int t) { return sum[q * M + t * 16]; }, acc);
+        }
+        fetch(d, i + D < PER ? kt0 + ct + D * WK : kt0 + CK + (i + D - PER) * WK + wk);
       }
     }
   }
 
-  // lane: rows 4 g + e of an output tile, row j of x
+  T* y = reinterpret_cast<T*>(a.y) + static_cast<int64_t>(model) * a.m * a.o;
+  const T* bias = a.bias ? reinterpret_cast<const T*>(a.bias) + static_cast<int64_t>(model) * a.o : nullptr;
+  __syncthreads();                   // x is done with: [WR][WK][M][RT * 16]
+  constexpr int N = RT * 16;
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int t = 0; t < MT; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        lds[(wave * MT * 16 + t * 16 + j) * (RT * 16) + r * 16 + g * 4 + e] = acc[r][t][e];
+      *reinterpret_cast<f32x4*>(lds + (wave * M + t * 16 + j) * N + r * 16 + g * 4) = acc[r][t];
   __syncthreads();
-  T* y = reinterpret_cast<T*>(a.y) + static_cast<int64_t>(model) * a.m * a.o;
-  for (int i = threadIdx.x; i < MT * 16 * RT * 16; i += NW * 64) {
-    const int row = row0 + i / (RT * 16), o = ot0 * 16 + i % (RT * 16);
+  for (int i = tid; i < WR * M * N / 4; i += NT) {
+    // neighbouring threads: neighbouring outputs of one row, four each
+    const int c = i % (WR * N / 4) * 4, v = c / N, mr = i / (WR * N / 4);
+    const int row = row0 + mr, o = (blockIdx.x - model * a.by_wg.d) * (WR * N) + c;
     if (row >= a.m || o >= a.o) continue;
-    float s = 0.f;
-    for (int w = 0; w < NW; ++w) s += lds[w * MT * 16 * RT * 16 + i];
-    if (a.bias) s += to_f32(reinterpret_cast<const T*>(a.bias)[static_cast<int64_t>(model) * a.o + o]);
-    y[static_cast<int64_t>(row) * a.o + o] = from_f32<T>(s);
+    f32x4 s = {};
+#pragma unroll
+    for (int k = 0; k < WK; ++k) s += *reinterpret_cast<const f32x4*>(lds + ((v * WK + k) * M + mr) * N + c % N);
+    store4(y + static_cast<int64_t>(row) * a.o, o, a.o, bias, s);
   }
 }
 
-template <typename T, int MT, int RT, int NW>
-void launch(Linear4 a, int64_t n, bool al, hipStream_t s) {
+// Calls go(m0, tiles of rows from m0) for grids of at most 65535 tiles of rows
+template <typename F>
+void over_rows(Linear4& a, int rows, F go) {
+  for (int64_t m0 = 0; m0 < a.m; m0 += 65535ll * rows) {
+    a.m0 = static_cast<int32_t>(m0);
+    go(static_cast<uint32_t>(std::min<int64_t>(cdiv(a.m - m0, rows), 65535)));
+  }
+}
+
+template <typename T, int GP, int RT, int NW>
+void launch_few(Linear4 a, int64_t n, hipStream_t s) {
   const int64_t per = cdiv(a.otiles, RT);
   a.by_wg = make_fastdiv(static_cast<uint32_t>(per));
-  const size_t lds = static_cast<size_t>(NW) * RT * 16 * MT * 16 * sizeof(float);
-  // grids of at most 65535 tiles of rows
-  for (int64_t m0 = 0; m0 < a.m; m0 += 65535ll * MT * 16) {
-    a.m0 = static_cast<int32_t>(m0);
-    const dim3 grid(static_cast<uint32_t>(n * per), static_cast<uint32_t>(std::min<int64_t>(cdiv(a.m - m0, MT * 16), 65535)));
-    if (al)
-      linear4_kernel<T, MT, RT, NW, true><<<grid, NW * 64, lds, s>>>(a);
-    else
-      linear4_kernel<T, MT, RT, NW, false><<<grid, NW * 64, lds, s>>>(a);
+  const auto kernel = a.vec ? linear4_few_kernel<T, GP, RT, NW, true> : linear4_few_kernel<T, GP, RT, NW, false>;
+  over_rows(a, 16, [&](uint32_t tiles) { kernel<<<dim3(static_cast<uint32_t>(n * per), tiles), NW * 64, 0, s>>>(a); });
+}
+
+template <typename T, int GP, int MT, int RT, int WR, int WK, int CK>
+void launch_rows(Linear4 a, int64_t n, hipStream_t s) {
+  constexpr int NX = sizeof(T) == 4 ? 3 : 1, M = MT * 16;
+  const int64_t per = cdiv(a.otiles, WR * RT);
+  a.by_wg = make_fastdiv(static_cast<uint32_t>(per));
+  const size_t staged = CK * (NX * M * kPad * 2 + 4 * M * 4), joined = WR * WK * M * RT * 16 * 4;
+  const size_t lds = std::max(staged, joined);
+  const auto kernel = a.vec ? linear4_rows_kernel<T, GP, MT, RT, WR, WK, CK, true> : linear4_rows_kernel<T, GP, MT, RT, WR, WK, CK, false>;
+  if (lds > 65536)
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+  over_rows(a, M, [&](uint32_t tiles) { kernel<<<dim3(static_cast<uint32_t>(n * per), tiles), WR * WK * 64, lds, s>>>(a); });
+}
+
+// Which kernel, by the tiles of output rows of all models and the tiles of 16 rows of x (us on an MI355X, launches of
+// a graph, bf16, groups of 128):
+//   few tiles: one tile a workgroup, its waves share the columns    64 tiles, 16 rows: 4.0 (two tiles: 4.5, LDS: 6.2)
+//   more: two tiles share what they bring of x                     512 tiles, 16 rows: 9.6 (12.5, 12.2)
+//   many: x through LDS                                           2048 tiles, 16 rows: 11.3 (25.8, 17.3)
+//   and of the forms through LDS the one that meets a weight with most rows of x at once where enough workgroups
+//   remain: 2048 tiles, 64 rows: 29 (16 rows at once: 37); 4096 tiles in fp16: 36 (32 rows at once: 49).
+template <typename T, int GP>
+void dispatch(const Linear4& a, int64_t n, hipStream_t s) {
+  constexpr bool F32 = sizeof(T) == 4;
+  const int64_t tiles = n * a.otiles, rows = cdiv(a.m, 16);
+  if (tiles * rows <= 256) return launch_few<T, GP, 1, 4>(a, n, s);
+  if (rows == 1 && tiles <= 1024) return launch_few<T, GP, 2, 4>(a, n, s);
+  if constexpr (F32) {
+    if (rows > 1 && tiles >= 1024) return launch_rows<T, GP, 2, 2, 4, 2, 2>(a, n, s);
+  } else {
+    if (rows > 2 && tiles >= 4096) return launch_rows<T, GP, 4, 2, 8, 1, 4>(a, n, s);
+    if (rows > 2 || (rows > 1 && tiles >= 1024)) return launch_rows<T, GP, 2, 1, 4, 2, 8>(a, n, s);
   }
+  launch_rows<T, GP, 1, 1, 4, 2, F32 ? 4 : 16>(a, n, s);
 }
 
 template <typename T>
-void dispatch(const Linear4& a, int64_t n, bool al, hipStream_t s) {
-  if (a.m <= 16)
-    launch<T, 1, 1, 4>(a, n, al, s);
-  else if (a.m <= 32)
-    launch<T, 2, 2, 4>(a, n, al, s);
+void dispatch(const Linear4& a, int64_t n, int group, hipStream_t s) {
+  if (group == 128)
+    dispatch<T, 1>(a, n, s);
+  else if (group == 64)
+    dispatch<T, 2>(a, n, s);
   else
-    launch<T, 4, 2, 4>(a, n, al, s);
+    dispatch<T, 4>(a, n, s);
 }
 
 }  // namespace
@@ -252,7 +498,7 @@ extern "C" int32_t wc_linear4(const wc_linear4_args* args, void* stream) {
              WC_ERR_LIMIT, "%s: sizes beyond 32 bits, or more than 2^22 tiles of output rows", what);
   if (p.n == 0 || p.m == 0 || p.o == 0) return WC_OK;
   WC_REQUIRE(p.k > 0, WC_ERR_SHAPE, "%s: no columns", what);
-  WC_REQUIRE(p.x && p.codes && p.scales && p.y, WC_ERR_NULL, "%s: null pointer", what);
+  WC_REQUIRE(p.x && p.codes && p.scales && p.zeros && p.y, WC_ERR_NULL, "%s: null pointer", what);
   WC_REQUIRE(p.x_rows_inner > 0, WC_ERR_ARG, "%s: rows_inner must be positive", what);
   WC_REQUIRE(p.x_rows_inner < (1ll << 31), WC_ERR_LIMIT, "%s: rows_inner beyond 32 bits", what);
   WC_REQUIRE(aligned(p.codes, 16) && aligned(p.scales, 16) && aligned(p.zeros, 4) && aligned(p.x, es) && aligned(p.y, es) &&
@@ -273,17 +519,16 @@ extern "C" int32_t wc_linear4(const wc_linear4_args* args, void* stream) {
   a.k = static_cast<int32_t>(p.k);
   a.otiles = static_cast<int32_t>(cdiv(p.o, 16));
   a.ktiles = static_cast<int32_t>(cdiv(p.k, 128));
-  a.steps_log2 = p.group == 32 ? 0 : p.group == 64 ? 1 : 2;
   a.by_rows = make_fastdiv(static_cast<uint32_t>(p.x_rows_inner));
   // whole vectors: of 8 columns in 16 bits, of 4 in fp32
-  const bool al = p.k * es % 16 == 0 && aligned(p.x, 16) && ubytes(p.x_stride_n, es) % 16 == 0 &&
+  a.vec = p.k * es % 16 == 0 && aligned(p.x, 16) && ubytes(p.x_stride_n, es) % 16 == 0 &&
                   ubytes(p.x_stride_outer, es) % 16 == 0 && ubytes(p.x_stride_inner, es) % 16 == 0;
   const hipStream_t s = as_stream(stream);
   if (p.dtype == WC_F32)
-    dispatch<float>(a, p.n, al, s);
+    dispatch<float>(a, p.n, p.group, s);
   else if (p.dtype == WC_BF16)
-    dispatch<bf16>(a, p.n, al, s);
+    dispatch<bf16>(a, p.n, p.group, s);
   else
-    dispatch<f16>(a, p.n, al, s);
+    dispatch<f16>(a, p.n, p.group, s);
   return check_launch(what);
 }

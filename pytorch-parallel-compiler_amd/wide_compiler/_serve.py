@@ -168,11 +168,11 @@ def paged_attention(cache, q: Tensor, o: Tensor, table: Tensor, lengths: Tensor,
 
 
 def linear4(*, n: int, m: int, o: int, k: int, group: int, x: Tensor, rows, codes: Tensor, scales: Tensor,
-            zeros: Optional[Tensor], bias: Optional[Tensor], y: Tensor) -> None:
+            zeros: Tensor, bias: Optional[Tensor], y: Tensor) -> None:
     _launch("wc_linear4", _Linear4Args, _pack_linear4(
         _hip.dtype_code(x.dtype, "linear4"), group, n, m, o, k, x.data_ptr(), rows.stride_n, rows.stride_outer,
         rows.stride_inner, rows.rows_inner, codes.data_ptr(), scales.data_ptr(),
-        0 if zeros is None else zeros.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr()), x)
+        zeros.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr()), x)
 
 
 for _name in ("head_norm_rotary", "cache_write", "cache_read", "paged_attention", "linear4"):

@@ -4,8 +4,7 @@ WideLinear4bit: N independent linear layers with weights of 4 bits, for few rows
     x [N, *batch, I]  ->  y [N, *batch, O],   y[i] = x[i] @ W[i].T + bias[i]
     W[i, o, k] = scale[i, o, k // group] * (code[i, o, k] - zero[i, o, k // group])
 
-with codes of 0 to 15, groups of 32, 64 or 128 columns and whole-number zero points (8 where there
-are none).  The forward (wc_linear4) reads every weight once for up to 64 rows, so that a token's
+with codes of 0 to 15, groups of 32, 64 or 128 columns and zero points of 0 to 15 (8 where none are given).  The forward (wc_linear4) reads every weight once for up to 64 rows, so that a token's
 products cost what reading half a byte a weight costs; more rows go 64 at a time.  Sums are fp32;
 the scale multiplies each group's sum.
 
@@ -31,7 +30,7 @@ _NIBBLE = (0, 4, 1, 5, 2, 6, 3, 7)
 
 class WideLinear4bit(nn.Module):
     def __init__(self, n: int, in_features: int, out_features: int, group_size: int = 128, bias: bool = True,
-                 zeros: bool = True, dtype: torch.dtype = torch.float32):
+                 dtype: torch.dtype = torch.float32):
         super().__init__()
         if group_size not in (32, 64, 128):
             raise ValueError(f"WideLinear4bit: group_size must be 32, 64 or 128, got {group_size}")
@@ -46,7 +45,7 @@ class WideLinear4bit(nn.Module):
         meta = (n, rt, kt * (128 // group_size), 16)
         self.register_buffer("packed", torch.zeros((n, rt, kt, 64, 4), dtype=torch.int32))
         self.register_buffer("scales", torch.zeros(meta, dtype=dtype))
-        self.register_buffer("zeros", torch.zeros(meta, dtype=torch.uint8) if zeros else None)
+        self.register_buffer("zeros", torch.full(meta, 8, dtype=torch.uint8))
         self.register_buffer("bias", torch.zeros((n, out_features), dtype=dtype) if bias else None)
 
     def forward(self, x: Tensor) -> Tensor:
@@ -79,7 +78,7 @@ class WideLinear4bit(nn.Module):
         words = half[..., 0::2] | (half[..., 1::2] << 4)                 # bytes, the low nibble first
         self.packed.copy_(words.contiguous().view(torch.int32).view(self.packed.shape))
         for dst, src in ((self.scales, scales), (self.zeros, zeros)):
-            if dst is not None:
+            if src is not None:
                 rows = torch.zeros((n, rt * 16, dst.shape[2]), dtype=dst.dtype, device=codes.device)
                 rows[:, :self.out_features, :src.shape[2]] = src
                 dst.copy_(rows.view(n, rt, 16, -1).transpose(2, 3))
@@ -100,7 +99,7 @@ class WideLinear4bit(nn.Module):
         if zeros is not None and zeros.numel() and int(zeros.max()) > 15:
             raise ValueError(f"{what}: zero points must be within [0, 15]")
         wide = cls(codes.shape[0], in_features, codes.shape[1], group_size, bias=bias is not None,
-                   zeros=zeros is not None, dtype=scales.dtype).to(codes.device)
+                   dtype=scales.dtype).to(codes.device)
         rows = torch.stack((codes & 15, codes >> 4), -1).flatten(-2)[..., :in_features]
         with torch.no_grad():
             wide._pack(rows, scales, zeros)
@@ -135,12 +134,11 @@ class WideLinear4bit(nn.Module):
         half = torch.stack((b & 15, b >> 4), -1).flatten(-2)             # nibbles in order
         c = half[..., list(_NIBBLE)].permute(0, 1, 4, 2, 5, 3, 6).reshape(n, rt * 16, kt * 128)
         rows = lambda t: t.transpose(2, 3).reshape(n, rt * 16, -1).float().repeat_interleave(self.group_size, -1)  # noqa: E731
-        w = (c.float() - (8.0 if self.zeros is None else rows(self.zeros))) * rows(self.scales)
+        w = (c.float() - rows(self.zeros)) * rows(self.scales)
         return w[:, :self.out_features, :self.in_features]
 
     def __repr__(self) -> str:
-        return (f"WideLinear4bit({self.n}x[{self.in_features}->{self.out_features}], group={self.group_size}"
-                f"{'' if self.zeros is None else ', zero points'})")
+        return (f"WideLinear4bit({self.n}x[{self.in_features}->{self.out_features}], group={self.group_size})")
 
 
 __all__ = ["WideLinear4bit"]

@@ -50,7 +50,8 @@ def _check(y, x, w, size, bias):
 @pytest.mark.parametrize("n,m,k,o,zeros,bias", [
     (1, 1, 128, 16, False, False), (2, 1, 1000, 500, True, True), (3, 5, 256, 33, True, False), (1, 16, 64, 100, False, True),
     (2, 17, 520, 64, True, True), (1, 33, 37, 5, True, True), (1, 64, 1024, 130, False, False), (2, 65, 129, 48, True, False),
-    (1, 200, 96, 17, True, True), (4, 1, 1, 1, True, True)])
+    (1, 200, 96, 17, True, True), (4, 1, 1, 1, True, True), (16, 3, 300, 500, True, True), (40, 16, 270, 600, True, False),
+    (20, 20, 200, 300, True, True), (30, 30, 390, 600, True, True), (20, 50, 513, 320, True, True), (64, 64, 150, 1030, True, False)])
 def test_linear4_sizes(n, m, k, o, zeros, bias, group, dtype):
     mod, w, size, b = _layer(n, k, o, group, zeros, bias, dtype, k + o + m)
     x = torch.randn(n, m, k, generator=gen(m)).to(DEV, dtype)
@@ -119,7 +120,7 @@ def test_linear4_from_modules_against_its_weights():
 def test_linear4_state_dict_and_graph():
     import wide_compiler as wc
     mod, w, size, b = _layer(2, 384, 80, 128, True, True, torch.float16, 19)
-    other = wc.WideLinear4bit(2, 384, 80, 128, bias=True, zeros=True, dtype=torch.float16).to(DEV)
+    other = wc.WideLinear4bit(2, 384, 80, 128, bias=True, dtype=torch.float16).to(DEV)
     other.load_state_dict(mod.state_dict(), strict=True)
     x = torch.randn(2, 3, 384, generator=gen(21)).to(DEV, torch.float16)
     y = mod(x)

@@ -128,7 +128,7 @@ def test_library_refuses_bad_arguments(serve):
     def linear(**kw):
         a = serve._Linear4Args()
         for f, v in dict(dtype=1, group=64, n=2, m=3, o=40, k=100, x=4096, x_rows_inner=3, codes=4096, scales=4096,
-                         y=4096).items():
+                         zeros=4096, y=4096).items():
             setattr(a, f, v)
         for f, v in kw.items():
             setattr(a, f, v)
