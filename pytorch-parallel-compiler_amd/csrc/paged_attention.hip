@@ -29,23 +29,30 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 32;          // tokens a wave takes at a time
+constexpr int kLeast = 8;          // tiles in a part at least
+
+constexpr int kTarget = 1024;      // shares at most
+constexpr int kWhole = 1024;       // tokens up to which sequences stay whole
 
 struct Paged {
   PagedTable t;
   const char *k, *v, *q;
   const float *ks, *vs;
   char* o;
-  float* part;               // [seqs * heads][splits][dh]
-  float2* ml;                // [seqs * heads][splits]: maximum and sum, a sum of -1 where there are no tokens
+  // parts, where sequences are split (budget > 0): [parts][heads][dh] outputs, [parts][heads] maximum and sum (-1 where
+  // there are no tokens), and for each sequence its first part and how many it has
+  float* part;
+  float2* ml;
+  int2* parts;
   const int32_t *lengths, *first;
   int64_t qn, qb, qh;
-  int32_t heads, group, qtiles, splits, dh, row_bytes, most;
-  FastDiv by_split, by_qtile, by_kvh, by_b;
+  int32_t seqs, heads, group, budget, dh, row_bytes, most, qvec;    // qvec: rows of q are whole 16-byte vectors
+  FastDiv by_qtile, by_kvh, by_b;
   float scale;               // of the scores, times log2 e
 };
 
 // exp2 of a difference of scores; a part that holds nothing has m = -infinity
-__device__ __forceinline__ float weight2(float m, float top) { return exp2f(m - top); }
+__device__ __forceinline__ float weight2(float m, float top) { return __builtin_amdgcn_exp2f(m - top); }
 __device__ __forceinline__ float finite_top(float m) { return m == -INFINITY ? 0.f : m; }
 
 template <typename MT>
@@ -72,7 +79,15 @@ __device__ __forceinline__ float unpack_hi(uint32_t v) {
   else
     return bf16_hi(v);
 }
-__device__ __forceinline__ float byte_f32(uint32_t v, int i) { return static_cast<float>(static_cast<int8_t>(v >> (8 * i))); }
+// byte i (a constant) of v as a float, in one instruction
+__device__ __forceinline__ float byte_f32(uint32_t v, int i) {
+  float f;
+  if (i == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f) : "v"(v));
+  if (i == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(v));
+  if (i == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(v));
+  if (i == 3) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(v));
+  return f;
+}
 
 // 8 floats as N planes of 16-bit values whose sum they are
 template <typename MT, int N>
@@ -130,6 +145,69 @@ __device__ __forceinline__ void clear(R& r) {
   r = R(0u);
 }
 
+// A sequence's tokens [lo, hi); its tiles are counted from the one that holds token lo.
+struct Span {
+  int lo, hi;
+  bool cut;                  // the length was beyond most
+};
+__device__ __forceinline__ Span span_of(const Paged& a, int64_t seq) {
+  const int length = a.lengths[seq];
+  return Span{a.first ? max(a.first[seq], 0) : 0, min(length, a.most), length > a.most};
+}
+__device__ __forceinline__ int tiles_of(const Span& s) {
+  return s.hi > s.lo ? (s.hi - (s.lo & ~(kTile - 1)) + kTile - 1) / kTile : 0;
+}
+
+// Where sequences are cut, the tiles of all of them count as one line, of which every workgroup (of a key head) has an
+// equal share however uneven the lengths are: share w is tiles [w size, (w + 1) size), of one sequence or the ends
+// and wholes of several.  What share w has of sequence s is part w + s: no two are alike, a sequence's parts are
+// neighbours, and there are at most shares + sequences of them.  Every wave finds its share from the lengths by itself.
+struct Line {
+  int size, total;           // tiles in a share, in all
+};
+__device__ __forceinline__ Line line_of(const Paged& a, int lane) {
+  int total = 0;
+  for (int s = lane; s < a.seqs; s += 64) total += tiles_of(span_of(a, s));
+#pragma unroll
+  for (int off = 32; off; off >>= 1) total += __shfl_xor(total, off, 64);
+  return Line{max((total + a.budget - 1) / a.budget, kLeast), total};
+}
+// the sum of v over the lanes before this one
+__device__ __forceinline__ int before(int v, int lane) {
+  int sum = v;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int up = __shfl_up(sum, off, 64);
+    if (lane >= off) sum += up;
+  }
+  return sum - v;
+}
+// the sequence that has tile `at` of the line (at < total), and the line's tiles before it
+__device__ __forceinline__ int2 find_tile(const Paged& a, int at, int lane) {
+  int done = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+    const int s = s0 + lane, n = s < a.seqs ? tiles_of(span_of(a, s)) : 0;
+    const int start = done + before(n, lane);
+    const uint64_t mine = __ballot(at >= start && at < start + n);
+    if (mine) {
+      const int l = __ffsll(static_cast<unsigned long long>(mine)) - 1;
+      return make_int2(s0 + l, __shfl(start, l, 64));
+    }
+    done = __shfl(start + n, 63, 64);
+  }
+  return make_int2(a.seqs, 0);
+}
+// each sequence's first part and how many it has, for the kernel that joins them
+__device__ __forceinline__ void list_parts(const Paged& a, int size, int lane) {
+  int done = 0;
+  for (int s0 = 0; s0 < a.seqs; s0 += 64) {
+    const int s = s0 + lane, n = s < a.seqs ? tiles_of(span_of(a, s)) : 0;
+    const int start = done + before(n, lane), w0 = start / size;
+    if (s < a.seqs) a.parts[s] = n ? make_int2(w0 + s, (start + n - 1) / size - w0 + 1) : make_int2(0, 0);
+    done = __shfl(start + n, 63, 64);
+  }
+}
+
 // QT: type of q and o; KT: stored type (int8_t for codes); DC: columns provided for; NW: waves
 template <typename QT, typename KT, int DC, int NW>
 __global__ __launch_bounds__(NW * 64) void paged_attention_kernel(Paged a) {
@@ -149,317 +227,419 @@ __global__ __launch_bounds__(NW * 64) void paged_attention_kernel(Paged a) {
   typedef typename Raw<CE * ES>::type VR;
   extern __shared__ float lds[];
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
+  const int lane0 = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint32_t id = blockIdx.x;
-  uint32_t up = fdiv(id, a.by_split);
-  const int split = id - up * a.by_split.d;
-  id = up;
-  up = fdiv(id, a.by_qtile);
+  uint32_t up = fdiv(id, a.by_qtile);
   const int qtile = id - up * a.by_qtile.d;
   id = up;
-  const uint32_t seq = fdiv(id, a.by_kvh);
-  const int kvh = id - seq * a.by_kvh.d;
-  const uint32_t model = fdiv(seq, a.by_b), b = seq - model * a.by_b.d;
-  const int gq = min(16, a.group - qtile * 16);                 // query heads of this workgroup
+  up = fdiv(id, a.by_kvh);
+  const int kvh = id - up * a.by_kvh.d;
+  const int gq0 = min(16, a.group - qtile * 16);                // query heads of this workgroup
   const int head0 = kvh * a.group + qtile * 16;
-
-  int hi = a.lengths[seq];
-  if (hi > a.most) {
-    hi = a.most;
-    if (threadIdx.x == 0) paged_fault(a.t);
+  // this workgroup's tiles: those of one sequence, or a share of the line
+  int seq = up, start = 0, from = 0, to = 1 << 30;
+  if (a.budget > 0) {
+    const Line line = line_of(a, lane0);
+    if (blockIdx.x == 0 && wave == 0) list_parts(a, line.size, lane0);
+    from = up * line.size;
+    if (from >= line.total) return;
+    to = min(from + line.size, line.total);
+    const int2 first = find_tile(a, from, lane0);
+    seq = first.x;
+    start = first.y;
   }
-  const int seq_lo = a.first ? max(a.first[seq], 0) : 0;
-  // this workgroup's share: whole tiles, counted from the tile that holds the first token
-  const int base = seq_lo & ~(kTile - 1);
-  const int tiles = hi > seq_lo ? (hi - base + kTile - 1) / kTile : 0;
-  const int per = (tiles + a.splits - 1) / a.splits;
-  const int tile_lo = split * per, tile_hi = min(tiles, tile_lo + per);
+  for (;; ++seq) {
+    // What depends on the lane and the sizes alone would be kept from one sequence to the next, in more registers than
+    // there are; it is worked out again.
+    int lane = lane0, gq = gq0, dh = a.dh;
+    asm volatile("" : "+v"(lane), "+s"(gq), "+s"(dh));
+    const int j = lane & 15, g = lane >> 4;
+    const uint32_t model = fdiv(seq, a.by_b), b = seq - model * a.by_b.d;
+    const Span span = span_of(a, seq);
+    const int seq_lo = span.lo, hi = span.hi, base = seq_lo & ~(kTile - 1), tiles = tiles_of(span);
+    if (span.cut && threadIdx.x == 0) paged_fault(a.t);
+    const int tile_lo = max(from - start, 0), tile_hi = min(tiles, to - start);
+    start += tiles;
+    if (a.budget > 0 && tile_lo >= tile_hi) continue;             // a sequence without tokens
 
-  // q: the same columns of each product as K's
-  u32x4 qf[kF32 ? 1 : NF][NQ];
-  float q32[kF32 ? NCK : 1][4];
-  {
-    const QT* q = reinterpret_cast<const QT*>(a.q) + model * a.qn + b * a.qb + (head0 + min(j, gq - 1)) * a.qh;
-    if constexpr (kF32) {
+    // q: the same columns of each product as K's
+    u32x4 qf[kF32 ? 1 : NF][NQ];
+    float q32[kF32 ? NCK : 1][4];
+    {
+      const QT* q = reinterpret_cast<const QT*>(a.q) + model * a.qn + b * a.qb + (head0 + min(j, gq - 1)) * a.qh;
+      // N values from column d, zeros for what a head doesn't have; loaded from column 0 instead of not at all, without
+      // branches that every load would wait in
+      auto columns = [&](int d, auto& x) {
+        constexpr int N = sizeof(x) / sizeof(float), V = 16 / sizeof(QT);
+        QT v[N];
+        if (a.qvec) {
 #pragma unroll
-      for (int c = 0; c < NCK; ++c)
+          for (int i = 0; i < N; i += V) *reinterpret_cast<u32x4*>(v + i) = *reinterpret_cast<const u32x4*>(q + (d + i < dh ? d + i : 0));
+        } else {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = (c * 4 + g) * 4 + e;
-          q32[c][e] = j < gq && d < a.dh ? to_f32(q[d]) : 0.f;
+          for (int i = 0; i < N; ++i) v[i] = q[d + i < dh ? d + i : 0];
         }
-    } else {
 #pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        float x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int d = kQ8 ? ((f / 2) * 4 + g) * 16 + (f % 2) * 8 + e : (f * 4 + g) * 8 + e;
-          x[e] = j < gq && d < a.dh ? to_f32(q[d]) : 0.f;
-        }
-        planes<MT, NQ>(x, qf[f]);
-      }
-    }
-  }
-
-  f32x4 acc[NCV][CE] = {};
-  float m = -INFINITY, l = 0.f;
-  bool any = false;
-
-  // the pool's row of token `lane % 32` of a tile, -1 for none
-  auto look = [&](int tile) {
-    const int tok = base + tile * kTile + (lane & 31);
-    int row = -1;
-    if (tile < tile_hi && tok >= seq_lo && tok < hi) {
-      row = paged_row(a.t, seq, tok, kvh);
-      if (row < 0) paged_fault(a.t);
-    }
-    return row;
-  };
-
-  int row = look(tile_lo + wave);
-  for (int tile = tile_lo + wave; tile < tile_hi; tile += NW) {
-    const int next = look(tile + NW);
-    const bool full = __all(row >= 0);
-    any |= __any(row >= 0);
-    // rows that no token has are read as row 0 of the pool and taken out afterwards
-    float ks = 0.f, vs = 0.f;
-    if constexpr (kQ8) {
-      ks = row >= 0 ? a.ks[row] : 0.f;
-      vs = row >= 0 ? a.vs[row] : 0.f;
-    }
-    u32x4 kf[2][NCK];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const char* p = a.k + static_cast<int64_t>(max(__shfl(row, s * 16 + j, 64), 0)) * a.row_bytes;
-#pragma unroll
-      for (int c = 0; c < NCK; ++c) {
-        const int at = (c * 4 + g) * 16;
-        kf[s][c] = *reinterpret_cast<const u32x4*>(p + (at < a.row_bytes ? at : 0));
-      }
-    }
-    int vrow[8];
-    VR vf[8][NCV];
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      vrow[u] = __shfl(row, (u >> 2) * 16 + g * 4 + (u & 3), 64);
-      const char* p = a.v + static_cast<int64_t>(max(vrow[u], 0)) * a.row_bytes;
-#pragma unroll
-      for (int c = 0; c < NCV; ++c) {
-        const int at = (c * 16 + j) * CE * ES;
-        vf[u][c] = *reinterpret_cast<const VR*>(p + (at < a.row_bytes ? at : 0));
-      }
-    }
-    // columns that a row doesn't have (their q is 0, but 0 times what stands elsewhere may not be)
-    if (a.row_bytes < DC * ES) {
-#pragma unroll
-      for (int c = 0; c < NCK; ++c)
-        if ((c * 4 + g) * 16 >= a.row_bytes) clear(kf[0][c]), clear(kf[1][c]);
-    }
-
-    f32x4 s2[2] = {};
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
+        for (int i = 0; i < N; ++i) x[i] = j < gq && d + i < dh ? to_f32(v[i]) : 0.f;
+      };
       if constexpr (kF32) {
 #pragma unroll
-        for (int c = 0; c < NCK; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s2[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, kf[s][c])[e], q32[c][e], s2[s], 0, 0, 0);
+        for (int c = 0; c < NCK; ++c) columns((c * 4 + g) * 4, q32[c]);
       } else {
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
-          u32x4 x;
-          if constexpr (kQ8) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t w = kf[s][f / 2][(f % 2) * 2 + e / 2];
-              x[e] = pack2<MT>(byte_f32(w, (e & 1) * 2), byte_f32(w, (e & 1) * 2 + 1));
-            }
-          } else {
-            x = kf[s][f];
-          }
-#pragma unroll
-          for (int n = NQ - 1; n >= 0; --n)
-            s2[s] = mma16<MT>(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, qf[f][n]), s2[s]);
+          float x[8];
+          columns(kQ8 ? ((f / 2) * 4 + g) * 16 + (f % 2) * 8 : (f * 4 + g) * 8, x);
+          planes<MT, NQ>(x, qf[f]);
         }
       }
     }
 
-    float p[8], top = -INFINITY;
+    f32x4 acc[NCV][CE] = {};
+    float m = -INFINITY, l = 0.f;
+    bool any = false;
+
+    // The table's entry for token `lane % 32` of a tile, two tiles ahead of its use; nothing looks at it (and so waits for
+    // it) before row_of, the pool's row of that token or -1 for none.
+    auto look = [&](int tile) {
+      const uint32_t block = fdiv(max(base + tile * kTile + (lane & 31), 0), a.t.by_page);
+      return a.t.table[seq * a.t.stride + min(block, static_cast<uint32_t>(a.t.len - 1))];
+    };
+    auto row_of = [&](int tile, int page) {
+      const int tok = base + tile * kTile + (lane & 31);
+      if (tile >= tile_hi || tok < seq_lo || tok >= hi) return -1;
+      const uint32_t block = fdiv(tok, a.t.by_page);
+      if (block >= static_cast<uint32_t>(a.t.len) || static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.t.pages)) {
+        paged_fault(a.t);
+        return -1;
+      }
+      return (page * a.t.heads + kvh) * a.t.page + static_cast<int>(tok - block * a.t.by_page.d);
+    };
+    // Rows that no token has are read as row 0 of the pool and taken out afterwards.  K comes one tile ahead, into the
+    // registers that the scores have just been taken from, while softmax and V keep the wave busy.
+    u32x4 kf[2][NCK];
+    float ks = 0.f;
+    auto load_k = [&](int row) {
+      if constexpr (kQ8) ks = a.ks[max(row, 0)];
 #pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      p[u] = s2[u >> 2][u & 3] * a.scale;
-      if constexpr (kQ8) p[u] *= __shfl(ks, (u >> 2) * 16 + g * 4 + (u & 3), 64);
-      if (!full && vrow[u] < 0) p[u] = -INFINITY;
-      top = fmaxf(top, p[u]);
-    }
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    const float mn = fmaxf(m, top), shrink = weight2(m, finite_top(mn)), use = finite_top(mn) - kShift;
-    m = mn;
-    l *= shrink;
+      for (int s = 0; s < 2; ++s) {
+        const char* p = a.k + static_cast<int64_t>(max(__shfl(row, s * 16 + j, 64), 0)) * a.row_bytes;
 #pragma unroll
-    for (int c = 0; c < NCV; ++c)
-#pragma unroll
-      for (int e = 0; e < CE; ++e) acc[c][e] *= shrink;
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-      p[u] = exp2f(p[u] - use);
-      l += p[u];
-      if constexpr (kQ8) p[u] *= __shfl(vs, (u >> 2) * 16 + g * 4 + (u & 3), 64);
-    }
-    if (!full) {
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        if (vrow[u] < 0) {
-          p[u] = 0.f;
-#pragma unroll
-          for (int c = 0; c < NCV; ++c) clear(vf[u][c]);
+        for (int c = 0; c < NCK; ++c) {
+          const int at = (c * 4 + g) * 16;
+          kf[s][c] = *reinterpret_cast<const u32x4*>(p + (at < a.row_bytes ? at : 0));
         }
+      }
+    };
+
+    int row = -1, next = -1;
+    if (tile_lo + wave < tile_hi) {
+      row = look(tile_lo + wave);
+      next = look(tile_lo + wave + NW);
+      row = row_of(tile_lo + wave, row);
+      load_k(row);
     }
-    if constexpr (kF32) {
+    for (int tile = tile_lo + wave; tile < tile_hi; tile += NW) {
+      const bool full = __all(row >= 0);
+      any |= __any(row >= 0);
+      float vs = 0.f;
+      if constexpr (kQ8) vs = a.vs[max(row, 0)];
+      int vrow[8];
+      VR vf[8][NCV];
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
+      for (int u = 0; u < 8; ++u) {
+        vrow[u] = __shfl(row, (u >> 2) * 16 + g * 4 + (u & 3), 64);
+        const char* p = a.v + static_cast<int64_t>(max(vrow[u], 0)) * a.row_bytes;
 #pragma unroll
-        for (int c = 0; c < NCV; ++c)
+        for (int c = 0; c < NCV; ++c) {
+          const int at = (c * 16 + j) * CE * ES;
+          vf[u][c] = *reinterpret_cast<const VR*>(p + (at < a.row_bytes ? at : 0));
+        }
+      }
+      // columns that a row doesn't have (their q is 0, but 0 times what stands elsewhere may not be)
+      if (a.row_bytes < DC * ES) {
 #pragma unroll
-          for (int e = 0; e < CE; ++e)
-            acc[c][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, dword(vf[u][c], e)), p[u], acc[c][e], 0, 0, 0);
-    } else {
-      u32x4 pf[NP];
-      if constexpr (NP == 2)
-        weight_planes<MT>(p, pf);
-      else
-        planes<MT, NP>(p, pf);
+        for (int c = 0; c < NCK; ++c)
+          if ((c * 4 + g) * 16 >= a.row_bytes) clear(kf[0][c]), clear(kf[1][c]);
+      }
+
+      f32x4 s2[2] = {};
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if constexpr (kF32) {
+#pragma unroll
+          for (int c = 0; c < NCK; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s2[s] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, kf[s][c])[e], q32[c][e], s2[s], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int f = 0; f < NF; ++f) {
+            u32x4 x;
+            if constexpr (kQ8) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t w = kf[s][f / 2][(f % 2) * 2 + e / 2];
+                x[e] = pack2<MT>(byte_f32(w, (e & 1) * 2), byte_f32(w, (e & 1) * 2 + 1));
+              }
+            } else {
+              x = kf[s][f];
+            }
+#pragma unroll
+            for (int n = NQ - 1; n >= 0; --n)
+              s2[s] = mma16<MT>(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, qf[f][n]), s2[s]);
+          }
+        }
+      }
+
+      float p[8], top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        p[u] = s2[u >> 2][u & 3] * a.scale;
+        if constexpr (kQ8) p[u] *= __shfl(ks, (u >> 2) * 16 + g * 4 + (u & 3), 64);
+      }
+      // behind the last tile too (as row 0): were there a way round these loads, the wait for V would have to be one for
+      // everything in flight
+      row = row_of(tile + NW, next);
+      load_k(row);
+      next = look(tile + 2 * NW);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        if (!full && vrow[u] < 0) p[u] = -INFINITY;
+        top = fmaxf(top, p[u]);
+      }
+      top = fmaxf(top, __shfl_xor(top, 16, 64));
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float mn = fmaxf(m, top), shrink = weight2(m, finite_top(mn)), use = finite_top(mn) - kShift;
+      m = mn;
+      l *= shrink;
 #pragma unroll
       for (int c = 0; c < NCV; ++c)
 #pragma unroll
-        for (int e = 0; e < CE; ++e) {
-          u32x4 x;
+        for (int e = 0; e < CE; ++e) acc[c][e] *= shrink;
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            if constexpr (kQ8)
-              x[u] = pack2<MT>(byte_f32(dword(vf[2 * u][c], e / 4), e & 3), byte_f32(dword(vf[2 * u + 1][c], e / 4), e & 3));
-            else
-              x[u] = __builtin_amdgcn_perm(dword(vf[2 * u + 1][c], e / 2), dword(vf[2 * u][c], e / 2),
-                                           e & 1 ? 0x07060302u : 0x05040100u);
+      for (int u = 0; u < 8; ++u) {
+        p[u] = __builtin_amdgcn_exp2f(p[u] - use);
+        l += p[u];
+        if constexpr (kQ8) p[u] *= __shfl(vs, (u >> 2) * 16 + g * 4 + (u & 3), 64);
+      }
+      if (!full) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (vrow[u] < 0) {
+            p[u] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NCV; ++c) clear(vf[u][c]);
           }
+      }
+      if constexpr (kF32) {
 #pragma unroll
-          for (int n = NP - 1; n >= 0; --n)
-            acc[c][e] = mma16<MT>(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, pf[n]), acc[c][e]);
-        }
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+          for (int c = 0; c < NCV; ++c)
+#pragma unroll
+            for (int e = 0; e < CE; ++e)
+              acc[c][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, dword(vf[u][c], e)), p[u], acc[c][e], 0, 0, 0);
+      } else {
+        u32x4 pf[NP];
+        if constexpr (NP == 2)
+          weight_planes<MT>(p, pf);
+        else
+          planes<MT, NP>(p, pf);
+#pragma unroll
+        for (int c = 0; c < NCV; ++c)
+#pragma unroll
+          for (int e = 0; e < CE; ++e) {
+            u32x4 x;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              if constexpr (kQ8)
+                x[u] = pack2<MT>(byte_f32(dword(vf[2 * u][c], e / 4), e & 3), byte_f32(dword(vf[2 * u + 1][c], e / 4), e & 3));
+              else
+                x[u] = __builtin_amdgcn_perm(dword(vf[2 * u + 1][c], e / 2), dword(vf[2 * u][c], e / 2),
+                                             e & 1 ? 0x07060302u : 0x05040100u);
+            }
+#pragma unroll
+            for (int n = NP - 1; n >= 0; --n)
+              acc[c][e] = mma16<MT>(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, pf[n]), acc[c][e]);
+          }
+      }
     }
-    row = next;
-  }
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
 
-  // join the waves: [NW][gq][DC] outputs, then [NW][gq] maxima and sums (a sum of -1: no tokens)
-  float* om = lds + NW * gq * DC;
-  float* ol = om + NW * gq;
-  if (j < gq) {
-    float* o = lds + (wave * gq + j) * DC;
+    // join the waves: [NW][gq][DC] outputs, then [NW][gq] maxima and sums (a sum of -1: no tokens), which become the
+    // weights of the waves' outputs and, for each head, the maximum and the sum of them all
+    float* om = lds + NW * gq * DC;
+    float* ol = om + NW * gq;
+    if (j < gq) {
+      float* o = lds + (wave * gq + j) * DC;
 #pragma unroll
-    for (int c = 0; c < NCV; ++c)
+      for (int c = 0; c < NCV; ++c)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
+        for (int r = 0; r < 4; ++r)
 #pragma unroll
-        for (int e = 0; e < CE; ++e) o[(c * 16 + g * 4 + r) * CE + e] = acc[c][e][r];
-    if (g == 0) {
-      om[wave * gq + j] = m;
-      ol[wave * gq + j] = any ? l : -1.f;
+          for (int e = 0; e < CE; ++e) o[(c * 16 + g * 4 + r) * CE + e] = acc[c][e][r];
+      if (g == 0) {
+        om[wave * gq + j] = m;
+        ol[wave * gq + j] = any ? l : -1.f;
+      }
     }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < gq * DC; i += NW * 64) {
-    const int h = i / DC, d = i - h * DC;
-    float top = -INFINITY;
-    for (int w = 0; w < NW; ++w) top = fmaxf(top, om[w * gq + h]);
-    const float use = finite_top(top);
-    float sum = 0.f, o = 0.f;
-    bool some = false;
-    for (int w = 0; w < NW; ++w) {
-      const float lw = ol[w * gq + h];
-      if (lw < 0.f) continue;
-      some = true;
-      const float f = weight2(om[w * gq + h], use);
-      sum += f * lw;
-      o += f * lds[(w * gq + h) * DC + d];
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) < gq) {
+      const int h = threadIdx.x;
+      float mw[NW], lw[NW], top = -INFINITY, sum = 0.f;
+      bool some = false;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        mw[w] = om[w * gq + h];
+        lw[w] = ol[w * gq + h];
+        top = fmaxf(top, mw[w]);
+        some |= !(lw[w] < 0.f);
+      }
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float f = weight2(mw[w], finite_top(top));            // 0 for a wave without tokens
+        om[w * gq + h] = f;
+        sum += lw[w] < 0.f ? 0.f : f * lw[w];
+      }
+      ol[h] = sum;
+      ol[gq + h] = some;
+      if (a.budget > 0) a.ml[static_cast<int64_t>(up + seq) * a.heads + head0 + h] = make_float2(top, some ? sum : -1.f);
     }
-    if (d >= a.dh) continue;
-    const int64_t at = static_cast<int64_t>(seq) * a.heads + head0 + h;
-    if (a.splits == 1) {
-      reinterpret_cast<QT*>(a.o)[at * a.dh + d] = from_f32<QT>(some ? o / sum : 0.f);
-    } else {
-      a.part[(at * a.splits + split) * a.dh + d] = o;
-      if (d == 0) a.ml[at * a.splits + split] = make_float2(top, some ? sum : -1.f);
+    __syncthreads();
+    for (int i = threadIdx.x; i < gq * DC / 4; i += NW * 64) {
+      const int h = i / (DC / 4), d = i % (DC / 4) * 4;
+      f32x4 o = {};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) o += om[w * gq + h] * *reinterpret_cast<const f32x4*>(lds + (w * gq + h) * DC + d);
+      if (a.budget == 0) {
+        QT* y = reinterpret_cast<QT*>(a.o) + (static_cast<int64_t>(seq) * a.heads + head0 + h) * dh;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < dh) y[d + e] = from_f32<QT>(ol[gq + h] != 0.f ? o[e] / ol[h] : 0.f);
+      } else {
+        float* y = a.part + (static_cast<int64_t>(up + seq) * a.heads + head0 + h) * dh;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (d + e < dh) y[d + e] = o[e];
+      }
     }
+    if (a.budget == 0 || start >= to) return;
+    __syncthreads();
   }
 }
 
-// Joins the workgroups' parts of one (sequence, query head).
+// Joins the parts of one (sequence, query head): their weights first, one thread a part, then their outputs, four
+// columns a thread and as many parts at a time as threads remain; no load waits for another.
 template <typename QT>
-__global__ __launch_bounds__(256) void paged_join_kernel(const float* part, const float2* parts, int splits, int dh, QT* out) {
-  const int64_t at = blockIdx.x;
-  const float2* ml = parts + at * splits;
+__global__ __launch_bounds__(256) void paged_join_kernel(Paged a) {
+  __shared__ float weight[kTarget], out[4 * 256], red[8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t at = blockIdx.x, seq = at / a.heads, head = at - seq * a.heads;
+  const int2 mine = a.parts[seq];
+  const int n = mine.y;                                            // at most the shares, which are at most kTarget
+  const float2* ml = a.ml + mine.x * static_cast<int64_t>(a.heads) + head;
+  const float* part = a.part + (mine.x * static_cast<int64_t>(a.heads) + head) * a.dh;
+  float2 x[kTarget / 256];
   float top = -INFINITY;
-  for (int s = 0; s < splits; ++s) top = fmaxf(top, ml[s].x);
-  const float use = finite_top(top);
-  float sum = 0.f;
   bool some = false;
-  for (int s = 0; s < splits; ++s) {
-    const float2 x = ml[s];
-    if (x.y < 0.f) continue;
-    some = true;
-    sum += weight2(x.x, use) * x.y;
+#pragma unroll
+  for (int i = 0; i < kTarget / 256; ++i) {
+    const int s = tid + i * 256;
+    x[i] = s < n ? ml[s * static_cast<int64_t>(a.heads)] : make_float2(-INFINITY, -1.f);
+    top = fmaxf(top, x[i].x);
+    some |= !(x[i].y < 0.f);
   }
-  for (int d = threadIdx.x; d < dh; d += 256) {
-    float o = 0.f;
-    for (int s = 0; s < splits; ++s) {
-      const float2 x = ml[s];
-      if (x.y < 0.f) continue;
-      o += weight2(x.x, use) * part[(at * splits + s) * dh + d];
+#pragma unroll
+  for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  if (lane == 0) red[wave] = top;
+  some = __syncthreads_or(some);
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kTarget / 256; ++i) {
+    const float f = x[i].y < 0.f ? 0.f : weight2(x[i].x, finite_top(top));
+    if (tid + i * 256 < n) weight[tid + i * 256] = f;
+    sum += x[i].y < 0.f ? 0.f : f * x[i].y;
+  }
+#pragma unroll
+  for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  if (lane == 0) red[4 + wave] = sum;
+  __syncthreads();
+  sum = red[4] + red[5] + red[6] + red[7];
+  const int quads = (a.dh + 3) / 4, rows = 256 / quads, q = tid % quads, r = tid / quads;
+  float o[4] = {};
+  if (r < rows) {
+#pragma unroll 4
+    for (int s = r; s < n; s += rows) {
+      const float f = weight[s];
+      const float* p = part + s * static_cast<int64_t>(a.heads) * a.dh + q * 4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] += f * p[q * 4 + e < a.dh ? e : 0];
     }
-    out[at * dh + d] = from_f32<QT>(some ? o / sum : 0.f);
   }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e * 256 + tid] = o[e];
+  __syncthreads();
+  if (tid >= a.dh) return;
+  float v = 0.f;
+  for (int i = 0; i < rows; ++i) v += out[(tid & 3) * 256 + i * quads + tid / 4];
+  reinterpret_cast<QT*>(a.o)[at * a.dh + tid] = from_f32<QT>(some ? v / sum : 0.f);
 }
 
-// Workgroups a sequence's key head is split over: enough of them for the machine to have three in every compute
-// unit, but none with less than a tile per wave.
-constexpr int kWaves = 4;
-int64_t splits_of(const wc_paged_attn_args& p) {
-  const int64_t group = p.q_heads / p.cache.heads;
-  const int64_t wgs = p.cache.n * p.cache.b * p.cache.heads * cdiv(group, 16);
-  const int64_t most = cdiv(std::min(p.max_length, p.cache.table_len * p.cache.page_size), kWaves * kTile);
-  return std::max<int64_t>(1, std::min({cdiv(768, wgs), most, int64_t(64)}));
+// How the work is spread: waves in a workgroup, and the shares of the line of all tiles (0: whole sequences).
+struct Plan {
+  int waves, budget;
+  int64_t parts;             // at most
+};
+Plan plan_of(const wc_paged_attn_args& p) {
+  const int64_t seqs = p.cache.n * p.cache.b, heads = p.cache.heads * cdiv(p.q_heads / p.cache.heads, 16);
+  const int64_t longest = std::min(p.max_length, p.cache.table_len * p.cache.page_size);
+  // shares for every compute unit to have as many workgroups as its registers hold, and no more: 64 sequences of
+  // 1000-4000 tokens in 8 bits (three fit) took 100 us in one share a unit, 91 in two, 86 in three, 101 in four
+  const int wide = p.cache.head_dim <= 64 ? 0 : p.cache.head_dim <= 128 ? 1 : 2;
+  static const int kFit[2][3][3] = {{{2, 1, 1}, {3, 2, 1}, {3, 2, 1}}, {{3, 2, 1}, {4, 3, 2}, {4, 2, 1}}};
+  const int target = 256 * kFit[p.cache.bits == 8][p.cache.dtype == WC_F32 ? 0 : p.cache.dtype == WC_BF16 ? 1 : 2][wide];
+  if (seqs * heads >= 2048 || longest <= kWhole || mul_sat({seqs, cdiv(longest, kTile) + 1}) >= (1ll << 31))
+    return Plan{seqs * heads >= 512 ? 4 : 8, 0, 0};
+  const int64_t budget = cdiv(target, heads);
+  return Plan{4, static_cast<int>(budget), budget + seqs};
+}
+int64_t workspace_of(const wc_paged_attn_args& p, const Plan& plan) {
+  if (plan.budget == 0) return 0;
+  return plan.parts * p.q_heads * (p.cache.head_dim + 2) * 4 + p.cache.n * p.cache.b * 8;
 }
 
-template <typename QT, typename KT, int DC>
+template <typename QT, typename KT, int DC, int NW>
 void launch(const Paged& a, int64_t grid, hipStream_t s) {
   const int gq = std::min(a.group, 16);
-  const size_t lds = static_cast<size_t>(kWaves) * gq * (DC + 2) * sizeof(float);
-  const auto kernel = paged_attention_kernel<QT, KT, DC, kWaves>;
+  const size_t lds = static_cast<size_t>(NW) * gq * (DC + 2) * sizeof(float);
+  const auto kernel = paged_attention_kernel<QT, KT, DC, NW>;
   if (lds > 65536)
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
-  kernel<<<static_cast<uint32_t>(grid), kWaves * 64, lds, s>>>(a);
+  kernel<<<static_cast<uint32_t>(grid), NW * 64, lds, s>>>(a);
 }
 
 template <typename QT>
-void dispatch(const Paged& a, bool q8, int64_t grid, hipStream_t s) {
-  auto go = [&](auto k) {
+void dispatch(const Paged& a, bool q8, int waves, int64_t grid, hipStream_t s) {
+  auto go = [&](auto k, auto dc) {
     typedef decltype(k) KT;
+    constexpr int DC = decltype(dc)::value;
+    waves == 8 ? launch<QT, KT, DC, 8>(a, grid, s) : launch<QT, KT, DC, 4>(a, grid, s);
+  };
+  auto width = [&](auto k) {
     if (a.dh <= 64)
-      launch<QT, KT, 64>(a, grid, s);
+      go(k, std::integral_constant<int, 64>());
     else if (a.dh <= 128)
-      launch<QT, KT, 128>(a, grid, s);
+      go(k, std::integral_constant<int, 128>());
     else
-      launch<QT, KT, 256>(a, grid, s);
+      go(k, std::integral_constant<int, 256>());
   };
   if (q8)
-    go(int8_t());
+    width(int8_t());
   else
-    go(QT());
+    width(QT());
 }
 
 int32_t check(const wc_paged_attn_args& p, const char* what) {
@@ -487,8 +667,7 @@ extern "C" int64_t wc_paged_attention_workspace_bytes(const wc_paged_attn_args* 
   }
   if (check(*args, "wc_paged_attention")) return -1;
   if (args->cache.n == 0 || args->cache.b == 0 || args->q_heads == 0) return 0;
-  const int64_t s = splits_of(*args);
-  return s == 1 ? 0 : args->cache.n * args->cache.b * args->q_heads * s * (args->cache.head_dim + 2) * 4;
+  return workspace_of(*args, plan_of(*args));
 }
 
 extern "C" int32_t wc_paged_attention(const wc_paged_attn_args* args, void* stream) {
@@ -519,33 +698,40 @@ extern "C" int32_t wc_paged_attention(const wc_paged_attn_args* args, void* stre
   a.qn = p.q_stride_n;
   a.qb = p.q_stride_b;
   a.qh = p.q_stride_h;
+  a.seqs = static_cast<int32_t>(seqs);
   a.heads = static_cast<int32_t>(p.q_heads);
   a.group = static_cast<int32_t>(p.q_heads / c.heads);
-  a.qtiles = static_cast<int32_t>(cdiv(a.group, 16));
+  const int64_t qtiles = cdiv(a.group, 16);
   a.dh = static_cast<int32_t>(c.head_dim);
   a.row_bytes = static_cast<int32_t>(c.row * paged_es(c));
-  a.most = static_cast<int32_t>(c.pages ? p.max_length : 0);      // a pool without pages has no row 0 either
+  // a pool without pages has no row 0, a table without entries no entry to look at
+  a.most = static_cast<int32_t>(c.pages && c.table_len ? p.max_length : 0);
   a.scale = p.scale * kLog2e;
-  const int64_t splits = splits_of(p);
-  a.splits = static_cast<int32_t>(splits);
-  const int64_t need = splits == 1 ? 0 : seqs * p.q_heads * splits * (c.head_dim + 2) * 4;
+  a.qvec = c.head_dim * es % 16 == 0 && aligned(p.q, 16) && ubytes(p.q_stride_n, es) % 16 == 0 &&
+           ubytes(p.q_stride_b, es) % 16 == 0 && ubytes(p.q_stride_h, es) % 16 == 0;
+  const Plan plan = plan_of(p);
+  const int64_t need = workspace_of(p, plan);
   WC_REQUIRE(need == 0 || (p.workspace && p.workspace_bytes >= need), WC_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what,
              (long long)p.workspace_bytes, (long long)need);
   WC_REQUIRE(need == 0 || aligned(p.workspace, 16), WC_ERR_ALIGN, "%s: workspace must be 16-byte aligned", what);
-  a.ml = static_cast<float2*>(p.workspace);
-  a.part = need ? static_cast<float*>(p.workspace) + 2 * seqs * p.q_heads * splits : nullptr;
-  a.by_split = make_fastdiv(static_cast<uint32_t>(splits));
-  a.by_qtile = make_fastdiv(static_cast<uint32_t>(a.qtiles));
+  a.budget = plan.budget;
+  a.part = nullptr;
+  a.ml = nullptr;
+  a.parts = nullptr;
+  if (need) {
+    a.ml = static_cast<float2*>(p.workspace);
+    a.parts = reinterpret_cast<int2*>(a.ml + plan.parts * p.q_heads);
+    a.part = reinterpret_cast<float*>(a.parts + seqs);
+  }
+  a.by_qtile = make_fastdiv(static_cast<uint32_t>(qtiles));
   a.by_kvh = make_fastdiv(static_cast<uint32_t>(c.heads));
   a.by_b = make_fastdiv(static_cast<uint32_t>(c.b));
-  const int64_t grid = seqs * c.heads * a.qtiles * splits;
+  const int64_t grid = (plan.budget ? plan.budget : seqs) * c.heads * qtiles;
   const hipStream_t s = as_stream(stream);
   auto go = [&](auto t) {
     typedef decltype(t) QT;
-    dispatch<QT>(a, c.bits == 8, grid, s);
-    if (splits > 1)
-      paged_join_kernel<QT><<<static_cast<uint32_t>(seqs * p.q_heads), 256, 0, s>>>(a.part, a.ml, a.splits, a.dh,
-                                                                                 reinterpret_cast<QT*>(a.o));
+    dispatch<QT>(a, c.bits == 8, plan.waves, grid, s);
+    if (plan.budget) paged_join_kernel<QT><<<static_cast<uint32_t>(seqs * p.q_heads), 256, 0, s>>>(a);
   };
   if (c.dtype == WC_F32)
     go(float());
