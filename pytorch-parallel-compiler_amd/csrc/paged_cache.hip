@@ -5,9 +5,9 @@
 // and that enough of them are in flight.
 //
 // 8 bits: scale = max(max |x| / 127, 2^-126), code = x / scale to the nearest, ties to even.  The quotient is
-// never formed: c = rint(x * (1 / scale)) is off by at most one, and then only next to a half; the remainder
+// never formed: c = x * (1 / scale) to the nearest is off by at most one, and then only next to a half; the remainder
 // x - c scale is exact (one fused multiply-add whose result fits 24 bits) and its place against scale / 2
-// puts c right.  The code is so a function of x and scale alone.
+// puts c right, for the lanes that have such a value.  The code is so a function of x and scale alone.
 #include <algorithm>
 
 #include "wc_paged.h"
@@ -16,21 +16,31 @@ namespace wc {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kRows = 4;           // rows of a group of lanes, all on their way at once
 
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
 
-__device__ __forceinline__ int8_t code8(float x, float scale, float inv) {
-  float c = rintf(x * inv);
+// x / scale to the nearest as the low byte of the result, by adding 1.5 2^23 (after which a float's last bit is 1), and
+// how far that is from x
+constexpr float kRound = 0x1.8p23f;
+__device__ __forceinline__ uint32_t code8(float x, float scale, float inv, float& off) {
+  const float c = fmaf(x, inv, kRound);
+  off = fabsf(fmaf(kRound - c, scale, x));
+  return __builtin_bit_cast(uint32_t, c);
+}
+// the code of a value whose quotient may be next to a half
+__device__ __forceinline__ uint32_t code8_near_half(float x, float scale, float inv) {
+  float c = fmaf(x, inv, kRound) - kRound;
   const float r = fmaf(-c, scale, x), half = 0.5f * scale;
   const bool odd = static_cast<int>(c) & 1;
   if (r > half || (r == half && odd))
     c += 1.f;
   else if (r < -half || (r == -half && odd))
     c -= 1.f;
-  return static_cast<int8_t>(static_cast<int>(c));
+  return __builtin_bit_cast(uint32_t, c + kRound);
 }
 
 struct Write {
@@ -41,73 +51,102 @@ struct Write {
   int64_t stride[2][4];
   const int32_t *start, *count;
   int32_t steps, dh, row, lanes_log2;
-  FastDiv by_b, by_tiles;      // sequences per model; workgroups per sequence
+  FastDiv by_b, by_tiles, by_heads;      // sequences per model; workgroups per sequence
 };
 
 // V: values a lane loads at once; NC: of those per lane
 template <typename T, bool Q8, int V, int NC>
 __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
   const int tid = threadIdx.x, kv = blockIdx.y;
-  const int lanes = 1 << a.lanes_log2, lane = tid & (lanes - 1);
+  const int lanes = 1 << a.lanes_log2, lane = tid & (lanes - 1), groups = kThreads >> a.lanes_log2;
   const uint32_t seq = fdiv(blockIdx.x, a.by_tiles), tile = blockIdx.x - seq * a.by_tiles.d;
-  const int64_t r = static_cast<int64_t>(tile) * (kThreads >> a.lanes_log2) + (tid >> a.lanes_log2);
-  const uint32_t step = static_cast<uint32_t>(r / a.t.heads), h = static_cast<uint32_t>(r - static_cast<int64_t>(step) * a.t.heads);
+  const uint32_t model = fdiv(seq, a.by_b), b = seq - model * a.by_b.d;
+  const int64_t* st = a.stride[kv];
+  const T* src = reinterpret_cast<const T*>(a.src[kv]) + model * st[0] + b * st[1];
   int n = a.count ? a.count[seq] : a.steps;
+  const int start = a.start[seq];
   if (n > a.steps) {
     n = a.steps;
     paged_fault(a.t);
   }
-  const int start = a.start[seq];
-  if (r >= static_cast<int64_t>(a.steps) * a.t.heads || static_cast<int>(step) >= n || start < 0) return;
-  const int64_t tok = static_cast<int64_t>(start) + step;
-  const int32_t row = tok > INT32_MAX ? -1 : paged_row(a.t, seq, static_cast<uint32_t>(tok), h);
-  if (row < 0) {
-    paged_fault(a.t);
-    return;
-  }
-  const uint32_t model = fdiv(seq, a.by_b), b = seq - model * a.by_b.d;
-  const int64_t* st = a.stride[kv];
-  const T* src = reinterpret_cast<const T*>(a.src[kv]) + model * st[0] + b * st[1] + step * st[2] + h * st[3];
-  Vec<T, V> x[NC];
+  if (start < 0) return;
+  const uint32_t rows = static_cast<uint32_t>(max(n, 0)) * a.t.heads;       // to write
+  const uint32_t r0 = tile * (groups * kRows) + (tid >> a.lanes_log2);
+  if (tile * (groups * kRows) >= rows) return;
+
+  // rows past the last are loaded as the last and not stored
+  Vec<T, V> x[kRows][NC];
+  int32_t row[kRows];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int d = (lane + c * lanes) * V;
-    if (d < a.dh) x[c] = *reinterpret_cast<const Vec<T, V>*>(src + d);
-  }
-  if constexpr (!Q8) {
-    T* dst = reinterpret_cast<T*>(a.pages[kv]) + static_cast<int64_t>(row) * a.row;
+  for (int u = 0; u < kRows; ++u) {
+    const uint32_t r = min(r0 + u * groups, rows - 1), step = fdiv(r, a.by_heads), h = r - step * a.by_heads.d;
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int d = (lane + c * lanes) * V;
-      if (d < a.dh) *reinterpret_cast<Vec<T, V>*>(dst + d) = x[c];
+      x[u][c] = *reinterpret_cast<const Vec<T, V>*>(src + step * st[2] + h * st[3] + (d < a.dh ? d : 0));
     }
-    for (int d = a.dh + lane; d < a.row; d += lanes) dst[d] = static_cast<T>(0.f);
-  } else {
-    // the largest magnitude by its bits, under which an infinity or NaN is larger than any finite value
-    uint32_t top = 0;
-    float f[NC][V];
+    const int64_t tok = static_cast<int64_t>(start) + step;
+    row[u] = tok > INT32_MAX ? -1 : paged_row(a.t, seq, static_cast<uint32_t>(tok), h);
+  }
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+  for (int u = 0; u < kRows; ++u) {
+    const bool mine = r0 + u * groups < rows;
+    if (mine && row[u] < 0) paged_fault(a.t);
+    const bool store = mine && row[u] >= 0;
+    const int64_t at = static_cast<int64_t>(row[u]) * a.row;
+    if constexpr (!Q8) {
+      if (!store) continue;
+      T* dst = reinterpret_cast<T*>(a.pages[kv]) + at;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        f[c][e] = (lane + c * lanes) * V < a.dh ? to_f32(x[c].v[e]) : 0.f;
-        top = max(top, __builtin_bit_cast(uint32_t, f[c][e]) & 0x7fffffffu);
+      for (int c = 0; c < NC; ++c) {
+        const int d = (lane + c * lanes) * V;
+        if (d < a.dh) *reinterpret_cast<Vec<T, V>*>(dst + d) = x[u][c];
       }
-    for (int off = lanes >> 1; off; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 64)));
-    const bool finite = top < 0x7f800000u;
-    const float scale = finite ? fmaxf(__builtin_bit_cast(float, top) / 127.f, 0x1p-126f) : __builtin_nanf("");
-    const float inv = 1.f / scale;
-    int8_t* dst = reinterpret_cast<int8_t*>(a.pages[kv]) + static_cast<int64_t>(row) * a.row;
+      for (int d = a.dh + lane; d < a.row; d += lanes) dst[d] = static_cast<T>(0.f);
+    } else {
+      // the largest magnitude by its bits, under which an infinity or NaN is larger than any finite value
+      uint32_t top = 0;
+      float f[NC][V];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      const int d = (lane + c * lanes) * V;
-      Vec<int8_t, V> o;
+      for (int c = 0; c < NC; ++c)
 #pragma unroll
-      for (int e = 0; e < V; ++e) o.v[e] = finite ? code8(f[c][e], scale, inv) : static_cast<int8_t>(0);
-      if (d < a.dh) *reinterpret_cast<Vec<int8_t, V>*>(dst + d) = o;
+        for (int e = 0; e < V; ++e) {
+          f[c][e] = (lane + c * lanes) * V < a.dh ? to_f32(x[u][c].v[e]) : 0.f;
+          top = max(top, __builtin_bit_cast(uint32_t, f[c][e]) & 0x7fffffffu);
+        }
+      for (int off = lanes >> 1; off; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 64)));
+      const bool finite = top < 0x7f800000u;
+      const float scale = finite ? fmaxf(__builtin_bit_cast(float, top) / 127.f, 0x1p-126f) : __builtin_nanf("");
+      const float inv = 1.f / scale;
+      uint32_t code[NC][V];
+      float far = 0.f;
+#pragma unroll
+      for (int c = 0; c < NC; ++c)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          float off;
+          code[c][e] = code8(f[c][e], scale, inv, off);
+          far = fmaxf(far, off);
+        }
+      // 2^-15 covers the product's rounding: 2^-23 of a quotient of up to 127, and inv's
+      if (far > scale * (0.5f - 0x1p-15f))
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+#pragma unroll
+          for (int e = 0; e < V; ++e) code[c][e] = code8_near_half(f[c][e], scale, inv);
+      if (!store) continue;
+      int8_t* dst = reinterpret_cast<int8_t*>(a.pages[kv]) + at;
+#pragma unroll
+      for (int c = 0; c < NC; ++c) {
+        const int d = (lane + c * lanes) * V;
+        Vec<int8_t, V> o;
+#pragma unroll
+        for (int e = 0; e < V; ++e) o.v[e] = static_cast<int8_t>(finite ? code[c][e] : 0u);
+        if (d < a.dh) *reinterpret_cast<Vec<int8_t, V>*>(dst + d) = o;
+      }
+      for (int d = a.dh + lane; d < a.row; d += lanes) dst[d] = 0;
+      if (lane == 0) a.scales[kv][row[u]] = scale;
     }
-    for (int d = a.dh + lane; d < a.row; d += lanes) dst[d] = 0;
-    if (lane == 0) a.scales[kv][row] = scale;
   }
 }
 
@@ -118,48 +157,60 @@ struct Read {
   char* out[2];
   const int32_t* lengths;
   int32_t most, dh, row, lanes_log2;
-  FastDiv by_tiles;
+  FastDiv by_tiles, by_heads;
 };
 
 template <typename T, bool Q8, int V, int NC>
 __global__ __launch_bounds__(kThreads) void cache_read_kernel(Read a) {
   typedef typename std::conditional<Q8, int8_t, T>::type S;
   const int tid = threadIdx.x, kv = blockIdx.y;
-  const int lanes = 1 << a.lanes_log2, lane = tid & (lanes - 1);
+  const int lanes = 1 << a.lanes_log2, lane = tid & (lanes - 1), groups = kThreads >> a.lanes_log2;
   const uint32_t seq = fdiv(blockIdx.x, a.by_tiles), tile = blockIdx.x - seq * a.by_tiles.d;
-  const int64_t rows = static_cast<int64_t>(a.most) * a.t.heads;
-  const int64_t r = static_cast<int64_t>(tile) * (kThreads >> a.lanes_log2) + (tid >> a.lanes_log2);
-  if (r >= rows) return;
-  const uint32_t tok = static_cast<uint32_t>(r / a.t.heads), h = static_cast<uint32_t>(r - static_cast<int64_t>(tok) * a.t.heads);
+  const uint32_t rows = static_cast<uint32_t>(a.most) * a.t.heads;
+  const uint32_t r0 = tile * (groups * kRows) + (tid >> a.lanes_log2);
   const int32_t length = a.lengths[seq];
-  int32_t row = -1;
-  if (static_cast<int32_t>(tok) < length) {
-    row = paged_row(a.t, seq, tok, h);
-    if (row < 0) paged_fault(a.t);
-  }
   if (length > a.most) paged_fault(a.t);
-  const float scale = Q8 && row >= 0 ? a.scales[kv][row] : 1.f;
-  const S* src = reinterpret_cast<const S*>(a.pages[kv]) + static_cast<int64_t>(row) * a.row;
-  T* out = reinterpret_cast<T*>(a.out[kv]) + (static_cast<int64_t>(seq) * rows + r) * a.dh;
+  int32_t row[kRows];
 #pragma unroll
-  for (int c = 0; c < NC; ++c) {
-    const int d = (lane + c * lanes) * V;
-    if (d >= a.dh) continue;
-    Vec<T, V> o;
-    if (row < 0) {
+  for (int u = 0; u < kRows; ++u) {
+    const uint32_t r = min(r0 + u * groups, rows - 1), tok = fdiv(r, a.by_heads), h = r - tok * a.by_heads.d;
+    const bool has = static_cast<int32_t>(tok) < length;
+    row[u] = has ? paged_row(a.t, seq, tok, h) : -1;
+    if (has && row[u] < 0) paged_fault(a.t);
+  }
+  // rows that aren't there are read as row 0 of the pool, if it has one, and become zeros
+  Vec<S, V> x[kRows][NC];
+  float scale[kRows];
 #pragma unroll
-      for (int e = 0; e < V; ++e) o.v[e] = static_cast<T>(0.f);
-    } else {
-      const Vec<S, V> x = *reinterpret_cast<const Vec<S, V>*>(src + d);
+  for (int u = 0; u < kRows; ++u) {
+    const int64_t at = max(row[u], 0);
+    if (a.t.pages == 0) continue;
+    scale[u] = Q8 ? a.scales[kv][at] : 1.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int d = (lane + c * lanes) * V;
+      x[u][c] = *reinterpret_cast<const Vec<S, V>*>(reinterpret_cast<const S*>(a.pages[kv]) + at * a.row + (d < a.dh ? d : 0));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const uint32_t r = r0 + u * groups;
+    if (r >= rows) continue;
+    T* out = reinterpret_cast<T*>(a.out[kv]) + (static_cast<int64_t>(seq) * rows + r) * a.dh;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const int d = (lane + c * lanes) * V;
+      if (d >= a.dh) continue;
+      Vec<T, V> o;
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         if constexpr (Q8)
-          o.v[e] = from_f32<T>(static_cast<float>(x.v[e]) * scale);
+          o.v[e] = from_f32<T>(row[u] < 0 ? 0.f : static_cast<float>(x[u][c].v[e]) * scale[u]);
         else
-          o.v[e] = x.v[e];
+          o.v[e] = row[u] < 0 ? static_cast<T>(0.f) : x[u][c].v[e];
       }
+      *reinterpret_cast<Vec<T, V>*>(out + d) = o;
     }
-    *reinterpret_cast<Vec<T, V>*>(out + d) = o;
   }
 }
 
@@ -209,7 +260,7 @@ extern "C" int32_t wc_cache_write(const wc_cache_write_args* args, void* stream)
   if (int32_t rc = paged_check(c, what)) return rc;
   const int es = dtype_size(c.dtype);
   WC_REQUIRE(p.t >= 0, WC_ERR_SHAPE, "%s: negative size", what);
-  WC_REQUIRE(mul_sat({p.t, c.heads}) < (1ll << 31), WC_ERR_LIMIT, "%s: more than 2^31 rows per sequence", what);
+  WC_REQUIRE(mul_sat({p.t, c.heads}) < (1ll << 30), WC_ERR_LIMIT, "%s: 2^30 rows per sequence or more", what);
   const int64_t seqs = c.n * c.b;
   if (seqs == 0 || p.t == 0 || c.heads == 0) return WC_OK;
   if (int32_t rc = paged_check_pointers(c, what)) return rc;
@@ -238,10 +289,11 @@ extern "C" int32_t wc_cache_write(const wc_cache_write_args* args, void* stream)
   a.dh = static_cast<int32_t>(c.head_dim);
   a.row = static_cast<int32_t>(c.row);
   a.lanes_log2 = log2_lanes(vec ? cdiv(c.head_dim * es, 16) : c.head_dim);
-  const int64_t tiles = cdiv(p.t * c.heads, kThreads >> a.lanes_log2);
+  const int64_t tiles = cdiv(p.t * c.heads, kRows * (kThreads >> a.lanes_log2));
   WC_REQUIRE(mul_sat({tiles, seqs}) < (1ll << 32) / kThreads, WC_ERR_LIMIT, "%s: too many rows for one launch", what);
   a.by_b = make_fastdiv(static_cast<uint32_t>(c.b));
   a.by_tiles = make_fastdiv(static_cast<uint32_t>(tiles));
+  a.by_heads = make_fastdiv(static_cast<uint32_t>(c.heads));
   dispatch<RunWrite>(c.dtype, c.bits, vec, a, dim3(static_cast<uint32_t>(tiles * seqs), 2), as_stream(stream));
   return check_launch(what);
 }
@@ -256,7 +308,7 @@ extern "C" int32_t wc_cache_read(const wc_cache_read_args* args, void* stream) {
   if (int32_t rc = paged_check(c, what)) return rc;
   const int es = dtype_size(c.dtype);
   WC_REQUIRE(p.max_length >= 0, WC_ERR_SHAPE, "%s: negative size", what);
-  WC_REQUIRE(mul_sat({p.max_length, c.heads}) < (1ll << 31), WC_ERR_LIMIT, "%s: more than 2^31 rows per sequence", what);
+  WC_REQUIRE(mul_sat({p.max_length, c.heads}) < (1ll << 30), WC_ERR_LIMIT, "%s: 2^30 rows per sequence or more", what);
   const int64_t seqs = c.n * c.b;
   if (seqs == 0 || p.max_length == 0 || c.heads == 0) return WC_OK;
   if (int32_t rc = paged_check_pointers(c, what)) return rc;
@@ -277,9 +329,10 @@ extern "C" int32_t wc_cache_read(const wc_cache_read_args* args, void* stream) {
   a.row = static_cast<int32_t>(c.row);
   const bool vec = c.head_dim * es % 16 == 0 && aligned(p.k, 16) && aligned(p.v, 16);
   a.lanes_log2 = log2_lanes(vec ? cdiv(c.head_dim * es, 16) : c.head_dim);
-  const int64_t tiles = cdiv(p.max_length * c.heads, kThreads >> a.lanes_log2);
+  const int64_t tiles = cdiv(p.max_length * c.heads, kRows * (kThreads >> a.lanes_log2));
   WC_REQUIRE(mul_sat({tiles, seqs}) < (1ll << 32) / kThreads, WC_ERR_LIMIT, "%s: too many rows for one launch", what);
   a.by_tiles = make_fastdiv(static_cast<uint32_t>(tiles));
+  a.by_heads = make_fastdiv(static_cast<uint32_t>(c.heads));
   dispatch<RunRead>(c.dtype, c.bits, vec, a, dim3(static_cast<uint32_t>(tiles * seqs), 2), as_stream(stream));
   return check_launch(what);
 }

@@ -118,63 +118,83 @@ def same_device(what: str, like: Tensor, *tensors: Optional[Tensor]) -> None:
             raise RuntimeError(f"{what}: tensors on {like.device} and {t.device}; one call takes one device")
 
 
-def head_norm_rotary(*, q: Tensor, k: Tensor, q_out: Tensor, k_out: Tensor, q_weight: Tensor, k_weight: Tensor,
-                     freq: Tensor, positions: Tensor, rotary_dim: int, interleaved: bool, eps: float) -> None:
-    """q [N, B, T, Hq, Dh], k [N, B, T, Hk, Dh] (unit last stride), positions expanded to [N, B, T]; q_out, k_out
-    contiguous; freq the turns per position as the bits of fp64."""
+# Plans: what a call's sizes, strides and types come to, worked out (and checked) once for each form of a call and
+# kept by the module or cache that is called: the leading fields of the argument struct.  The tensors' addresses are
+# read on every call.
+
+class Plans(dict):
+    """Plans by the form of a call; a program that never repeats a form does not fill memory with them."""
+
+    def keep(self, form, plan):
+        if len(self) >= 256:
+            self.clear()
+        self[form] = plan
+        return plan
+
+
+def head_norm_plan(*, q: Tensor, k: Tensor, q_weight: Tensor, positions: Tensor, rotary_dim: int,
+                   interleaved: bool) -> Tuple:
+    """q [N, B, T, Hq, Dh], k [N, B, T, Hk, Dh] (unit last stride), positions expanded to [N, B, T]."""
     n, b, t, hq, dh = q.shape
+    return ((_hip.dtype_code(q.dtype, "head_norm"), _hip.dtype_code(q_weight.dtype, "head_norm"),
+             1 if interleaved else 0, positions.element_size(), n, b, t, hq, k.shape[3], dh, rotary_dim),
+            q.stride()[:4], k.stride()[:4], positions.stride())
+
+
+def head_norm_rotary(plan, q: Tensor, k: Tensor, q_out: Tensor, k_out: Tensor, q_weight: Tensor, k_weight: Tensor,
+                     freq: Tensor, positions: Tensor, eps: float) -> None:
+    """q_out, k_out contiguous; freq the turns per position as the bits of fp64."""
+    sizes, q_strides, k_strides, p_strides = plan
     _launch("wc_head_norm_rotary", _HeadNormArgs, _pack_head_norm(
-        _hip.dtype_code(q.dtype, "head_norm"), _hip.dtype_code(q_weight.dtype, "head_norm"), 1 if interleaved else 0,
-        positions.element_size(), n, b, t, hq, k.shape[3], dh, rotary_dim,
-        q.data_ptr(), *q.stride()[:4], k.data_ptr(), *k.stride()[:4], q_out.data_ptr(), k_out.data_ptr(),
-        q_weight.data_ptr(), k_weight.data_ptr(), freq.data_ptr(), positions.data_ptr(), *positions.stride(), eps), q)
+        *sizes, q.data_ptr(), *q_strides, k.data_ptr(), *k_strides, q_out.data_ptr(), k_out.data_ptr(),
+        q_weight.data_ptr(), k_weight.data_ptr(), freq.data_ptr(), positions.data_ptr(), *p_strides, eps), q)
 
 
-def _cache_fields(cache, table: Tensor, n: int, b: int) -> Tuple:
-    return (*cache._sizes[:2], n, b, *cache._sizes[2:], cache.k_pages.data_ptr(), cache.v_pages.data_ptr(),
-            0 if cache.k_scales is None else cache.k_scales.data_ptr(),
-            0 if cache.v_scales is None else cache.v_scales.data_ptr(),
-            table.data_ptr(), table.shape[2], table.shape[2], cache._err.data_ptr())
+def _cache_fields(cache, sizes: Tuple, table: Tensor) -> Tuple:
+    k, v, ks, vs = cache._pools
+    m = table.shape[2]
+    return (*sizes, k.data_ptr(), v.data_ptr(), 0 if ks is None else ks.data_ptr(), 0 if vs is None else vs.data_ptr(),
+            table.data_ptr(), m, m, cache._err.data_ptr())
 
 
-def cache_write(cache, k: Tensor, v: Tensor, table: Tensor, start: Tensor, count: Optional[Tensor]) -> None:
-    n, b, t = k.shape[:3]
+def cache_write(cache, sizes: Tuple, k: Tensor, v: Tensor, table: Tensor, start: Tensor,
+                count: Optional[Tensor]) -> None:
     _launch("wc_cache_write", _CacheWriteArgs, _pack_write(
-        *_cache_fields(cache, table, n, b), t, k.data_ptr(), *k.stride()[:4], v.data_ptr(), *v.stride()[:4],
+        *_cache_fields(cache, sizes, table), k.shape[2], k.data_ptr(), *k.stride()[:4], v.data_ptr(), *v.stride()[:4],
         start.data_ptr(), 0 if count is None else count.data_ptr()), k)
 
 
-def cache_read(cache, table: Tensor, lengths: Tensor, max_length: int, k: Tensor, v: Tensor) -> None:
-    n, b = table.shape[:2]
+def cache_read(cache, sizes: Tuple, table: Tensor, lengths: Tensor, max_length: int, k: Tensor, v: Tensor) -> None:
     _launch("wc_cache_read", _CacheReadArgs, _pack_read(
-        *_cache_fields(cache, table, n, b), lengths.data_ptr(), max_length, k.data_ptr(), v.data_ptr()), table)
+        *_cache_fields(cache, sizes, table), lengths.data_ptr(), max_length, k.data_ptr(), v.data_ptr()), table)
 
 
-def paged_attention(cache, q: Tensor, o: Tensor, table: Tensor, lengths: Tensor, first: Optional[Tensor],
-                    scale: float, max_length: int, workspace_of) -> None:
-    """workspace_of(bytes): a workspace tensor; called only where the sizes need one."""
-    n, b, heads = q.shape[:3]
-    fields = (*_cache_fields(cache, table, n, b), heads, max_length, q.data_ptr(), *q.stride()[:3], o.data_ptr(),
-              lengths.data_ptr(), 0 if first is None else first.data_ptr())
-    block = _pack_attn(*fields, 0, 0, scale)
-    need = int(lib().wc_paged_attention_workspace_bytes(ctypes.byref(_PagedAttnArgs.from_buffer_copy(block))))
+def paged_attention_workspace(cache, sizes: Tuple, table: Tensor, heads: int, max_length: int) -> int:
+    """Bytes of workspace that attention of `heads` query heads takes."""
+    a = _PagedAttnArgs.from_buffer_copy(_pack_attn(*_cache_fields(cache, sizes, table), heads, max_length, 0, 0, 0, 0,
+                                                   0, 0, 0, 0, 0, 0.0))
+    need = int(lib().wc_paged_attention_workspace_bytes(ctypes.byref(a)))
     if need < 0:
         raise _hip.WideKernelError(f"wc_paged_attention: {_hip.last_error()}")
-    ws = None
-    if need:
-        ws = workspace_of(need)
-        block = _pack_attn(*fields, ws.data_ptr(), need, scale)
-    _launch("wc_paged_attention", _PagedAttnArgs, block, q)
+    return need
 
 
-def linear4(*, n: int, m: int, o: int, k: int, group: int, x: Tensor, rows, codes: Tensor, scales: Tensor,
-            zeros: Tensor, bias: Optional[Tensor], y: Tensor) -> None:
+def paged_attention(cache, sizes: Tuple, q: Tensor, o: Tensor, table: Tensor, lengths: Tensor, first: Optional[Tensor],
+                    scale: float, max_length: int, workspace: Optional[Tensor]) -> None:
+    _launch("wc_paged_attention", _PagedAttnArgs, _pack_attn(
+        *_cache_fields(cache, sizes, table), q.shape[2], max_length, q.data_ptr(), *q.stride()[:3], o.data_ptr(),
+        lengths.data_ptr(), 0 if first is None else first.data_ptr(),
+        *((0, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())), scale), q)
+
+
+def linear4(sizes: Tuple, rows, x: Tensor, codes: Tensor, scales: Tensor, zeros: Tensor, bias: Optional[Tensor],
+            y: Tensor) -> None:
+    """sizes: dtype, group, n, m, o, k; rows the strides of x (_layout.Rows)."""
     _launch("wc_linear4", _Linear4Args, _pack_linear4(
-        _hip.dtype_code(x.dtype, "linear4"), group, n, m, o, k, x.data_ptr(), rows.stride_n, rows.stride_outer,
-        rows.stride_inner, rows.rows_inner, codes.data_ptr(), scales.data_ptr(),
-        zeros.data_ptr(), 0 if bias is None else bias.data_ptr(), y.data_ptr()), x)
+        *sizes, x.data_ptr(), rows[0], rows[1], rows[2], rows[3], codes.data_ptr(), scales.data_ptr(), zeros.data_ptr(),
+        0 if bias is None else bias.data_ptr(), y.data_ptr()), x)
 
 
-for _name in ("head_norm_rotary", "cache_write", "cache_read", "paged_attention", "linear4"):
+for _name in ("head_norm_rotary", "cache_write", "cache_read", "paged_attention_workspace", "paged_attention", "linear4"):
     globals()[_name] = torch.compiler.disable(globals()[_name])
 del _name

@@ -82,60 +82,95 @@ class WidePagedCache:
         if page_size < 1 or row * k_pages.element_size() % 16 or row > 512:
             raise ValueError(f"{what}: pages of at least one token, rows of whole 16 bytes and at most 512 elements, "
                              f"got {page_size} and {row}")
-        self.k_pages, self.v_pages, self.k_scales, self.v_scales = k_pages, v_pages, k_scales, v_scales
+        self._pools = (k_pages, v_pages, k_scales, v_scales)
         self.num_pages, self.n_kv_heads, self.page_size, self.head_dim = pages, heads, page_size, head_dim
         self.dtype, self.quantized, self.device = dtype, quantized, k_pages.device
         self._err = torch.zeros(1, dtype=torch.int32, device=self.device)
         self._sizes = (code, 8 if quantized else 0, pages, page_size, heads, head_dim, row)
+        self._plans = _serve.Plans()
 
-    def _table(self, what: str, table: Tensor, n: int, b: int) -> Tensor:
-        if table.dim() != 3 or table.dtype != torch.int32 or table.shape[0] != n or table.shape[1] != b:
-            raise RuntimeError(f"{what}: block_table must be int32 [N={n}, B={b}, M], got {table.dtype} {list(table.shape)}")
-        return table if table.is_contiguous() else table.contiguous()
+    def _sizes_for(self, n: int, b: int) -> Tuple:
+        return (*self._sizes[:2], n, b, *self._sizes[2:])
+
+    # The pools are this cache's for good: its plans hold their sizes.
+    @property
+    def k_pages(self) -> Tensor:
+        return self._pools[0]
+
+    @property
+    def v_pages(self) -> Tensor:
+        return self._pools[1]
+
+    @property
+    def k_scales(self) -> Optional[Tensor]:
+        return self._pools[2]
+
+    @property
+    def v_scales(self) -> Optional[Tensor]:
+        return self._pools[3]
 
     @staticmethod
-    def _per_sequence(what: str, name: str, t: Tensor, n: int, b: int) -> Tensor:
-        if t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != n or t.shape[1] != b:
+    def _check_table(what: str, table: Tensor, n: int, b: int) -> None:
+        if table.dim() != 3 or table.dtype != torch.int32 or table.shape[0] != n or table.shape[1] != b:
+            raise RuntimeError(f"{what}: block_table must be int32 [N={n}, B={b}, M], got {table.dtype} {list(table.shape)}")
+
+    @staticmethod
+    def _check_per_sequence(what: str, name: str, t: Optional[Tensor], n: int, b: int) -> None:
+        if t is not None and (t.dtype != torch.int32 or t.dim() != 2 or t.shape[0] != n or t.shape[1] != b):
             raise RuntimeError(f"{what}: {name} must be int32 [N={n}, B={b}], got {t.dtype} {list(t.shape)}")
-        return t if t.is_contiguous() else t.contiguous()
+
+    @staticmethod
+    def _dense(t: Optional[Tensor]) -> Optional[Tensor]:
+        return t if t is None or t.is_contiguous() else t.contiguous()
 
     def write(self, k: Tensor, v: Tensor, block_table: Tensor, start: Tensor, count: Optional[Tensor] = None) -> None:
         """Rows [0, count[n, b]) of k, v [N, B, T, Hkv, Dh] become tokens start[n, b] + 0, 1, ... of their
         sequences (count None: all T).  Rows from count on are padding, and a sequence of negative start takes part in
         nothing: neither is written."""
-        what = "WidePagedCache.write"
-        _hip.require_device(what, k, v, block_table, start, count)
-        _hip.require_forward_only(what, k, v)
-        if k.dim() != 5 or k.shape != v.shape or k.shape[3] != self.n_kv_heads or k.shape[4] != self.head_dim:
-            raise RuntimeError(f"{what}: k and v must be [N, B, T, {self.n_kv_heads}, {self.head_dim}], got "
-                               f"{list(k.shape)} and {list(v.shape)}")
-        if k.dtype != self.dtype or v.dtype != self.dtype:
-            raise RuntimeError(f"{what}: k {k.dtype} and v {v.dtype} in a cache for {self.dtype}")
-        n, b = k.shape[:2]
-        table = self._table(what, block_table, n, b)
-        start = self._per_sequence(what, "start", start, n, b)
-        if count is not None:
-            count = self._per_sequence(what, "count", count, n, b)
-        _serve.same_device(what, self.k_pages, k, v, table, start, count)
+        form = (k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, block_table.shape,
+                block_table.dtype, block_table.device, start.shape, start.dtype, start.device,
+                None if count is None else (count.shape, count.dtype, count.device))
+        plan = self._plans.get(form)
+        if plan is None:
+            what = "WidePagedCache.write"
+            _hip.require_device(what, k, v, block_table, start, count)
+            if k.dim() != 5 or k.shape != v.shape or k.shape[3] != self.n_kv_heads or k.shape[4] != self.head_dim:
+                raise RuntimeError(f"{what}: k and v must be [N, B, T, {self.n_kv_heads}, {self.head_dim}], got "
+                                   f"{list(k.shape)} and {list(v.shape)}")
+            if k.dtype != self.dtype or v.dtype != self.dtype:
+                raise RuntimeError(f"{what}: k {k.dtype} and v {v.dtype} in a cache for {self.dtype}")
+            n, b = k.shape[:2]
+            self._check_table(what, block_table, n, b)
+            self._check_per_sequence(what, "start", start, n, b)
+            self._check_per_sequence(what, "count", count, n, b)
+            _serve.same_device(what, self.k_pages, k, v, block_table, start, count)
+            plan = self._plans.keep(form, self._sizes_for(n, b))
+        if torch.is_grad_enabled():
+            _hip.require_forward_only("WidePagedCache.write", k, v)
         k = k if k.stride(4) == 1 else k.contiguous()
         v = v if v.stride(4) == 1 else v.contiguous()
-        _serve.cache_write(self, k, v, table, start, count)
+        _serve.cache_write(self, plan, k, v, self._dense(block_table), self._dense(start), self._dense(count))
 
     def read(self, block_table: Tensor, lengths: Tensor, max_length: int) -> Tuple[Tensor, Tensor]:
         """K and V of tokens [0, lengths[n, b]) as [N, B, max_length, Hkv, Dh]; zeros from a sequence's length on."""
-        what = "WidePagedCache.read"
-        _hip.require_device(what, block_table, lengths)
-        if max_length < 0:
-            raise RuntimeError(f"{what}: max_length must not be negative, got {max_length}")
-        n, b = block_table.shape[:2]
-        table = self._table(what, block_table, n, b)
-        lengths = self._per_sequence(what, "lengths", lengths, n, b)
-        _serve.same_device(what, self.k_pages, table, lengths)
-        shape = (n, b, max_length, self.n_kv_heads, self.head_dim)
+        form = (block_table.shape, block_table.dtype, block_table.device, lengths.shape, lengths.dtype, lengths.device,
+                max_length)
+        plan = self._plans.get(form)
+        if plan is None:
+            what = "WidePagedCache.read"
+            _hip.require_device(what, block_table, lengths)
+            if max_length < 0:
+                raise RuntimeError(f"{what}: max_length must not be negative, got {max_length}")
+            n, b = block_table.shape[:2]
+            self._check_table(what, block_table, n, b)
+            self._check_per_sequence(what, "lengths", lengths, n, b)
+            _serve.same_device(what, self.k_pages, block_table, lengths)
+            plan = self._plans.keep(form, (self._sizes_for(n, b), (n, b, max_length, self.n_kv_heads, self.head_dim)))
+        sizes, shape = plan
         k = torch.empty(shape, dtype=self.dtype, device=self.device)
         v = torch.empty(shape, dtype=self.dtype, device=self.device)
         if k.numel():
-            _serve.cache_read(self, table, lengths, max_length, k, v)
+            _serve.cache_read(self, sizes, self._dense(block_table), self._dense(lengths), max_length, k, v)
         return k, v
 
     def attend(self, q: Tensor, block_table: Tensor, lengths: Tensor, first: Optional[Tensor] = None,
@@ -145,31 +180,46 @@ class WidePagedCache:
         head h reads key head h // (Hq // Hkv); scale defaults to Dh ** -0.5.  A sequence without tokens gets
         zeros.  ``max_length`` bounds the lengths (default: what the block table can name); a tight bound splits
         short sequences less."""
+        form = (q.shape, q.dtype, q.device, block_table.shape, block_table.dtype, block_table.device, lengths.shape,
+                lengths.dtype, lengths.device, None if first is None else (first.shape, first.dtype, first.device),
+                max_length)
+        plan = self._plans.get(form)
+        if plan is None:
+            plan = self._plans.keep(form, self._plan_attend(q, block_table, lengths, first, max_length))
+        sizes, most, need = plan
+        if torch.is_grad_enabled():
+            _hip.require_forward_only("WidePagedCache.attend", q)
+        q = q if q.stride(3) == 1 else q.contiguous()
+        o = q.new_empty(q.shape)
+        if o.numel():
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
+            _serve.paged_attention(self, sizes, q, o, self._dense(block_table), self._dense(lengths), self._dense(first),
+                                   self.head_dim ** -0.5 if scale is None else scale, most, ws)
+        return o
+
+    def _plan_attend(self, q: Tensor, block_table: Tensor, lengths: Tensor, first: Optional[Tensor],
+                     max_length: Optional[int]) -> Tuple:
         what = "WidePagedCache.attend"
         _hip.require_device(what, q, block_table, lengths, first)
-        _hip.require_forward_only(what, q)
         if q.dim() != 4 or q.shape[3] != self.head_dim or q.shape[2] % self.n_kv_heads:
             raise RuntimeError(f"{what}: q must be [N, B, a multiple of {self.n_kv_heads} heads, {self.head_dim}], got "
                                f"{list(q.shape)}")
         if q.dtype != self.dtype:
             raise RuntimeError(f"{what}: q {q.dtype} over a cache for {self.dtype}")
         n, b = q.shape[:2]
-        table = self._table(what, block_table, n, b)
-        lengths = self._per_sequence(what, "lengths", lengths, n, b)
-        if first is not None:
-            first = self._per_sequence(what, "first", first, n, b)
-        _serve.same_device(what, self.k_pages, q, table, lengths, first)
-        most = table.shape[2] * self.page_size
+        self._check_table(what, block_table, n, b)
+        self._check_per_sequence(what, "lengths", lengths, n, b)
+        self._check_per_sequence(what, "first", first, n, b)
+        _serve.same_device(what, self.k_pages, q, block_table, lengths, first)
         if max_length is None:
-            max_length = min(most, 2 ** 31 - 65)
+            max_length = min(block_table.shape[2] * self.page_size, 2 ** 31 - 65)
         elif max_length < 0:
             raise RuntimeError(f"{what}: max_length must not be negative, got {max_length}")
-        q = q if q.stride(3) == 1 else q.contiguous()
-        o = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if o.numel():
-            _serve.paged_attention(self, q, o, table, lengths, first, self.head_dim ** -0.5 if scale is None else scale,
-                                   max_length, lambda need: torch.empty(need, dtype=torch.uint8, device=q.device))
-        return o
+        sizes = self._sizes_for(n, b)
+        need = 0
+        if q.numel():
+            need = _serve.paged_attention_workspace(self, sizes, block_table, q.shape[2], max_length)
+        return sizes, max_length, need
 
     def index_error(self) -> None:
         """Raise IndexError if any call since the last check met a page outside the pool, or a token, count or length

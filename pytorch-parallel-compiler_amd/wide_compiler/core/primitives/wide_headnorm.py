@@ -47,15 +47,35 @@ class WideHeadNormRotary(nn.Module):
                             dtype=torch.float64)
         # turns per position, as the bits of fp64: .to(dtype) leaves integer buffers as they are
         self.register_buffer("_freq_bits", freq.view(torch.int64), persistent=False)
+        self._plans = _serve.Plans()
 
     def forward(self, q: Tensor, k: Tensor, positions: Tensor) -> Tuple[Tensor, Tensor]:
+        params = self._parameters
+        qw, kw, freq = params["q_weight"], params["k_weight"], self._buffers["_freq_bits"]
+        form = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, positions.shape,
+                positions.stride(), positions.dtype, positions.device, qw.shape, qw.dtype, qw.device, kw.shape, kw.dtype, kw.device)
+        plan = self._plans.get(form)
+        if plan is None:
+            plan = self._plan(form, q, k, positions, qw, kw, freq)
+        if torch.is_grad_enabled():
+            _hip.require_forward_only("WideHeadNormRotary", q, k, qw, kw)
+        q = q if q.stride(4) == 1 else q.contiguous()
+        k = k if k.stride(4) == 1 else k.contiguous()
+        if not (qw.is_contiguous() and kw.is_contiguous()):
+            qw, kw = qw.contiguous(), kw.contiguous()
+        q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
+        _serve.head_norm_rotary(plan, q, k, q_out, k_out, qw, kw, freq, positions, self.eps)
+        return q_out, k_out
+
+    def _plan(self, form, q: Tensor, k: Tensor, positions: Tensor, qw: Tensor, kw: Tensor, freq: Tensor):
         what = "WideHeadNormRotary"
-        qw, kw, freq = self.q_weight, self.k_weight, self._freq_bits
         _hip.require_device(what, q, k, positions, qw, kw)
-        _hip.require_forward_only(what, q, k, qw, kw)
         for name, t in (("q", q), ("k", k)):
             if t.dim() != 5 or t.shape[0] != self.n or t.shape[4] != self.head_dim:
                 raise RuntimeError(f"{what}: {name} must be [N={self.n}, B, T, heads, {self.head_dim}], got {list(t.shape)}")
+        for name, t in (("q_weight", qw), ("k_weight", kw)):
+            if tuple(t.shape) != (self.n, self.head_dim):
+                raise RuntimeError(f"{what}: {name} must be [{self.n}, {self.head_dim}], got {list(t.shape)}")
         if q.shape[:3] != k.shape[:3]:
             raise RuntimeError(f"{what}: q {list(q.shape)} and k {list(k.shape)} differ in [N, B, T]")
         if q.dtype != k.dtype or qw.dtype != kw.dtype:
@@ -71,14 +91,8 @@ class WideHeadNormRotary(nn.Module):
                                f"{list(q.shape[:3])}") from None
         q = q if q.stride(4) == 1 else q.contiguous()
         k = k if k.stride(4) == 1 else k.contiguous()
-        qw = qw if qw.is_contiguous() else qw.contiguous()
-        kw = kw if kw.is_contiguous() else kw.contiguous()
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-        _serve.head_norm_rotary(q=q, k=k, q_out=q_out, k_out=k_out, q_weight=qw, k_weight=kw, freq=freq,
-                                positions=positions, rotary_dim=self.rotary_dim, interleaved=self.interleaved,
-                                eps=self.eps)
-        return q_out, k_out
+        return self._plans.keep(form, _serve.head_norm_plan(q=q, k=k, q_weight=qw, positions=positions,
+                                                            rotary_dim=self.rotary_dim, interleaved=self.interleaved))
 
     @classmethod
     def from_modules(cls, q_norms: List[nn.RMSNorm], k_norms: List[nn.RMSNorm], rotary_dim: Optional[int] = None,

@@ -47,24 +47,37 @@ class WideLinear4bit(nn.Module):
         self.register_buffer("scales", torch.zeros(meta, dtype=dtype))
         self.register_buffer("zeros", torch.full(meta, 8, dtype=torch.uint8))
         self.register_buffer("bias", torch.zeros((n, out_features), dtype=dtype) if bias else None)
+        self._plans = _serve.Plans()
 
     def forward(self, x: Tensor) -> Tensor:
+        bufs = self._buffers
+        packed, scales, zeros, bias = bufs["packed"], bufs["scales"], bufs["zeros"], bufs["bias"]
+        form = (x.shape, x.stride(), x.dtype, x.device, packed.device, scales.dtype, scales.device, zeros.device,
+                None if bias is None else (bias.dtype, bias.device))
+        plan = self._plans.get(form)
+        if plan is None:
+            plan = self._plan(form, x, packed, scales, zeros, bias)
+        if torch.is_grad_enabled():
+            _hip.require_forward_only("WideLinear4bit", x)
+        dense, rows, sizes, shape = plan
+        if not dense:
+            x = x.contiguous()
+        y = x.new_empty(shape)
+        if y.numel():
+            _serve.linear4(sizes, rows, x, packed, scales, zeros, bias, y)
+        return y
+
+    def _plan(self, form, x: Tensor, packed: Tensor, scales: Tensor, zeros: Tensor, bias: Optional[Tensor]):
         what = "WideLinear4bit"
         if x.dim() < 2 or x.shape[0] != self.n or x.shape[-1] != self.in_features:
             raise RuntimeError(f"{what}: expected input [N={self.n}, ..., {self.in_features}], got {list(x.shape)}")
-        bufs = self._buffers
-        packed, scales, zeros, bias = bufs["packed"], bufs["scales"], bufs["zeros"], bufs["bias"]
         _hip.require_device(what, x, packed)
-        _hip.require_forward_only(what, x)
         if x.dtype != scales.dtype or (bias is not None and bias.dtype != x.dtype):
             raise RuntimeError(f"{what}: input dtype {x.dtype} != {scales.dtype} of scales and bias")
         _serve.same_device(what, x, packed, scales, zeros, bias)
-        x, r = rows_or_contiguous(x)
-        y = torch.empty((*x.shape[:-1], self.out_features), dtype=x.dtype, device=x.device)
-        if y.numel():
-            _serve.linear4(n=self.n, m=r.rows, o=self.out_features, k=self.in_features, group=self.group_size, x=x,
-                           rows=r, codes=packed, scales=scales, zeros=zeros, bias=bias, y=y)
-        return y
+        dense, rows = rows_or_contiguous(x)
+        sizes = (_hip.dtype_code(x.dtype, "linear4"), self.group_size, self.n, rows.rows, self.out_features, self.in_features)
+        return self._plans.keep(form, (dense is x, rows, sizes, (*x.shape[:-1], self.out_features)))
 
     def _pack(self, codes: Tensor, scales: Tensor, zeros: Optional[Tensor]) -> None:
         """codes [N, O, I] uint8 of 0-15, scales and zeros [N, O, ceil(I / group)] into the buffers."""

@@ -159,6 +159,7 @@ def anywhere(monkeypatch):
     monkeypatch.setattr(_hip, "require_device", lambda *a: None)
     for name in ("head_norm_rotary", "cache_write", "cache_read", "paged_attention", "linear4"):
         monkeypatch.setattr(_serve, name, reached)
+    monkeypatch.setattr(_serve, "paged_attention_workspace", lambda *a: 0)
 
 
 def test_head_norm_refusals(anywhere):
