@@ -43,6 +43,31 @@ __device__ __forceinline__ uint32_t code8_near_half(float x, float scale, float 
   return __builtin_bit_cast(uint32_t, c + kRound);
 }
 
+// The largest magnitude of a lane's values as the bits of a float, under which an infinity or NaN is larger than any
+// finite value; 16-bit values are compared two at a time.
+template <typename T, int V, int NC>
+__device__ __forceinline__ uint32_t largest(const Vec<T, V> (&x)[NC]) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  uint32_t top = 0;
+  if constexpr (sizeof(T) == 2 && V == 8) {
+    u16x2 t = {};
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      const u32x4 w = __builtin_bit_cast(u32x4, x[c]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t = __builtin_elementwise_max(t, __builtin_bit_cast(u16x2, static_cast<uint32_t>(w[e]) & 0x7fff7fffu));
+    }
+    const uint16_t m = max(t[0], t[1]);
+    top = __builtin_bit_cast(uint32_t, to_f32(__builtin_bit_cast(T, m)));
+  } else {
+#pragma unroll
+    for (int c = 0; c < NC; ++c)
+#pragma unroll
+      for (int e = 0; e < V; ++e) top = max(top, __builtin_bit_cast(uint32_t, to_f32(x[c].v[e])) & 0x7fffffffu);
+  }
+  return top;
+}
+
 struct Write {
   PagedTable t;
   const char *src[2];
@@ -74,7 +99,7 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
   const uint32_t r0 = tile * (groups * kRows) + (tid >> a.lanes_log2);
   if (tile * (groups * kRows) >= rows) return;
 
-  // rows past the last are loaded as the last and not stored
+  // rows past the last are loaded as the last and not stored; lanes past a row's end hold its first values again
   Vec<T, V> x[kRows][NC];
   int32_t row[kRows];
 #pragma unroll
@@ -104,20 +129,11 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
       }
       for (int d = a.dh + lane; d < a.row; d += lanes) dst[d] = static_cast<T>(0.f);
     } else {
-      // the largest magnitude by its bits, under which an infinity or NaN is larger than any finite value
-      uint32_t top = 0;
-      float f[NC][V];
-#pragma unroll
-      for (int c = 0; c < NC; ++c)
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          f[c][e] = (lane + c * lanes) * V < a.dh ? to_f32(x[u][c].v[e]) : 0.f;
-          top = max(top, __builtin_bit_cast(uint32_t, f[c][e]) & 0x7fffffffu);
-        }
+      uint32_t top = largest<T, V, NC>(x[u]);
       for (int off = lanes >> 1; off; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 64)));
       const bool finite = top < 0x7f800000u;
       const float scale = finite ? fmaxf(__builtin_bit_cast(float, top) / 127.f, 0x1p-126f) : __builtin_nanf("");
-      const float inv = 1.f / scale;
+      const float inv = __builtin_amdgcn_rcpf(scale);
       uint32_t code[NC][V];
       float far = 0.f;
 #pragma unroll
@@ -125,24 +141,33 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           float off;
-          code[c][e] = code8(f[c][e], scale, inv, off);
+          code[c][e] = code8(to_f32(x[u][c].v[e]), scale, inv, off);
           far = fmaxf(far, off);
         }
-      // 2^-15 covers the product's rounding: 2^-23 of a quotient of up to 127, and inv's
+      // 2^-15 covers the product's rounding and inv's: 2^-22 of a quotient of up to 127
       if (far > scale * (0.5f - 0x1p-15f))
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int e = 0; e < V; ++e) code[c][e] = code8_near_half(f[c][e], scale, inv);
+          for (int e = 0; e < V; ++e) code[c][e] = code8_near_half(to_f32(x[u][c].v[e]), scale, inv);
       if (!store) continue;
       int8_t* dst = reinterpret_cast<int8_t*>(a.pages[kv]) + at;
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const int d = (lane + c * lanes) * V;
-        Vec<int8_t, V> o;
+        if (d >= a.dh) continue;
+        if constexpr (V == 1) {
+          dst[d] = static_cast<int8_t>(finite ? code[c][0] : 0u);
+        } else {
+          Vec<uint32_t, V / 4> o;
 #pragma unroll
-        for (int e = 0; e < V; ++e) o.v[e] = static_cast<int8_t>(finite ? code[c][e] : 0u);
-        if (d < a.dh) *reinterpret_cast<Vec<int8_t, V>*>(dst + d) = o;
+          for (int q = 0; q < V / 4; ++q) {
+            const uint32_t* k = code[c] + 4 * q;
+            const uint32_t lo = __builtin_amdgcn_perm(k[1], k[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(k[3], k[2], 0x0c0c0400u);
+            o.v[q] = finite ? lo | hi << 16 : 0u;
+          }
+          *reinterpret_cast<Vec<uint32_t, V / 4>*>(dst + d) = o;
+        }
       }
       for (int d = a.dh + lane; d < a.row; d += lanes) dst[d] = 0;
       if (lane == 0) a.scales[kv][row[u]] = scale;
