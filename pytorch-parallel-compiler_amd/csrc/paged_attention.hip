@@ -29,10 +29,8 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 32;          // tokens a wave takes at a time
-constexpr int kLeast = 8;          // tiles in a part at least
-
-constexpr int kTarget = 1024;      // shares at most
-constexpr int kWhole = 1024;       // tokens up to which sequences stay whole
+constexpr int kLeast = 8;          // tiles in a part at least: two for each of its waves
+constexpr int kTarget = 1024;      // shares of the line at most
 
 struct Paged {
   PagedTable t;
@@ -588,6 +586,10 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Paged a) {
   reinterpret_cast<QT*>(a.o)[at * a.dh + tid] = from_f32<QT>(some ? v / sum : 0.f);
 }
 
+// Whether 8 waves of a workgroup find registers for their rows (two waves a SIMD).
+template <typename QT, typename KT, int DC>
+constexpr bool kRoom8 = DC <= (std::is_same<KT, float>::value ? 64 : 128);
+
 // How the work is spread: waves in a workgroup, and the shares of the line of all tiles (0: whole sequences).
 struct Plan {
   int waves, budget;
@@ -601,8 +603,12 @@ Plan plan_of(const wc_paged_attn_args& p) {
   const int wide = p.cache.head_dim <= 64 ? 0 : p.cache.head_dim <= 128 ? 1 : 2;
   static const int kFit[2][3][3] = {{{2, 1, 1}, {3, 2, 1}, {3, 2, 1}}, {{3, 2, 1}, {4, 3, 2}, {4, 2, 1}}};
   const int target = 256 * kFit[p.cache.bits == 8][p.cache.dtype == WC_F32 ? 0 : p.cache.dtype == WC_BF16 ? 1 : 2][wide];
-  if (seqs * heads >= 2048 || longest <= kWhole || mul_sat({seqs, cdiv(longest, kTile) + 1}) >= (1ll << 31))
-    return Plan{seqs * heads >= 512 ? 4 : 8, 0, 0};
+  // Sequences stay whole where they fill the machine by themselves, or are so short that the second launch costs more
+  // than it saves: 8 sequences of 2 heads of 64 took 10.6 us whole at 1024 tokens and 14.0 in parts at 1500; of 128
+  // fp32 columns 20.1 whole and 23.2 in parts at 600, 28.1 and 23.9 at 1024
+  const int64_t whole = p.cache.bits == 0 && p.cache.dtype == WC_F32 && wide > 0 ? 512 : 1024;
+  if (seqs * heads >= 2048 || longest <= whole || mul_sat({seqs, cdiv(longest, kTile) + 1}) >= (1ll << 31))
+    return Plan{seqs * heads >= 512 ? 4 : 8, 0, 0};      // two workgroups a unit hide each other's waits
   const int64_t budget = cdiv(target, heads);
   return Plan{4, static_cast<int>(budget), budget + seqs};
 }
@@ -626,7 +632,9 @@ void dispatch(const Paged& a, bool q8, int waves, int64_t grid, hipStream_t s) {
   auto go = [&](auto k, auto dc) {
     typedef decltype(k) KT;
     constexpr int DC = decltype(dc)::value;
-    waves == 8 ? launch<QT, KT, DC, 8>(a, grid, s) : launch<QT, KT, DC, 4>(a, grid, s);
+    if constexpr (kRoom8<QT, KT, DC>)
+      if (waves == 8) return launch<QT, KT, DC, 8>(a, grid, s);
+    launch<QT, KT, DC, 4>(a, grid, s);
   };
   auto width = [&](auto k) {
     if (a.dh <= 64)

@@ -235,3 +235,74 @@ def test_attend_rows_beyond_four_gigabytes():
     _check(cache.attend(q, table, lens), q, k, v, lens)
     rk, rv = cache.read(table, lens, 300)
     assert torch.equal(rk, k) and torch.equal(rv, v)
+
+
+# long sequences are cut into parts that a second kernel joins
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("quantized", [False, True])
+@pytest.mark.parametrize("hq,hkv,d,page", [(1, 1, 64, 16), (17, 1, 80, 24), (40, 2, 32, 128), (16, 1, 256, 16), (6, 2, 128, 64),
+                                           (3, 1, 1, 5), (4, 2, 250, 33)])
+def test_attend_parts_layouts(hq, hkv, d, page, quantized, dtype):
+    lens = [0, 2500, 1, 31, 0, 1300]
+    cache, q, k, v, table, lens = _setup(2, 3, hq, hkv, d, page, lens, dtype, quantized, hq * 100 + d + 1)
+    got = cache.attend(q, table, lens)
+    _check(got, q, k, v, lens)
+    assert (got[(lens == 0)] == 0).all()
+    cache.index_error()
+
+
+@pytest.mark.parametrize("first", [[0, 0, 0, 0], [2999, 1, 1400, 0], [3000, 0, 31, 5], [-9, -1, 33, 2600], [1234, 77, 1501, 4]])
+@pytest.mark.parametrize("dtype,quantized", [(torch.bfloat16, False), (torch.float16, True), (torch.float32, False)])
+def test_attend_parts_windows(first, dtype, quantized):
+    cache, q, k, v, table, lens = _setup(2, 2, 4, 2, 64, 16, [3000, 1, 1500, 2600], dtype, quantized, 41)
+    first = torch.tensor(first, dtype=torch.int32, device=DEV).view(2, 2)
+    got = cache.attend(q, table, lens, first=first)
+    _check(got, q, k, v, lens, first)
+    assert (got[(first >= lens)] == 0).all()
+
+
+@pytest.mark.parametrize("n,b", [(1, 63), (1, 64), (5, 13), (3, 50), (2, 257)])
+@pytest.mark.parametrize("dtype,quantized", [(torch.bfloat16, False), (torch.float32, True)])
+def test_attend_parts_of_many_sequences(n, b, dtype, quantized):
+    """More sequences than a wave has lanes; most are short or empty, a few long, the last one as well."""
+    g = gen(n * 1000 + b)
+    lens = torch.randint(0, 60, (n * b,), generator=g) * (torch.rand(n * b, generator=g) < 0.6)
+    lens[torch.randint(0, n * b, (4,), generator=g)] = 1400
+    lens[-1] = 1100
+    cache, q, k, v, table, lens = _setup(n, b, 2, 1, 32, 16, lens.tolist(), dtype, quantized, b)
+    got = cache.attend(q, table, lens)
+    _check(got, q, k, v, lens)
+    assert (got[(lens == 0)] == 0).all()
+
+
+def test_attend_many_long_sequences():
+    """As many sequences as fill the machine stay whole at any length."""
+    g = gen(43)
+    lens = torch.randint(0, 40, (512,), generator=g)
+    lens[100], lens[511] = 1200, 1100
+    cache, q, k, v, table, lens = _setup(4, 128, 4, 4, 16, 16, lens.tolist(), torch.bfloat16, False, 43)
+    _check(cache.attend(q, table, lens), q, k, v, lens)
+
+
+def test_attend_parts_scores_of_minus_infinity():
+    """A part whose keys all score -infinity weighs nothing next to one that has a score."""
+    cache, q, k, v, table, lens = _setup(1, 1, 2, 1, 64, 16, [4000], torch.float32, False, 47)
+    q = q.abs() + 0.1
+    k[0, 0, :3000, 0] = -float("inf")
+    cache.write(k, v, table, torch.zeros_like(lens), lens)
+    got = cache.attend(q, table, lens)
+    ref, _ = attend(q, k[:, :, 3000:], v[:, :, 3000:], lens - 3000)
+    within(got, ref, HALF[torch.float32], attend_slack(torch.float32, 64.0, 64, 4000, v.double().abs().amax().item()))
+
+
+def test_attend_forms_one_after_the_other():
+    """The same cache under other queries, tables and lengths than those of the call before."""
+    cache, q, k, v, table, lens = _setup(2, 2, 8, 2, 64, 16, [1500, 300, 17, 64], torch.bfloat16, False, 53)
+    for cut in (2, 1, 2):
+        for heads in (8, 2, 4):
+            for most in (None, 1500, 1024):
+                length = lens if most != 1024 else lens.clamp(max=1024)
+                part = q[:, :cut, :heads]
+                _check(cache.attend(part, table[:, :cut], length[:, :cut], max_length=most), part, k[:, :cut], v[:, :cut],
+                       length[:, :cut])
+    cache.index_error()
