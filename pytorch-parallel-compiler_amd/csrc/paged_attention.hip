@@ -253,56 +253,51 @@ __global__ __launch_bounds__(NW * 64) void paged_attention_kernel(Paged a) {
     asm volatile("" : "+v"(lane), "+s"(gq), "+s"(dh));
     const int j = lane & 15, g = lane >> 4;
     const uint32_t model = fdiv(seq, a.by_b), b = seq - model * a.by_b.d;
-    const Span span = span_of(a, seq);
-    const int seq_lo = span.lo, hi = span.hi, base = seq_lo & ~(kTile - 1), tiles = tiles_of(span);
+    // What every load here depends on is the sequence alone, so that one wait serves them all: its length, the table's
+    // entries for the wave's first two tiles, and q.
+    const int begin = a.first ? max(a.first[seq], 0) : 0, length = a.lengths[seq], base = begin & ~(kTile - 1);
+    const int tile_lo = max(from - start, 0);
+    // The table's entry for token `lane % 32` of a tile, two tiles ahead of its use; nothing looks at it (and so waits for
+    // it) before row_of, the pool's row of that token or -1 for none.
+    auto look = [&](int tile) {
+      const uint32_t block = fdiv(static_cast<uint32_t>(base) + tile * kTile + (lane & 31), a.t.by_page);
+      return a.t.table[seq * a.t.stride + min(block, static_cast<uint32_t>(a.t.len - 1))];
+    };
+    int row = look(tile_lo + wave), next = look(tile_lo + wave + NW);
+    // N values of q from column d, loaded from column 0 instead of not at all, without branches that every load would
+    // wait in
+    const QT* q = reinterpret_cast<const QT*>(a.q) + model * a.qn + b * a.qb + (head0 + min(j, gq - 1)) * a.qh;
+    constexpr int N = kF32 ? 4 : 8, NX = kF32 ? NCK : NF;
+    auto column = [&](int i) {                                    // the same columns of each product as K's
+      return kF32 ? (i * 4 + g) * 4 : kQ8 ? ((i / 2) * 4 + g) * 16 + (i % 2) * 8 : (i * 4 + g) * 8;
+    };
+    constexpr int NV = 16 / sizeof(QT);
+    u32x4 raw[NX][N / NV];
+#pragma unroll
+    for (int i = 0; i < NX * N / NV; ++i) {
+      const int d = column(i / (N / NV)) + i % (N / NV) * NV;
+      u32x4& r = raw[i / (N / NV)][i % (N / NV)];
+      if (a.qvec) {
+        r = *reinterpret_cast<const u32x4*>(q + (d < dh ? d : 0));
+      } else {
+        QT v[NV];
+#pragma unroll
+        for (int e = 0; e < NV; ++e) v[e] = q[d + e < dh ? d + e : 0];
+        __builtin_memcpy(&r, v, sizeof v);
+      }
+    }
+    const Span span{begin, min(length, a.most), length > a.most};
+    const int seq_lo = span.lo, hi = span.hi, tiles = tiles_of(span), tile_hi = min(tiles, to - start);
     if (span.cut && threadIdx.x == 0) paged_fault(a.t);
-    const int tile_lo = max(from - start, 0), tile_hi = min(tiles, to - start);
     start += tiles;
     if (a.budget > 0 && tile_lo >= tile_hi) continue;             // a sequence without tokens
 
-    // q: the same columns of each product as K's
     u32x4 qf[kF32 ? 1 : NF][NQ];
     float q32[kF32 ? NCK : 1][4];
-    {
-      const QT* q = reinterpret_cast<const QT*>(a.q) + model * a.qn + b * a.qb + (head0 + min(j, gq - 1)) * a.qh;
-      // N values from column d, zeros for what a head doesn't have; loaded from column 0 instead of not at all, without
-      // branches that every load would wait in
-      auto columns = [&](int d, auto& x) {
-        constexpr int N = sizeof(x) / sizeof(float), V = 16 / sizeof(QT);
-        QT v[N];
-        if (a.qvec) {
-#pragma unroll
-          for (int i = 0; i < N; i += V) *reinterpret_cast<u32x4*>(v + i) = *reinterpret_cast<const u32x4*>(q + (d + i < dh ? d + i : 0));
-        } else {
-#pragma unroll
-          for (int i = 0; i < N; ++i) v[i] = q[d + i < dh ? d + i : 0];
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = j < gq && d + i < dh ? to_f32(v[i]) : 0.f;
-      };
-      if constexpr (kF32) {
-#pragma unroll
-        for (int c = 0; c < NCK; ++c) columns((c * 4 + g) * 4, q32[c]);
-      } else {
-#pragma unroll
-        for (int f = 0; f < NF; ++f) {
-          float x[8];
-          columns(kQ8 ? ((f / 2) * 4 + g) * 16 + (f % 2) * 8 : (f * 4 + g) * 8, x);
-          planes<MT, NQ>(x, qf[f]);
-        }
-      }
-    }
-
     f32x4 acc[NCV][CE] = {};
     float m = -INFINITY, l = 0.f;
     bool any = false;
 
-    // The table's entry for token `lane % 32` of a tile, two tiles ahead of its use; nothing looks at it (and so waits for
-    // it) before row_of, the pool's row of that token or -1 for none.
-    auto look = [&](int tile) {
-      const uint32_t block = fdiv(max(base + tile * kTile + (lane & 31), 0), a.t.by_page);
-      return a.t.table[seq * a.t.stride + min(block, static_cast<uint32_t>(a.t.len - 1))];
-    };
     auto row_of = [&](int tile, int page) {
       const int tok = base + tile * kTile + (lane & 31);
       if (tile >= tile_hi || tok < seq_lo || tok >= hi) return -1;
@@ -330,12 +325,23 @@ __global__ __launch_bounds__(NW * 64) void paged_attention_kernel(Paged a) {
       }
     };
 
-    int row = -1, next = -1;
     if (tile_lo + wave < tile_hi) {
-      row = look(tile_lo + wave);
-      next = look(tile_lo + wave + NW);
       row = row_of(tile_lo + wave, row);
       load_k(row);
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        QT v[N];
+        float x[N];
+        __builtin_memcpy(v, raw[i], sizeof v);
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = j < gq && column(i) + e < dh ? to_f32(v[e]) : 0.f;
+        if constexpr (kF32) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q32[i][e] = x[e];
+        } else {
+          planes<MT, NQ>(x, qf[i]);
+        }
+      }
     }
     for (int tile = tile_lo + wave; tile < tile_hi; tile += NW) {
       const bool full = __all(row >= 0);
@@ -712,8 +718,13 @@ extern "C" int32_t wc_paged_attention(const wc_paged_attn_args* args, void* stre
   const int64_t qtiles = cdiv(a.group, 16);
   a.dh = static_cast<int32_t>(c.head_dim);
   a.row_bytes = static_cast<int32_t>(c.row * paged_es(c));
-  // a pool without pages has no row 0, a table without entries no entry to look at
+  // a pool without pages has no row 0; a table without entries none to look at, for which another number does
   a.most = static_cast<int32_t>(c.pages && c.table_len ? p.max_length : 0);
+  if (c.table_len == 0) {
+    a.t.table = p.lengths;
+    a.t.stride = 0;
+    a.t.len = 1;
+  }
   a.scale = p.scale * kLog2e;
   a.qvec = c.head_dim * es % 16 == 0 && aligned(p.q, 16) && ubytes(p.q_stride_n, es) % 16 == 0 &&
            ubytes(p.q_stride_b, es) % 16 == 0 && ubytes(p.q_stride_h, es) % 16 == 0;
