@@ -2,9 +2,9 @@
 //
 //   y = x / sqrt(mean x^2 + eps) * w,   (y_a, y_b) -> (y_a cos - y_b sin, y_b cos + y_a sin)
 //
-// A pair of columns turns by 2 pi pos f, f turns per position.  pos f is taken in fp64 and only its
-// fraction of a turn goes on in fp32, so that a token's angle is good to 2^-25 of a turn however far it
-// stands (in fp32 the product itself would be off by 2^-24 of pos f turns).
+// A pair of columns turns by 2 pi pos f, f turns per position, at most 1 / 2 pi.  pos f is taken in fp64, off by
+// 2^-52 of itself with f's own rounding, and only its fraction of a turn goes on in fp32, so that a token's angle is
+// good to 2^-25 of a turn at any position up to 2^28 (in fp32 the product itself would be off by 2^-24 of pos f turns).
 //
 // Both halves of a pair belong to one lane: it loads V columns from each half (V neighbouring pairs when
 // pairs are neighbours), so a row needs no exchange but the sum of its squares.  A workgroup takes some

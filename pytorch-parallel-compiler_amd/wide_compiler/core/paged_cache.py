@@ -79,6 +79,8 @@ class WidePagedCache:
         _serve.same_device(what, k_pages, v_pages, k_scales, v_scales)
         if not 0 < head_dim <= min(row, 256):
             raise ValueError(f"{what}: head_dim {head_dim} must be within [1, {min(row, 256)}]")
+        if heads < 1:
+            raise ValueError(f"{what}: n_kv_heads must be positive")
         if page_size < 1 or row * k_pages.element_size() % 16 or row > 512:
             raise ValueError(f"{what}: pages of at least one token, rows of whole 16 bytes and at most 512 elements, "
                              f"got {page_size} and {row}")

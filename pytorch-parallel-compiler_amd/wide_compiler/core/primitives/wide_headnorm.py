@@ -9,8 +9,9 @@ Every head of every token is divided by its root mean square, multiplied by its 
     (y_a, y_b) -> (y_a cos a - y_b sin a, y_b cos a + y_a sin a)
 
 for the pairs p of the first ``rotary_dim`` columns: columns (p, p + rotary_dim / 2), or
-neighbours (2p, 2p + 1) when ``interleaved``.  Angles are taken in 64 bits, so that any position
-an int64 holds turns as exactly as the first.  ``positions`` is an integer tensor that broadcasts
+neighbours (2p, 2p + 1) when ``interleaved``.  Angles are taken in 64 bits, so that a token at any
+position up to 2^28 turns as exactly as the first (fp32 would be off by a radian at 2^24).  Squares
+are summed in fp32, as nn.RMSNorm sums them.  ``positions`` is an integer tensor that broadcasts
 to [N, B, T].  q and k may be views (of one projection's output, say) with unit last stride.  One
 launch of wc_head_norm_rotary; the reference has no counterpart.
 """

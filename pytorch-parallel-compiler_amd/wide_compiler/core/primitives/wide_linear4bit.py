@@ -4,9 +4,12 @@ WideLinear4bit: N independent linear layers with weights of 4 bits, for few rows
     x [N, *batch, I]  ->  y [N, *batch, O],   y[i] = x[i] @ W[i].T + bias[i]
     W[i, o, k] = scale[i, o, k // group] * (code[i, o, k] - zero[i, o, k // group])
 
-with codes of 0 to 15, groups of 32, 64 or 128 columns and zero points of 0 to 15 (8 where none are given).  The forward (wc_linear4) reads every weight once for up to 64 rows, so that a token's
-products cost what reading half a byte a weight costs; more rows go 64 at a time.  Sums are fp32;
-the scale multiplies each group's sum.
+with codes of 0 to 15, groups of 32, 64 or 128 columns and zero points of 0 to 15 (8 where none are
+given).  The forward (wc_linear4) brings each weight from memory once for up to 16, 32 or 64 rows (the
+more weights there are, the more), so that a token's products cost what reading half a byte a weight
+costs.  It is made for few rows: hundreds of them are faster through dequantize() and a product in
+16 bits.  Sums are fp32; the scale multiplies each group's sum.  An infinity in a row of x gives that
+row NaN in bf16 and fp32, also where the formula has an infinity.
 
 The buffers hold the weights as the kernel reads them (``packed`` [N, O / 16, I / 128, 64, 4] int32,
 ``scales`` and ``zeros`` [N, O / 16, groups, 16], sizes rounded up); ``from_codes`` packs them from
@@ -52,8 +55,9 @@ class WideLinear4bit(nn.Module):
     def forward(self, x: Tensor) -> Tensor:
         bufs = self._buffers
         packed, scales, zeros, bias = bufs["packed"], bufs["scales"], bufs["zeros"], bufs["bias"]
-        form = (x.shape, x.stride(), x.dtype, x.device, packed.device, scales.dtype, scales.device, zeros.device,
-                None if bias is None else (bias.dtype, bias.device))
+        form = (x.shape, x.stride(), x.dtype, x.device, packed.shape, packed.dtype, packed.device, scales.shape,
+                scales.dtype, scales.device, zeros.shape, zeros.dtype, zeros.device,
+                None if bias is None else (bias.shape, bias.dtype, bias.device))
         plan = self._plans.get(form)
         if plan is None:
             plan = self._plan(form, x, packed, scales, zeros, bias)
@@ -62,6 +66,10 @@ class WideLinear4bit(nn.Module):
         dense, rows, sizes, shape = plan
         if not dense:
             x = x.contiguous()
+        if not (packed.is_contiguous() and scales.is_contiguous() and zeros.is_contiguous()):
+            packed, scales, zeros = packed.contiguous(), scales.contiguous(), zeros.contiguous()
+        if bias is not None and not bias.is_contiguous():
+            bias = bias.contiguous()
         y = x.new_empty(shape)
         if y.numel():
             _serve.linear4(sizes, rows, x, packed, scales, zeros, bias, y)
@@ -74,6 +82,12 @@ class WideLinear4bit(nn.Module):
         _hip.require_device(what, x, packed)
         if x.dtype != scales.dtype or (bias is not None and bias.dtype != x.dtype):
             raise RuntimeError(f"{what}: input dtype {x.dtype} != {scales.dtype} of scales and bias")
+        rt, kt = -(-self.out_features // 16), -(-self.in_features // 128)
+        meta = (self.n, rt, kt * (128 // self.group_size), 16)
+        for name, t, shape, dtype in (("packed", packed, (self.n, rt, kt, 64, 4), torch.int32), ("scales", scales, meta, x.dtype),
+                                      ("zeros", zeros, meta, torch.uint8), ("bias", bias, (self.n, self.out_features), x.dtype)):
+            if t is not None and (t.dtype != dtype or tuple(t.shape) != shape):
+                raise RuntimeError(f"{what}: {name} must be {dtype} {list(shape)}, got {t.dtype} {list(t.shape)}")
         _serve.same_device(what, x, packed, scales, zeros, bias)
         dense, rows = rows_or_contiguous(x)
         sizes = (_hip.dtype_code(x.dtype, "linear4"), self.group_size, self.n, rows.rows, self.out_features, self.in_features)
@@ -102,6 +116,8 @@ class WideLinear4bit(nn.Module):
         """codes [N, O, ceil(I / 2)] uint8, two to a byte, the even column in the low half; scales
         [N, O, ceil(I / group)] of the dtype of the inputs; zeros the same of uint8 (0 to 15) or None; bias [N, O]."""
         what = "WideLinear4bit.from_codes"
+        if group_size not in (32, 64, 128):
+            raise ValueError(f"{what}: group_size must be 32, 64 or 128, got {group_size}")
         if codes.dim() != 3 or codes.dtype != torch.uint8 or codes.shape[2] != (in_features + 1) // 2:
             raise ValueError(f"{what}: codes must be uint8 [N, O, {(in_features + 1) // 2}], got {codes.dtype} {list(codes.shape)}")
         meta = (*codes.shape[:2], -(-in_features // group_size))

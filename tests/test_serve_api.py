@@ -199,7 +199,7 @@ def test_cache_refusals(anywhere):
                      ((pages, pages), dict(head_dim=65)), ((pages, pages), dict(head_dim=0)),
                      ((pages[..., :60].contiguous(), pages[..., :60].contiguous()), {}),
                      ((pages.transpose(1, 2), pages.transpose(1, 2)), {}), ((pages[:, :, :0], pages[:, :, :0]), {}),
-                     ((i8, i8, scales, None), dict(dtype=torch.bfloat16))):
+                     ((i8, i8, scales, None), dict(dtype=torch.bfloat16)), ((pages[:, :0], pages[:, :0]), {})):
         with pytest.raises(ValueError):
             f(*args, **kw)
     with pytest.raises(TypeError):
@@ -239,7 +239,8 @@ def test_linear4_refusals(anywhere):
     zeros = torch.zeros(2, 16, 1, dtype=torch.uint8)
     f = wc.WideLinear4bit.from_codes
     for kw in (dict(codes=codes.int()), dict(codes=codes[0]), dict(in_features=66), dict(scales=scales[:, :8]),
-               dict(zeros=zeros + 16), dict(zeros=zeros.int()), dict(bias=torch.zeros(2, 15)), dict(group_size=32)):
+               dict(zeros=zeros + 16), dict(zeros=zeros.int()), dict(bias=torch.zeros(2, 15)), dict(group_size=32),
+               dict(group_size=0)):
         kw = dict(codes=codes, scales=scales, in_features=64, group_size=64, zeros=zeros) | kw
         with pytest.raises(ValueError):
             f(kw.pop("codes"), kw.pop("scales"), **kw)
@@ -249,6 +250,17 @@ def test_linear4_refusals(anywhere):
     for x in (torch.zeros(2, 3, 32), torch.zeros(1, 3, 64), torch.zeros(2, 3, 64).half(), torch.zeros(64)):
         with pytest.raises(RuntimeError):
             mod(x)
+    # buffers that were replaced since the last call
+    x = torch.zeros(2, 3, 64)
+    for name, t in (("packed", mod.packed[:, :, :, :32]), ("packed", mod.packed.long()), ("scales", mod.scales[..., :8]),
+                    ("zeros", mod.zeros[:1]), ("zeros", mod.zeros.int()), ("bias", torch.zeros(2, 15))):
+        old = getattr(mod, name)
+        setattr(mod, name, t)
+        with pytest.raises(RuntimeError, match=name):
+            mod(x)
+        setattr(mod, name, old)
+    with pytest.raises(AssertionError, match="launched"):
+        mod(x)
 
 
 @pytest.mark.parametrize("n,o,k,group,zeros", [(2, 500, 1000, 32, True), (1, 16, 128, 128, False), (3, 5, 37, 64, True),
