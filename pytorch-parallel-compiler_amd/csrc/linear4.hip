@@ -290,7 +290,7 @@ __global__ __launch_bounds__(NW * 64) void linear4_few_kernel(Linear4 a) {
   }
 }
 
-// More rows, through LDS: a workgroup of 8 waves, WR of them over output rows (RT tiles each) and WK over columns,
+// More rows, through LDS: a workgroup of 8 or 16 waves, WR of them over output rows (RT tiles each) and WK over columns,
 // brings CK tiles of 128 columns of x at a time, split into planes (fp32) and with the sums over 32 columns that the
 // zero points want, once for all its output rows.  Weights come straight into registers, D tiles ahead of their use.
 constexpr int kPad = 136;          // 16-bit values in a staged row: 128, and 8 that move the rows to other banks
@@ -447,13 +447,23 @@ void launch_rows(Linear4 a, int64_t n, hipStream_t s) {
   over_rows(a, M, [&](uint32_t tiles) { kernel<<<dim3(static_cast<uint32_t>(n * per), tiles), WR * WK * 64, lds, s>>>(a); });
 }
 
-// Which kernel, by the tiles of output rows of all models and the tiles of 16 rows of x (us on an MI355X, launches of
-// a graph, bf16, groups of 128):
-//   few tiles: one tile a workgroup, its waves share the columns    64 tiles, 16 rows: 4.0 (two tiles: 4.5, LDS: 6.2)
-//   more: two tiles share what they bring of x                     512 tiles, 16 rows: 9.6 (12.5, 12.2)
-//   many: x through LDS                                           2048 tiles, 16 rows: 11.3 (25.8, 17.3)
-//   and of the forms through LDS the one that meets a weight with most rows of x at once where enough workgroups
-//   remain: 2048 tiles, 64 rows: 29 (16 rows at once: 37); 4096 tiles in fp16: 36 (32 rows at once: 49).
+// Which kernel, for `tiles` tiles of output rows of all models and `rows` tiles of 16 rows of x (us on an MI355X,
+// launches of a graph).  Few tiles: a tile for each workgroup, its waves share the columns (bf16, groups of 128, 64
+// tiles of 16 rows: 4.0; two tiles each 4.5, through LDS 6.2), then two that share what they bring of x (512 tiles: 9.6;
+// one each 12.5, through LDS 12.2).  More go through LDS, with as much of x and W in a workgroup as leaves one for every
+// compute unit:
+//   fp16, groups of 64            16 waves, 64 rows   16 waves, 32 rows   8 x 2, 32 rows   4 x 2, 32 rows
+//   4096 tiles, 64 rows                   31                  43                 50               48
+//   2048 tiles, 64 rows                   29                  21                 27               27
+//   1024 tiles, 64 rows, K 4096           47                  33                 22               25
+//    512 tiles, 64 rows, K 4096           46                  31                 21               16
+// and likewise for 16 rows (4096 tiles: 17.5, of 4 x 2 waves 19.1) and in fp32, whose three planes of x leave less room.
+template <typename T, int GP, int MT, int RT, int WR, int WK, int CK>
+bool launch_if_full(const Linear4& a, int64_t n, hipStream_t s) {
+  if (n * cdiv(a.otiles, WR * RT) * cdiv(a.m, MT * 16) < 256) return false;
+  launch_rows<T, GP, MT, RT, WR, WK, CK>(a, n, s);
+  return true;
+}
 template <typename T, int GP>
 void dispatch(const Linear4& a, int64_t n, hipStream_t s) {
   constexpr bool F32 = sizeof(T) == 4;
@@ -461,12 +471,16 @@ void dispatch(const Linear4& a, int64_t n, hipStream_t s) {
   if (tiles * rows <= 256) return launch_few<T, GP, 1, 4>(a, n, s);
   if (rows == 1 && tiles <= 1024) return launch_few<T, GP, 2, 4>(a, n, s);
   if constexpr (F32) {
-    if (rows > 1 && tiles >= 1024) return launch_rows<T, GP, 2, 2, 4, 2, 2>(a, n, s);
+    if (rows > 1 && (launch_if_full<T, GP, 2, 2, 8, 1, 1>(a, n, s) || launch_if_full<T, GP, 2, 1, 8, 2, 2>(a, n, s))) return;
+    if (launch_if_full<T, GP, 1, 1, 16, 1, 4>(a, n, s) || launch_if_full<T, GP, 1, 1, 8, 2, 4>(a, n, s)) return;
+    launch_rows<T, GP, 1, 1, 4, 2, 4>(a, n, s);
   } else {
-    if (rows > 2 && tiles >= 4096) return launch_rows<T, GP, 4, 2, 8, 1, 4>(a, n, s);
-    if (rows > 2 || (rows > 1 && tiles >= 1024)) return launch_rows<T, GP, 2, 1, 4, 2, 8>(a, n, s);
+    if (rows > 2 && launch_if_full<T, GP, 4, 1, 16, 1, 2>(a, n, s)) return;
+    if (rows > 1 && (launch_if_full<T, GP, 2, 1, 16, 1, 4>(a, n, s) || launch_if_full<T, GP, 2, 1, 8, 2, 4>(a, n, s))) return;
+    if (rows > 2) return launch_rows<T, GP, 2, 1, 4, 2, 8>(a, n, s);
+    if (rows == 1 && launch_if_full<T, GP, 1, 1, 16, 1, 8>(a, n, s)) return;
+    launch_rows<T, GP, 1, 1, 4, 2, 16>(a, n, s);
   }
-  launch_rows<T, GP, 1, 1, 4, 2, F32 ? 4 : 16>(a, n, s);
 }
 
 template <typename T>

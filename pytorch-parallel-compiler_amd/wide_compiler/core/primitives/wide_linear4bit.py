@@ -7,8 +7,8 @@ WideLinear4bit: N independent linear layers with weights of 4 bits, for few rows
 with codes of 0 to 15, groups of 32, 64 or 128 columns and zero points of 0 to 15 (8 where none are
 given).  The forward (wc_linear4) brings each weight from memory once for up to 16, 32 or 64 rows (the
 more weights there are, the more), so that a token's products cost what reading half a byte a weight
-costs.  It is made for few rows: hundreds of them are faster through dequantize() and a product in
-16 bits.  Sums are fp32; the scale multiplies each group's sum.  An infinity in a row of x gives that
+costs; it is faster than WideLinear up to about 500 rows in 16 bits, and at any in fp32.  Sums are
+fp32; the scale multiplies each group's sum.  An infinity in a row of x gives that
 row NaN in bf16 and fp32, also where the formula has an infinity.
 
 The buffers hold the weights as the kernel reads them (``packed`` [N, O / 16, I / 128, 64, 4] int32,
