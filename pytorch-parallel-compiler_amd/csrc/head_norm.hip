@@ -268,11 +268,15 @@ extern "C" int32_t wc_head_norm_rotary(const wc_head_norm_args* args, void* stre
   const int pairs = a.dh / 2, need = static_cast<int>(cdiv(pairs, v));
   a.lanes_log2 = 0;
   while ((1 << a.lanes_log2) < need && a.lanes_log2 < 6) ++a.lanes_log2;
-  // A workgroup takes about 4 rows per group of lanes: all heads of some tokens, or a part of the heads
-  const int target = 4 * (kThreads >> a.lanes_log2);
-  a.chunk = a.heads <= target ? a.heads : target;
-  a.tile = std::max(1, target / a.chunk);
-  a.tile = std::min({a.tile, 4096 / pairs, a.tokens});      // at most 32 KB of cosines and sines
+  // A workgroup takes about 4 rows per group of lanes, all heads of some tokens or a part of the heads, or fewer where
+  // that would leave compute units without work (us on an MI355X, 8 heads of 128 columns for 32 heads of queries, bf16:
+  // 4 models of 4096 tokens 70 with 4 rows, 76 with 2, 77 with 8; 8 models of 4 tokens 7.1 with 4, 5.0 with 2)
+  int target = 4 * (kThreads >> a.lanes_log2);
+  for (;; target >>= 1) {
+    a.chunk = std::min(a.heads, target);
+    a.tile = std::min({std::max(1, target / a.chunk), 4096 / pairs, a.tokens});    // at most 32 KB of cosines and sines
+    if (target <= kThreads >> a.lanes_log2 || p.n * cdiv(a.tokens, a.tile) * cdiv(a.heads, a.chunk) >= 256) break;
+  }
   a.by_t = make_fastdiv(static_cast<uint32_t>(p.t));
   a.by_chunk = make_fastdiv(static_cast<uint32_t>(a.chunk));
   a.by_pairs = make_fastdiv(static_cast<uint32_t>(pairs));

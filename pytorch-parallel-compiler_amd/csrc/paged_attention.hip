@@ -259,10 +259,7 @@ __global__ __launch_bounds__(NW * 64) void paged_attention_kernel(Paged a) {
     const int tile_lo = max(from - start, 0);
     // The table's entry for token `lane % 32` of a tile, two tiles ahead of its use; nothing looks at it (and so waits for
     // it) before row_of, the pool's row of that token or -1 for none.
-    auto look = [&](int tile) {
-      const uint32_t block = fdiv(static_cast<uint32_t>(base) + tile * kTile + (lane & 31), a.t.by_page);
-      return a.t.table[seq * a.t.stride + min(block, static_cast<uint32_t>(a.t.len - 1))];
-    };
+    auto look = [&](int tile) { return paged_entry(a.t, seq, static_cast<uint32_t>(base) + tile * kTile + (lane & 31)); };
     int row = look(tile_lo + wave), next = look(tile_lo + wave + NW);
     // N values of q from column d, loaded from column 0 instead of not at all, without branches that every load would
     // wait in
@@ -301,12 +298,9 @@ __global__ __launch_bounds__(NW * 64) void paged_attention_kernel(Paged a) {
     auto row_of = [&](int tile, int page) {
       const int tok = base + tile * kTile + (lane & 31);
       if (tile >= tile_hi || tok < seq_lo || tok >= hi) return -1;
-      const uint32_t block = fdiv(tok, a.t.by_page);
-      if (block >= static_cast<uint32_t>(a.t.len) || static_cast<uint32_t>(page) >= static_cast<uint32_t>(a.t.pages)) {
-        paged_fault(a.t);
-        return -1;
-      }
-      return (page * a.t.heads + kvh) * a.t.page + static_cast<int>(tok - block * a.t.by_page.d);
+      const int r = paged_row(a.t, page, tok, kvh);
+      if (r < 0) paged_fault(a.t);
+      return r;
     };
     // Rows that no token has are read as row 0 of the pool and taken out afterwards.  K comes one tile ahead, into the
     // registers that the scores have just been taken from, while softmax and V keep the wave busy.
@@ -700,7 +694,7 @@ extern "C" int32_t wc_paged_attention(const wc_paged_attn_args* args, void* stre
   WC_REQUIRE(aligned(p.q, es) && aligned(p.o, es) && aligned(p.lengths, 4) && aligned(p.first, 4), WC_ERR_ALIGN,
              "%s: pointers must be aligned to their elements", what);
   Paged a;
-  a.t = paged_table(c);
+  a.t = paged_table(c, p.lengths);
   a.k = static_cast<const char*>(c.k_pages);
   a.v = static_cast<const char*>(c.v_pages);
   a.ks = c.k_scales;
@@ -718,13 +712,8 @@ extern "C" int32_t wc_paged_attention(const wc_paged_attn_args* args, void* stre
   const int64_t qtiles = cdiv(a.group, 16);
   a.dh = static_cast<int32_t>(c.head_dim);
   a.row_bytes = static_cast<int32_t>(c.row * paged_es(c));
-  // a pool without pages has no row 0; a table without entries none to look at, for which another number does
+  // a pool without pages has no row 0, a table without entries no tokens
   a.most = static_cast<int32_t>(c.pages && c.table_len ? p.max_length : 0);
-  if (c.table_len == 0) {
-    a.t.table = p.lengths;
-    a.t.stride = 0;
-    a.t.len = 1;
-  }
   a.scale = p.scale * kLog2e;
   a.qvec = c.head_dim * es % 16 == 0 && aligned(p.q, 16) && ubytes(p.q_stride_n, es) % 16 == 0 &&
            ubytes(p.q_stride_b, es) % 16 == 0 && ubytes(p.q_stride_h, es) % 16 == 0;

@@ -110,8 +110,12 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
       const int d = (lane + c * lanes) * V;
       x[u][c] = *reinterpret_cast<const Vec<T, V>*>(src + step * st[2] + h * st[3] + (d < a.dh ? d : 0));
     }
-    const int64_t tok = static_cast<int64_t>(start) + step;
-    row[u] = tok > INT32_MAX ? -1 : paged_row(a.t, seq, static_cast<uint32_t>(tok), h);
+    row[u] = paged_entry(a.t, seq, start + step);                 // at most 2^32 - 2
+  }
+#pragma unroll
+  for (int u = 0; u < kRows; ++u) {
+    const uint32_t r = min(r0 + u * groups, rows - 1), step = fdiv(r, a.by_heads), tok = start + step;
+    row[u] = tok > INT32_MAX ? -1 : paged_row(a.t, row[u], tok, r - step * a.by_heads.d);
   }
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
@@ -197,10 +201,12 @@ __global__ __launch_bounds__(kThreads) void cache_read_kernel(Read a) {
   if (length > a.most) paged_fault(a.t);
   int32_t row[kRows];
 #pragma unroll
+  for (int u = 0; u < kRows; ++u) row[u] = paged_entry(a.t, seq, fdiv(min(r0 + u * groups, rows - 1), a.by_heads));
+#pragma unroll
   for (int u = 0; u < kRows; ++u) {
     const uint32_t r = min(r0 + u * groups, rows - 1), tok = fdiv(r, a.by_heads), h = r - tok * a.by_heads.d;
     const bool has = static_cast<int32_t>(tok) < length;
-    row[u] = has ? paged_row(a.t, seq, tok, h) : -1;
+    row[u] = has ? paged_row(a.t, row[u], tok, h) : -1;
     if (has && row[u] < 0) paged_fault(a.t);
   }
   // rows that aren't there are read as row 0 of the pool, if it has one, and become zeros
@@ -293,7 +299,7 @@ extern "C" int32_t wc_cache_write(const wc_cache_write_args* args, void* stream)
   WC_REQUIRE(aligned(p.k, es) && aligned(p.v, es) && aligned(p.start, 4) && aligned(p.count, 4), WC_ERR_ALIGN,
              "%s: pointers must be aligned to their elements", what);
   Write a;
-  a.t = paged_table(c);
+  a.t = paged_table(c, p.start);
   a.src[0] = static_cast<const char*>(p.k);
   a.src[1] = static_cast<const char*>(p.v);
   a.pages[0] = static_cast<char*>(c.k_pages);
@@ -341,7 +347,7 @@ extern "C" int32_t wc_cache_read(const wc_cache_read_args* args, void* stream) {
   WC_REQUIRE(aligned(p.k, es) && aligned(p.v, es) && aligned(p.lengths, 4), WC_ERR_ALIGN,
              "%s: pointers must be aligned to their elements", what);
   Read a;
-  a.t = paged_table(c);
+  a.t = paged_table(c, p.lengths);
   a.pages[0] = static_cast<const char*>(c.k_pages);
   a.pages[1] = static_cast<const char*>(c.v_pages);
   a.scales[0] = c.k_scales;

@@ -14,13 +14,16 @@ struct PagedTable {
   FastDiv by_page;
 };
 
-// The row of the pool (in units of rows) that holds token `tok` (>= 0) of sequence `seq` for head `h`, or -1
-// where the table names no page of the pool.  Rows of a pool fit 31 bits (paged_check).
-__device__ __forceinline__ int32_t paged_row(const PagedTable& t, int64_t seq, uint32_t tok, int h) {
+// The table's entry for token `tok` of sequence `seq`, behind its end the last: loaded without a condition, so that
+// neighbouring loads need not wait for each other
+__device__ __forceinline__ int32_t paged_entry(const PagedTable& t, int64_t seq, uint32_t tok) {
+  return t.table[seq * t.stride + min(fdiv(tok, t.by_page), static_cast<uint32_t>(max(t.len, 1) - 1))];
+}
+// The row of the pool (in units of rows) that holds token `tok` for head `h` in page `id` of the table, or -1 where the
+// table has none.  Rows of a pool fit 31 bits (paged_check).
+__device__ __forceinline__ int32_t paged_row(const PagedTable& t, int32_t id, uint32_t tok, int h) {
   const uint32_t block = fdiv(tok, t.by_page);
-  if (block >= static_cast<uint32_t>(t.len)) return -1;
-  const int32_t id = t.table[seq * t.stride + block];
-  if (static_cast<uint32_t>(id) >= static_cast<uint32_t>(t.pages)) return -1;
+  if (block >= static_cast<uint32_t>(t.len) || static_cast<uint32_t>(id) >= static_cast<uint32_t>(t.pages)) return -1;
   return (id * t.heads + h) * t.page + static_cast<int32_t>(tok - block * t.by_page.d);
 }
 
@@ -28,10 +31,11 @@ __device__ __forceinline__ void paged_fault(const PagedTable& t) {
   if (t.err) *t.err = 1;
 }
 
-inline PagedTable paged_table(const wc_paged_cache& c) {
+// instead: as many int32 as there are sequences, for a table without entries, of which one is loaded all the same
+inline PagedTable paged_table(const wc_paged_cache& c, const int32_t* instead) {
   PagedTable t;
-  t.table = c.table;
-  t.stride = c.table_stride;
+  t.table = c.table_len ? c.table : instead;
+  t.stride = c.table_len ? c.table_stride : 0;
   t.len = static_cast<int32_t>(c.table_len);
   t.pages = static_cast<int32_t>(c.pages);
   t.page = static_cast<int32_t>(c.page_size);
