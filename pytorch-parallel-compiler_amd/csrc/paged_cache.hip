@@ -88,8 +88,9 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
   const uint32_t model = fdiv(seq, a.by_b), b = seq - model * a.by_b.d;
   const int64_t* st = a.stride[kv];
   const T* src = reinterpret_cast<const T*>(a.src[kv]) + model * st[0] + b * st[1];
-  int n = a.count ? a.count[seq] : a.steps;
   const int start = a.start[seq];
+  int n = a.steps;
+  if (a.count) n = a.count[seq];
   if (n > a.steps) {
     n = a.steps;
     paged_fault(a.t);
@@ -100,7 +101,8 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
   if (tile * (groups * kRows) >= rows) return;
 
   // rows past the last are loaded as the last and not stored; lanes past a row's end hold its first values again
-  Vec<T, V> x[kRows][NC];
+  typedef typename std::conditional<V == 1, T, u32x4>::type Piece;      // an array of structs would not stay in registers
+  Piece x[kRows][NC];
   int32_t row[kRows];
 #pragma unroll
   for (int u = 0; u < kRows; ++u) {
@@ -108,7 +110,7 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       const int d = (lane + c * lanes) * V;
-      x[u][c] = *reinterpret_cast<const Vec<T, V>*>(src + step * st[2] + h * st[3] + (d < a.dh ? d : 0));
+      x[u][c] = *reinterpret_cast<const Piece*>(src + step * st[2] + h * st[3] + (d < a.dh ? d : 0));
     }
     row[u] = paged_entry(a.t, seq, start + step);                 // at most 2^32 - 2
   }
@@ -129,11 +131,14 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
 #pragma unroll
       for (int c = 0; c < NC; ++c) {
         const int d = (lane + c * lanes) * V;
-        if (d < a.dh) *reinterpret_cast<Vec<T, V>*>(dst + d) = x[u][c];
+        if (d < a.dh) *reinterpret_cast<Piece*>(dst + d) = x[u][c];
       }
       for (int d = a.dh + lane; d < a.row; d += lanes) dst[d] = static_cast<T>(0.f);
     } else {
-      uint32_t top = largest<T, V, NC>(x[u]);
+      Vec<T, V> v[NC];
+#pragma unroll
+      for (int c = 0; c < NC; ++c) v[c] = __builtin_bit_cast(Vec<T, V>, x[u][c]);
+      uint32_t top = largest<T, V, NC>(v);
       for (int off = lanes >> 1; off; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 64)));
       const bool finite = top < 0x7f800000u;
       const float scale = finite ? fmaxf(__builtin_bit_cast(float, top) / 127.f, 0x1p-126f) : __builtin_nanf("");
@@ -145,7 +150,7 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           float off;
-          code[c][e] = code8(to_f32(x[u][c].v[e]), scale, inv, off);
+          code[c][e] = code8(to_f32(v[c].v[e]), scale, inv, off);
           far = fmaxf(far, off);
         }
       // 2^-15 covers the product's rounding and inv's: 2^-22 of a quotient of up to 127
@@ -153,7 +158,7 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll
-          for (int e = 0; e < V; ++e) code[c][e] = code8_near_half(to_f32(x[u][c].v[e]), scale, inv);
+          for (int e = 0; e < V; ++e) code[c][e] = code8_near_half(to_f32(v[c].v[e]), scale, inv);
       if (!store) continue;
       int8_t* dst = reinterpret_cast<int8_t*>(a.pages[kv]) + at;
 #pragma unroll
