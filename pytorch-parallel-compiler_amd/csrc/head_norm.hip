@@ -6,6 +6,9 @@
 // 2^-52 of itself with f's own rounding, and only its fraction of a turn goes on in fp32, so that a token's angle is
 // good to 2^-25 of a turn at any position up to 2^28 (in fp32 the product itself would be off by 2^-24 of pos f turns).
 //
+// Memory bounds it: rows in, rows out, some 8 flops a value.  4 models' 4096 tokens of 32 + 8 heads of 128 columns in
+// bf16, 335 MB: 70 us, 4.8 TB/s (a large copy here: 4.7 to 5.1).
+//
 // Both halves of a pair belong to one lane: it loads V columns from each half (V neighbouring pairs when
 // pairs are neighbours), so a row needs no exchange but the sum of its squares.  A workgroup takes some
 // tokens of one model: their cosines and sines are computed once, one thread a pair, and kept in LDS for all
@@ -19,7 +22,7 @@ namespace wc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 2;        // rows in flight per group of lanes
+constexpr int kUnroll = 2;        // rows in flight per group of lanes (those 335 MB: 70 us; one row 72, four 80)
 
 struct HeadNorm {
   const char *q, *k, *qw, *kw, *pos;

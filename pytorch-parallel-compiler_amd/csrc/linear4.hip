@@ -13,6 +13,10 @@
 // rounding in fp32 is 2^-24 of 128 |sum x|.  fp32 goes as three bf16 planes of x (every bit of it down to 2^-110)
 // against codes converted to bf16, without the 128.  A row of x with an infinity or NaN gives NaN in bf16 and fp32.
 //
+// 4 models' [4096 -> 4096] in bf16, one row (35 MB): 10.8 us, of which an empty launch is 3.3; 8 models' [2048 -> 8192]
+// in fp16, 64 rows (84 MB, 17 GFLOP): 31 us, half of it the instructions that make numbers of codes and scale the
+// groups' sums, which with two to four waves a unit's quarter only partly hide behind the loads.
+//
 // The columns are dealt to the waves of a workgroup, which add their sums up through LDS at the end.
 #include <algorithm>
 

@@ -4,8 +4,10 @@
 //
 // in one pass over the sequence.  A query head group shares a key head, so up to 16 query heads are the columns of
 // one MFMA tile and every K and V row is read once for all of them.  What bounds it is that reading: 4 flops per
-// stored value and query head, far under the machine's balance; the matrix instructions run mostly empty for
-// small groups and still cost a tenth of the time their rows take to arrive.
+// stored value and query head, far under the machine's balance.  The matrix instructions run mostly empty for small
+// groups and in 16 bits still cost a tenth of the time their rows take to arrive.  32 query heads over 8 key heads of
+// 128 columns: 2 sequences of 131072 and 32768 tokens in bf16 (671 MB) 121 us, 5.5 TB/s; 64 sequences of 1000 to 4000
+// tokens in 8 bits (335 MB) 76 us, 4.4 TB/s, where turning codes into numbers takes half the instructions.
 //
 // A wave takes 32 tokens at a time, and nothing but the sum over its lanes ever leaves its registers:
 //   scores   S [token][query] = K Q^T, K rows as the A operand: lane l brings 16-byte pieces of token l % 16, Q the
@@ -29,7 +31,8 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kTile = 32;          // tokens a wave takes at a time
-constexpr int kLeast = 8;          // tiles in a part at least: two for each of its waves
+constexpr int kLeast = 8;          // tiles in a part at least, two for each of its waves (2 sequences of 2000 and 500 tokens:
+                                   // 13.8 us; 4 tiles 13.4, 16 tiles 15.8; 8 of 3000 to 750: 22.3, 22.2, 21.1)
 constexpr int kTarget = 1024;      // shares of the line at most
 
 struct Paged {
@@ -586,9 +589,11 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Paged a) {
   reinterpret_cast<QT*>(a.o)[at * a.dh + tid] = from_f32<QT>(some ? v / sum : 0.f);
 }
 
-// Whether 8 waves of a workgroup find registers for their rows (two waves a SIMD).
-template <typename QT, typename KT, int DC>
-constexpr bool kRoom8 = DC <= (std::is_same<KT, float>::value ? 64 : 128);
+// Whether whole sequences may have 8 waves: over codes, whose instructions two waves a SIMD share, and where both find
+// registers.  8 sequences of 600 and 1024 tokens of 2 heads of 128 columns: in 8 bits 9.8 and 13.1 us with 8 waves, 11.3
+// and 15.7 with 4; in bf16 10.2 and 14.2 with 8, 9.9 and 13.5 with 4.
+template <typename KT, int DC>
+constexpr bool kEight = std::is_same<KT, int8_t>::value && DC <= 128;
 
 // How the work is spread: waves in a workgroup, and the shares of the line of all tiles (0: whole sequences).
 struct Plan {
@@ -608,7 +613,7 @@ Plan plan_of(const wc_paged_attn_args& p) {
   // fp32 columns 20.1 whole and 23.2 in parts at 600, 28.1 and 23.9 at 1024
   const int64_t whole = p.cache.bits == 0 && p.cache.dtype == WC_F32 && wide > 0 ? 512 : 1024;
   if (seqs * heads >= 2048 || longest <= whole || mul_sat({seqs, cdiv(longest, kTile) + 1}) >= (1ll << 31))
-    return Plan{seqs * heads >= 512 ? 4 : 8, 0, 0};      // two workgroups a unit hide each other's waits
+    return Plan{seqs * heads >= 512 ? 4 : 8, 0, 0};      // 8 only where two workgroups a unit don't come anyway
   const int64_t budget = cdiv(target, heads);
   return Plan{4, static_cast<int>(budget), budget + seqs};
 }
@@ -632,7 +637,7 @@ void dispatch(const Paged& a, bool q8, int waves, int64_t grid, hipStream_t s) {
   auto go = [&](auto k, auto dc) {
     typedef decltype(k) KT;
     constexpr int DC = decltype(dc)::value;
-    if constexpr (kRoom8<QT, KT, DC>)
+    if constexpr (kEight<KT, DC>)
       if (waves == 8) return launch<QT, KT, DC, 8>(a, grid, s);
     launch<QT, KT, DC, 4>(a, grid, s);
   };

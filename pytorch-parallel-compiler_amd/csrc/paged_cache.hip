@@ -2,7 +2,9 @@
 //
 // One group of lanes has a row: head_dim values of one head of one token, 16 bytes of them a lane.  Both
 // kernels only move rows, so they are bound by memory; what decides is that every access is a whole vector
-// and that enough of them are in flight.
+// and that enough of them are in flight.  16 sequences' 750 to 1500 new tokens of 8 heads of 128 columns in bf16:
+// written as they are (147 MB) 32 us, 4.6 TB/s; as codes (112 MB) 32 us, which the search for each row's scale and the
+// codes' arithmetic keep from 25; codes read back (145 MB) 26 us, 5.5 TB/s.
 //
 // 8 bits: scale = max(max |x| / 127, 2^-126), code = x / scale to the nearest, ties to even.  The quotient is
 // never formed: c = x * (1 / scale) to the nearest is off by at most one, and then only next to a half; the remainder
@@ -16,7 +18,8 @@ namespace wc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kRows = 4;           // rows of a group of lanes, all on their way at once
+constexpr int kRows = 4;           // rows of a group of lanes, all on their way at once (those codes written and read: 61 us;
+                                   // one row 68, two 64, eight 73)
 
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
