@@ -452,19 +452,26 @@ void launch_rows(Linear4 a, int64_t n, hipStream_t s) {
 }
 
 // Which kernel, for `tiles` tiles of output rows of all models and `rows` tiles of 16 rows of x (us on an MI355X,
-// launches of a graph).  Few tiles: a tile for each workgroup, its waves share the columns (bf16, groups of 128, 64
-// tiles of 16 rows: 4.0; two tiles each 4.5, through LDS 6.2), then two that share what they bring of x (512 tiles: 9.6;
-// one each 12.5, through LDS 12.2).  More go through LDS, with as much of x and W in a workgroup as leaves one for every
-// compute unit:
-//   fp16, groups of 64            16 waves, 64 rows   16 waves, 32 rows   8 x 2, 32 rows   4 x 2, 32 rows
-//   4096 tiles, 64 rows                   31                  43                 50               48
-//   2048 tiles, 64 rows                   29                  21                 27               27
-//   1024 tiles, 64 rows, K 4096           47                  33                 22               25
-//    512 tiles, 64 rows, K 4096           46                  31                 21               16
-// and likewise for 16 rows (4096 tiles: 17.5, of 4 x 2 waves 19.1) and in fp32, whose three planes of x leave less room.
+// launches of a graph, bf16, groups of 128).
+//
+// Few tiles: a tile for each workgroup, its waves share the columns (64 tiles of 16 rows: 4.0; two tiles each 4.5, through
+// LDS 6.2), then two that share what they bring of x (512 tiles, K 4096: 8.9; one each 10.1, through LDS 12.6).
+//
+// More go through LDS.  16 waves fill a unit, with as much of x and W as registers take, where their workgroups come to
+// whole rounds of all units, nearly; else 8 waves with 32 rows, of which a unit has two; else as many workgroups as can be:
+//                                 16 waves, 64 rows   16 waves, 32 rows   8 waves, 32 rows   4 x 2 waves, 32 rows
+//   4096 tiles, 64 rows, K 2048         35                  42                  41                 53
+//   2048 tiles, 64 rows, K 2048         32                  21                  22                 29
+//   1235 tiles, 64 rows, K 2048         32                  21                  22                 24
+//   1235 tiles, 200 rows, K 2048        62                  59                  50                 60
+//    512 tiles, 64 rows, K 2048         31                  19                  14                 12
+// and by the same reasons in fp32, whose three planes of x leave less room.  Sixteen rows or fewer: 16 waves again where
+// they come to whole rounds (4096 tiles, K 2048: 18, of 4 x 2 waves 20), and two waves over two tiles, without LDS,
+// where there are too few columns for it to pay (1235 tiles, K 1024: 7.5 against 8.9).
 template <typename T, int GP, int MT, int RT, int WR, int WK, int CK>
 bool launch_if_full(const Linear4& a, int64_t n, hipStream_t s) {
-  if (n * cdiv(a.otiles, WR * RT) * cdiv(a.m, MT * 16) < 256) return false;
+  const int64_t wgs = n * cdiv(a.otiles, WR * RT) * cdiv(a.m, MT * 16);
+  if (wgs * 5 < cdiv(wgs, 256) * 256 * 4) return false;              // the last round included, 4 of 5 units at work
   launch_rows<T, GP, MT, RT, WR, WK, CK>(a, n, s);
   return true;
 }
@@ -475,14 +482,17 @@ void dispatch(const Linear4& a, int64_t n, hipStream_t s) {
   if (tiles * rows <= 256) return launch_few<T, GP, 1, 4>(a, n, s);
   if (rows == 1 && tiles <= 1024) return launch_few<T, GP, 2, 4>(a, n, s);
   if constexpr (F32) {
-    if (rows > 1 && (launch_if_full<T, GP, 2, 2, 8, 1, 1>(a, n, s) || launch_if_full<T, GP, 2, 1, 8, 2, 2>(a, n, s))) return;
-    if (launch_if_full<T, GP, 1, 1, 16, 1, 4>(a, n, s) || launch_if_full<T, GP, 1, 1, 8, 2, 4>(a, n, s)) return;
+    if (rows > 1 && launch_if_full<T, GP, 2, 2, 8, 1, 1>(a, n, s)) return;
+    if (launch_if_full<T, GP, 1, 1, 16, 1, 4>(a, n, s)) return;
+    if (tiles * rows > 1024) return launch_rows<T, GP, 1, 1, 8, 1, 2>(a, n, s);
     launch_rows<T, GP, 1, 1, 4, 2, 4>(a, n, s);
   } else {
     if (rows > 2 && launch_if_full<T, GP, 4, 1, 16, 1, 2>(a, n, s)) return;
-    if (rows > 1 && (launch_if_full<T, GP, 2, 1, 16, 1, 4>(a, n, s) || launch_if_full<T, GP, 2, 1, 8, 2, 4>(a, n, s))) return;
+    if (rows > 1 && launch_if_full<T, GP, 2, 1, 16, 1, 4>(a, n, s)) return;
+    if (rows > 1 && (tiles * cdiv(rows, 2) > 1024 || a.ktiles <= 4)) return launch_rows<T, GP, 2, 1, 8, 1, 2>(a, n, s);
     if (rows > 2) return launch_rows<T, GP, 2, 1, 4, 2, 8>(a, n, s);
     if (rows == 1 && launch_if_full<T, GP, 1, 1, 16, 1, 8>(a, n, s)) return;
+    if (rows == 1 && a.ktiles <= 8) return launch_few<T, GP, 2, 2>(a, n, s);
     launch_rows<T, GP, 1, 1, 4, 2, 16>(a, n, s);
   }
 }

@@ -7,7 +7,7 @@ WideLinear4bit: N independent linear layers with weights of 4 bits, for few rows
 with codes of 0 to 15, groups of 32, 64 or 128 columns and zero points of 0 to 15 (8 where none are
 given).  The forward (wc_linear4) brings each weight from memory once for up to 16, 32 or 64 rows (the
 more weights there are, the more), so that a token's products cost what reading half a byte a weight
-costs; it is faster than WideLinear up to about 500 rows in 16 bits, and at any in fp32.  Sums are
+costs; it is faster than WideLinear up to some 250 rows in 16 bits, and at any in fp32.  Sums are
 fp32; the scale multiplies each group's sum.  An infinity in a row of x gives that
 row NaN in bf16 and fp32, also where the formula has an infinity.
 
