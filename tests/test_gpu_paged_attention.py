@@ -306,3 +306,31 @@ def test_attend_forms_one_after_the_other():
                 _check(cache.attend(part, table[:, :cut], length[:, :cut], max_length=most), part, k[:, :cut], v[:, :cut],
                        length[:, :cut])
     cache.index_error()
+
+
+def test_attend_two_graphs_at_once():
+    """Two captured calls that cut sequences into parts, replayed on two streams at the same time, with eager calls of
+    other lengths between the replays: every call has a workspace of its own."""
+    cache, q, k, v, table, lens = _setup(2, 2, 8, 2, 128, 16, [3000, 40, 1700, 2500], torch.bfloat16, False, 59)
+    short = (lens // 2).contiguous()
+    graphs, outs, streams = [], [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for part in (lens, short):
+        cache.attend(q, table, part)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(cache.attend(q, table, part))
+        graphs.append(g)
+    for step in range(4):
+        q.mul_(0.9)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        between = cache.attend(q, table, short)
+        torch.cuda.synchronize()
+        for out, part in zip(outs, (lens, short)):
+            assert torch.equal(out, cache.attend(q, table, part)), step
+        assert torch.equal(between, outs[1])
+    _check(outs[0], q, k, v, lens)
+    cache.index_error()

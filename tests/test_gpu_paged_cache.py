@@ -195,3 +195,24 @@ def test_write_and_read_in_a_graph():
         cache.write(k, v, table, start, count)
         ek, ev = cache.read(table, lens, most)
         assert torch.equal(a, ek) and torch.equal(c, ev)
+
+
+@pytest.mark.parametrize("quantized", [False, True])
+def test_a_table_without_entries(quantized):
+    """Nothing to follow: what is asked of it is reported and reads as zeros, what isn't asked is fine."""
+    import wide_compiler as wc
+    cache = wc.WidePagedCache(4, 16, 2, 64, quantized=quantized)
+    table = torch.zeros(2, 3, 0, dtype=torch.int32, device=DEV)
+    k = torch.randn(2, 3, 5, 2, 64, device=DEV, dtype=torch.bfloat16)
+    q = torch.randn(2, 3, 4, 64, device=DEV, dtype=torch.bfloat16)
+    none, some = (torch.full((2, 3), x, dtype=torch.int32, device=DEV) for x in (0, 2))
+    for lens in (none, some):
+        for call in (lambda: cache.write(k, k, table, none, lens), lambda: cache.read(table, lens, 5),
+                     lambda: (cache.attend(q, table, lens),)):
+            out = call()
+            assert out is None or all((o == 0).all() for o in out)
+            if lens is some:
+                with pytest.raises(IndexError):
+                    cache.index_error()
+            cache.index_error()
+    assert (cache.k_pages == 0).all() and (cache.v_pages == 0).all()
