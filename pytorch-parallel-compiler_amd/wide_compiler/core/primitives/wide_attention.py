@@ -250,6 +250,8 @@ class WideAttention(nn.Module):
         n, d, hh, dh = self.n, self.d_model, self.n_heads, self.d_head
         if x.dim() != 4 or x.shape[0] != n or x.shape[3] != d:
             raise RuntimeError(f"{what}: x must be [N={n}, B, T, {d}], got {list(x.shape)}")
+        if dh > (128 if x.dtype == torch.float32 else 256):          # what wc_attention takes, before the cache is written
+            raise RuntimeError(f"{what}: heads of {dh} columns are not supported in {x.dtype}")
         b, t = x.shape[1:3]
         q, k, v = self._cached_heads(what, x, cache, torch.arange(t, device=x.device), head_norm)
         cache.write(k, v, block_table, torch.zeros_like(lengths), lengths)

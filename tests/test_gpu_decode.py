@@ -154,3 +154,16 @@ def test_a_decoder_step_with_shared_heads(dtype):
             start.add_((start >= 0).to(torch.int32))
             lens.copy_(start + 1)
     cache.index_error()
+
+
+def test_a_refused_prompt_leaves_the_cache():
+    import wide_compiler as wc
+    attn = wc.WideAttention(2, 256, 1).to(DEV).eval()
+    cache = wc.WidePagedCache(8, 16, 1, 256, dtype=torch.float32)
+    table = torch.arange(2, dtype=torch.int32, device=DEV).view(2, 1, 1)
+    lens = torch.full((2, 1), 5, dtype=torch.int32, device=DEV)
+    with torch.no_grad():
+        with pytest.raises(RuntimeError, match="256 columns"):
+            attn.prompt(torch.randn(2, 1, 5, 256, device=DEV), cache, table, lens)
+        assert (cache.k_pages == 0).all()
+        assert torch.isfinite(attn.step(torch.randn(2, 1, 256, device=DEV), cache, table, lens)).all()
