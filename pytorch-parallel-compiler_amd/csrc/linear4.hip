@@ -13,8 +13,8 @@
 // rounding in fp32 is 2^-24 of 128 |sum x|.  fp32 goes as three bf16 planes of x (every bit of it down to 2^-110)
 // against codes converted to bf16, without the 128.  A row of x with an infinity or NaN gives NaN in bf16 and fp32.
 //
-// 4 models' [4096 -> 4096] in bf16, one row (35 MB): 10.8 us, of which an empty launch is 3.3; 8 models' [2048 -> 8192]
-// in fp16, 64 rows (84 MB, 17 GFLOP): 31 us, half of it the instructions that make numbers of codes and scale the
+// 4 models' [4096 -> 4096] in bf16, one row (35 MB): 10.4 us, of which an empty launch is 3.3; 8 models' [2048 -> 8192]
+// in fp16, 64 rows (84 MB, 17 GFLOP): 30 us, half of it the instructions that make numbers of codes and scale the
 // groups' sums, which with two to four waves a unit's quarter only partly hide behind the loads.
 //
 // The columns are dealt to the waves of a workgroup, which add their sums up through LDS at the end.
@@ -202,12 +202,12 @@ __device__ __forceinline__ void store4(T* y, int o, int end, const T* bias, f32x
       if (o + e < end) y[o + e] = r.v[e];
 }
 
-// Up to 16 rows of x, straight from memory: a workgroup has one tile of output rows, its waves every NW-th tile of
+// Up to 16 rows of x, straight from memory: a workgroup has RT tiles of output rows, its waves every NW-th tile of
 // columns.  Weights come D tiles ahead of their use, x (which all workgroups share, in L2) one.
 template <typename T, int GP, int RT, int NW, bool AL>
 __global__ __launch_bounds__(NW * 64) void linear4_few_kernel(Linear4 a) {
   constexpr bool kF32 = sizeof(T) == 4, kF16 = std::is_same<T, f16>::value;
-  constexpr int NX = kF32 ? 3 : 1, D = RT * GP > 4 || (kF32 && RT > 1) ? 2 : 4, E = 16 / sizeof(T), P = 8 / E;
+  constexpr int NX = kF32 ? 3 : 1, D = NW > 4 || RT * GP > 4 || (kF32 && RT > 1) ? 2 : 4, E = 16 / sizeof(T), P = 8 / E;
   __shared__ float lds[NW * 16 * RT * 16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
   const uint32_t model = fdiv(blockIdx.x, a.by_wg);
@@ -455,7 +455,9 @@ void launch_rows(Linear4 a, int64_t n, hipStream_t s) {
 // launches of a graph, bf16, groups of 128).
 //
 // Few tiles: a tile for each workgroup, its waves share the columns (64 tiles of 16 rows: 4.0; two tiles each 4.5, through
-// LDS 6.2), then two that share what they bring of x (512 tiles, K 4096: 8.9; one each 10.1, through LDS 12.6).
+// LDS 6.2), then two that share what they bring of x, for 8 waves where their workgroups all find room at once (1024 tiles,
+// K 4096: 10.9; for 4 waves 11.9; one tile for 4 waves 12.3; in fp16 with groups of 64: 11.6, 13.4, 12.7.  Groups of 32, K
+// 2048, whose registers leave room for half: 11.6 with 8, 9.6 with 4).
 //
 // More go through LDS.  16 waves fill a unit, with as much of x and W as registers take, where their workgroups come to
 // whole rounds of all units, nearly; else 8 waves with 32 rows, of which a unit has two; else as many workgroups as can be:
@@ -480,6 +482,7 @@ void dispatch(const Linear4& a, int64_t n, hipStream_t s) {
   constexpr bool F32 = sizeof(T) == 4;
   const int64_t tiles = n * a.otiles, rows = cdiv(a.m, 16);
   if (tiles * rows <= 256) return launch_few<T, GP, 1, 4>(a, n, s);
+  if (rows == 1 && tiles <= (F32 || GP > 2 ? 512 : 1024)) return launch_few<T, GP, 2, 8>(a, n, s);
   if (rows == 1 && tiles <= 1024) return launch_few<T, GP, 2, 4>(a, n, s);
   if constexpr (F32) {
     if (rows > 1 && launch_if_full<T, GP, 2, 2, 8, 1, 1>(a, n, s)) return;

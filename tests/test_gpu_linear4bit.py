@@ -64,7 +64,7 @@ def test_linear4_sizes(n, m, k, o, zeros, bias, group, dtype):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("n,m", [(52, 3), (52, 20), (90, 5), (90, 32), (52, 90), (90, 70), (90, 64), (83, 5), (83, 32), (83, 60),
-                                 (10, 20), (6, 50)])
+                                 (10, 20), (6, 50), (20, 3)])
 @pytest.mark.parametrize("k", [150, 264, 600, 1160])
 def test_linear4_many_layers(n, m, k, group, dtype):
     """Enough output rows for every form of the kernel, with widths of whole vectors and not."""
