@@ -195,6 +195,9 @@ def linear4(sizes: Tuple, rows, x: Tensor, codes: Tensor, scales: Tensor, zeros:
         0 if bias is None else bias.data_ptr(), y.data_ptr()), x)
 
 
-for _name in ("head_norm_rotary", "cache_write", "cache_read", "paged_attention_workspace", "paged_attention", "linear4"):
-    globals()[_name] = torch.compiler.disable(globals()[_name])
-del _name
+
+@torch.compiler.disable
+def uncompiled(call, *args):
+    """call(*args) outside a region that torch.compile traces: what the modules' and the cache's calls do there, whose
+    plans and launches are nothing to trace.  A check of is_compiling() costs a call less than the decorator does."""
+    return call(*args)

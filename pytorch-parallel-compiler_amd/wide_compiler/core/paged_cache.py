@@ -129,9 +129,11 @@ class WidePagedCache:
         """Rows [0, count[n, b]) of k, v [N, B, T, Hkv, Dh] become tokens start[n, b] + 0, 1, ... of their
         sequences (count None: all T).  Rows from count on are padding, and a sequence of negative start takes part in
         nothing: neither is written."""
-        form = (k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(), v.dtype, v.device, block_table.shape,
-                block_table.dtype, block_table.device, start.shape, start.dtype, start.device,
-                None if count is None else (count.shape, count.dtype, count.device))
+        if torch.compiler.is_compiling():
+            return _serve.uncompiled(self.write, k, v, block_table, start, count)
+        form = (k.shape, k.stride(), k.dtype, k.get_device(), v.shape, v.stride(), v.dtype, v.get_device(),
+                block_table.shape, block_table.dtype, block_table.get_device(), start.shape, start.dtype, start.get_device(),
+                None if count is None else (count.shape, count.dtype, count.get_device()))
         plan = self._plans.get(form)
         if plan is None:
             what = "WidePagedCache.write"
@@ -155,8 +157,10 @@ class WidePagedCache:
 
     def read(self, block_table: Tensor, lengths: Tensor, max_length: int) -> Tuple[Tensor, Tensor]:
         """K and V of tokens [0, lengths[n, b]) as [N, B, max_length, Hkv, Dh]; zeros from a sequence's length on."""
-        form = (block_table.shape, block_table.dtype, block_table.device, lengths.shape, lengths.dtype, lengths.device,
-                max_length)
+        if torch.compiler.is_compiling():
+            return _serve.uncompiled(self.read, block_table, lengths, max_length)
+        form = (block_table.shape, block_table.dtype, block_table.get_device(), lengths.shape, lengths.dtype,
+                lengths.get_device(), max_length)
         plan = self._plans.get(form)
         if plan is None:
             what = "WidePagedCache.read"
@@ -182,9 +186,11 @@ class WidePagedCache:
         head h reads key head h // (Hq // Hkv); scale defaults to Dh ** -0.5.  A sequence without tokens gets
         zeros.  ``max_length`` bounds the lengths (default: what the block table can name); a tight bound splits
         short sequences less."""
-        form = (q.shape, q.dtype, q.device, block_table.shape, block_table.dtype, block_table.device, lengths.shape,
-                lengths.dtype, lengths.device, None if first is None else (first.shape, first.dtype, first.device),
-                max_length)
+        if torch.compiler.is_compiling():
+            return _serve.uncompiled(self.attend, q, block_table, lengths, first, scale, max_length)
+        form = (q.shape, q.dtype, q.get_device(), block_table.shape, block_table.dtype, block_table.get_device(),
+                lengths.shape, lengths.dtype, lengths.get_device(),
+                None if first is None else (first.shape, first.dtype, first.get_device()), max_length)
         plan = self._plans.get(form)
         if plan is None:
             plan = self._plans.keep(form, self._plan_attend(q, block_table, lengths, first, max_length))

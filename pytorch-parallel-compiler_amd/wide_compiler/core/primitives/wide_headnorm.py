@@ -51,10 +51,13 @@ class WideHeadNormRotary(nn.Module):
         self._plans = _serve.Plans()
 
     def forward(self, q: Tensor, k: Tensor, positions: Tensor) -> Tuple[Tensor, Tensor]:
+        if torch.compiler.is_compiling():
+            return _serve.uncompiled(self.forward, q, k, positions)
         params = self._parameters
         qw, kw, freq = params["q_weight"], params["k_weight"], self._buffers["_freq_bits"]
-        form = (q.shape, q.stride(), q.dtype, q.device, k.shape, k.stride(), k.dtype, k.device, positions.shape,
-                positions.stride(), positions.dtype, positions.device, qw.shape, qw.dtype, qw.device, kw.shape, kw.dtype, kw.device)
+        form = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), positions.shape,
+                positions.stride(), positions.dtype, positions.get_device(), qw.shape, qw.dtype, qw.get_device(), kw.shape,
+                kw.dtype, kw.get_device())
         plan = self._plans.get(form)
         if plan is None:
             plan = self._plan(form, q, k, positions, qw, kw, freq)

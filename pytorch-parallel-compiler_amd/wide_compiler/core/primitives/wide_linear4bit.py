@@ -53,11 +53,13 @@ class WideLinear4bit(nn.Module):
         self._plans = _serve.Plans()
 
     def forward(self, x: Tensor) -> Tensor:
+        if torch.compiler.is_compiling():
+            return _serve.uncompiled(self.forward, x)
         bufs = self._buffers
         packed, scales, zeros, bias = bufs["packed"], bufs["scales"], bufs["zeros"], bufs["bias"]
-        form = (x.shape, x.stride(), x.dtype, x.device, packed.shape, packed.dtype, packed.device, scales.shape,
-                scales.dtype, scales.device, zeros.shape, zeros.dtype, zeros.device,
-                None if bias is None else (bias.shape, bias.dtype, bias.device))
+        form = (x.shape, x.stride(), x.dtype, x.get_device(), packed.shape, packed.dtype, packed.get_device(), scales.shape,
+                scales.dtype, scales.get_device(), zeros.shape, zeros.dtype, zeros.get_device(),
+                None if bias is None else (bias.shape, bias.dtype, bias.get_device()))
         plan = self._plans.get(form)
         if plan is None:
             plan = self._plan(form, x, packed, scales, zeros, bias)

@@ -167,3 +167,28 @@ def test_a_refused_prompt_leaves_the_cache():
             attn.prompt(torch.randn(2, 1, 5, 256, device=DEV), cache, table, lens)
         assert (cache.k_pages == 0).all()
         assert torch.isfinite(attn.step(torch.randn(2, 1, 256, device=DEV), cache, table, lens)).all()
+
+
+def test_under_torch_compile():
+    """A compiled function ends its regions at these calls, and gives what the function itself gives."""
+    import wide_compiler as wc
+    n, b, h, d = 2, 3, 2, 64
+    attn = wc.WideAttention(n, h * d, h).to(DEV, torch.bfloat16).eval()
+    norm = wc.WideHeadNormRotary(n, d).to(DEV, torch.bfloat16)
+    proj = wc.WideLinear4bit.from_modules([torch.nn.Linear(h * d, 40).to(DEV, torch.bfloat16) for _ in range(n)], group_size=32)
+    lens = torch.tensor([[5, 1, 0], [9, 30, 2]], dtype=torch.int32)
+    table, pages = make_table(lens, 16, gen(3))
+    table, lens = table.to(DEV), lens.to(DEV)
+    x = torch.randn(n, b, h * d, device=DEV, dtype=torch.bfloat16)
+    outs = []
+    for wrap in (lambda f: f, lambda f: torch.compile(f, backend="eager")):
+        cache = wc.WidePagedCache(pages, 16, h, d)
+
+        def step(x, table, lens):
+            y = attn.step(x, cache, table, lens, norm)
+            k, v = cache.read(table, lens, 30)
+            return proj(y + 1), k, v
+        with torch.no_grad():
+            outs.append(wrap(step)(x, table, lens))
+    for a, c in zip(*outs):
+        assert torch.equal(a, c)
