@@ -154,35 +154,41 @@ __device__ __forceinline__ const T* x_row(const Linear4& a, uint32_t model, int 
 }
 
 // 16 bytes of a row of x at column k, and its values from the row's end on as zeros: apart, because what looks at a
-// loaded value waits for it
+// loaded value waits for it.  Rows that aren't whole vectors (AL false) are loaded at any address all the same, the piece
+// over the end from further left, and moved down afterwards; value by value only where a row is shorter than a vector.
 template <typename T, bool AL>
 __device__ __forceinline__ u32x4 x_load(const T* x, int k, int end) {
-  if constexpr (AL) {
-    return *reinterpret_cast<const u32x4*>(x + (k < end ? k : 0));
+  constexpr int E = 16 / sizeof(T);
+  if constexpr (AL) return *reinterpret_cast<const u32x4*>(x + (k < end ? k : 0));
+  u32x4 v;
+  if (end >= E) {
+    __builtin_memcpy(&v, x + std::min(k, end - E), sizeof v);
   } else {
-    constexpr int E = 16 / sizeof(T);
-    struct alignas(16) {
-      T v[E];
-    } s;
+    T s[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) s.v[e] = x[k + e < end ? k + e : 0];
-    return __builtin_bit_cast(u32x4, s);
+    for (int e = 0; e < E; ++e) s[e] = x[k + e < end ? k + e : 0];
+    __builtin_memcpy(&v, s, sizeof v);
   }
+  return v;
 }
 template <typename T, bool AL>
 __device__ __forceinline__ u32x4 x_keep(u32x4 v, int k, int end) {
-  if constexpr (AL) {
-    return k < end ? v : u32x4{};
-  } else {
-    constexpr int E = 16 / sizeof(T);
-    struct alignas(16) {
-      T v[E];
-    } s = __builtin_bit_cast(decltype(s), v);
-#pragma unroll
-    for (int e = 0; e < E; ++e)
-      if (k + e >= end) s.v[e] = static_cast<T>(0.f);
-    return __builtin_bit_cast(u32x4, s);
+  constexpr int E = 16 / sizeof(T);
+  if constexpr (AL) return k < end ? v : u32x4{};
+  if (end >= E) {
+    const int down = std::max(k - (end - E), 0) * static_cast<int>(sizeof(T)) * 8;      // bits
+    typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+    const u64x2 w = __builtin_bit_cast(u64x2, v);
+    const u64x2 part = down < 64 ? u64x2{w[0] >> (down & 63) | w[1] << 1 << (~down & 63), w[1] >> (down & 63)} : u64x2{w[1] >> (down & 63), 0};
+    return down == 0 ? v : down < 128 ? __builtin_bit_cast(u32x4, part) : u32x4{};
   }
+  T s[E];
+  __builtin_memcpy(s, &v, sizeof v);
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (k + e >= end) s[e] = static_cast<T>(0.f);
+  __builtin_memcpy(&v, s, sizeof v);
+  return v;
 }
 
 // outputs o..o + 3 of a row of y, those it has
@@ -207,7 +213,7 @@ __device__ __forceinline__ void store4(T* y, int o, int end, const T* bias, f32x
 template <typename T, int GP, int RT, int NW, bool AL>
 __global__ __launch_bounds__(NW * 64) void linear4_few_kernel(Linear4 a) {
   constexpr bool kF32 = sizeof(T) == 4, kF16 = std::is_same<T, f16>::value;
-  constexpr int NX = kF32 ? 3 : 1, D = NW > 4 || RT * GP > 4 || (kF32 && RT > 1) ? 2 : 4, E = 16 / sizeof(T), P = 8 / E;
+  constexpr int NX = kF32 ? 3 : 1, D = RT * GP > 4 || (RT > 1 && (kF32 || NW > 4)) ? 2 : 4, E = 16 / sizeof(T), P = 8 / E;
   __shared__ float lds[NW * 16 * RT * 16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
   const uint32_t model = fdiv(blockIdx.x, a.by_wg);
@@ -455,7 +461,7 @@ void launch_rows(Linear4 a, int64_t n, hipStream_t s) {
 // launches of a graph, bf16, groups of 128).
 //
 // Few tiles: a tile for each workgroup, its waves share the columns (64 tiles of 16 rows: 4.0; two tiles each 4.5, through
-// LDS 6.2), then two that share what they bring of x, for 8 waves where their workgroups all find room at once (1024 tiles,
+// LDS 6.2; 8 waves where columns are long: 256 tiles, K 4096, fp16: 5.9, with 4 6.3), then two that share what they bring of x, for 8 waves where their workgroups all find room at once (1024 tiles,
 // K 4096: 10.9; for 4 waves 11.9; one tile for 4 waves 12.3; in fp16 with groups of 64: 11.6, 13.4, 12.7.  Groups of 32, K
 // 2048, whose registers leave room for half: 11.6 with 8, 9.6 with 4).
 //
@@ -481,6 +487,7 @@ template <typename T, int GP>
 void dispatch(const Linear4& a, int64_t n, hipStream_t s) {
   constexpr bool F32 = sizeof(T) == 4;
   const int64_t tiles = n * a.otiles, rows = cdiv(a.m, 16);
+  if (tiles * rows <= 256 && a.ktiles >= 32) return launch_few<T, GP, 1, 8>(a, n, s);
   if (tiles * rows <= 256) return launch_few<T, GP, 1, 4>(a, n, s);
   if (rows == 1 && tiles <= (F32 || GP > 2 ? 512 : 1024)) return launch_few<T, GP, 2, 8>(a, n, s);
   if (rows == 1 && tiles <= 1024) return launch_few<T, GP, 2, 4>(a, n, s);
