@@ -16,8 +16,9 @@
 //   output   O^T [column][query] = V^T P: those 8 tokens are what the B operand of one 32-token product wants from
 //            the lane, if V^T takes tokens in the same order: lane l loads the 8 tokens' rows, at columns of its
 //            own (l % 16), as whole vectors; operand e pairs up their e-th values, one v_perm per two.
-// P goes into the product as the sum of two 16-bit numbers (three for fp32 queries over 8-bit pages), because its
-// rounding to one would be as large an error as the rounding of the result.  fp32 pages use the fp32 MFMA.
+// P goes into the product as the sum of three bf16 numbers, or two fp16 ones: of two bf16 its last 2^-17 would be lost, which
+// values that cancel show (and which moves 0.4 % of bf16 outputs by a step where fp32 sums move 0.1 %); the third costs
+// nothing where memory bounds it and 3 % over codes.  fp32 pages use the fp32 MFMA.
 // 8-bit codes are exact in bf16 and fp16; a row's scale multiplies its score, or its weight in P.
 //
 // Work is split over waves, over workgroups and joined with the usual weights exp(m_part - m): waves of a
@@ -109,20 +110,27 @@ __device__ __forceinline__ void planes(const float (&v)[8], u32x4 (&out)[N]) {
     }
 }
 
-// 8 weights >= 0 as two planes, both over 0 where the weight is: the first is what 16 bits hold of a value just under
-// the weight, so that an infinite value in V takes the sum to its infinity and not, by 0 or the other sign, to NaN.
-template <typename MT>
-__device__ __forceinline__ void weight_planes(const float (&p)[8], u32x4 (&out)[2]) {
+// 8 weights >= 0 as N planes that leave out at most 2^-23 of them (two fp16 ones: 2^-21), all over 0 where the weight
+// is: each but the last is what 16 bits hold of a value just under what is left, so that an infinite value in V takes the
+// sum to its infinity and not, by 0 or the other sign, to NaN.
+template <typename MT, int N>
+__device__ __forceinline__ void weight_planes(const float (&p)[8], u32x4 (&out)[N]) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const float a = p[2 * e], b = p[2 * e + 1], under = 0x1.fffffep-1f;
-    uint32_t w;
-    if constexpr (std::is_same<MT, f16>::value)
-      w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a * under, b * under));
-    else
-      w = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b * under), __builtin_bit_cast(uint32_t, a * under), 0x07060302u);
-    out[0][e] = w;
-    out[1][e] = pack2<MT>(a - unpack_lo<MT>(w), b - unpack_hi<MT>(w));
+    float a = p[2 * e], b = p[2 * e + 1];
+    constexpr float under = 0x1.fffffep-1f;
+#pragma unroll
+    for (int n = 0; n + 1 < N; ++n) {
+      uint32_t w;
+      if constexpr (std::is_same<MT, f16>::value)
+        w = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a * under, b * under));
+      else
+        w = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b * under), __builtin_bit_cast(uint32_t, a * under), 0x07060302u);
+      out[n][e] = w;
+      a -= unpack_lo<MT>(w);
+      b -= unpack_hi<MT>(w);
+    }
+    out[N - 1][e] = pack2<MT>(a, b);
   }
 }
 
@@ -222,7 +230,7 @@ __global__ __launch_bounds__(NW * 64) void paged_attention_kernel(Paged a) {
   constexpr int VE = DC / 16, CE = VE * ES > 16 ? CH : VE, NCV = VE / CE;   // columns of V per lane
   constexpr int NF = DC / 32;                                   // 16-bit score products per 16 tokens
   constexpr int NQ = std::is_same<QT, float>::value ? 3 : std::is_same<QT, MT>::value ? 1 : 2;   // planes of q
-  constexpr int NP = std::is_same<QT, float>::value ? 3 : 2;                                    // and of P
+  constexpr int NP = std::is_same<MT, f16>::value ? 2 : 3;                                      // and of P
   // fp16 weights are taken 2^14 times as large (m - 14 in their exponents), so that those far under 1 keep their bits
   constexpr float kShift = std::is_same<MT, f16>::value ? 14.f : 0.f;
   typedef typename Raw<CE * ES>::type VR;
@@ -443,10 +451,10 @@ __global__ __launch_bounds__(NW * 64) void paged_attention_kernel(Paged a) {
               acc[c][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, dword(vf[u][c], e)), p[u], acc[c][e], 0, 0, 0);
       } else {
         u32x4 pf[NP];
-        if constexpr (NP == 2)
-          weight_planes<MT>(p, pf);
-        else
+        if constexpr (std::is_same<QT, float>::value)
           planes<MT, NP>(p, pf);
+        else
+          weight_planes<MT, NP>(p, pf);
 #pragma unroll
         for (int c = 0; c < NCV; ++c)
 #pragma unroll

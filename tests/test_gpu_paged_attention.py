@@ -334,3 +334,42 @@ def test_attend_two_graphs_at_once():
         assert torch.equal(between, outs[1])
     _check(outs[0], q, k, v, lens)
     cache.index_error()
+
+
+@pytest.mark.parametrize("dtype,quantized", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float16, False),
+                                             (torch.float16, True), (torch.float32, False), (torch.float32, True)])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_attend_values_that_cancel(d, dtype, quantized):
+    """Softmax weights count with all their bits: every token's values take away what those before it left over, so that
+    the result is the rounding of the weights.  Scores are one product each, of at most 2, so a weight is off by 10 2^-24
+    of itself (scale, product, difference and 2^x, of an exponent up to 2.9) and 2^-21 by its planes, a sum of 4 tokens by
+    4 2^-24: 2^-19 of the sum of magnitudes in all."""
+    import wide_compiler as wc
+    n, b, heads, length = 2, 16, 4, 4
+    g = gen(d)
+    score = (2 * torch.rand(n, b, length, heads, generator=g) - 1).to(dtype).double()
+    p = torch.softmax(score, 2)
+    k = torch.zeros(n, b, length, heads, d, dtype=torch.float64)
+    k[..., 0] = score
+    if quantized:
+        k = quantise(k)                                     # one value a row: its code is 127
+        p = torch.softmax(k[..., 0], 2)
+    v, left = [], torch.zeros(n, b, heads, d, dtype=torch.float64)
+    for t in range(length):
+        x = 1 + torch.rand(n, b, heads, d, generator=g, dtype=torch.float64) if t == 0 else -left / p[:, :, t, :, None]
+        x = x.to(dtype)
+        v.append(x)
+        left = left + p[:, :, t, :, None] * (quantise(x) if quantized else x.double())
+    v = torch.stack(v, 2)
+    stored = quantise(v) if quantized else v.double()
+    size = (p[..., None] * stored.abs()).sum(2)
+    assert (left.abs() < 2.0 ** -13 * size).all()
+    lens = torch.full((n, b), length, dtype=torch.int32)
+    table, pages = make_table(lens, 16, g)
+    cache = wc.WidePagedCache(pages, 16, heads, d, dtype=dtype, quantized=quantized)
+    table, lens = table.to(DEV), lens.to(DEV)
+    cache.write((score[..., None] * (torch.arange(d) == 0)).to(DEV, dtype), v.to(DEV), table, torch.zeros_like(lens))
+    q = torch.zeros(n, b, heads, d, device=DEV, dtype=dtype)
+    q[..., 0] = 1
+    got = cache.attend(q, table, lens, scale=1.0).cpu()
+    within(got, left, HALF[dtype], 2.0 ** -19 * size)
