@@ -206,11 +206,15 @@ __device__ __forceinline__ int2 find_tile(const Paged& a, int at, int lane) {
   }
   return make_int2(a.seqs, 0);
 }
-// each sequence's first part and how many it has, for the kernel that joins them
+// each sequence's first part and how many it has, for the kernel that joins them; and the fault of lengths that were cut,
+// of sequences without a tile (which no share visits) too
 __device__ __forceinline__ void list_parts(const Paged& a, int size, int lane) {
   int done = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += 64) {
-    const int s = s0 + lane, n = s < a.seqs ? tiles_of(span_of(a, s)) : 0;
+    const int s = s0 + lane;
+    const Span span = s < a.seqs ? span_of(a, s) : Span{0, 0, false};
+    if (span.cut) paged_fault(a.t);
+    const int n = tiles_of(span);
     const int start = done + before(n, lane), w0 = start / size;
     if (s < a.seqs) a.parts[s] = n ? make_int2(w0 + s, (start + n - 1) / size - w0 + 1) : make_int2(0, 0);
     done = __shfl(start + n, 63, 64);
@@ -296,7 +300,7 @@ __global__ __launch_bounds__(NW * 64) void paged_attention_kernel(Paged a) {
     }
     const Span span{begin, min(length, a.most), length > a.most};
     const int seq_lo = span.lo, hi = span.hi, tiles = tiles_of(span), tile_hi = min(tiles, to - start);
-    if (span.cut && threadIdx.x == 0) paged_fault(a.t);
+    if (a.budget == 0 && span.cut && threadIdx.x == 0) paged_fault(a.t);
     start += tiles;
     if (a.budget > 0 && tile_lo >= tile_hi) continue;             // a sequence without tokens
 

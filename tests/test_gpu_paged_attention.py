@@ -373,3 +373,29 @@ def test_attend_values_that_cancel(d, dtype, quantized):
     q[..., 0] = 1
     got = cache.attend(q, table, lens, scale=1.0).cpu()
     within(got, left, HALF[dtype], 2.0 ** -19 * size)
+
+
+def test_attend_lengths_out_of_range_of_sequences_without_a_tile():
+    """A length beyond its bound is reported in either form, also where none of the sequence's tokens is left: a pool
+    without pages, a first token at or behind the bound, alone and next to sequences that have tokens."""
+    import wide_compiler as wc
+    for blocks in (1, 200):                                 # whole, in parts
+        cache = wc.WidePagedCache(0, 16, 2, 64)
+        q = torch.randn(1, 2, 4, 64, device=DEV, dtype=torch.bfloat16)
+        table = torch.zeros(1, 2, blocks, dtype=torch.int32, device=DEV)
+        for lens, bad in (([0, 0], False), ([0, 5], True), ([3, 0], True)):
+            assert (cache.attend(q, table, torch.tensor([lens], dtype=torch.int32, device=DEV)) == 0).all()
+            if bad:
+                with pytest.raises(IndexError):
+                    cache.index_error()
+            cache.index_error()
+    for most, lens in ((1000, [40, 1001, 30]), (2000, [1500, 2001, 1700])):
+        cache, q, k, v, table, lens = _setup(1, 3, 4, 2, 64, 16, lens, torch.bfloat16, False, most)
+        for first in ([0, most, 0], [3000, most, 3000]):
+            first = torch.tensor([first], dtype=torch.int32, device=DEV)
+            got = cache.attend(q, table, lens, first=first, max_length=most)
+            with pytest.raises(IndexError):
+                cache.index_error()
+            cut = lens.clamp(max=most)
+            assert torch.equal(got, cache.attend(q, table, cut, first=first, max_length=most))
+            cache.index_error()
