@@ -31,7 +31,7 @@ namespace wc {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kTile = 32;          // tokens a wave takes at a time
+constexpr int kTile = kPagedTile;  // tokens a wave takes at a time
 constexpr int kLeast = 8;          // tiles in a part at least, two for each of its waves (2 sequences of 2000 and 500 tokens:
                                    // 13.8 us; 4 tiles 13.4, 16 tiles 15.8; 8 of 3000 to 750: 22.3, 22.2, 21.1)
 constexpr int kTarget = 1024;      // shares of the line at most
@@ -154,17 +154,8 @@ __device__ __forceinline__ void clear(R& r) {
   r = R(0u);
 }
 
-// A sequence's tokens [lo, hi); its tiles are counted from the one that holds token lo.
-struct Span {
-  int lo, hi;
-  bool cut;                  // the length was beyond most
-};
-__device__ __forceinline__ Span span_of(const Paged& a, int64_t seq) {
-  const int length = a.lengths[seq];
-  return Span{a.first ? max(a.first[seq], 0) : 0, min(length, a.most), length > a.most};
-}
-__device__ __forceinline__ int tiles_of(const Span& s) {
-  return s.hi > s.lo ? (s.hi - (s.lo & ~(kTile - 1)) + kTile - 1) / kTile : 0;
+__device__ __forceinline__ PagedSpan span_of(const Paged& a, int64_t seq) {
+  return paged_span(a.first ? a.first[seq] : 0, a.lengths[seq], a.most);
 }
 
 // Where sequences are cut, the tiles of all of them count as one line, of which every workgroup (of a key head) has an
@@ -176,7 +167,7 @@ struct Line {
 };
 __device__ __forceinline__ Line line_of(const Paged& a, int lane) {
   int total = 0;
-  for (int s = lane; s < a.seqs; s += 64) total += tiles_of(span_of(a, s));
+  for (int s = lane; s < a.seqs; s += 64) total += paged_tiles(span_of(a, s));
 #pragma unroll
   for (int off = 32; off; off >>= 1) total += __shfl_xor(total, off, 64);
   return Line{max((total + a.budget - 1) / a.budget, kLeast), total};
@@ -195,7 +186,7 @@ __device__ __forceinline__ int before(int v, int lane) {
 __device__ __forceinline__ int2 find_tile(const Paged& a, int at, int lane) {
   int done = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += 64) {
-    const int s = s0 + lane, n = s < a.seqs ? tiles_of(span_of(a, s)) : 0;
+    const int s = s0 + lane, n = s < a.seqs ? paged_tiles(span_of(a, s)) : 0;
     const int start = done + before(n, lane);
     const uint64_t mine = __ballot(at >= start && at < start + n);
     if (mine) {
@@ -212,9 +203,9 @@ __device__ __forceinline__ void list_parts(const Paged& a, int size, int lane) {
   int done = 0;
   for (int s0 = 0; s0 < a.seqs; s0 += 64) {
     const int s = s0 + lane;
-    const Span span = s < a.seqs ? span_of(a, s) : Span{0, 0, false};
+    const PagedSpan span = s < a.seqs ? span_of(a, s) : PagedSpan{0, 0, false};
     if (span.cut) paged_fault(a.t);
-    const int n = tiles_of(span);
+    const int n = paged_tiles(span);
     const int start = done + before(n, lane), w0 = start / size;
     if (s < a.seqs) a.parts[s] = n ? make_int2(w0 + s, (start + n - 1) / size - w0 + 1) : make_int2(0, 0);
     done = __shfl(start + n, 63, 64);
@@ -298,8 +289,8 @@ __global__ __launch_bounds__(NW * 64) void paged_attention_kernel(Paged a) {
         __builtin_memcpy(&r, v, sizeof v);
       }
     }
-    const Span span{begin, min(length, a.most), length > a.most};
-    const int seq_lo = span.lo, hi = span.hi, tiles = tiles_of(span), tile_hi = min(tiles, to - start);
+    const PagedSpan span = paged_span(begin, length, a.most);
+    const int seq_lo = span.lo, hi = span.hi, tiles = paged_tiles(span), tile_hi = min(tiles, to - start);
     if (a.budget == 0 && span.cut && threadIdx.x == 0) paged_fault(a.t);
     start += tiles;
     if (a.budget > 0 && tile_lo >= tile_hi) continue;             // a sequence without tokens
@@ -558,7 +549,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(Paged a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t at = blockIdx.x, seq = at / a.heads, head = at - seq * a.heads;
   const int2 mine = a.parts[seq];
-  const int n = mine.y;                                            // at most the shares, which are at most kTarget
+  const int n = min(mine.y, kTarget);                              // at most the shares, which are at most kTarget
   const float2* ml = a.ml + mine.x * static_cast<int64_t>(a.heads) + head;
   const float* part = a.part + (mine.x * static_cast<int64_t>(a.heads) + head) * a.dh;
   const int quads = (a.dh + 3) / 4, rows = 256 / quads, q = tid % quads, r = tid / quads;
@@ -633,7 +624,7 @@ struct Plan {
 };
 Plan plan_of(const wc_paged_attn_args& p) {
   const int64_t seqs = p.cache.n * p.cache.b, heads = p.cache.heads * cdiv(p.q_heads / p.cache.heads, 16);
-  const int64_t longest = std::min(p.max_length, p.cache.table_len * p.cache.page_size);
+  const int64_t most = paged_most(p.cache, p.max_length);
   // shares for every compute unit to have as many workgroups as its registers hold, and no more: 64 sequences of
   // 1000-4000 tokens in 8 bits (three fit) took 100 us in one share a unit, 91 in two, 86 in three, 101 in four
   const int wide = p.cache.head_dim <= 64 ? 0 : p.cache.head_dim <= 128 ? 1 : 2;
@@ -643,7 +634,7 @@ Plan plan_of(const wc_paged_attn_args& p) {
   // than it saves: 8 sequences of 2 heads of 64 took 10.6 us whole at 1024 tokens and 14.0 in parts at 1500; of 128
   // fp32 columns 20.1 whole and 23.2 in parts at 600, 28.1 and 23.9 at 1024
   const int64_t whole = p.cache.bits == 0 && p.cache.dtype == WC_F32 && wide > 0 ? 512 : 1024;
-  if (seqs * heads >= 2048 || longest <= whole || mul_sat({seqs, cdiv(longest, kTile) + 1}) >= (1ll << 31))
+  if (seqs * heads >= 2048 || most <= whole || !paged_countable(seqs, most))
     return Plan{seqs * heads >= 512 ? 4 : 8, 0, 0};      // 8 only where two workgroups a unit don't come anyway
   const int64_t budget = cdiv(target, heads);
   return Plan{4, static_cast<int>(budget), budget + seqs};
@@ -748,8 +739,8 @@ extern "C" int32_t wc_paged_attention(const wc_paged_attn_args* args, void* stre
   const int64_t qtiles = cdiv(a.group, 16);
   a.dh = static_cast<int32_t>(c.head_dim);
   a.row_bytes = static_cast<int32_t>(c.row * paged_es(c));
-  // a pool without pages has no row 0, a table without entries no tokens
-  a.most = static_cast<int32_t>(c.pages && c.table_len ? p.max_length : 0);
+  // the bound of plan_of's count too; a pool without pages has no row 0, a table without entries no tokens
+  a.most = static_cast<int32_t>(paged_most(c, p.max_length));
   a.scale = p.scale * kLog2e;
   a.qvec = c.head_dim * es % 16 == 0 && aligned(p.q, 16) && ubytes(p.q_stride_n, es) % 16 == 0 &&
            ubytes(p.q_stride_b, es) % 16 == 0 && ubytes(p.q_stride_h, es) % 16 == 0;

@@ -1,6 +1,8 @@
 // What the kernels over a paged key-value cache share: its addressing and the host checks of its description.
 #pragma once
 
+#include <algorithm>
+
 #include "wc_common.h"
 #include "wc_serve_abi.h"
 
@@ -43,6 +45,28 @@ inline PagedTable paged_table(const wc_paged_cache& c, const int32_t* instead) {
   t.err = c.err_flag;
   t.by_page = make_fastdiv(static_cast<uint32_t>(c.page_size));
   return t;
+}
+
+// What attention walks: a sequence's tokens [lo, hi) in tiles of kPagedTile, counted from the one that holds token lo.
+constexpr int kPagedTile = 32;
+struct PagedSpan {
+  int32_t lo, hi;
+  bool cut;                  // the length was beyond most
+};
+__host__ __device__ inline PagedSpan paged_span(int32_t first, int32_t length, int32_t most) {
+  return PagedSpan{first > 0 ? first : 0, length < most ? length : most, length > most};
+}
+__host__ __device__ inline int32_t paged_tiles(const PagedSpan& s) {
+  return s.hi > s.lo ? (s.hi - (s.lo & ~(kPagedTile - 1)) + kPagedTile - 1) / kPagedTile : 0;
+}
+// The tokens that a sequence has at most, whatever its length says: those its table can name and max_length allows, which
+// is under 2^31 - 64; none of a pool without pages.
+inline int64_t paged_most(const wc_paged_cache& c, int64_t max_length) {
+  return c.pages ? std::min(max_length, c.table_len * c.page_size) : 0;
+}
+// Whether the tiles of all sequences, and a share's end behind the last of them, can be counted in 32 bits
+inline bool paged_countable(int64_t seqs, int64_t most) {
+  return mul_sat({seqs, (most + kPagedTile - 1) / kPagedTile}) < (1ll << 30);
 }
 
 // Bytes of a stored element

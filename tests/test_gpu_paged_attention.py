@@ -399,3 +399,21 @@ def test_attend_lengths_out_of_range_of_sequences_without_a_tile():
             cut = lens.clamp(max=most)
             assert torch.equal(got, cache.attend(q, table, cut, first=first, max_length=most))
             cache.index_error()
+
+
+@pytest.mark.parametrize("n,b,blocks", [(1, 3, 100), (8, 8, 70), (4, 512, 70)])
+def test_attend_lengths_far_beyond_the_table(n, b, blocks):
+    """Lengths that say anything, under a max_length far over what the tables name: every sequence has the tokens of its
+    table, and the flag is raised; in parts, and of so many sequences that they stay whole."""
+    page, d = 16, 32
+    full = [blocks * page] + [0] * (n * b - 1)
+    cache, q, k, v, table, lens = _setup(n, b, 1, 1, d, page, full, torch.bfloat16, False, blocks)
+    table[:] = table[0, 0]                                  # all of them over the same pages
+    lens[:] = blocks * page
+    expect = cache.attend(q, table, lens)
+    cache.index_error()
+    for length in (2 ** 31 - 1, 2 ** 31 - 65, blocks * page + 1):
+        got = cache.attend(q, table, torch.full_like(lens, length), max_length=2 ** 31 - 65)
+        with pytest.raises(IndexError):
+            cache.index_error()
+        within(got, expect.double(), 2 * HALF[q.dtype], attend_slack(q.dtype, 32.0, d, blocks * page, 4.5))

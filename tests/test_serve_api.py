@@ -5,6 +5,7 @@ import ctypes
 import hashlib
 import os
 import re
+import shutil
 import subprocess
 import sys
 
@@ -290,3 +291,65 @@ def test_serve_host_side_clean_under_sanitizers():
     assert r.returncode == 0, r.stderr[-6000:]
     assert "runtime error" not in r.stderr and "AddressSanitizer" not in r.stderr, r.stderr[-6000:]
     assert "no sanitizer report" in r.stdout
+
+
+COUNT = r"""
+#include <cstdio>
+#include <cstdlib>
+
+#include "wc_paged.h"
+
+// What the attention kernel counts in 32 bits (the tiles of all sequences, a share's end), here in 64 beside it, for lengths
+// that say anything: none may differ, and a share's parts are at most the shares.
+int main() {
+  using namespace wc;
+  srand(20261206);
+  const int64_t extreme = (1ll << 31) - 65, budgets[] = {1, 7, 256, 768, 1024};
+  const int32_t garbage[] = {2147483647, 2147483583, 2147483640, 1 << 30, -1, 1025, 0, 100, 1048577};
+  int cut = 0, counted = 0;
+  for (int it = 0; it < 20000; ++it) {
+    wc_paged_cache c = {};
+    c.pages = rand() % 8 ? 4 : 0;
+    c.page_size = 1ll << rand() % 25;
+    c.table_len = rand() % 3 ? rand() % 4096 : extreme;
+    const int64_t seqs = 1 + rand() % (rand() % 2 ? 2047 : 40), budget = budgets[rand() % 5];
+    const int64_t max_length = rand() % 3 ? extreme : rand() % 4096, most = paged_most(c, max_length);
+    if (most > max_length || most > c.table_len * c.page_size || (!c.pages && most)) return 1;
+    if (!paged_countable(seqs, most)) continue;
+    int64_t total = 0;
+    uint32_t total32 = 0;                                  // as the kernel adds, without undefined overflow here
+    for (int64_t s = 0; s < seqs; ++s) {
+      const int32_t length = garbage[rand() % 9], first = rand() % 2 ? 0 : garbage[rand() % 9];
+      const PagedSpan span = paged_span(first, length, static_cast<int32_t>(most));
+      if (span.hi > most || span.lo < 0 || span.cut != (length > most)) return 2;
+      const int64_t lo = span.lo / 32 * 32, want = span.hi > span.lo ? (span.hi - lo + 31) / 32 : 0;
+      if (paged_tiles(span) != want) return 3;
+      cut += span.cut;
+      total += want;
+      total32 += static_cast<uint32_t>(paged_tiles(span));
+    }
+    const int64_t size = std::max<int64_t>((total + budget - 1) / budget, 8);
+    if (total != static_cast<int32_t>(total32) || (budget - 1) * size + size > 2147483647ll + 8 * 1024 || total + size > 2147483647ll) return 4;
+    if (total && (total - 1) / size + 1 > budget) return 5;
+    ++counted;
+  }
+  printf("%d counted, %d cut\n", counted, cut);
+  return counted > 1000 && cut > 1000 ? 0 : 6;
+}
+"""
+
+
+def test_attention_counts_tiles_within_32_bits(tmp_path):
+    """The bound of a sequence's tokens is the one that the count of all tiles is checked with: neither lengths that say
+    anything nor a max_length far over what the tables name take the line of tiles, its shares or a join's parts out of
+    their range."""
+    hipcc = next((h for h in ("/opt/rocm/bin/hipcc", "hipcc") if shutil.which(h)), None)
+    if hipcc is None:
+        pytest.skip("no hipcc")
+    src, exe = tmp_path / "count.cpp", tmp_path / "count"
+    src.write_text(COUNT)
+    r = subprocess.run([hipcc, "-x", "hip", "--offload-host-only", "-std=c++17", "-O1", "-w", "-I", os.path.join(PKG, "csrc"), "-I",
+                        os.path.join(ROOT, "include"), str(src), "-o", str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-4000:]
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, (r.returncode, r.stdout)
