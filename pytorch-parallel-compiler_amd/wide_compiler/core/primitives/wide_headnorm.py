@@ -109,8 +109,8 @@ class WideHeadNormRotary(nn.Module):
         if len(t.normalized_shape) != 1:
             raise ValueError("WideHeadNormRotary supports a single normalized dimension")
         w = t.weight
-        # nn.RMSNorm's eps None: the dtype's epsilon
-        eps = t.eps if t.eps is not None else torch.finfo(torch.float32 if w is None else w.dtype).eps
+        # nn.RMSNorm's eps None is fp32's epsilon in 16 bits too: what it computes in
+        eps = t.eps if t.eps is not None else torch.finfo(torch.float32).eps
         wide = cls(len(q_norms), t.normalized_shape[0], rotary_dim=rotary_dim, base=base, eps=eps,
                    interleaved=interleaved)
         if w is not None:

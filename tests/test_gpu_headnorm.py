@@ -160,3 +160,22 @@ def test_head_norm_empty_and_graph():
             a, c = mod(q, k, pos)
             torch.cuda.synchronize()
             assert torch.equal(a, qo) and torch.equal(c, ko)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_head_norm_from_modules_of_default_eps(dtype):
+    """nn.RMSNorm without an eps, on rows as small as its default; torch rounds the norm and the product with the weight
+    apart, two half steps more."""
+    import wide_compiler as wc
+    norms = [torch.nn.RMSNorm(64).to(DEV, dtype) for _ in range(2)]
+    for m in norms:
+        torch.nn.init.normal_(m.weight, 1.0, 0.2)
+    mod = wc.WideHeadNormRotary.from_modules(norms, norms, rotary_dim=0)
+    pos = torch.zeros(1, dtype=torch.int64, device=DEV)
+    for size in (1.0, 1e-2, 1e-3):
+        q = (size * torch.randn(2, 2, 5, 4, 64, generator=gen(9))).to(DEV, dtype)
+        with torch.no_grad():
+            qo, _ = mod(q, q, pos)
+            _check(qo, q, mod.q_weight, torch.zeros(2, 2, 5, device=DEV), 0, 1.0, 2.0 ** -23, False)
+            for i in range(2):
+                within(qo[i], norms[i](q[i]).double(), 4 * HALF[dtype] + 72 * 2.0 ** -24, 0.0)

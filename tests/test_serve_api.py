@@ -353,3 +353,19 @@ def test_attention_counts_tiles_within_32_bits(tmp_path):
     assert r.returncode == 0, r.stderr[-4000:]
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, (r.returncode, r.stdout)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("eps", [None, 1e-5])
+def test_head_norm_from_modules_has_the_eps_that_rms_norm_uses(eps, dtype):
+    """Rows as small as eps: what nn.RMSNorm gives (up to its roundings of the norm, the weight's product and the sum:
+    4 steps) is the formula with the converted module's eps."""
+    import wide_compiler as wc
+    norm = torch.nn.RMSNorm(96, eps=eps).to(dtype)
+    mod = wc.WideHeadNormRotary.from_modules([norm], [norm])
+    for size in (1.0, 1e-2, 1e-3):
+        x = (size * torch.randn(50, 96, generator=gen(3))).to(dtype)
+        ref = x.double() / (x.double().square().mean(-1, keepdim=True) + mod.eps).sqrt()
+        step = torch.finfo(dtype).eps
+        with torch.no_grad():
+            assert ((norm(x).double() - ref).abs() <= 4 * step * ref.abs() + 4 * torch.finfo(dtype).tiny * step + 100 * 2.0 ** -24 * ref.abs()).all()
