@@ -108,7 +108,10 @@ class WideHeadNormRotary(nn.Module):
             raise ValueError("WideHeadNormRotary.from_modules needs as many q norms as k norms, of one shape and eps")
         if len(t.normalized_shape) != 1:
             raise ValueError("WideHeadNormRotary supports a single normalized dimension")
-        w = t.weight
+        weights = [m.weight for m in (*q_norms, *k_norms) if m.weight is not None]
+        w = weights[0] if weights else None
+        if any(x.dtype != w.dtype or x.device != w.device for x in weights):
+            raise ValueError("WideHeadNormRotary.from_modules needs norms of one dtype on one device")
         # nn.RMSNorm's eps None is fp32's epsilon in 16 bits too: what it computes in
         eps = t.eps if t.eps is not None else torch.finfo(torch.float32).eps
         wide = cls(len(q_norms), t.normalized_shape[0], rotary_dim=rotary_dim, base=base, eps=eps,

@@ -369,3 +369,16 @@ def test_head_norm_from_modules_has_the_eps_that_rms_norm_uses(eps, dtype):
         step = torch.finfo(dtype).eps
         with torch.no_grad():
             assert ((norm(x).double() - ref).abs() <= 4 * step * ref.abs() + 4 * torch.finfo(dtype).tiny * step + 100 * 2.0 ** -24 * ref.abs()).all()
+
+
+def test_head_norm_from_modules_of_norms_with_and_without_weights():
+    """The type is that of the weights there are, wherever they stand; norms of several types are refused."""
+    import wide_compiler as wc
+    plain, own = torch.nn.RMSNorm(32, elementwise_affine=False), torch.nn.RMSNorm(32, dtype=torch.bfloat16)
+    torch.nn.init.normal_(own.weight)
+    mod = wc.WideHeadNormRotary.from_modules([plain, plain], [own, plain])
+    assert mod.k_weight.dtype == mod.q_weight.dtype == torch.bfloat16
+    assert torch.equal(mod.k_weight[0], own.weight) and (mod.k_weight[1] == 1).all() and (mod.q_weight == 1).all()
+    assert wc.WideHeadNormRotary.from_modules([plain], [plain]).q_weight.dtype == torch.float32
+    with pytest.raises(ValueError, match="one dtype"):
+        wc.WideHeadNormRotary.from_modules([own], [torch.nn.RMSNorm(32)])
