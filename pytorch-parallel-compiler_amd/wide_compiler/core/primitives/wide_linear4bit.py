@@ -149,7 +149,11 @@ class WideLinear4bit(nn.Module):
             w = torch.stack([m.weight for m in modules]).float()
             pad = torch.nn.functional.pad(w, (0, groups * group_size - i)).view(n, o, groups, group_size)
             lo, hi = pad.amin(-1).clamp_max(0), pad.amax(-1).clamp_min(0)
-            scales = ((hi - lo) / 15).clamp_min(torch.finfo(t.weight.dtype).tiny).to(t.weight.dtype)
+            # a step, under the type's normal values rounded up (to the nearest it may be half as large, or 0); 1 of zeros
+            step, info = hi.double() / 15 - lo.double() / 15, torch.finfo(t.weight.dtype)
+            least = info.tiny * info.eps
+            step = torch.where(step < info.tiny, torch.ceil(step / least) * least, step)
+            scales = torch.where(step == 0, 1.0, step).to(t.weight.dtype)
             s = scales.float()
             zeros = torch.round(-lo / s).clamp(0, 15)
             codes = (torch.round(pad / s[..., None]) + zeros[..., None]).clamp(0, 15)

@@ -147,3 +147,22 @@ def test_linear4_state_dict_and_graph():
         eager = mod(x)
         torch.cuda.synchronize()
         assert torch.equal(out, eager)
+
+
+@pytest.mark.parametrize("m", [1, 20, 70])
+@pytest.mark.parametrize("dtype,size", [(torch.float16, 3e-4), (torch.float16, 2e-6), (torch.bfloat16, 1e-36), (torch.float32, 1e-36)])
+def test_linear4_small_weights(m, dtype, size):
+    """Scales under the type's normal values (fp16) and next to them count as they are."""
+    import wide_compiler as wc
+    torch.manual_seed(7)
+    lin = [torch.nn.Linear(200, 50, bias=False).to(DEV, dtype) for _ in range(2)]
+    for layer in lin:
+        torch.nn.init.uniform_(layer.weight, -size, size)
+    mod = wc.WideLinear4bit.from_modules(lin, group_size=32)
+    w = mod.dequantize().double()
+    assert (w.abs().amax() >= size / 2).item()
+    x = (8 * torch.randn(2, m, 200, generator=gen(17))).to(DEV, dtype)
+    with torch.no_grad():
+        y = mod(x)
+    extra = 160 if dtype == torch.bfloat16 else 30          # codes, zero points and (bf16) 128, times the scale
+    _check(y, x, w, w.abs() + extra * mod.scales.amax().double(), None)

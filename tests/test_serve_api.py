@@ -382,3 +382,29 @@ def test_head_norm_from_modules_of_norms_with_and_without_weights():
     assert wc.WideHeadNormRotary.from_modules([plain], [plain]).q_weight.dtype == torch.float32
     with pytest.raises(ValueError, match="one dtype"):
         wc.WideHeadNormRotary.from_modules([own], [torch.nn.RMSNorm(32)])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("size", [1.0, 1e-3, 3e-4, 3e-5, 1e-6, 6e-8, 2e-38, 0.0])
+@pytest.mark.parametrize("group", [32, 128])
+def test_linear4_from_modules_spans_small_weights(group, size, dtype):
+    """Codes span a group's values at any size that the type has: a value is off by half of the stored scale s, or, at the
+    upper end, by s / 2 and what s is under (max - min) / 15 (at most half a rounding step of it, 15 times); s is at most
+    that step's rounding, or up to the type's smallest value more."""
+    import wide_compiler as wc
+    torch.manual_seed(5)
+    lin = [torch.nn.Linear(150, 40, bias=False).to(dtype) for _ in range(2)]
+    for m in lin:
+        torch.nn.init.uniform_(m.weight, -size, size)
+        m.weight.data[3] = m.weight.data[3].abs()             # a row of one sign
+        m.weight.data[4] = 0
+    mod = wc.WideLinear4bit.from_modules(lin, group_size=group)
+    groups = -(-150 // group)
+    w = torch.stack([m.weight for m in lin]).detach().double()
+    pad = torch.nn.functional.pad(w, (0, groups * group - 150)).unflatten(-1, (groups, group))
+    step = (pad.amax(-1).clamp_min(0) - pad.amin(-1).clamp_max(0)) / 15
+    s = mod.scales.transpose(2, 3).reshape(2, -1, mod.scales.shape[2])[:, :40, :groups].double()
+    info = torch.finfo(dtype)
+    off = (torch.nn.functional.pad(mod.dequantize().double() - w, (0, groups * group - 150))).unflatten(-1, pad.shape[2:]).abs().amax(-1)
+    assert (off <= s * (0.5 + 8 * info.eps + 1e-5)).where(step > 0, off == 0).all()
+    assert (s <= step * (1 + info.eps) + info.tiny * info.eps).where(step > 0, s > 0).all()
