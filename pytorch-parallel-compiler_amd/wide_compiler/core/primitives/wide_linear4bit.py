@@ -142,6 +142,11 @@ class WideLinear4bit(nn.Module):
     def from_modules(cls, modules: List[nn.Linear], group_size: int = 128) -> "WideLinear4bit":
         """Quantises N nn.Linear: each group's codes span its values and zero, code = round(w / scale) + zero."""
         t = modules[0]
+        form = lambda m: (tuple(m.weight.shape), m.weight.dtype, m.weight.device,  # noqa: E731
+                          None if m.bias is None else (m.bias.dtype, m.bias.device))
+        if any(form(m) != form(t) for m in modules):
+            raise ValueError("WideLinear4bit.from_modules needs modules of one shape, dtype and device, all with a bias or all "
+                             "without")
         n, o, i = len(modules), t.out_features, t.in_features
         wide = cls(n, i, o, group_size, bias=t.bias is not None, dtype=t.weight.dtype).to(t.weight.device)
         groups = -(-i // group_size)

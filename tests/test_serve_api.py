@@ -408,3 +408,13 @@ def test_linear4_from_modules_spans_small_weights(group, size, dtype):
     off = (torch.nn.functional.pad(mod.dequantize().double() - w, (0, groups * group - 150))).unflatten(-1, pad.shape[2:]).abs().amax(-1)
     assert (off <= s * (0.5 + 8 * info.eps + 1e-5)).where(step > 0, off == 0).all()
     assert (s <= step * (1 + info.eps) + info.tiny * info.eps).where(step > 0, s > 0).all()
+
+
+def test_linear4_from_modules_of_several_kinds_are_refused():
+    """A bias would be lost, a type rounded, where only the first module were looked at."""
+    import wide_compiler as wc
+    lin = torch.nn.Linear
+    for a, b in ((lin(64, 16, bias=False), lin(64, 16)), (lin(64, 16), lin(64, 16, bias=False)), (lin(64, 16), lin(64, 17)),
+                 (lin(64, 16), lin(32, 16)), (lin(64, 16).half(), lin(64, 16))):
+        with pytest.raises(ValueError, match="one shape, dtype and device"):
+            wc.WideLinear4bit.from_modules([a, b], group_size=32)
