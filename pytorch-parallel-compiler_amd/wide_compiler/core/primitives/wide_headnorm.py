@@ -38,10 +38,8 @@ class WideHeadNormRotary(nn.Module):
             raise ValueError(f"WideHeadNormRotary: rotary_dim must be even and within [0, {head_dim}], got {rotary_dim}")
         self.n = n
         self.head_dim = head_dim
-        self.rotary_dim = rotary_dim
-        self.base = base
+        self._rotation = (rotary_dim, base, interleaved)
         self.eps = eps
-        self.interleaved = interleaved
         self.q_weight = nn.Parameter(torch.ones(n, head_dim))
         self.k_weight = nn.Parameter(torch.ones(n, head_dim))
         freq = torch.tensor([base ** (-2.0 * p / rotary_dim) / (2.0 * math.pi) for p in range(rotary_dim // 2)],
@@ -49,6 +47,19 @@ class WideHeadNormRotary(nn.Module):
         # turns per position, as the bits of fp64: .to(dtype) leaves integer buffers as they are
         self.register_buffer("_freq_bits", freq.view(torch.int64), persistent=False)
         self._plans = _serve.Plans()
+
+    # What turns the heads is a module's for good: its frequencies and its plans are made of it.
+    @property
+    def rotary_dim(self) -> int:
+        return self._rotation[0]
+
+    @property
+    def base(self) -> float:
+        return self._rotation[1]
+
+    @property
+    def interleaved(self) -> bool:
+        return self._rotation[2]
 
     def forward(self, q: Tensor, k: Tensor, positions: Tensor) -> Tuple[Tensor, Tensor]:
         if torch.compiler.is_compiling():

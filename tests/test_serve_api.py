@@ -418,3 +418,22 @@ def test_linear4_from_modules_of_several_kinds_are_refused():
                  (lin(64, 16), lin(32, 16)), (lin(64, 16).half(), lin(64, 16))):
         with pytest.raises(ValueError, match="one shape, dtype and device"):
             wc.WideLinear4bit.from_modules([a, b], group_size=32)
+
+
+def test_head_norm_rotation_is_fixed(monkeypatch, anywhere):
+    """A call's plan and the frequencies are made from the rotation's numbers: they cannot be set apart from them.  eps,
+    which every call reads, can."""
+    import wide_compiler as wc
+    from wide_compiler import _serve
+    mod = wc.WideHeadNormRotary(1, 64, rotary_dim=32, base=500.0, interleaved=True).requires_grad_(False)
+    assert (mod.rotary_dim, mod.base, mod.interleaved) == (32, 500.0, True)
+    for name, value in (("rotary_dim", 64), ("base", 10000.0), ("interleaved", False)):
+        with pytest.raises(AttributeError):
+            setattr(mod, name, value)
+    seen = []
+    monkeypatch.setattr(_serve, "head_norm_rotary", lambda plan, *a: seen.append((plan[0][2], plan[0][9], a[-1])))
+    q, pos = torch.zeros(1, 1, 2, 3, 64), torch.zeros(2, dtype=torch.int64)
+    mod(q, q, pos)
+    mod.eps = 1e-3
+    mod(q, q, pos)
+    assert seen == [(1, 32, 1e-6), (1, 32, 1e-3)]
