@@ -431,7 +431,7 @@ def test_head_norm_rotation_is_fixed(monkeypatch, anywhere):
         with pytest.raises(AttributeError):
             setattr(mod, name, value)
     seen = []
-    monkeypatch.setattr(_serve, "head_norm_rotary", lambda plan, *a: seen.append((plan[0][2], plan[0][9], a[-1])))
+    monkeypatch.setattr(_serve, "head_norm_rotary", lambda plan, *a: seen.append((plan[0][2], plan[0][10], a[-1])))
     q, pos = torch.zeros(1, 1, 2, 3, 64), torch.zeros(2, dtype=torch.int64)
     mod(q, q, pos)
     mod.eps = 1e-3
