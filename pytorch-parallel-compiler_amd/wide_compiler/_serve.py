@@ -195,9 +195,11 @@ def linear4(sizes: Tuple, rows, x: Tensor, codes: Tensor, scales: Tensor, zeros:
         0 if bias is None else bias.data_ptr(), y.data_ptr()), x)
 
 
-
 @torch.compiler.disable
 def uncompiled(call, *args):
     """call(*args) outside a region that torch.compile traces: what the modules' and the cache's calls do there, whose
-    plans and launches are nothing to trace.  A check of is_compiling() costs a call less than the decorator does."""
+    plans and launches are nothing to trace.  A check of is_compiling() costs a call less than the decorator does.  An
+    export has no outside: it would come back here for ever."""
+    if torch.compiler.is_compiling():
+        raise RuntimeError(f"{getattr(call, '__qualname__', call)}: a kernel's launch cannot be exported")
     return call(*args)

@@ -437,3 +437,26 @@ def test_head_norm_rotation_is_fixed(monkeypatch, anywhere):
     mod.eps = 1e-3
     mod(q, q, pos)
     assert seen == [(1, 32, 1e-6), (1, 32, 1e-3)]
+
+
+def test_exports_are_refused(anywhere):
+    """torch.export traces through what torch.compile steps out of: an error that says so, not a recursion."""
+    import wide_compiler as wc
+    pages = torch.zeros(5, 2, 16, 64)
+    cache = wc.WidePagedCache.from_pages(pages, pages)
+    table, n = torch.zeros(1, 3, 4, dtype=torch.int32), torch.zeros(1, 3, dtype=torch.int32)
+    k, q = torch.zeros(1, 3, 7, 2, 64), torch.zeros(1, 3, 4, 64)
+
+    class Calls(torch.nn.Module):
+        def __init__(self, f):
+            super().__init__()
+            self.f = f
+
+        def forward(self, x):
+            return self.f(x)
+    norm = wc.WideHeadNormRotary(1, 64).requires_grad_(False)
+    for f, x in ((wc.WideLinear4bit(1, 64, 16), torch.zeros(1, 2, 64)), (lambda x: norm(x, x, n[0, 0]), k),
+                 (lambda x: cache.attend(x, table, n), q), (lambda x: cache.write(x, x, table, n), k),
+                 (lambda x: cache.read(table, n, 4), k)):
+        with torch.no_grad(), pytest.raises(RuntimeError, match="cannot be exported"):
+            torch.export.export(Calls(f), (x,), strict=False)
