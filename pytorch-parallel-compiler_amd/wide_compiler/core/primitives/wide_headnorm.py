@@ -65,7 +65,10 @@ class WideHeadNormRotary(nn.Module):
         if torch.compiler.is_compiling():
             return _serve.uncompiled(self.forward, q, k, positions)
         params = self._parameters
-        qw, kw, freq = params["q_weight"], params["k_weight"], self._buffers["_freq_bits"]
+        try:
+            qw, kw, freq = params["q_weight"], params["k_weight"], self._buffers["_freq_bits"]
+        except KeyError:                                     # a parametrised weight is no parameter of the module's own
+            qw, kw, freq = self.q_weight, self.k_weight, self._freq_bits
         form = (q.shape, q.stride(), q.dtype, q.get_device(), k.shape, k.stride(), k.dtype, k.get_device(), positions.shape,
                 positions.stride(), positions.dtype, positions.get_device(), qw.shape, qw.dtype, qw.get_device(), kw.shape,
                 kw.dtype, kw.get_device())

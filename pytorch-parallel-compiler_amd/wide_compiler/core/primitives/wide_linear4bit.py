@@ -56,7 +56,10 @@ class WideLinear4bit(nn.Module):
         if torch.compiler.is_compiling():
             return _serve.uncompiled(self.forward, x)
         bufs = self._buffers
-        packed, scales, zeros, bias = bufs["packed"], bufs["scales"], bufs["zeros"], bufs["bias"]
+        try:
+            packed, scales, zeros, bias = bufs["packed"], bufs["scales"], bufs["zeros"], bufs["bias"]
+        except KeyError:                                     # one that was parametrised, or became something else
+            packed, scales, zeros, bias = self.packed, self.scales, self.zeros, self.bias
         form = (x.shape, x.stride(), x.dtype, x.get_device(), packed.shape, packed.dtype, packed.get_device(), scales.shape,
                 scales.dtype, scales.get_device(), zeros.shape, zeros.dtype, zeros.get_device(),
                 None if bias is None else (bias.shape, bias.dtype, bias.get_device()))
@@ -64,7 +67,7 @@ class WideLinear4bit(nn.Module):
         if plan is None:
             plan = self._plan(form, x, packed, scales, zeros, bias)
         if torch.is_grad_enabled():
-            _hip.require_forward_only("WideLinear4bit", x)
+            _hip.require_forward_only("WideLinear4bit", x, scales, bias)
         dense, rows, sizes, shape = plan
         if not dense:
             x = x.contiguous()

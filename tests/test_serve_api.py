@@ -460,3 +460,32 @@ def test_exports_are_refused(anywhere):
                  (lambda x: cache.read(table, n, 4), k)):
         with torch.no_grad(), pytest.raises(RuntimeError, match="cannot be exported"):
             torch.export.export(Calls(f), (x,), strict=False)
+
+
+def test_parametrised_weights_count(monkeypatch, anywhere):
+    """A weight or scale that torch parametrises, or a bias that became a parameter, is read as any other module reads it."""
+    import wide_compiler as wc
+    from torch.nn.utils import parametrize
+    from wide_compiler import _serve
+
+    class Twice(torch.nn.Module):
+        def forward(self, w):
+            return 2 * w
+    seen = []
+    monkeypatch.setattr(_serve, "head_norm_rotary", lambda plan, q, k, qo, ko, qw, kw, *a: seen.append((qw, kw)))
+    monkeypatch.setattr(_serve, "linear4", lambda sizes, rows, x, codes, scales, zeros, bias, y: seen.append((scales, bias)))
+    norm = wc.WideHeadNormRotary(1, 64)
+    parametrize.register_parametrization(norm, "k_weight", Twice())
+    lin = wc.WideLinear4bit(1, 64, 16, group_size=64)
+    lin.scales.fill_(1)
+    parametrize.register_parametrization(lin, "scales", Twice())
+    del lin.bias
+    lin.bias = torch.nn.Parameter(torch.ones(1, 16))
+    q = torch.zeros(1, 1, 2, 3, 64)
+    with torch.no_grad():
+        norm(q, q, torch.zeros(2, dtype=torch.int64))
+        lin(torch.zeros(1, 2, 64))
+    (qw, kw), (scales, bias) = seen
+    assert (qw == 1).all() and (kw == 2).all() and (scales == 2).all() and (bias == 1).all()
+    with pytest.raises(RuntimeError, match="forward-only"):
+        lin(torch.zeros(1, 2, 64))                          # its bias asks for a gradient
