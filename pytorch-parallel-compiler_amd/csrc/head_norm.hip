@@ -123,6 +123,8 @@ __global__ __launch_bounds__(kThreads) void head_norm_kernel(HeadNorm a) {
   }
   __syncthreads();
 
+  // columns that aren't turned are left alone by their neighbours, whatever those hold
+  const bool some_rest = a.rot < a.dh;
   for (int r0 = group; r0 < rows; r0 += kUnroll * groups) {
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -164,7 +166,8 @@ __global__ __launch_bounds__(kThreads) void head_norm_kernel(HeadNorm a) {
           // interleaved: pair e is values 2e and 2e + 1 of the 2V
           const float s = INTER ? y[(2 * e) / V][(2 * e) % V] : y[0][e];
           const float t = INTER ? y[(2 * e + 1) / V][(2 * e + 1) % V] : y[1][e];
-          const float s2 = s * cs[e].x - t * cs[e].y, t2 = t * cs[e].x + s * cs[e].y;
+          float s2 = s * cs[e].x - t * cs[e].y, t2 = t * cs[e].x + s * cs[e].y;
+          if (some_rest && p + e >= (a.rot >> 1)) s2 = s, t2 = t;
           if (INTER) {
             ((2 * e) / V ? o1 : o0).v[(2 * e) % V] = from_f32<T>(s2);
             ((2 * e + 1) / V ? o1 : o0).v[(2 * e + 1) % V] = from_f32<T>(t2);

@@ -179,3 +179,27 @@ def test_head_norm_from_modules_of_default_eps(dtype):
             _check(qo, q, mod.q_weight, torch.zeros(2, 2, 5, device=DEV), 0, 1.0, 2.0 ** -23, False)
             for i in range(2):
                 within(qo[i], norms[i](q[i]).double(), 4 * HALF[dtype] + 72 * 2.0 ** -24, 0.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("d,rot", [(64, 0), (64, 32), (80, 12), (18, 6)])
+def test_head_norm_columns_that_are_not_turned_stand_alone(d, rot, inter, dtype):
+    """What isn't finite in a column from rotary_dim on shows there alone: a row with an infinity is NaN in that column and
+    zero in the others that aren't turned, a weight that is infinite makes its own column infinite."""
+    mod = _module(1, d, rot, 10000.0, inter, dtype, 11)
+    q = torch.randn(1, 1, d, 3, d, generator=gen(12)).to(DEV, dtype)
+    pos = torch.arange(d, device=DEV)
+    rest = [c for c in range(rot, d)]
+    for c in rest:
+        q[0, 0, c, 1, c] = float("inf")
+    with torch.no_grad():
+        qo, _ = mod(q, q, pos)
+        ref, _ = _ref(q, mod.q_weight, pos.expand(1, 1, d), rot, 10000.0, 1e-6, inter)
+        for c in rest:
+            assert torch.isnan(qo[0, 0, c, 1, c])
+            assert (qo[0, 0, c, 1, [x for x in rest if x != c]] == 0).all()
+        assert torch.equal(torch.isnan(qo), torch.isnan(ref))
+        mod.k_weight[0, d - 1] = float("inf")
+        _, ko = mod(q[:, :, :, :1], q[:, :, :, :1], pos)
+    assert torch.isinf(ko[..., d - 1]).all() and torch.isfinite(ko[..., :d - 1]).all()
