@@ -203,3 +203,28 @@ def test_head_norm_columns_that_are_not_turned_stand_alone(d, rot, inter, dtype)
         mod.k_weight[0, d - 1] = float("inf")
         _, ko = mod(q[:, :, :, :1], q[:, :, :, :1], pos)
     assert torch.isinf(ko[..., d - 1]).all() and torch.isfinite(ko[..., :d - 1]).all()
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_head_norm_turns_by_the_whole_angle(inter):
+    """Rows whose norm is exact (a quarter of their columns 2, the others 0) come out as 2 cos and 2 sin of the angle.  Two
+    roundings each, the function's and its correction's: an independent one has a variance of u^2 / 12 for the unit u of the
+    last place, which over all angles is 0.716 2^-48 / 12 on average, and a function that is off by up to a unit has
+    0.16 u^2 at most.  Root mean square of the pair: sqrt(2 0.716 (0.16 + 1 / 12)) 2^-24 = 0.59 2^-24; an angle rounded
+    to fp32 adds 0.7 2^-24, 0.9 in all.  The bar is 0.65."""
+    n, b, t, h, d = 1, 4, 512, 8, 128
+    import wide_compiler as wc
+    mod = wc.WideHeadNormRotary(n, d, base=500.0, eps=0.0, interleaved=inter).to(DEV)
+    pairs = torch.rand(n, b, t, h, d // 2, generator=gen(13)).argsort(-1) < d // 4    # half of the pairs
+    q = torch.zeros(n, b, t, h, d)
+    if inter:
+        q[..., 0::2] = 2.0 * pairs
+    else:
+        q[..., :d // 2] = 2.0 * pairs
+    pos = torch.randint(0, 100000, (n, b, t), generator=gen(14))
+    with torch.no_grad():
+        qo, _ = mod(q.to(DEV), q[..., :0, :].to(DEV), pos.to(DEV))
+    assert torch.equal(q.square().mean(-1), torch.ones(n, b, t, h))
+    ref, _ = _ref(q, torch.ones(n, d), pos, d, 500.0, 0.0, inter)
+    off = ((qo.cpu().double() - ref).square().sum(-1) / (2 * 2 * pairs.sum(-1))).mean().sqrt().item()
+    assert off <= 0.65 * 2.0 ** -24, off / 2.0 ** -24
