@@ -137,7 +137,7 @@ int32_t wc_paged_attention(const wc_paged_attn_args* args, void* stream);
  *   codes   [n, row tiles, column tiles, 64, 4] 32-bit words; word q of lane l holds row l % 16 and columns
  *           32 q + 8 (l / 16) + e of the tile, e = 0..7 in nibbles 0, 4, 1, 5, 2, 6, 3, 7
  *   scales  [n, row tiles, column tiles * 128 / group, 16] of `dtype`
- *   zeros   the same of uint8
+ *   zeros   the same of uint8, each at most 127
  */
 typedef struct wc_linear4_args {
   int32_t dtype;                  /* of x, scales, bias and y */

@@ -4,14 +4,16 @@
 // 2 flops a row.  So the weights are read once, as whole kilobytes per wave (a tile of 16 output rows x 128 columns
 // is laid out in the order in which the lanes want it), and all rows of x meet them there, 16 to an MFMA tile.
 //
-//   y = sum_g scale_g (sum_k code x - zero_g sum_k x)
+//   y = sum_g scale_g sum_k (code - zero_g) x
 //
-// The codes enter the product without their scale, as whole numbers in 16 bits, and the scale multiplies the fp32 sum
-// of each group.  A nibble becomes a number by the bits above it: 0x4300 | code is 128 + code in bf16, 0x6400 | code
-// is 1024 + code in fp16, two to an instruction.  fp16 then takes 1024 + zero off (exact); bf16 has no packed
-// subtraction, so there the sum of x, by one more product with ones, takes (128 + zero) sum_k x off, whose
-// rounding in fp32 is 2^-24 of 128 |sum x|.  fp32 goes as three bf16 planes of x (every bit of it down to 2^-110)
-// against codes converted to bf16, without the 128.  A row of x with an infinity or NaN gives NaN in bf16 and fp32.
+// A code less its zero point is a whole number that bf16 and fp16 hold, so what enters the product is exact, a weight of 0
+// takes no part however large x is there, and the scale multiplies the fp32 sum of each group.  fp16: 0x6400 | code is
+// 1024 + code, two to an instruction, and 1024 + zero is taken off two at a time.  bf16 has no packed subtraction: four
+// codes a register lose their zero points as bytes, and each becomes a float and one half of a bf16 pair.  (Numbers
+// 128 + code, with 128 + zero times the sum of x taken off afterwards, are half the instructions for the codes, but as many
+// more for those sums: 4 models' [4096 -> 4096], one row, 11.8 us against 12.6, 8 models' [2048 -> 8192], 64 rows, 47 against
+// 42, weights from memory; and they lose 2^-24 of 143 sum |x|, also where weights are 0, and overflow from x of 2^114 on.)
+// fp32 goes as three bf16 planes of x (every bit of it down to 2^-110); a row of x with an infinity gives NaN there.
 //
 // 4 models' [4096 -> 4096] in bf16, one row (35 MB): 10.4 us, of which an empty launch is 3.3; 8 models' [2048 -> 8192]
 // in fp16, 64 rows (84 MB, 17 GFLOP): 30 us, half of it the instructions that make numbers of codes and scale the
@@ -41,29 +43,43 @@ struct alignas(4 * sizeof(T)) Four {
   T v[4];
 };
 
-// 8 codes as 16-bit numbers with 128 (bf16) or 1024 (fp16) added, or exact bf16 (fp32); `over` holds the bits above a
-// nibble in a register, so that mask and bits are one instruction
+// 8 codes of a word less their zero point, as bf16 (fp32 too) or fp16.  `zero`: the zero point in each byte (bf16) or 1024
+// and it in each half (fp16); `over`: the bits that stand above a code meanwhile, in a register, so that mask and bits are
+// one instruction.  bf16: a byte 128 + code takes a zero point of up to 127 off without borrowing, then its top bit is the
+// sign's again, and a signed byte becomes a float in one instruction.
 template <typename T>
-__device__ __forceinline__ u32x4 numbers(uint32_t w, uint32_t over) {
+__device__ __forceinline__ u32x4 numbers(uint32_t w, uint32_t zero, uint32_t over) {
   u32x4 r;
+  if constexpr (std::is_same<T, f16>::value) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if constexpr (sizeof(T) == 4)
-      r[e] = pack_bf16x2(static_cast<float>((w >> (4 * e)) & 15u), static_cast<float>((w >> (4 * e + 16)) & 15u));
-    else
-      r[e] = ((w >> (4 * e)) & 0x000f000fu) | over;
+    for (int e = 0; e < 4; ++e)
+      r[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, ((w >> (4 * e)) & 0x000f000fu) | over) - __builtin_bit_cast(h2, zero));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t v = ((((w >> (4 * (e & 1))) & 0x0f0f0f0fu) | over) - zero) ^ over;
+      r[e] = pack_bf16x2(byte_f32(v, e / 2), byte_f32(v, e / 2 + 2));
+    }
+  }
   return r;
 }
 template <typename T>
 __device__ __forceinline__ uint32_t bits_over() {
-  uint32_t v = 0;
-  if constexpr (std::is_same<T, bf16>::value) asm("v_mov_b32 %0, 0x43004300" : "=v"(v));
-  if constexpr (std::is_same<T, f16>::value) asm("v_mov_b32 %0, 0x64006400" : "=v"(v));
+  uint32_t v;
+  if constexpr (std::is_same<T, f16>::value)
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(v));
+  else
+    asm("v_mov_b32 %0, 0x80808080" : "=v"(v));
   return v;
 }
+template <typename T>
+__device__ __forceinline__ uint32_t zero_point(uint32_t z) {
+  return std::is_same<T, f16>::value ? __builtin_amdgcn_perm(0u, z, 0x01000100u) + 0x64006400u : __builtin_amdgcn_perm(0u, z, 0u);
+}
 
-// A tile of weights in a lane's registers: codes, and for each of the GP groups of its 128 columns the scales of rows
-// 4 g + 0..3 and the zero points of the same rows (fp16: of row j, which is where they are taken off)
+// A tile of weights in a lane's registers: codes of row j and, for each of the GP groups of its 128 columns, that row's zero
+// point, and the scales of rows 4 g + 0..3, whose sums the lane has
 template <typename T, int GP>
 struct Tile {
   u32x4 w;
@@ -80,7 +96,7 @@ struct TileSource {
     const int64_t t = static_cast<int64_t>(model) * a.otiles + std::min(ot, a.otiles - 1);
     codes = reinterpret_cast<const u32x4*>(a.codes) + t * a.ktiles * 64 + lane;
     scales = reinterpret_cast<const T*>(a.scales) + t * a.ktiles * (GP * 16) + (lane >> 4) * 4;
-    zeros = a.zeros + t * a.ktiles * (GP * 16) + (std::is_same<T, f16>::value ? lane & 15 : (lane >> 4) * 4);
+    zeros = a.zeros + t * a.ktiles * (GP * 16) + (lane & 15);
     last = a.ktiles - 1;
   }
   __device__ __forceinline__ void load(Tile<T, GP>& t, int kt) const {      // past the last: the last again
@@ -90,57 +106,41 @@ struct TileSource {
     for (int s = 0; s < GP; ++s) {
       const int64_t m = static_cast<int64_t>(k) * GP * 16 + s * 16;
       t.scale[s] = *reinterpret_cast<const Four<T>*>(scales + m);
-      if constexpr (std::is_same<T, f16>::value)
-        t.zero[s] = zeros[m];
-      else
-        t.zero[s] = *reinterpret_cast<const uint32_t*>(zeros + m);
+      t.zero[s] = zeros[m];
     }
   }
 };
 
-// acc += RT tiles of weights times MT * 16 rows of x; x(q, xf): the planes of all rows of columns 32 q.., sum(q, t): the
-// sum of rows t over those columns (bf16, fp32)
-template <typename T, int GP, int RT, int MT, typename X, typename S>
-__device__ __forceinline__ void multiply(const Tile<T, GP> (&tile)[RT], uint32_t over, X x, S sum, f32x4 (&acc)[RT][MT]) {
-  constexpr bool kF32 = sizeof(T) == 4, kF16 = std::is_same<T, f16>::value;
+// acc += RT tiles of weights times MT * 16 rows of x; x(q, xf): the planes of all rows of columns 32 q..
+template <typename T, int GP, int RT, int MT, typename X>
+__device__ __forceinline__ void multiply(const Tile<T, GP> (&tile)[RT], uint32_t over, X x, f32x4 (&acc)[RT][MT]) {
+  constexpr bool kF32 = sizeof(T) == 4;
   constexpr int NX = kF32 ? 3 : 1, STEPS = 4 / GP;
-  typedef typename std::conditional<kF16, f16, bf16>::type MM;
+  typedef typename std::conditional<std::is_same<T, f16>::value, f16, bf16>::type MM;
 #pragma unroll
   for (int s = 0; s < GP; ++s) {
     f32x4 part[RT][MT] = {};
-    float total[MT] = {};
 #pragma unroll
     for (int q = s * STEPS; q < (s + 1) * STEPS; ++q) {
       u32x4 xf[MT][NX];
       x(q, xf);
 #pragma unroll
       for (int r = 0; r < RT; ++r) {
-        u32x4 c = numbers<T>(tile[r].w[q], over);
-        if constexpr (kF16) {
-          typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-          const f16 zero = static_cast<f16>(static_cast<float>(tile[r].zero[s] + 1024u));
-          const h2 zz = {zero, zero};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) c[e] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, static_cast<uint32_t>(c[e])) - zz);
-        }
+        const u32x4 c = numbers<T>(tile[r].w[q], zero_point<T>(tile[r].zero[s]), over);
 #pragma unroll
         for (int t = 0; t < MT; ++t)
 #pragma unroll
           for (int n = NX - 1; n >= 0; --n)
             part[r][t] = mma16<MM>(__builtin_bit_cast(bf16x8, c), __builtin_bit_cast(bf16x8, xf[t][n]), part[r][t]);
       }
-      if constexpr (!kF16)
-#pragma unroll
-        for (int t = 0; t < MT; ++t) total[t] += sum(q, t);
     }
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float scale = to_f32(tile[r].scale[s].v[e]);
-        const float zero = static_cast<float>((tile[r].zero[s] >> (8 * e)) & 255u) + (kF32 ? 0.f : 128.f);
 #pragma unroll
-        for (int t = 0; t < MT; ++t) acc[r][t][e] += scale * (kF16 ? part[r][t][e] : part[r][t][e] - zero * total[t]);
+        for (int t = 0; t < MT; ++t) acc[r][t][e] += scale * part[r][t][e];
       }
   }
 }
@@ -212,7 +212,7 @@ __device__ __forceinline__ void store4(T* y, int o, int end, const T* bias, f32x
 // columns.  Weights come D tiles ahead of their use, x (which all workgroups share, in L2) one.
 template <typename T, int GP, int RT, int NW, bool AL>
 __global__ __launch_bounds__(NW * 64) void linear4_few_kernel(Linear4 a) {
-  constexpr bool kF32 = sizeof(T) == 4, kF16 = std::is_same<T, f16>::value;
+  constexpr bool kF32 = sizeof(T) == 4;
   constexpr int NX = kF32 ? 3 : 1, D = RT * GP > 4 || (RT > 1 && (kF32 || NW > 4)) ? 2 : 4, E = 16 / sizeof(T), P = 8 / E;
   __shared__ float lds[NW * 16 * RT * 16];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
@@ -221,7 +221,6 @@ __global__ __launch_bounds__(NW * 64) void linear4_few_kernel(Linear4 a) {
   const int row0 = a.m0 + blockIdx.y * 16;
   const T* x = x_row<T>(a, model, row0 + j);
   const uint32_t over = bits_over<T>();
-  const u32x4 one = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
 
   struct Columns {
     u32x4 v[4][P];                       // 8 columns of each 32
@@ -250,7 +249,6 @@ __global__ __launch_bounds__(NW * 64) void linear4_few_kernel(Linear4 a) {
       if (kt < a.ktiles) {
         bring(cols[(i + 1) & 1], kt + NW);
         u32x4 xf[4][NX];
-        float sums[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           u32x4 v[P];
@@ -267,20 +265,13 @@ __global__ __launch_bounds__(NW * 64) void linear4_few_kernel(Linear4 a) {
           } else {
             xf[q][0] = v[0];
           }
-          if constexpr (!kF16) {
-            f32x4 s = {};
-#pragma unroll
-            for (int n = NX - 1; n >= 0; --n)
-              s = mma16<bf16>(__builtin_bit_cast(bf16x8, one), __builtin_bit_cast(bf16x8, xf[q][n]), s);
-            sums[q] = s[0];
-          }
         }
         multiply<T, GP, RT, 1>(tile[i], over,
                                [&](int q, u32x4(&f)[1][NX]) {
 #pragma unroll
                                  for (int n = 0; n < NX; ++n) f[0][n] = xf[q][n];
                                },
-                               [&](int q, int) { return sums[q]; }, acc);
+                               acc);
         fetch(i, kt + D * NW);
       }
     }
@@ -301,13 +292,12 @@ __global__ __launch_bounds__(NW * 64) void linear4_few_kernel(Linear4 a) {
 }
 
 // More rows, through LDS: a workgroup of 8 or 16 waves, WR of them over output rows (RT tiles each) and WK over columns,
-// brings CK tiles of 128 columns of x at a time, split into planes (fp32) and with the sums over 32 columns that the
-// zero points want, once for all its output rows.  Weights come straight into registers, D tiles ahead of their use.
+// brings CK tiles of 128 columns of x at a time, split into planes (fp32), once for all its output rows.  Weights come straight into registers, D tiles ahead of their use.
 constexpr int kPad = 136;          // 16-bit values in a staged row: 128, and 8 that move the rows to other banks
 
 template <typename T, int GP, int MT, int RT, int WR, int WK, int CK, bool AL>
 __global__ __launch_bounds__(WR * WK * 64) void linear4_rows_kernel(Linear4 a) {
-  constexpr bool kF32 = sizeof(T) == 4, kF16 = std::is_same<T, f16>::value;
+  constexpr bool kF32 = sizeof(T) == 4;
   constexpr int NX = kF32 ? 3 : 1, M = MT * 16, NT = WR * WK * 64;
   static_assert(CK % WK == 0, "every wave has whole tiles of a chunk");
   constexpr int PER = CK / WK, D = PER < 2 ? PER : 2;                   // tiles of a wave in a chunk; in flight
@@ -315,7 +305,6 @@ __global__ __launch_bounds__(WR * WK * 64) void linear4_rows_kernel(Linear4 a) {
   static_assert(PER % D == 0 && CK * M * 16 % NT == 0, "slots repeat with the chunk, pieces with the threads");
   extern __shared__ float lds[];
   uint16_t* xs = reinterpret_cast<uint16_t*>(lds);                      // [CK][NX][M][kPad]
-  float* sums = lds + CK * NX * M * kPad / 2;                           // [CK][4][M]
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, j = lane & 15, g = lane >> 4;
   const int wr = wave / WK, wk = wave % WK;
   const uint32_t model = fdiv(blockIdx.x, a.by_wg);
@@ -340,11 +329,11 @@ __global__ __launch_bounds__(WR * WK * 64) void linear4_rows_kernel(Linear4 a) {
     for (int i = 0; i < PC; ++i) {
       const int p = tid / 16 + i * (NT / 16), r = p % M, k = p / M, c = tid % 16;
       uint16_t* dst = xs + (k * NX * M + r) * kPad + c * 8;
-      float f[8];
       u32x4 v[P];
 #pragma unroll
       for (int h = 0; h < P; ++h) v[h] = x_keep<T, AL>(xr[i][h], (kt0 + k) * 128 + c * 8 + h * E, a.k);
       if constexpr (kF32) {
+        float f[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) f[e] = __builtin_bit_cast(f32x4, v[e / 4])[e % 4];
         uint4 pl[3];
@@ -353,16 +342,6 @@ __global__ __launch_bounds__(WR * WK * 64) void linear4_rows_kernel(Linear4 a) {
         for (int n = 0; n < 3; ++n) *reinterpret_cast<uint4*>(dst + n * M * kPad) = pl[n];
       } else {
         *reinterpret_cast<u32x4*>(dst) = v[0];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[2 * e] = bf16_lo(v[0][e]), f[2 * e + 1] = bf16_hi(v[0][e]);
-      }
-      if constexpr (!kF16) {
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum += f[e];
-        sum += __shfl_xor(sum, 1, 64);
-        sum += __shfl_xor(sum, 2, 64);
-        if ((c & 3) == 0) sums[(k * 4 + c / 4) * M + r] = sum;
       }
     }
   };
@@ -389,7 +368,6 @@ __global__ __launch_bounds__(WR * WK * 64) void linear4_rows_kernel(Linear4 a) {
         const int i = i0 + d, ct = i * WK + wk;            // tile of the chunk
         if (kt0 + ct < a.ktiles) {
           const uint16_t* x = xs + ct * NX * M * kPad + j * kPad + g * 8;
-          const float* sum = sums + ct * 4 * M + j;
           multiply<T, GP, RT, MT>(tile[d], over,
                                   [&](int q, u32x4(&f)[MT][NX]) {
 #pragma unroll
@@ -398,7 +376,7 @@ __global__ __launch_bounds__(WR * WK * 64) void linear4_rows_kernel(Linear4 a) {
                                       for (int n = 0; n < NX; ++n)
                                         f[t][n] = *reinterpret_cast<const u32x4*>(x + (n * M + t * 16) * kPad + q * 32);
                                   },
-                                  [&](int q, int t) { return sum[q * M + t * 16]; }, acc);
+                                  acc);
         }
         fetch(d, i + D < PER ? kt0 + ct + D * WK : kt0 + CK + (i + D - PER) * WK + wk);
       }
@@ -449,7 +427,7 @@ void launch_rows(Linear4 a, int64_t n, hipStream_t s) {
   constexpr int NX = sizeof(T) == 4 ? 3 : 1, M = MT * 16;
   const int64_t per = cdiv(a.otiles, WR * RT);
   a.by_wg = make_fastdiv(static_cast<uint32_t>(per));
-  const size_t staged = CK * (NX * M * kPad * 2 + 4 * M * 4), joined = WR * WK * M * RT * 16 * 4;
+  const size_t staged = CK * NX * M * kPad * 2, joined = WR * WK * M * RT * 16 * 4;
   const size_t lds = std::max(staged, joined);
   const auto kernel = a.vec ? linear4_rows_kernel<T, GP, MT, RT, WR, WK, CK, true> : linear4_rows_kernel<T, GP, MT, RT, WR, WK, CK, false>;
   if (lds > 65536)

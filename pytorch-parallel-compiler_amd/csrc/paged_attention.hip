@@ -81,16 +81,6 @@ __device__ __forceinline__ float unpack_hi(uint32_t v) {
   else
     return bf16_hi(v);
 }
-// byte i (a constant) of v as a float, in one instruction
-__device__ __forceinline__ float byte_f32(uint32_t v, int i) {
-  float f;
-  if (i == 0) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_0" : "=v"(f) : "v"(v));
-  if (i == 1) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_1" : "=v"(f) : "v"(v));
-  if (i == 2) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_2" : "=v"(f) : "v"(v));
-  if (i == 3) asm("v_cvt_f32_i32_sdwa %0, sext(%1) dst_sel:DWORD dst_unused:UNUSED_PAD src0_sel:BYTE_3" : "=v"(f) : "v"(v));
-  return f;
-}
-
 // 8 floats as N planes of 16-bit values whose sum they are
 template <typename MT, int N>
 __device__ __forceinline__ void planes(const float (&v)[8], u32x4 (&out)[N]) {

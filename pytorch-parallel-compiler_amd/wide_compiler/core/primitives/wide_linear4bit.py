@@ -7,9 +7,9 @@ WideLinear4bit: N independent linear layers with weights of 4 bits, for few rows
 with codes of 0 to 15, groups of 32, 64 or 128 columns and zero points of 0 to 15 (8 where none are
 given).  The forward (wc_linear4) brings each weight from memory once for up to 16, 32 or 64 rows (the
 more weights there are, the more), so that a token's products cost what reading half a byte a weight
-costs; it is faster than WideLinear up to some 250 rows in 16 bits, and at any in fp32.  Sums are
-fp32; the scale multiplies each group's sum.  An infinity in a row of x gives that
-row NaN in bf16 and fp32, also where the formula has an infinity.
+costs.  Whole numbers code - zero meet x, exactly, sums are fp32, and the scale multiplies each group's sum: products with
+x of 2^117 and more can overflow where scaled ones would not.  An infinity in a row of x gives that row NaN in fp32, also
+where the formula has an infinity.
 
 The buffers hold the weights as the kernel reads them (``packed`` [N, O / 16, I / 128, 64, 4] int32,
 ``scales`` and ``zeros`` [N, O / 16, groups, 16], sizes rounded up); ``from_codes`` packs them from

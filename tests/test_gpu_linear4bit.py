@@ -166,3 +166,42 @@ def test_linear4_small_weights(m, dtype, size):
         y = mod(x)
     extra = 160 if dtype == torch.bfloat16 else 30          # codes, zero points and (bf16) 128, times the scale
     _check(y, x, w, w.abs() + extra * mod.scales.amax().double(), None)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n,m,k,o", [(1, 1, 512, 200), (3, 5, 4100, 40), (2, 20, 1000, 300), (90, 8, 600, 300), (52, 40, 390, 600), (20, 70, 300, 300)])
+def test_linear4_weights_of_zero_take_no_part(n, m, k, o, group, dtype):
+    """Where a column's codes are their zero points, nothing of x counts, however large it is, and what x sums up to
+    counts nowhere: the loss is 2^-24 of the sum of |x w| for each addition, as above."""
+    import wide_compiler as wc
+    g = gen(k + m)
+    groups, at = -(-k // group), torch.arange(k) // group
+    codes = torch.randint(0, 16, (n, o, k), generator=g, dtype=torch.uint8)
+    z = torch.randint(0, 16, (n, o, groups), generator=g, dtype=torch.uint8)
+    none = torch.rand(k, generator=g) < 0.05
+    none[7], none[k - 1], none[k - 2] = True, True, False
+    codes = torch.where(none, z[..., at], codes)
+    scales = (0.02 * (0.5 + torch.rand(n, o, groups, generator=g))).to(dtype)
+    even = torch.nn.functional.pad(codes, (0, k % 2))
+    mod = wc.WideLinear4bit.from_codes((even[..., 0::2] | even[..., 1::2] << 4).to(DEV), scales.to(DEV), in_features=k,
+                                       group_size=group, zeros=z.to(DEV))
+    w = ((codes.double() - z.double()[..., at]) * scales.double()[..., at]).to(DEV)
+    assert (w[..., none.to(DEV)] == 0).all()
+    x = 3 + torch.randn(n, m, k, generator=g)
+    x[..., none] = 3e4 if dtype == torch.float16 else 1e37
+    x = x.to(DEV, dtype)
+    _check(mod(x), x, w, w.abs(), None)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m", [1, 20, 70])
+def test_linear4_infinities_in_16_bits(m, dtype):
+    """An infinity in x comes out as the formula has it: of its weights' sign, NaN where one is zero."""
+    mod, w, size, b = _layer(2, 500, 300, 64, True, True, dtype, 23)
+    x = torch.randn(2, m, 500, generator=gen(m)).to(DEV, dtype)
+    x[0, 0, 77], x[1, m // 2, 499] = float("inf"), -float("inf")
+    ref = torch.stack([(x[i].double()[:, None] * w[i]).sum(-1) for i in range(2)]) + b.to(DEV).double()[:, None]
+    y = mod(x)
+    assert torch.equal(torch.isnan(y), torch.isnan(ref)) and torch.equal(torch.isinf(y), torch.isinf(ref))
+    assert torch.equal(y[torch.isinf(ref)].double(), ref[torch.isinf(ref)]) and 0 < torch.isinf(ref).sum() < 600
