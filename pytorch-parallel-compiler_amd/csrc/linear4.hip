@@ -436,24 +436,26 @@ void launch_rows(Linear4 a, int64_t n, hipStream_t s) {
 }
 
 // Which kernel, for `tiles` tiles of output rows of all models and `rows` tiles of 16 rows of x (us on an MI355X,
-// launches of a graph, bf16, groups of 128).
+// launches of a graph, weights from memory, bf16, groups of 128 where nothing else is said).
 //
-// Few tiles: a tile for each workgroup, its waves share the columns (64 tiles of 16 rows: 4.0; two tiles each 4.5, through
-// LDS 6.2; 8 waves where columns are long: 256 tiles, K 4096, fp16: 5.9, with 4 6.3), then two that share what they bring of x, for 8 waves where their workgroups all find room at once (1024 tiles,
-// K 4096: 10.9; for 4 waves 11.9; one tile for 4 waves 12.3; in fp16 with groups of 64: 11.6, 13.4, 12.7.  Groups of 32, K
-// 2048, whose registers leave room for half: 11.6 with 8, 9.6 with 4).
+// Few tiles: a tile for each workgroup, its waves share the columns (64 tiles, 16 rows, K 2048: 6.6; through LDS 7.5; 8 waves
+// where columns are long: 256 tiles, K 4096: 6.2, with 4 waves 6.5, with two tiles a workgroup 7.5), then two that share what
+// they bring of x, for 8 waves where their workgroups all find room at once, which takes 128 registers (1024 tiles, K 4096:
+// 12.6; for 4 waves 13.6; one tile for 4 waves 14.1; in fp16 with groups of 64: 12.6, 13.8, 14.2).  There is less room with
+// groups of 32 (K 2048: 12.8 with 8, 10.9 with 4), and in bf16 with groups of 64 where x isn't whole vectors (K 2047: 14.4
+// with 8, 13.0 with 4).
 //
 // More go through LDS.  16 waves fill a unit, with as much of x and W as registers take, where their workgroups come to
 // whole rounds of all units, nearly; else 8 waves with 32 rows, of which a unit has two; else as many workgroups as can be:
 //                                 16 waves, 64 rows   16 waves, 32 rows   8 waves, 32 rows   4 x 2 waves, 32 rows
-//   4096 tiles, 64 rows, K 2048         35                  42                  41                 53
-//   2048 tiles, 64 rows, K 2048         32                  21                  22                 29
-//   1235 tiles, 64 rows, K 2048         32                  21                  22                 24
-//   1235 tiles, 200 rows, K 2048        62                  59                  50                 60
-//    512 tiles, 64 rows, K 2048         31                  19                  14                 12
+//   4096 tiles, 64 rows, K 2048         42                  54                  51                 62
+//   2048 tiles, 64 rows, K 2048         31                  26                  26                 33
+//   1235 tiles, 64 rows, K 2048         29                  23                  23                 23
+//   1235 tiles, 200 rows, K 2048        58                  63                  55                 63
+//    512 tiles, 64 rows, K 2048         27                  21                  14                 11
 // and by the same reasons in fp32, whose three planes of x leave less room.  Sixteen rows or fewer: 16 waves again where
-// they come to whole rounds (4096 tiles, K 2048: 18, of 4 x 2 waves 20), and two waves over two tiles, without LDS,
-// where there are too few columns for it to pay (1235 tiles, K 1024: 7.5 against 8.9).
+// they come to whole rounds (4096 tiles, K 2048: 23, of 4 x 2 waves 27), and two waves over two tiles, without LDS,
+// where there are too few columns for it to pay (1235 tiles, K 1024: 9.2 against 9.7; K 2048: 13.3 against 12.2).
 template <typename T, int GP, int MT, int RT, int WR, int WK, int CK>
 bool launch_if_full(const Linear4& a, int64_t n, hipStream_t s) {
   const int64_t wgs = n * cdiv(a.otiles, WR * RT) * cdiv(a.m, MT * 16);
@@ -467,7 +469,8 @@ void dispatch(const Linear4& a, int64_t n, hipStream_t s) {
   const int64_t tiles = n * a.otiles, rows = cdiv(a.m, 16);
   if (tiles * rows <= 256 && a.ktiles >= 32) return launch_few<T, GP, 1, 8>(a, n, s);
   if (tiles * rows <= 256) return launch_few<T, GP, 1, 4>(a, n, s);
-  if (rows == 1 && tiles <= (F32 || GP > 2 ? 512 : 1024)) return launch_few<T, GP, 2, 8>(a, n, s);
+  const bool room = !F32 && (GP == 1 || (GP == 2 && (a.vec || std::is_same<T, f16>::value)));
+  if (rows == 1 && tiles <= (room ? 1024 : 512)) return launch_few<T, GP, 2, 8>(a, n, s);
   if (rows == 1 && tiles <= 1024) return launch_few<T, GP, 2, 4>(a, n, s);
   if constexpr (F32) {
     if (rows > 1 && launch_if_full<T, GP, 2, 2, 8, 1, 1>(a, n, s)) return;
