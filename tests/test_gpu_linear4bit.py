@@ -205,3 +205,29 @@ def test_linear4_infinities_in_16_bits(m, dtype):
     y = mod(x)
     assert torch.equal(torch.isnan(y), torch.isnan(ref)) and torch.equal(torch.isinf(y), torch.isinf(ref))
     assert torch.equal(y[torch.isinf(ref)].double(), ref[torch.isinf(ref)]) and 0 < torch.isinf(ref).sum() < 600
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("n,o,m,k", [
+    (1, 600, 1, 2999), (1, 600, 1, 4097), (1, 600, 33, 4999), (1, 600, 5, 8192), (1, 600, 1, 8191),      # one tile of outputs
+    (4, 2100, 1, 4999), (4, 4096, 3, 4096), (4, 4096, 1, 8191), (5, 2048, 9, 2047),                      # two, 8 and 4 waves
+    (16, 2048, 1, 8192), (16, 2048, 3, 4999), (16, 2048, 7, 8191),                                       # chunks of 16 tiles
+    (32, 2048, 16, 4097), (32, 2048, 50, 2056), (9, 2000, 70, 4097)])                                    # 16 and 8 waves
+def test_linear4_long_columns(n, o, m, k, group, dtype):
+    """Every form's loops over the columns come round again, with rows of x that are whole vectors and not; a chain of
+    additions as above, each off by 2^-24 of the sum of |x w|."""
+    import wide_compiler as wc
+    g = torch.Generator(device=DEV).manual_seed(n + o + m + k)
+    groups = -(-k // group)
+    codes = torch.randint(0, 256, (n, o, (k + 1) // 2), generator=g, dtype=torch.uint8, device=DEV)
+    scales = (0.02 * (0.5 + torch.rand(n, o, groups, generator=g, device=DEV))).to(dtype)
+    z = torch.randint(0, 16, (n, o, groups), generator=g, dtype=torch.uint8, device=DEV)
+    mod = wc.WideLinear4bit.from_codes(codes, scales, in_features=k, group_size=group, zeros=z)
+    x = torch.randn(n, m, k, generator=g, device=DEV).to(dtype)
+    y = mod(x)
+    at = torch.arange(k, device=DEV) // group
+    for i in range(n):
+        c = torch.stack((codes[i] & 15, codes[i] >> 4), -1).flatten(-2)[:, :k].double()
+        w = ((c - z[i].double()[:, at]) * scales[i].double()[:, at])[None]
+        _check(y[i:i + 1], x[i:i + 1], w, w.abs(), None)

@@ -417,3 +417,23 @@ def test_attend_lengths_far_beyond_the_table(n, b, blocks):
         with pytest.raises(IndexError):
             cache.index_error()
         within(got, expect.double(), 2 * HALF[q.dtype], attend_slack(q.dtype, 32.0, d, blocks * page, 4.5))
+
+
+@pytest.mark.parametrize("dtype,quantized", [(torch.bfloat16, False), (torch.bfloat16, True), (torch.float16, False), (torch.float32, False)])
+@pytest.mark.parametrize("hq,hkv,d,lens", [
+    (8, 8, 64, [20000, 60000, 3000]),                       # shares of many tiles, of one sequence and of two
+    (4, 1, 64, [131072]), (2, 1, 128, [300000, 17]),        # hundreds of parts, so that a thread of the join has several
+    (1, 1, 32, [300000]), (16, 2, 256, [40000, 1, 9000])])
+def test_attend_long_shares_and_many_parts(hq, hkv, d, lens, dtype, quantized):
+    """A part adds up at most 256 products in a chain (a share's tiles over its waves, 32 tokens at a time), the join at
+    most 1024 / 4 outputs: 512 additions of 2^-24 of the sum of |p v|, in numerator and sum each; a score and its
+    exponential as attend_slack has them."""
+    cache, q, k, v, table, lens = _setup(1, len(lens), hq, hkv, d, 64, lens, dtype, quantized, d + hq)
+    got = cache.attend(q, table, lens)
+    for i in range(lens.shape[1]):
+        length = int(lens[0, i])
+        one, part = lens[:, i:i + 1], [t[:, i:i + 1, :length] for t in (k, v)]
+        ref, big = attend(q[:, i:i + 1], *part, one)
+        size, _ = attend(q[:, i:i + 1], part[0], part[1].abs(), one)
+        within(got[:, i:i + 1], ref, HALF[dtype], size * (2 * (d + 4) * 2.0 ** -24 * big + 2.0 ** -20 + 2 * 512 * 2.0 ** -24 + 2.0 ** -21))
+    cache.index_error()
