@@ -160,19 +160,19 @@ class WidePagedCache:
         if torch.compiler.is_compiling():
             return _serve.uncompiled(self.read, block_table, lengths, max_length)
         form = (block_table.shape, block_table.dtype, block_table.get_device(), lengths.shape, lengths.dtype,
-                lengths.get_device(), max_length)
-        plan = self._plans.get(form)
-        if plan is None:
+                lengths.get_device())
+        sizes = self._plans.get(form)
+        if max_length < 0:
+            raise RuntimeError(f"WidePagedCache.read: max_length must not be negative, got {max_length}")
+        if sizes is None:
             what = "WidePagedCache.read"
             _hip.require_device(what, block_table, lengths)
-            if max_length < 0:
-                raise RuntimeError(f"{what}: max_length must not be negative, got {max_length}")
             n, b = block_table.shape[:2]
             self._check_table(what, block_table, n, b)
             self._check_per_sequence(what, "lengths", lengths, n, b)
             _serve.same_device(what, self.k_pages, block_table, lengths)
-            plan = self._plans.keep(form, (self._sizes_for(n, b), (n, b, max_length, self.n_kv_heads, self.head_dim)))
-        sizes, shape = plan
+            sizes = self._plans.keep(form, self._sizes_for(n, b))
+        shape = (*lengths.shape, max_length, self.n_kv_heads, self.head_dim)
         k = torch.empty(shape, dtype=self.dtype, device=self.device)
         v = torch.empty(shape, dtype=self.dtype, device=self.device)
         if k.numel():
@@ -190,11 +190,15 @@ class WidePagedCache:
             return _serve.uncompiled(self.attend, q, block_table, lengths, first, scale, max_length)
         form = (q.shape, q.dtype, q.get_device(), block_table.shape, block_table.dtype, block_table.get_device(),
                 lengths.shape, lengths.dtype, lengths.get_device(),
-                None if first is None else (first.shape, first.dtype, first.get_device()), max_length)
+                None if first is None else (first.shape, first.dtype, first.get_device()))
         plan = self._plans.get(form)
         if plan is None:
-            plan = self._plans.keep(form, self._plan_attend(q, block_table, lengths, first, max_length))
-        sizes, most, need = plan
+            plan = self._plans.keep(form, self._plan_attend(q, block_table, lengths, first))
+        sizes, reach, needs = plan
+        most = reach if max_length is None else max_length
+        need = needs.get(most)
+        if need is None:
+            need = needs.keep(most, self._workspace(sizes, q, block_table, most))
         if torch.is_grad_enabled():
             _hip.require_forward_only("WidePagedCache.attend", q)
         q = q if q.stride(3) == 1 else q.contiguous()
@@ -205,8 +209,7 @@ class WidePagedCache:
                                    self.head_dim ** -0.5 if scale is None else scale, most, ws)
         return o
 
-    def _plan_attend(self, q: Tensor, block_table: Tensor, lengths: Tensor, first: Optional[Tensor],
-                     max_length: Optional[int]) -> Tuple:
+    def _plan_attend(self, q: Tensor, block_table: Tensor, lengths: Tensor, first: Optional[Tensor]) -> Tuple:
         what = "WidePagedCache.attend"
         _hip.require_device(what, q, block_table, lengths, first)
         if q.dim() != 4 or q.shape[3] != self.head_dim or q.shape[2] % self.n_kv_heads:
@@ -219,15 +222,13 @@ class WidePagedCache:
         self._check_per_sequence(what, "lengths", lengths, n, b)
         self._check_per_sequence(what, "first", first, n, b)
         _serve.same_device(what, self.k_pages, q, block_table, lengths, first)
-        if max_length is None:
-            max_length = min(block_table.shape[2] * self.page_size, 2 ** 31 - 65)
-        elif max_length < 0:
-            raise RuntimeError(f"{what}: max_length must not be negative, got {max_length}")
-        sizes = self._sizes_for(n, b)
-        need = 0
-        if q.numel():
-            need = _serve.paged_attention_workspace(self, sizes, block_table, q.shape[2], max_length)
-        return sizes, max_length, need
+        # workspaces by max_length, which a caller may raise with every token: apart from the checks above
+        return self._sizes_for(n, b), min(block_table.shape[2] * self.page_size, 2 ** 31 - 65), _serve.Plans()
+
+    def _workspace(self, sizes: Tuple, q: Tensor, block_table: Tensor, max_length: int) -> int:
+        if max_length < 0:
+            raise RuntimeError(f"WidePagedCache.attend: max_length must not be negative, got {max_length}")
+        return _serve.paged_attention_workspace(self, sizes, block_table, q.shape[2], max_length) if q.numel() else 0
 
     def index_error(self) -> None:
         """Raise IndexError if any call since the last check met a page outside the pool, or a token, count or length

@@ -489,3 +489,27 @@ def test_parametrised_weights_count(monkeypatch, anywhere):
     assert (qw == 1).all() and (kw == 2).all() and (scales == 2).all() and (bias == 1).all()
     with pytest.raises(RuntimeError, match="forward-only"):
         lin(torch.zeros(1, 2, 64))                          # its bias asks for a gradient
+
+
+def test_a_growing_bound_keeps_the_plans(monkeypatch, anywhere):
+    """max_length raised with every token, as a tight bound is: the call's form stays checked, and no other form's plan is
+    lost to it."""
+    import wide_compiler as wc
+    from wide_compiler import _serve
+    for name in ("cache_write", "cache_read", "paged_attention"):
+        monkeypatch.setattr(_serve, name, lambda *a: None)
+    pages = torch.zeros(5, 2, 16, 64)
+    cache = wc.WidePagedCache.from_pages(pages, pages)
+    table, n = torch.zeros(1, 3, 4, dtype=torch.int32), torch.zeros(1, 3, dtype=torch.int32)
+    k, q = torch.zeros(1, 3, 7, 2, 64), torch.zeros(1, 3, 4, 64)
+    cache.write(k, k, table, n)
+    checked = []
+    monkeypatch.setattr(wc.WidePagedCache, "_check_table", staticmethod(lambda *a: checked.append(a)))
+    for length in range(1000):
+        cache.attend(q, table, n, max_length=length)
+        assert cache.read(table, n, length % 9)[0].shape == (1, 3, length % 9, 2, 64)
+    cache.write(k, k, table, n)
+    assert len(checked) == 2                                 # the first attend and the first read
+    for call in (lambda: cache.attend(q, table, n, max_length=-1), lambda: cache.read(table, n, -1)):
+        with pytest.raises(RuntimeError, match="negative"):
+            call()
