@@ -59,6 +59,7 @@ int32_t wc_head_norm_rotary(const wc_head_norm_args* args, void* stream);
  *   pages + ((page * heads + head) * page_size + slot) * row      (row elements, head_dim of them used)
  * in `dtype` (bits 0), or as 8-bit codes (bits 8) with one fp32 scale at the same index of the scales:
  *   scale = max(max |x| / 127, 2^-126),  code = x / scale to the nearest, ties to even (exactly),
+ * (a unit of the last place less for the largest fp32 value, so that 127 times it is finite),
  * and a row that holds an infinity or NaN gets scale NaN and codes 0: it reads back as NaN.
  * A table entry outside [0, pages), or a token past the table's end, is never followed: its row is
  * not written, reads as zeros, takes no part in the attention, and stores 1 in *err_flag.

@@ -6,7 +6,7 @@
 // written as they are (147 MB) 32 us, 4.6 TB/s; as codes (112 MB) 32 us, which the search for each row's scale and the
 // codes' arithmetic keep from 25; codes read back (145 MB) 26 us, 5.5 TB/s.
 //
-// 8 bits: scale = max(max |x| / 127, 2^-126), code = x / scale to the nearest, ties to even.  The quotient is
+// 8 bits: scale = max(max |x| / 127, 2^-126) (one unit less for fp32's largest value), code = x / scale to the nearest, ties to even.  The quotient is
 // never formed: c = x * (1 / scale) to the nearest is off by at most one, and then only next to a half; the remainder
 // x - c scale is exact (one fused multiply-add whose result fits 24 bits) and its place against scale / 2
 // puts c right, for the lanes that have such a value.  The code is so a function of x and scale alone.
@@ -18,6 +18,7 @@ namespace wc {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr float kMost = 0x1.020406p121f;      // the largest scale: 127 of the next one round to infinity in fp32
 constexpr int kRows = 4;           // rows of a group of lanes, all on their way at once (those codes written and read: 61 us;
                                    // one row 68, two 64, eight 73)
 
@@ -144,7 +145,7 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
       uint32_t top = largest<T, V, NC>(v);
       for (int off = lanes >> 1; off; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 64)));
       const bool finite = top < 0x7f800000u;
-      const float scale = finite ? fmaxf(__builtin_bit_cast(float, top) / 127.f, 0x1p-126f) : __builtin_nanf("");
+      const float scale = finite ? fminf(fmaxf(__builtin_bit_cast(float, top) / 127.f, 0x1p-126f), kMost) : __builtin_nanf("");
       const float inv = __builtin_amdgcn_rcpf(scale);
       uint32_t code[NC][V];
       float far = 0.f;

@@ -216,3 +216,23 @@ def test_a_table_without_entries(quantized):
                     cache.index_error()
             cache.index_error()
     assert (cache.k_pages == 0).all() and (cache.v_pages == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_codes_of_the_largest_values_are_finite(dtype):
+    """A row that holds the type's largest value reads back as that value, to a unit of fp32's and its own last place, and
+    the others as multiples of 1/127 of it, half of one off."""
+    import wide_compiler as wc
+    top = torch.finfo(dtype).max
+    x = torch.linspace(-1, 1, 64).to(dtype).double() * top
+    x[0], x[63], x[5] = -top, top, 0
+    x = x.to(dtype).to(DEV).view(1, 1, 1, 1, 64)
+    cache = wc.WidePagedCache(1, 16, 1, 64, dtype=dtype, quantized=True)
+    table, start = torch.zeros(1, 1, 1, dtype=torch.int32, device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    cache.write(x, x / 2, table, start)
+    k, v = cache.read(table, start + 1, 1)
+    assert torch.isfinite(k).all() and torch.isfinite(v).all()
+    for got, ref in ((k.double(), x.double()), (v.double(), x.double() / 2)):
+        big = ref.abs().max()
+        assert ((got - ref).abs() <= big * (1 / 254 + torch.finfo(dtype).eps + 2.0 ** -22)).all()
+        assert ((got[..., [0, 63]] - ref[..., [0, 63]]).abs() <= big * (torch.finfo(dtype).eps + 2.0 ** -22)).all()
