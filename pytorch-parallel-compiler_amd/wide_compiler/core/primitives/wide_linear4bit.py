@@ -98,22 +98,23 @@ class WideLinear4bit(nn.Module):
         sizes = (_hip.dtype_code(x.dtype, "linear4"), self.group_size, self.n, rows.rows, self.out_features, self.in_features)
         return self._plans.keep(form, (dense is x, rows, sizes, (*x.shape[:-1], self.out_features)))
 
-    def _pack(self, codes: Tensor, scales: Tensor, zeros: Optional[Tensor]) -> None:
-        """codes [N, O, I] uint8 of 0-15, scales and zeros [N, O, ceil(I / group)] into the buffers."""
-        n, rt, kt = self.packed.shape[:3]
-        full = torch.zeros((n, rt * 16, kt * 128), dtype=torch.uint8, device=codes.device)
-        full[:, :self.out_features, :self.in_features] = codes
-        # [n, row tile, row, column tile, word, lane group, column] -> [.., lane group, row, word, column]
-        c = full.view(n, rt, 16, kt, 4, 4, 8).permute(0, 1, 3, 5, 2, 4, 6)
+    def _pack(self, i: int, codes: Tensor, scales: Tensor, zeros: Optional[Tensor]) -> None:
+        """codes [O, I] uint8 of 0-15, scales and zeros [O, ceil(I / group)] into model i's part of the buffers: one model
+        at a time, because that takes some bytes a weight on the way."""
+        rt, kt = self.packed.shape[1:3]
+        full = torch.zeros((rt * 16, kt * 128), dtype=torch.uint8, device=codes.device)
+        full[:self.out_features, :self.in_features] = codes
+        # [row tile, row, column tile, word, lane group, column] -> [.., lane group, row, word, column]
+        c = full.view(rt, 16, kt, 4, 4, 8).permute(0, 2, 4, 1, 3, 5)
         half = torch.empty((*c.shape[:-1], 8), dtype=torch.uint8, device=codes.device)
         half[..., list(_NIBBLE)] = c
         words = half[..., 0::2] | (half[..., 1::2] << 4)                 # bytes, the low nibble first
-        self.packed.copy_(words.contiguous().view(torch.int32).view(self.packed.shape))
-        for dst, src in ((self.scales, scales), (self.zeros, zeros)):
+        self.packed[i].copy_(words.contiguous().view(torch.int32).view(self.packed.shape[1:]))
+        for dst, src in ((self.scales[i], scales), (self.zeros[i], zeros)):
             if src is not None:
-                rows = torch.zeros((n, rt * 16, dst.shape[2]), dtype=dst.dtype, device=codes.device)
-                rows[:, :self.out_features, :src.shape[2]] = src
-                dst.copy_(rows.view(n, rt, 16, -1).transpose(2, 3))
+                rows = torch.zeros((rt * 16, dst.shape[1]), dtype=dst.dtype, device=codes.device)
+                rows[:self.out_features, :src.shape[1]] = src
+                dst.copy_(rows.view(rt, 16, -1).transpose(1, 2))
 
     @classmethod
     def from_codes(cls, codes: Tensor, scales: Tensor, *, in_features: int, group_size: int = 128,
@@ -134,9 +135,10 @@ class WideLinear4bit(nn.Module):
             raise ValueError(f"{what}: zero points must be within [0, 15]")
         wide = cls(codes.shape[0], in_features, codes.shape[1], group_size, bias=bias is not None,
                    dtype=scales.dtype).to(codes.device)
-        rows = torch.stack((codes & 15, codes >> 4), -1).flatten(-2)[..., :in_features]
         with torch.no_grad():
-            wide._pack(rows, scales, zeros)
+            for i, c in enumerate(codes):
+                rows = torch.stack((c & 15, c >> 4), -1).flatten(-2)[:, :in_features]
+                wide._pack(i, rows, scales[i], None if zeros is None else zeros[i])
             if bias is not None:
                 wide.bias.copy_(bias)
         return wide
@@ -150,24 +152,23 @@ class WideLinear4bit(nn.Module):
         if any(form(m) != form(t) for m in modules):
             raise ValueError("WideLinear4bit.from_modules needs modules of one shape, dtype and device, all with a bias or all "
                              "without")
-        n, o, i = len(modules), t.out_features, t.in_features
-        wide = cls(n, i, o, group_size, bias=t.bias is not None, dtype=t.weight.dtype).to(t.weight.device)
-        groups = -(-i // group_size)
+        o, k = t.out_features, t.in_features
+        wide = cls(len(modules), k, o, group_size, bias=t.bias is not None, dtype=t.weight.dtype).to(t.weight.device)
+        groups, info = -(-k // group_size), torch.finfo(t.weight.dtype)
         with torch.no_grad():
-            w = torch.stack([m.weight for m in modules]).float()
-            pad = torch.nn.functional.pad(w, (0, groups * group_size - i)).view(n, o, groups, group_size)
-            lo, hi = pad.amin(-1).clamp_max(0), pad.amax(-1).clamp_min(0)
-            # a step, under the type's normal values rounded up (to the nearest it may be half as large, or 0); 1 of zeros
-            step, info = hi.double() / 15 - lo.double() / 15, torch.finfo(t.weight.dtype)
-            least = info.tiny * info.eps
-            step = torch.where(step < info.tiny, torch.ceil(step / least) * least, step)
-            scales = torch.where(step == 0, 1.0, step).to(t.weight.dtype)
-            s = scales.float()
-            zeros = torch.round(-lo / s).clamp(0, 15)
-            codes = (torch.round(pad / s[..., None]) + zeros[..., None]).clamp(0, 15)
-            wide._pack(codes.to(torch.uint8).flatten(-2)[..., :i], scales, zeros.to(torch.uint8))
-            if t.bias is not None:
-                wide.bias.copy_(torch.stack([m.bias for m in modules]))
+            for i, m in enumerate(modules):
+                w = torch.nn.functional.pad(m.weight.float(), (0, groups * group_size - k)).view(o, groups, group_size)
+                lo, hi = w.amin(-1).clamp_max(0), w.amax(-1).clamp_min(0)
+                # a step, under the type's normal values rounded up (to the nearest it may be half as large, or 0); 1 of zeros
+                step, least = hi.double() / 15 - lo.double() / 15, info.tiny * info.eps
+                step = torch.where(step < info.tiny, torch.ceil(step / least) * least, step)
+                scales = torch.where(step == 0, 1.0, step).to(t.weight.dtype)
+                s = scales.float()
+                zeros = torch.round(-lo / s).clamp(0, 15)
+                codes = (torch.round(w / s[..., None]) + zeros[..., None]).clamp(0, 15)
+                wide._pack(i, codes.to(torch.uint8).flatten(-2)[:, :k], scales, zeros.to(torch.uint8))
+                if m.bias is not None:
+                    wide.bias[i].copy_(m.bias)
         return wide
 
     def dequantize(self) -> Tensor:

@@ -231,3 +231,21 @@ def test_linear4_long_columns(n, o, m, k, group, dtype):
         c = torch.stack((codes[i] & 15, codes[i] >> 4), -1).flatten(-2)[:, :k].double()
         w = ((c - z[i].double()[:, at]) * scales[i].double()[:, at])[None]
         _check(y[i:i + 1], x[i:i + 1], w, w.abs(), None)
+
+
+def test_linear4_packs_one_model_at_a_time():
+    """What packing takes beside the weights does not grow with the number of models: of 32, at most 4 bytes a weight with
+    the packed half byte, where one model's own passes through fp32, its codes and their nibbles take 20 and more."""
+    import wide_compiler as wc
+    n, d = 32, 1024
+    lin = [torch.nn.Linear(d, d, bias=False, device=DEV, dtype=torch.bfloat16) for _ in range(n)]
+    codes = torch.randint(0, 256, (n, d, d // 2), dtype=torch.uint8, device=DEV)
+    scales = torch.ones(n, d, d // 128, device=DEV)
+    for make in (lambda: wc.WideLinear4bit.from_modules(lin), lambda: wc.WideLinear4bit.from_codes(codes, scales, in_features=d)):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        mod = make()
+        torch.cuda.synchronize()
+        assert torch.cuda.max_memory_allocated() - before <= 4 * n * d * d
+        del mod
