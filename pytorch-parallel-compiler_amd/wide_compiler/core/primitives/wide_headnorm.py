@@ -42,11 +42,22 @@ class WideHeadNormRotary(nn.Module):
         self.eps = eps
         self.q_weight = nn.Parameter(torch.ones(n, head_dim))
         self.k_weight = nn.Parameter(torch.ones(n, head_dim))
-        freq = torch.tensor([base ** (-2.0 * p / rotary_dim) / (2.0 * math.pi) for p in range(rotary_dim // 2)],
-                            dtype=torch.float64)
         # turns per position, as the bits of fp64: .to(dtype) leaves integer buffers as they are
-        self.register_buffer("_freq_bits", freq.view(torch.int64), persistent=False)
+        self.register_buffer("_freq_bits", self._frequencies(None), persistent=False)
         self._plans = _serve.Plans()
+
+    def _frequencies(self, device: Optional[torch.device]) -> Tensor:
+        rotary_dim, base, _ = self._rotation
+        turns = [base ** (-2.0 * p / rotary_dim) / (2.0 * math.pi) for p in range(rotary_dim // 2)]
+        return torch.tensor(turns, dtype=torch.float64, device=device).view(torch.int64)
+
+    def _apply(self, fn, recurse: bool = True):
+        """No state_dict holds the frequencies, and to_empty() leaves a module that was made on the meta device with whatever
+        stood in memory: wherever the module goes they are made again."""
+        super()._apply(fn, recurse)
+        device = self._buffers["_freq_bits"].device
+        self._buffers["_freq_bits"] = self._frequencies(device)
+        return self
 
     # What turns the heads is a module's for good: its frequencies and its plans are made of it.
     @property

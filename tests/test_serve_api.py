@@ -513,3 +513,19 @@ def test_a_growing_bound_keeps_the_plans(monkeypatch, anywhere):
     for call in (lambda: cache.attend(q, table, n, max_length=-1), lambda: cache.read(table, n, -1)):
         with pytest.raises(RuntimeError, match="negative"):
             call()
+
+
+def test_head_norm_made_on_the_meta_device_turns_as_any_other():
+    """Frequencies are no part of a state_dict: a module that gets its memory later has them all the same."""
+    import wide_compiler as wc
+    made = wc.WideHeadNormRotary(2, 64, rotary_dim=32, base=500.0)
+    with torch.device("meta"):
+        later = wc.WideHeadNormRotary(2, 64, rotary_dim=32, base=500.0)
+    assert later._freq_bits.is_meta and later.half()._freq_bits.is_meta
+    torch.full((16,), 7)                                     # what to_empty may find in memory
+    later = later.to_empty(device="cpu")
+    later.load_state_dict(made.state_dict(), strict=True)
+    assert torch.equal(later._freq_bits, made._freq_bits) and later._freq_bits.view(torch.float64)[0] > 0.1
+    assert torch.equal(made.to(torch.bfloat16)._freq_bits, later._freq_bits)
+    none = wc.WideHeadNormRotary(1, 64, rotary_dim=0).double()
+    assert none._freq_bits.numel() == 0
