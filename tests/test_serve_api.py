@@ -6,8 +6,10 @@ import hashlib
 import os
 import re
 import shutil
+import struct
 import subprocess
 import sys
+import tempfile
 
 import pytest
 import torch
@@ -529,3 +531,51 @@ def test_head_norm_made_on_the_meta_device_turns_as_any_other():
     assert torch.equal(made.to(torch.bfloat16)._freq_bits, later._freq_bits)
     none = wc.WideHeadNormRotary(1, 64, rotary_dim=0).double()
     assert none._freq_bits.numel() == 0
+
+
+def _kernel_registers(part):
+    """{mangled name: (VGPRs with AGPRs, bytes of scratch)} of the kernels in the built library whose name has `part`: what
+    the compiler wrote into the notes of its code objects."""
+    readelf = next((r for r in ("/opt/rocm/llvm/bin/llvm-readelf", "llvm-readelf") if shutil.which(r)), None)
+    if readelf is None:
+        pytest.skip("no llvm-readelf")
+    data = open(os.path.join(PKG, "wide_compiler", "libwide_hip.so"), "rb").read()
+    magic, found, at = b"__CLANG_OFFLOAD_BUNDLE__", {}, -1
+    while (at := data.find(magic, at + 1)) >= 0:
+        entry = at + 32
+        for _ in range(struct.unpack_from("<Q", data, at + 24)[0]):
+            offset, size, length = struct.unpack_from("<QQQ", data, entry)
+            target = data[entry + 24:entry + 24 + length]
+            entry += 24 + length
+            code = data[at + offset:at + offset + size]
+            if b"gfx950" not in target or part.encode() not in code:
+                continue
+            with tempfile.NamedTemporaryFile() as f:
+                f.write(code)
+                f.flush()
+                notes = subprocess.run([readelf, "--notes", f.name], capture_output=True, text=True, timeout=60).stdout
+            for kernel in notes.split("  - .agpr_count:")[1:]:
+                field = lambda name: re.search(r"\.%s:\s+(\S+)" % name, kernel).group(1)  # noqa: E731
+                if part in field("symbol"):
+                    found[field("symbol")] = (int(field("vgpr_count")), int(field("private_segment_fixed_size")))
+    return found
+
+
+def test_attention_shares_follow_the_registers():
+    """The number of workgroups a compute unit has room for, by which paged attention cuts its line of tiles, is what the
+    built kernels' registers leave: of 512 a lane and quarter of a unit, in steps of 8, for workgroups of a wave each."""
+    source = open(os.path.join(PKG, "csrc", "paged_attention.hip")).read()
+    fit = re.search(r"kFit\[2\]\[3\]\[3\] = \{(.*)\};", source).group(1)
+    fit = [int(x) for x in re.findall(r"\d+", fit)]
+    kernels = _kernel_registers("paged_attention_kernel")
+    seen = 0
+    for q8 in (0, 1):
+        for t, name in enumerate(("f", "DF16b", "DF16_")):
+            for w, dc in enumerate((64, 128, 256)):
+                stored = "a" if q8 else "S3_" if name != "f" else "f"
+                match = [k for k in kernels if re.search(r"kernelI%s(%s|%s)Li%dELi4E" % (name, stored, "a" if q8 else name, dc), k)]
+                assert len(match) == 1, (name, q8, dc, match)
+                registers = -(-kernels[match[0]][0] // 8) * 8
+                assert fit[(q8 * 3 + t) * 3 + w] == min(512 // registers, 8), (match[0], registers)
+                seen += 1
+    assert seen == 18
