@@ -16,7 +16,9 @@ may go to the same slot.  Pools stand as
 
 With ``quantized=True`` a row (one head of one token) is 8-bit codes and one fp32 scale: scale =
 max(max |x| / 127, 2^-126), code = x / scale to the nearest, ties to even; a row with an infinity
-or NaN reads back as NaN.
+or NaN reads back as NaN.  ``attend`` sums a score before the key's scale multiplies it and takes a
+weight times the value's scale as bf16 numbers: queries from 2^110 on can overflow over 8 bits, and
+values whose row's largest is under 2^-90 lose bits.
 
 A block-table entry outside the pool, a token past the table's end or a count or length beyond the
 call's is never followed: nothing is written there, it reads as zeros, takes no part in the
