@@ -15,7 +15,7 @@
 // 42, weights from memory; and they lose 2^-24 of 143 sum |x|, also where weights are 0, and overflow from x of 2^114 on.)
 // fp32 goes as three bf16 planes of x (every bit of it down to 2^-110); a row of x with an infinity gives NaN there.
 //
-// 4 models' [4096 -> 4096] in bf16, one row (35 MB): 10.4 us, of which an empty launch is 3.3; 8 models' [2048 -> 8192]
+// 4 models' [4096 -> 4096] in bf16, one row (35 MB): 11.1 us, of which an empty launch is 3.3; 8 models' [2048 -> 8192]
 // in fp16, 64 rows (84 MB, 17 GFLOP): 30 us, half of it the instructions that make numbers of codes and scale the
 // groups' sums, which with two to four waves a unit's quarter only partly hide behind the loads.
 //

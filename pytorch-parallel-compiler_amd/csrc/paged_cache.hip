@@ -3,7 +3,7 @@
 // One group of lanes has a row: head_dim values of one head of one token, 16 bytes of them a lane.  Both
 // kernels only move rows, so they are bound by memory; what decides is that every access is a whole vector
 // and that enough of them are in flight.  16 sequences' 750 to 1500 new tokens of 8 heads of 128 columns in bf16:
-// written as they are (147 MB) 32 us, 4.6 TB/s; as codes (112 MB) 32 us, which the search for each row's scale and the
+// written as they are (154 MB) 26 us, 6.0 TB/s; as codes (112 MB) 32 us, which the search for each row's scale and the
 // codes' arithmetic keep from 25; codes read back (145 MB) 26 us, 5.5 TB/s.
 //
 // 8 bits: scale = max(max |x| / 127, 2^-126) (one unit less for fp32's largest value), code = x / scale to the nearest, ties to even.  The quotient is
