@@ -95,11 +95,11 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
   const int start = a.start[seq];
   int n = a.steps;
   if (a.count) n = a.count[seq];
+  if (start < 0) return;                 // whatever its count says
   if (n > a.steps) {
     n = a.steps;
     paged_fault(a.t);
   }
-  if (start < 0) return;
   const uint32_t rows = static_cast<uint32_t>(max(n, 0)) * a.t.heads;       // to write
   const uint32_t r0 = tile * (groups * kRows) + (tid >> a.lanes_log2);
   if (tile * (groups * kRows) >= rows) return;

@@ -236,3 +236,18 @@ def test_codes_of_the_largest_values_are_finite(dtype):
         big = ref.abs().max()
         assert ((got - ref).abs() <= big * (1 / 254 + torch.finfo(dtype).eps + 2.0 ** -22)).all()
         assert ((got[..., [0, 63]] - ref[..., [0, 63]]).abs() <= big * (torch.finfo(dtype).eps + 2.0 ** -22)).all()
+
+
+def test_sequences_that_take_no_part_raise_nothing():
+    """A sequence of negative start is left out, whatever its count says; a count beyond the rows of another is reported."""
+    cache, k, v, table, start, count = _write(torch.bfloat16, False, 2, 2, 5, 2, 64, 16, 9, 71)
+    start[0, 1], count[0, 1] = -1, 99
+    before = cache.k_pages.clone()
+    expect = _expect(before, k, table, start, torch.where(start < 0, 0, count), 16, 64)
+    cache.write(k, v, table, start, count)
+    cache.index_error()
+    assert torch.equal(cache.k_pages, expect)
+    count[1, 1] = 6
+    cache.write(k, v, table, start, count)
+    with pytest.raises(IndexError):
+        cache.index_error()
