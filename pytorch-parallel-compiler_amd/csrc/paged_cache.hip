@@ -5,20 +5,16 @@
 // and that enough of them are in flight.  16 sequences' 750 to 1500 new tokens of 8 heads of 128 columns in bf16:
 // written as they are (154 MB) 26 us, 6.0 TB/s; as codes (112 MB) 32 us, which the search for each row's scale and the
 // codes' arithmetic keep from 25; codes read back (145 MB) 26 us, 5.5 TB/s.
-//
-// 8 bits: scale = max(max |x| / 127, 2^-126) (one unit less for fp32's largest value), code = x / scale to the nearest, ties to even.  The quotient is
-// never formed: c = x * (1 / scale) to the nearest is off by at most one, and then only next to a half; the remainder
-// x - c scale is exact (one fused multiply-add whose result fits 24 bits) and its place against scale / 2
-// puts c right, for the lanes that have such a value.  The code is so a function of x and scale alone.
+// How a row's codes come about is in wc_codes.h.
 #include <algorithm>
 
+#include "wc_codes.h"
 #include "wc_paged.h"
 
 namespace wc {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kMost = 0x1.020406p121f;      // the largest scale: 127 of the next one round to infinity in fp32
 constexpr int kRows = 4;           // rows of a group of lanes, all on their way at once (those codes written and read: 61 us;
                                    // one row 68, two 64, eight 73)
 
@@ -26,26 +22,6 @@ template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
   T v[V];
 };
-
-// x / scale to the nearest as the low byte of the result, by adding 1.5 2^23 (after which a float's last bit is 1), and
-// how far that is from x
-constexpr float kRound = 0x1.8p23f;
-__device__ __forceinline__ uint32_t code8(float x, float scale, float inv, float& off) {
-  const float c = fmaf(x, inv, kRound);
-  off = fabsf(fmaf(kRound - c, scale, x));
-  return __builtin_bit_cast(uint32_t, c);
-}
-// the code of a value whose quotient may be next to a half
-__device__ __forceinline__ uint32_t code8_near_half(float x, float scale, float inv) {
-  float c = fmaf(x, inv, kRound) - kRound;
-  const float r = fmaf(-c, scale, x), half = 0.5f * scale;
-  const bool odd = static_cast<int>(c) & 1;
-  if (r > half || (r == half && odd))
-    c += 1.f;
-  else if (r < -half || (r == -half && odd))
-    c -= 1.f;
-  return __builtin_bit_cast(uint32_t, c + kRound);
-}
 
 // The largest magnitude of a lane's values as the bits of a float, under which an infinity or NaN is larger than any
 // finite value; 16-bit values are compared two at a time.
@@ -145,7 +121,7 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
       uint32_t top = largest<T, V, NC>(v);
       for (int off = lanes >> 1; off; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 64)));
       const bool finite = top < 0x7f800000u;
-      const float scale = finite ? fminf(fmaxf(__builtin_bit_cast(float, top) / 127.f, 0x1p-126f), kMost) : __builtin_nanf("");
+      const float scale = finite ? row_scale(top) : __builtin_nanf("");
       const float inv = __builtin_amdgcn_rcpf(scale);
       uint32_t code[NC][V];
       float far = 0.f;
@@ -157,8 +133,7 @@ __global__ __launch_bounds__(kThreads) void cache_write_kernel(Write a) {
           code[c][e] = code8(to_f32(v[c].v[e]), scale, inv, off);
           far = fmaxf(far, off);
         }
-      // 2^-15 covers the product's rounding and inv's: 2^-22 of a quotient of up to 127
-      if (far > scale * (0.5f - 0x1p-15f))
+      if (far > scale * kNearHalf)
 #pragma unroll
         for (int c = 0; c < NC; ++c)
 #pragma unroll

@@ -1,0 +1,708 @@
+// Attention of one new token of every sequence over a prefix that groups of sequences share and over tokens of its own.
+//
+//   o = sum_i exp(s_i - m) v_i / sum_i exp(s_i - m),   s_i = scale q . k_i,   i over the prefix and the own tokens
+//
+// The softmax is joined from parts that have a maximum, a sum and an output each, so a prefix is walked once for all
+// its sequences: their query heads are the rows that every K and V row meets, 16 for each tile of the matrix instructions.
+// Both walks are one kernel, of stretches of tokens with rows that read them: a prefix with the heads of its sequences,
+// and a sequence's own tokens with its heads.  A second kernel joins the parts.
+//
+// A wave takes 32 tokens at a time, K and V straight from memory into the operands of MFMAs:
+//   scores   S [token][row] = K Q^T, lane l brings 16-byte pieces of token l % 16
+//   softmax  the accumulator has row l % 16 and tokens 4 (l / 16) + r, of two tiles of 16 tokens
+//   output   O^T [column][row] = V^T P, lane l loads those 8 tokens' rows at columns of its own, and operand e pairs
+//            up their e-th values
+#include <algorithm>
+
+#include "wc_answer_abi.h"
+#include "wc_paged_attn.h"
+
+namespace wc {
+namespace {
+
+constexpr int kTile = kPagedTile;    // tokens a wave takes at a time
+constexpr int kLeast = 8;            // tiles in a share at least, two for each of its waves
+constexpr int kTarget = 1024;        // shares of a line at most
+constexpr int kWaves = 4;
+
+// Stretches of tokens and the sequences that read them
+struct Walk {
+  PagedTable t;
+  const int32_t* lengths;            // [units]
+  float* part;                       // [parts][share][heads][dh]
+  float2* ml;                        // [parts][share][heads]: maximum and sum, -1 where there are no tokens
+  int2* parts;                       // [units]: first part and how many, where the line of all tiles is cut (budget > 0)
+  int32_t units, share, budget, most, rows;          // rows: query heads of a unit that read one key head
+  FastDiv by_tiles, by_units;        // tiles of rows; units of a model
+};
+struct Shared {
+  Walk walk[2];                      // prefixes, own tokens
+  const char *k, *v, *q;
+  const float *ks, *vs;
+  char* o;
+  int64_t qn, qb, qh;
+  int32_t heads, group, dh, row_bytes, qvec, blocks;  // blocks: workgroups of the prefixes' walk
+  FastDiv by_kvh, by_group, by_heads, by_share;
+  float scale;                       // of the scores, times log2 e
+};
+
+__device__ __forceinline__ PagedSpan span_of(const Walk& w, int unit) { return paged_span(0, w.lengths[unit], w.most); }
+
+// Where stretches are cut, the tiles of all of them count as one line, of which every workgroup (of a key head and a tile of rows)
+// has an equal share however uneven the lengths are: share w is tiles [w size, (w + 1) size), of one unit or the ends and
+// wholes of several.  What share w has of unit s is part w + s: no two are alike, a unit's parts are neighbours, and there
+// are at most shares + units of them.  Every wave finds its share from the lengths by itself.
+struct Line {
+  int size, total;
+};
+__device__ __forceinline__ Line line_of(const Walk& w, int lane) {
+  int total = 0;
+  for (int s = lane; s < w.units; s += 64) total += paged_tiles(span_of(w, s));
+#pragma unroll
+  for (int off = 32; off; off >>= 1) total += __shfl_xor(total, off, 64);
+  return Line{max((total + w.budget - 1) / w.budget, kLeast), total};
+}
+// the unit that has tile `at` of the line (at < total), and the line's tiles before it
+__device__ __forceinline__ int2 find_tile(const Walk& w, int at, int lane) {
+  int done = 0;
+  for (int s0 = 0; s0 < w.units; s0 += 64) {
+    const int s = s0 + lane, n = s < w.units ? paged_tiles(span_of(w, s)) : 0;
+    const int start = done + before(n, lane);
+    const uint64_t mine = __ballot(at >= start && at < start + n);
+    if (mine) {
+      const int l = __ffsll(static_cast<unsigned long long>(mine)) - 1;
+      return make_int2(s0 + l, __shfl(start, l, 64));
+    }
+    done = __shfl(start + n, 63, 64);
+  }
+  return make_int2(w.units, 0);
+}
+// each unit's first part and how many it has, for the kernel that joins them; and the fault of lengths that were cut
+__device__ __forceinline__ void list_parts(const Walk& w, int size, int lane) {
+  int done = 0;
+  for (int s0 = 0; s0 < w.units; s0 += 64) {
+    const int s = s0 + lane;
+    const PagedSpan span = s < w.units ? span_of(w, s) : PagedSpan{0, 0, false};
+    if (span.cut) paged_fault(w.t);
+    const int n = paged_tiles(span);
+    const int start = done + before(n, lane), w0 = start / size;
+    if (s < w.units) w.parts[s] = n ? make_int2(w0 + s, (start + n - 1) / size - w0 + 1) : make_int2(0, 0);
+    done = __shfl(start + n, 63, 64);
+  }
+}
+
+// QT: type of q and o; KT: stored type (int8_t for codes); DC: columns provided for; RT: tiles of 16 rows
+template <typename QT, typename KT, int DC, int RT>
+__device__ __forceinline__ void walk(const Shared& a, const Walk& w, uint32_t id, float* lds) {
+  constexpr bool kF32 = std::is_same<KT, float>::value;
+  constexpr bool kQ8 = std::is_same<KT, int8_t>::value;
+  // fp16 has no room for a weight times a row's scale: over codes, fp16 queries go as two bf16 planes
+  typedef typename std::conditional<std::is_same<QT, f16>::value && !kQ8, f16, bf16>::type MT;
+  constexpr int ES = sizeof(KT);
+  constexpr int CH = 16 / ES;                                   // columns in 16 bytes
+  constexpr int NCK = DC / (4 * CH);                            // 16-byte pieces of a K row per lane
+  constexpr int VE = DC / 16, CE = VE * ES > 16 ? CH : VE, NCV = VE / CE;   // columns of V per lane
+  constexpr int NF = DC / 32;                                   // 16-bit score products per 16 tokens
+  constexpr int NQ = std::is_same<QT, float>::value ? 3 : std::is_same<QT, MT>::value ? 1 : 2;   // planes of q
+  constexpr int NP = std::is_same<MT, f16>::value ? 2 : 3;                                      // and of P
+  // fp16 weights are taken 2^14 times as large (m - 14 in their exponents), so that those far under 1 keep their bits
+  constexpr float kShift = std::is_same<MT, f16>::value ? 14.f : 0.f;
+  constexpr int NW = kWaves;
+  typedef typename Raw<CE * ES>::type VR;
+
+  const int lane0 = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t up = fdiv(id, w.by_tiles);
+  const int row0 = (id - up * w.by_tiles.d) * (RT * 16);
+  id = up;
+  up = fdiv(id, a.by_kvh);
+  const int kvh = id - up * a.by_kvh.d;
+  // this workgroup's tiles: those of one unit, or a share of the line
+  int unit = up, start = 0, from = 0, to = 1 << 30;
+  if (w.budget > 0) {
+    const Line line = line_of(w, lane0);
+    if (id == 0 && row0 == 0 && wave == 0) list_parts(w, line.size, lane0);
+    from = up * line.size;
+    if (from >= line.total) return;
+    to = min(from + line.size, line.total);
+    const int2 first = find_tile(w, from, lane0);
+    unit = first.x;
+    start = first.y;
+  }
+  for (;; ++unit) {
+    // What depends on the lane and the sizes alone would be kept from one unit to the next, in more registers than there
+    // are; it is worked out again.
+    int lane = lane0, rows = w.rows, dh = a.dh;
+    asm volatile("" : "+v"(lane), "+s"(rows), "+s"(dh));
+    const int j = lane & 15, g = lane >> 4;
+    const uint32_t model = fdiv(unit, w.by_units), b0 = (unit - model * w.by_units.d) * w.share;
+    const int tile_lo = max(from - start, 0);
+    // The table's entry for token `lane % 32` of a tile, two tiles ahead of its use; nothing looks at it (and so waits for
+    // it) before row_of, the pool's row of that token or -1 for none.
+    auto look = [&](int tile) { return paged_entry(w.t, unit, static_cast<uint32_t>(tile) * kTile + (lane & 31)); };
+    int row = look(tile_lo + wave), next = look(tile_lo + wave + NW);
+    const PagedSpan span = span_of(w, unit);
+    const int hi = span.hi, tiles = paged_tiles(span), tile_hi = min(tiles, to - start);
+    if (w.budget == 0 && span.cut && threadIdx.x == 0) paged_fault(w.t);
+    start += tiles;
+    if (w.budget > 0 && tile_lo >= tile_hi) continue;             // a unit without tokens
+
+    // the rows of q: row r is head r % group of sequence r / group; past the last the last again
+    constexpr int N = kF32 ? 4 : 8, NX = kF32 ? NCK : NF;
+    auto column = [&](int i) {                                    // the same columns of each product as K's
+      return kF32 ? (i * 4 + g) * 4 : kQ8 ? ((i / 2) * 4 + g) * 16 + (i % 2) * 8 : (i * 4 + g) * 8;
+    };
+    constexpr int NV = 16 / sizeof(QT);
+    u32x4 qf[RT][kF32 ? 1 : NF][NQ];
+    float q32[RT][kF32 ? NCK : 1][4];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int r = min(row0 + t * 16 + j, rows - 1);
+      const uint32_t s = fdiv(r, a.by_group), h = r - s * a.by_group.d;
+      const QT* q = reinterpret_cast<const QT*>(a.q) + model * a.qn + (b0 + s) * a.qb + (kvh * a.group + h) * a.qh;
+#pragma unroll
+      for (int i = 0; i < NX; ++i) {
+        QT v[N];
+        if (a.qvec) {
+#pragma unroll
+          for (int e = 0; e < N; e += NV) {
+            const int d = column(i) + e;
+            __builtin_memcpy(v + e, __builtin_assume_aligned(q + (d < dh ? d : 0), 16), 16);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < N; ++e) v[e] = q[column(i) + e < dh ? column(i) + e : 0];
+        }
+        float x[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = column(i) + e < dh ? to_f32(v[e]) : 0.f;
+        if constexpr (kF32) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q32[t][i][e] = x[e];
+        } else {
+          planes<MT, NQ>(x, qf[t][i]);
+        }
+      }
+    }
+
+    f32x4 acc[RT][NCV][CE] = {};
+    float m[RT], l[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) m[t] = -INFINITY, l[t] = 0.f;
+    bool any = false;
+
+    auto row_of = [&](int tile, int page) {
+      const int tok = tile * kTile + (lane & 31);
+      if (tile >= tile_hi || tok >= hi) return -1;
+      const int r = paged_row(w.t, page, tok, kvh);
+      if (r < 0) paged_fault(w.t);
+      return r;
+    };
+    // Rows that no token has are read as row 0 of the pool and taken out afterwards.  K comes one tile ahead, into the
+    // registers that the scores have just been taken from, while softmax and V keep the wave busy.
+    u32x4 kf[2][NCK];
+    float ks = 0.f;
+    auto load_k = [&](int row) {
+      if constexpr (kQ8) ks = a.ks[max(row, 0)];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const char* p = a.k + static_cast<int64_t>(max(__shfl(row, s * 16 + j, 64), 0)) * a.row_bytes;
+#pragma unroll
+        for (int c = 0; c < NCK; ++c) {
+          const int at = (c * 4 + g) * 16;
+          kf[s][c] = *reinterpret_cast<const u32x4*>(p + (at < a.row_bytes ? at : 0));
+        }
+      }
+    };
+    if (tile_lo + wave < tile_hi) {
+      row = row_of(tile_lo + wave, row);
+      load_k(row);
+    }
+    for (int tile = tile_lo + wave; tile < tile_hi; tile += NW) {
+      const bool full = __all(row >= 0);
+      any |= __any(row >= 0);
+      float vs = 0.f;
+      if constexpr (kQ8) vs = a.vs[max(row, 0)];
+      int vrow[8];
+      VR vf[8][NCV];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        vrow[u] = __shfl(row, (u >> 2) * 16 + g * 4 + (u & 3), 64);
+        const char* p = a.v + static_cast<int64_t>(max(vrow[u], 0)) * a.row_bytes;
+#pragma unroll
+        for (int c = 0; c < NCV; ++c) {
+          const int at = (c * 16 + j) * CE * ES;
+          vf[u][c] = *reinterpret_cast<const VR*>(p + (at < a.row_bytes ? at : 0));
+        }
+      }
+      // columns that a row doesn't have (their q is 0, but 0 times what stands elsewhere may not be)
+      if (a.row_bytes < DC * ES) {
+#pragma unroll
+        for (int c = 0; c < NCK; ++c)
+          if ((c * 4 + g) * 16 >= a.row_bytes) clear(kf[0][c]), clear(kf[1][c]);
+      }
+
+      f32x4 s2[RT][2] = {};
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if constexpr (kF32) {
+#pragma unroll
+          for (int c = 0; c < NCK; ++c)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int t = 0; t < RT; ++t)
+                s2[t][s] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(f32x4, kf[s][c])[e], q32[t][c][e], s2[t][s], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int f = 0; f < NF; ++f) {
+            u32x4 x;
+            if constexpr (kQ8) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t c = kf[s][f / 2][(f % 2) * 2 + e / 2];
+                x[e] = pack2<MT>(byte_f32(c, (e & 1) * 2), byte_f32(c, (e & 1) * 2 + 1));
+              }
+            } else {
+              x = kf[s][f];
+            }
+#pragma unroll
+            for (int n = NQ - 1; n >= 0; --n)
+#pragma unroll
+              for (int t = 0; t < RT; ++t)
+                s2[t][s] = mma16<MT>(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, qf[t][f][n]), s2[t][s]);
+          }
+        }
+      }
+      float kscale[kQ8 ? 8 : 1], vscale[kQ8 ? 8 : 1];
+      if constexpr (kQ8) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          kscale[u] = __shfl(ks, (u >> 2) * 16 + g * 4 + (u & 3), 64);
+          vscale[u] = __shfl(vs, (u >> 2) * 16 + g * 4 + (u & 3), 64);
+        }
+      }
+      // behind the last tile too (as row 0): were there a way round these loads, the wait for V would have to be one for
+      // everything in flight
+      row = row_of(tile + NW, next);
+      load_k(row);
+      next = look(tile + 2 * NW);
+      if (!full) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (vrow[u] < 0) {
+#pragma unroll
+            for (int c = 0; c < NCV; ++c) clear(vf[u][c]);
+          }
+      }
+      u32x4 pf[RT][NP];
+      float p[RT][8];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          p[t][u] = s2[t][u >> 2][u & 3] * a.scale;
+          if constexpr (kQ8) p[t][u] *= kscale[u];
+          if (!full && vrow[u] < 0) p[t][u] = -INFINITY;
+          top = fmaxf(top, p[t][u]);
+        }
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        top = fmaxf(top, __shfl_xor(top, 32, 64));
+        const float mn = fmaxf(m[t], top), use = finite_top(mn) - kShift;
+        if (__any(mn > m[t])) {
+          const float shrink = weight2(m[t], finite_top(mn));
+          l[t] *= shrink;
+#pragma unroll
+          for (int c = 0; c < NCV; ++c)
+#pragma unroll
+            for (int e = 0; e < CE; ++e) acc[t][c][e] *= shrink;
+        }
+        m[t] = mn;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          p[t][u] = __builtin_amdgcn_exp2f(p[t][u] - use);
+          if (!full && vrow[u] < 0) p[t][u] = 0.f;
+          l[t] += p[t][u];
+          if constexpr (kQ8) p[t][u] = !full && vrow[u] < 0 ? 0.f : p[t][u] * vscale[u];
+        }
+        if constexpr (!kF32) {
+          if constexpr (std::is_same<QT, float>::value)
+            planes<MT, NP>(p[t], pf[t]);
+          else
+            weight_planes<MT, NP>(p[t], pf[t]);
+        }
+      }
+      if constexpr (kF32) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+          for (int c = 0; c < NCV; ++c)
+#pragma unroll
+            for (int e = 0; e < CE; ++e)
+#pragma unroll
+              for (int t = 0; t < RT; ++t)
+                acc[t][c][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, dword(vf[u][c], e)), p[t][u], acc[t][c][e], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int c = 0; c < NCV; ++c)
+#pragma unroll
+          for (int e = 0; e < CE; ++e) {
+            u32x4 x;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              if constexpr (kQ8)
+                x[u] = pack2<MT>(byte_f32(dword(vf[2 * u][c], e / 4), e & 3), byte_f32(dword(vf[2 * u + 1][c], e / 4), e & 3));
+              else
+                x[u] = __builtin_amdgcn_perm(dword(vf[2 * u + 1][c], e / 2), dword(vf[2 * u][c], e / 2),
+                                             e & 1 ? 0x07060302u : 0x05040100u);
+            }
+#pragma unroll
+            for (int n = NP - 1; n >= 0; --n)
+#pragma unroll
+              for (int t = 0; t < RT; ++t)
+                acc[t][c][e] = mma16<MT>(__builtin_bit_cast(bf16x8, x), __builtin_bit_cast(bf16x8, pf[t][n]), acc[t][c][e]);
+          }
+      }
+    }
+
+    // join the waves, a tile of rows at a time: [NW][16][DC] outputs, then [NW][16] maxima and sums (a sum of -1: no tokens),
+    // which become the weights of the waves' outputs
+    float* om = lds + NW * 16 * DC;
+    float* ol = om + NW * 16;
+    const int64_t first = static_cast<int64_t>(w.budget > 0 ? up + unit : unit) * w.share;      // part's first (sequence, ..)
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      if (row0 + t * 16 >= rows) break;
+      l[t] += __shfl_xor(l[t], 16, 64);
+      l[t] += __shfl_xor(l[t], 32, 64);
+      __syncthreads();
+      float* o = lds + (wave * 16 + j) * DC;
+#pragma unroll
+      for (int c = 0; c < NCV; ++c)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+          for (int e = 0; e < CE; ++e) o[(c * 16 + g * 4 + r) * CE + e] = acc[t][c][e][r];
+      if (g == 0) {
+        om[wave * 16 + j] = m[t];
+        ol[wave * 16 + j] = any ? l[t] : -1.f;
+      }
+      __syncthreads();
+      auto at = [&](int h) {                         // of row h of the tile: its place among the part's (sequence, head)
+        const uint32_t r = row0 + t * 16 + h, s = fdiv(r, a.by_group);
+        return (first + s) * a.heads + kvh * a.group + (r - s * a.by_group.d);
+      };
+      if (static_cast<int>(threadIdx.x) < min(16, rows - row0 - t * 16)) {
+        const int h = threadIdx.x;
+        float mw[NW], lw[NW], top = -INFINITY, sum = 0.f;
+        bool some = false;
+#pragma unroll
+        for (int v = 0; v < NW; ++v) {
+          mw[v] = om[v * 16 + h];
+          lw[v] = ol[v * 16 + h];
+          top = fmaxf(top, mw[v]);
+          some |= !(lw[v] < 0.f);
+        }
+#pragma unroll
+        for (int v = 0; v < NW; ++v) {
+          const float f = weight2(mw[v], finite_top(top));            // 0 for a wave without tokens
+          om[v * 16 + h] = f;
+          sum += lw[v] < 0.f ? 0.f : f * lw[v];
+        }
+        w.ml[at(h)] = make_float2(top, some ? sum : -1.f);
+      }
+      __syncthreads();
+      for (int i = threadIdx.x; i < min(16, rows - row0 - t * 16) * (DC / 4); i += NW * 64) {
+        const int h = i / (DC / 4), d = i % (DC / 4) * 4;
+        f32x4 sum = {};
+#pragma unroll
+        for (int v = 0; v < NW; ++v) sum += om[v * 16 + h] * *reinterpret_cast<const f32x4*>(lds + (v * 16 + h) * DC + d);
+        float* y = w.part + at(h) * dh;
+        if (dh % 4 == 0) {
+          if (d < dh) *reinterpret_cast<f32x4*>(y + d) = sum;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < dh) y[d + e] = sum[e];
+        }
+      }
+    }
+    if (w.budget == 0 || start >= to) return;
+    __syncthreads();
+  }
+}
+
+template <typename QT, typename KT, int DC, int RT>
+__global__ __launch_bounds__(kWaves * 64) void shared_attention_kernel(Shared a) {
+  extern __shared__ float lds[];
+  const int own = static_cast<int>(blockIdx.x) >= a.blocks;
+  const uint32_t id = blockIdx.x - (own ? a.blocks : 0);
+  if constexpr (RT == 1) {
+    walk<QT, KT, DC, 1>(a, a.walk[own], id, lds);
+  } else {
+    if (own)
+      walk<QT, KT, DC, 1>(a, a.walk[1], id, lds);
+    else
+      walk<QT, KT, DC, RT>(a, a.walk[0], id, lds);
+  }
+}
+
+// Joins the parts of one (sequence, query head): their weights first, then their outputs, four columns a thread and as
+// many parts at a time as threads remain.  VEC: rows are whole vectors.
+template <typename QT, bool VEC>
+__global__ __launch_bounds__(256) void shared_join_kernel(Shared a) {
+  constexpr int kMost = 2 * kTarget;
+  __shared__ float weight[kMost], out[4 * 256], red[8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t at = blockIdx.x, seq = fdiv(at, a.by_heads), head = at - seq * a.by_heads.d;
+  const uint32_t unit = fdiv(seq, a.by_share), place = seq - unit * a.by_share.d;
+  const Walk &w0 = a.walk[0], &w1 = a.walk[1];
+  const int2 p0 = w0.parts[unit], p1 = w1.budget > 0 ? w1.parts[seq] : make_int2(seq, 1);
+  const int n0 = min(p0.y, kTarget), n = w1.lengths[seq] < 0 ? 0 : n0 + min(p1.y, kTarget);
+  // row of part s of these: the prefix's, then the own
+  auto row = [&](int s) {
+    return s < n0 ? ((p0.x + s) * static_cast<int64_t>(w0.share) + place) * a.heads + head
+                  : (p1.x + s - n0) * static_cast<int64_t>(a.heads) + head;
+  };
+  const int quads = (a.dh + 3) / 4, rows = 256 / quads, q = tid % quads, r = tid / quads;
+  float top = -INFINITY;
+  bool some = false;
+  for (int s = tid; s < n; s += 256) {
+    const float2 x = (s < n0 ? w0.ml : w1.ml)[row(s)];
+    top = fmaxf(top, x.x);
+    some |= !(x.y < 0.f);
+  }
+#pragma unroll
+  for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  if (lane == 0) red[wave] = top;
+  some = __syncthreads_or(some);
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  float sum = 0.f;
+  for (int s = tid; s < n; s += 256) {
+    const float2 x = (s < n0 ? w0.ml : w1.ml)[row(s)];
+    const float f = x.y < 0.f ? 0.f : weight2(x.x, finite_top(top));
+    weight[s] = f;
+    sum += x.y < 0.f ? 0.f : f * x.y;
+  }
+#pragma unroll
+  for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  if (lane == 0) red[4 + wave] = sum;
+  __syncthreads();
+  sum = red[4] + red[5] + red[6] + red[7];
+  f32x4 o = {};
+  if (r < rows) {
+    for (int s = r; s < n; s += rows) {
+      const float* p = (s < n0 ? w0.part : w1.part) + row(s) * a.dh + q * 4;
+      f32x4 v;
+      if constexpr (VEC) {
+        v = *reinterpret_cast<const f32x4*>(p);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = p[q * 4 + e < a.dh ? e : 0];
+      }
+      // a part without tokens holds zeros
+      o += weight[s] * v;
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e * 256 + tid] = o[e];
+  __syncthreads();
+  if (tid >= a.dh) return;
+  float v = 0.f;
+  for (int i = 0; i < rows; ++i) v += out[(tid & 3) * 256 + i * quads + tid / 4];
+  reinterpret_cast<QT*>(a.o)[static_cast<int64_t>(at) * a.dh + tid] = from_f32<QT>(some ? v / sum : 0.f);
+}
+
+// How the work is spread: tiles of 16 rows that a workgroup of the prefixes' walk has, and shares of both lines (own tokens
+// 0: whole sequences)
+struct Plan {
+  int rt;
+  int64_t budget[2], parts[2];
+};
+int tiles_of_rows(const wc_shared_attn_args& p) {
+  return p.share * (p.q_heads / p.cache.heads) <= 16 || (p.cache.head_dim > 128 && p.cache.dtype == WC_F32) ? 1 : 2;
+}
+Plan plan_of(const wc_shared_attn_args& p) {
+  Plan plan;
+  plan.rt = tiles_of_rows(p);
+  const int64_t group = p.q_heads / p.cache.heads, units = p.cache.n * (p.cache.b / p.share), seqs = p.cache.n * p.cache.b;
+  const int64_t heads0 = p.cache.heads * cdiv(p.share * group, plan.rt * 16), heads1 = p.cache.heads * cdiv(group, 16);
+  const int64_t target = 512;
+  plan.budget[0] = std::min<int64_t>(cdiv(target, heads0), kTarget);
+  plan.parts[0] = plan.budget[0] + units;
+  const bool whole = seqs * heads1 >= 2048 || p.max_length <= 1024;
+  plan.budget[1] = whole ? 0 : std::min<int64_t>(cdiv(target, heads1), kTarget);
+  plan.parts[1] = plan.budget[1] + seqs;
+  return plan;
+}
+// outputs of both walks, their maxima and sums, the lists of parts
+struct Space {
+  int64_t part[2], ml[2], list[2], bytes;
+};
+Space space_of(const wc_shared_attn_args& p, const Plan& plan) {
+  const int64_t units = p.cache.n * (p.cache.b / p.share), seqs = p.cache.n * p.cache.b;
+  const int64_t rows[2] = {plan.parts[0] * p.share * p.q_heads, plan.parts[1] * p.q_heads};
+  Space s;
+  int64_t at = 0;
+  for (int i = 0; i < 2; ++i) {
+    s.part[i] = at;
+    at += (rows[i] * p.cache.head_dim * 4 + 15) / 16 * 16;
+  }
+  for (int i = 0; i < 2; ++i) {
+    s.ml[i] = at;
+    at += rows[i] * 8;
+  }
+  s.list[0] = at;
+  s.list[1] = at + units * 8;
+  s.bytes = s.list[1] + seqs * 8;
+  return s;
+}
+
+template <typename QT, typename KT, int DC, int RT>
+void launch(const Shared& a, int64_t grid, hipStream_t s) {
+  constexpr size_t lds = static_cast<size_t>(kWaves) * 16 * (DC + 2) * sizeof(float);
+  const auto kernel = shared_attention_kernel<QT, KT, DC, RT>;
+  if (lds > 65536)
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
+  kernel<<<static_cast<uint32_t>(grid), kWaves * 64, lds, s>>>(a);
+}
+
+template <typename QT>
+void dispatch(const Shared& a, bool q8, int rt, int64_t grid, hipStream_t s) {
+  auto go = [&](auto k, auto dc) {
+    typedef decltype(k) KT;
+    constexpr int DC = decltype(dc)::value;
+    if (rt == 1) return launch<QT, KT, DC, 1>(a, grid, s);
+    if constexpr (DC <= 128 || sizeof(QT) == 2) launch<QT, KT, DC, 2>(a, grid, s);
+  };
+  auto width = [&](auto k) {
+    if (a.dh <= 64)
+      go(k, std::integral_constant<int, 64>());
+    else if (a.dh <= 128)
+      go(k, std::integral_constant<int, 128>());
+    else
+      go(k, std::integral_constant<int, 256>());
+  };
+  if (q8)
+    width(int8_t());
+  else
+    width(QT());
+}
+
+int64_t most_of(const wc_shared_attn_args& p, int i) {
+  const int64_t len = i ? p.cache.table_len : p.prefix_len, most = i ? p.max_length : p.max_prefix;
+  return p.cache.pages ? std::min(most, len * p.cache.page_size) : 0;
+}
+
+int32_t check(const wc_shared_attn_args& p, const char* what) {
+  const wc_paged_cache& c = p.cache;
+  if (int32_t rc = paged_check(c, what)) return rc;
+  WC_REQUIRE(p.q_heads >= 0 && p.max_prefix >= 0 && p.max_length >= 0 && p.prefix_len >= 0, WC_ERR_SHAPE, "%s: negative size", what);
+  WC_REQUIRE(p.share > 0 && c.b % p.share == 0, WC_ERR_SHAPE, "%s: %lld sequences in groups of %lld", what, (long long)c.b, (long long)p.share);
+  WC_REQUIRE(c.heads > 0 ? p.q_heads % c.heads == 0 : p.q_heads == 0, WC_ERR_SHAPE, "%s: %lld query heads over %lld key heads", what,
+             (long long)p.q_heads, (long long)c.heads);
+  WC_REQUIRE(p.q_heads <= 65535 && p.max_prefix < (1ll << 31) - 64 && p.max_length < (1ll << 31) - 64 && p.prefix_len < (1ll << 31),
+             WC_ERR_LIMIT, "%s: more than 65535 heads or 2^31 tokens", what);
+  WC_REQUIRE(p.prefix_len <= 1 || p.prefix_stride >= 0, WC_ERR_ARG, "%s: negative table stride", what);
+  // a launch holds fewer than 2^32 threads, and counts tiles in 32 bits
+  WC_REQUIRE(mul_sat({c.n, c.b, p.q_heads}) < (1ll << 22), WC_ERR_LIMIT, "%s: 2^22 rows or more", what);
+  WC_REQUIRE(c.row * paged_es(c) <= 1024, WC_ERR_LIMIT, "%s: rows above 1024 bytes", what);
+  WC_REQUIRE(paged_countable(c.n * (c.b / p.share), most_of(p, 0)) && paged_countable(c.n * c.b, most_of(p, 1)), WC_ERR_LIMIT,
+             "%s: more than 2^35 tokens by the bounds", what);
+  return WC_OK;
+}
+
+}  // namespace
+}  // namespace wc
+
+extern "C" int64_t wc_shared_attention_workspace_bytes(const wc_shared_attn_args* args) {
+  using namespace wc;
+  clear_error();
+  if (!args) {
+    set_error(WC_ERR_NULL, "wc_shared_attention: null args");
+    return -1;
+  }
+  if (check(*args, "wc_shared_attention")) return -1;
+  if (args->cache.n == 0 || args->cache.b == 0 || args->q_heads == 0) return 0;
+  return space_of(*args, plan_of(*args)).bytes;
+}
+
+extern "C" int32_t wc_shared_attention(const wc_shared_attn_args* args, void* stream) {
+  using namespace wc;
+  clear_error();
+  const char* what = "wc_shared_attention";
+  WC_REQUIRE(args, WC_ERR_NULL, "%s: null args", what);
+  const wc_shared_attn_args& p = *args;
+  const wc_paged_cache& c = p.cache;
+  if (int32_t rc = check(p, what)) return rc;
+  const int64_t seqs = c.n * c.b, units = seqs / p.share;
+  if (seqs == 0 || p.q_heads == 0) return WC_OK;
+  if (int32_t rc = paged_check_pointers(c, what)) return rc;
+  const int es = dtype_size(c.dtype);
+  WC_REQUIRE(p.q && p.o && p.lengths && p.prefix_lengths && (p.prefix_len == 0 || p.prefix_table), WC_ERR_NULL, "%s: null pointer", what);
+  WC_REQUIRE(aligned(p.q, es) && aligned(p.o, es) && aligned(p.lengths, 4) && aligned(p.prefix_lengths, 4) && aligned(p.prefix_table, 4),
+             WC_ERR_ALIGN, "%s: pointers must be aligned to their elements", what);
+  const Plan plan = plan_of(p);
+  const Space space = space_of(p, plan);
+  WC_REQUIRE(p.workspace && p.workspace_bytes >= space.bytes, WC_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what,
+             (long long)p.workspace_bytes, (long long)space.bytes);
+  WC_REQUIRE(aligned(p.workspace, 16), WC_ERR_ALIGN, "%s: workspace must be 16-byte aligned", what);
+  Shared a;
+  a.k = static_cast<const char*>(c.k_pages);
+  a.v = static_cast<const char*>(c.v_pages);
+  a.ks = c.k_scales;
+  a.vs = c.v_scales;
+  a.q = static_cast<const char*>(p.q);
+  a.o = static_cast<char*>(p.o);
+  a.qn = p.q_stride_n;
+  a.qb = p.q_stride_b;
+  a.qh = p.q_stride_h;
+  a.heads = static_cast<int32_t>(p.q_heads);
+  a.group = static_cast<int32_t>(p.q_heads / c.heads);
+  a.dh = static_cast<int32_t>(c.head_dim);
+  a.row_bytes = static_cast<int32_t>(c.row * paged_es(c));
+  a.qvec = c.head_dim * es % 16 == 0 && aligned(p.q, 16) && ubytes(p.q_stride_n, es) % 16 == 0 &&
+           ubytes(p.q_stride_b, es) % 16 == 0 && ubytes(p.q_stride_h, es) % 16 == 0;
+  a.scale = p.scale * kLog2e;
+  a.by_kvh = make_fastdiv(static_cast<uint32_t>(c.heads));
+  a.by_group = make_fastdiv(static_cast<uint32_t>(a.group));
+  a.by_heads = make_fastdiv(static_cast<uint32_t>(a.heads));
+  a.by_share = make_fastdiv(static_cast<uint32_t>(p.share));
+  wc_paged_cache prefix = c;
+  prefix.table = p.prefix_table;
+  prefix.table_len = p.prefix_len;
+  prefix.table_stride = p.prefix_stride;
+  int64_t blocks[2];
+  for (int i = 0; i < 2; ++i) {
+    Walk& w = a.walk[i];
+    w.lengths = i ? p.lengths : p.prefix_lengths;
+    w.t = paged_table(i ? c : prefix, w.lengths);
+    char* ws = static_cast<char*>(p.workspace);
+    w.part = reinterpret_cast<float*>(ws + space.part[i]);
+    w.ml = reinterpret_cast<float2*>(ws + space.ml[i]);
+    w.parts = reinterpret_cast<int2*>(ws + space.list[i]);
+    w.units = static_cast<int32_t>(i ? seqs : units);
+    w.share = static_cast<int32_t>(i ? 1 : p.share);
+    w.budget = static_cast<int32_t>(plan.budget[i]);
+    w.most = static_cast<int32_t>(most_of(p, i));
+    w.rows = w.share * a.group;
+    const int64_t tiles = cdiv(w.rows, i ? 16 : plan.rt * 16);
+    w.by_tiles = make_fastdiv(static_cast<uint32_t>(tiles));
+    w.by_units = make_fastdiv(static_cast<uint32_t>(i ? c.b : c.b / p.share));
+    blocks[i] = (w.budget ? w.budget : w.units) * c.heads * tiles;
+  }
+  a.blocks = static_cast<int32_t>(blocks[0]);
+  const hipStream_t s = as_stream(stream);
+  auto go = [&](auto t) {
+    typedef decltype(t) QT;
+    dispatch<QT>(a, c.bits == 8, plan.rt, blocks[0] + blocks[1], s);
+    (c.head_dim % 4 ? shared_join_kernel<QT, false> : shared_join_kernel<QT, true>)<<<static_cast<uint32_t>(seqs * p.q_heads), 256, 0, s>>>(a);
+  };
+  if (c.dtype == WC_F32)
+    go(float());
+  else if (c.dtype == WC_BF16)
+    go(bf16());
+  else
+    go(f16());
+  return check_launch(what);
+}

@@ -17,7 +17,7 @@ from .core.ensemble_util import pack_inputs, unpack_outputs
 from .core.primitives import (
     WideAttention, WideBatchNorm1d, WideBatchNorm2d, WideConv1d, WideConv2d, WideConv3d, WideEmbedding,
     WideGRU, WideGroupNorm, WideHeadNormRotary, WideInstanceNorm1d, WideInstanceNorm2d, WideLayerNorm, WideLinear,
-    WideLinear4bit, WideLSTM,
+    WideLinear4bit, WideLinear8bit, WideLSTM, WideSampler,
 )
 from .core.paged_cache import WidePagedCache
 from .api import benchmark_custom, benchmark_primitive
@@ -38,7 +38,8 @@ __all__ = [
     "TracedWideModel", "FunctionalOp", "BinaryOp", "print_trace", "pack_inputs", "unpack_outputs",
     "WideLinear", "WideConv1d", "WideConv2d", "WideConv3d", "WideBatchNorm1d", "WideBatchNorm2d",
     "WideLayerNorm", "WideGroupNorm", "WideInstanceNorm1d", "WideInstanceNorm2d", "WideEmbedding",
-    "WideAttention", "WideGRU", "WideLSTM", "WideHeadNormRotary", "WideLinear4bit", "WidePagedCache",
+    "WideAttention", "WideGRU", "WideLSTM", "WideHeadNormRotary", "WideLinear4bit", "WideLinear8bit", "WidePagedCache",
+    "WideSampler",
     "benchmark_primitive", "benchmark_multi", "benchmark_all", "benchmark_custom",
     "list_benchmark_primitives", "BenchmarkResult", "SweepParams",
 ]

@@ -4,6 +4,8 @@ WidePagedCache: the keys and values of many sequences of N models, in pages of o
     cache.write(k, v, block_table, start, count)      new tokens into the pages
     cache.read(block_table, lengths, max_length)      back to dense [N, B, max_length, Hkv, Dh]
     cache.attend(q, block_table, lengths)             one new token of every sequence over its pages
+    cache.attend_shared(q, prefix_table, prefix_lengths, block_table, lengths)
+                                                      the same where sequences share prefixes, read once for all of them
 
 Token i of sequence (n, b) stands in slot i % page_size of page block_table[n, b, i // page_size] of
 the pool (int32 [N, B, M]; entries behind a sequence's last page are not followed and may hold
@@ -34,7 +36,7 @@ from typing import Optional, Tuple, Union
 import torch
 from torch import Tensor
 
-from .. import _hip, _serve
+from .. import _answer, _hip, _serve
 
 
 class WidePagedCache:
@@ -231,6 +233,65 @@ class WidePagedCache:
         if max_length < 0:
             raise RuntimeError(f"WidePagedCache.attend: max_length must not be negative, got {max_length}")
         return _serve.paged_attention_workspace(self, sizes, block_table, q.shape[2], max_length) if q.numel() else 0
+
+    def attend_shared(self, q: Tensor, prefix_table: Tensor, prefix_lengths: Tensor, block_table: Tensor, lengths: Tensor,
+                      scale: Optional[float] = None, max_prefix: Optional[int] = None,
+                      max_length: Optional[int] = None) -> Tensor:
+        """softmax(scale q k^T) v of one new token per sequence, q [N, B, Hq, Dh], over the tokens of a prefix and then its
+        own.  B / G neighbouring sequences of a model share each of the G prefixes that ``prefix_table`` (int32 [N, G, M])
+        and ``prefix_lengths`` (int32 [N, G]) name; ``block_table`` (int32 [N, B, M']) and ``lengths`` (int32 [N, B]) name
+        the tokens behind the prefix that a sequence has of its own, 0 for none.  A sequence of negative length takes
+        part in nothing and gets zeros, as does one without any token.  The pages of a prefix are read once for all its
+        sequences, where ``attend`` reads them for each.  ``max_prefix`` and ``max_length`` bound the lengths (default: what
+        the tables can name); tight bounds split short ones less.  In 16 bits the weights enter the products with a
+        prefix of more than 16 query heads a key head as two numbers of 16 bits (off by at most 2^-17 of a weight)."""
+        if torch.compiler.is_compiling():
+            return _serve.uncompiled(self.attend_shared, q, prefix_table, prefix_lengths, block_table, lengths, scale,
+                                     max_prefix, max_length)
+        form = (q.shape, q.dtype, q.get_device(), prefix_table.shape, prefix_table.dtype, prefix_table.get_device(),
+                prefix_lengths.shape, prefix_lengths.dtype, prefix_lengths.get_device(), block_table.shape, block_table.dtype,
+                block_table.get_device(), lengths.shape, lengths.dtype, lengths.get_device())
+        plan = self._plans.get(form)
+        if plan is None:
+            plan = self._plans.keep(form, self._plan_shared(q, prefix_table, prefix_lengths, block_table, lengths))
+        sizes, share, reach, needs = plan
+        most = (reach[0] if max_prefix is None else max_prefix, reach[1] if max_length is None else max_length)
+        need = needs.get(most)
+        if need is None:
+            if min(most) < 0:
+                raise RuntimeError(f"WidePagedCache.attend_shared: max_prefix and max_length must not be negative, got {most}")
+            need = needs.keep(most, _answer.shared_attention_workspace(sizes, block_table.shape[2], share, prefix_table.shape[2],
+                                                                       q.shape[2], *most) if q.numel() else 0)
+        if torch.is_grad_enabled():
+            _hip.require_forward_only("WidePagedCache.attend_shared", q)
+        q = q if q.stride(3) == 1 else q.contiguous()
+        o = q.new_empty(q.shape)
+        if o.numel():
+            _answer.shared_attention(self, sizes, share, q, o, self._dense(prefix_table), self._dense(prefix_lengths),
+                                     self._dense(block_table), self._dense(lengths),
+                                     self.head_dim ** -0.5 if scale is None else scale, most, need)
+        return o
+
+    def _plan_shared(self, q: Tensor, prefix_table: Tensor, prefix_lengths: Tensor, block_table: Tensor, lengths: Tensor) -> Tuple:
+        what = "WidePagedCache.attend_shared"
+        _hip.require_device(what, q, prefix_table, prefix_lengths, block_table, lengths)
+        if q.dim() != 4 or q.shape[3] != self.head_dim or q.shape[2] % self.n_kv_heads:
+            raise RuntimeError(f"{what}: q must be [N, B, a multiple of {self.n_kv_heads} heads, {self.head_dim}], got "
+                               f"{list(q.shape)}")
+        if q.dtype != self.dtype:
+            raise RuntimeError(f"{what}: q {q.dtype} over a cache for {self.dtype}")
+        n, b = q.shape[:2]
+        if prefix_table.dim() != 3 or prefix_table.dtype != torch.int32 or prefix_table.shape[0] != n:
+            raise RuntimeError(f"{what}: prefix_table must be int32 [N={n}, G, M], got {prefix_table.dtype} {list(prefix_table.shape)}")
+        g = prefix_table.shape[1]
+        if b % g if g else b:
+            raise RuntimeError(f"{what}: {b} sequences of a model do not come in {g} groups of one size")
+        self._check_per_sequence(what, "prefix_lengths", prefix_lengths, n, g)
+        self._check_table(what, block_table, n, b)
+        self._check_per_sequence(what, "lengths", lengths, n, b)
+        _serve.same_device(what, self.k_pages, q, prefix_table, prefix_lengths, block_table, lengths)
+        reach = tuple(min(t.shape[2] * self.page_size, 2 ** 31 - 65) for t in (prefix_table, block_table))
+        return self._sizes_for(n, b), max(b // g if g else 1, 1), reach, _serve.Plans()
 
     def index_error(self) -> None:
         """Raise IndexError if any call since the last check met a page outside the pool, or a token, count or length

@@ -14,6 +14,7 @@ from .wide_conv2d import (
 from .wide_conv3d import WideConv3d, Conv3dStrategy
 from .wide_linear import WideLinear, WideMLP2, LinearStrategy, select_linear_strategy, LINEAR_THRESHOLDS
 from .wide_linear4bit import WideLinear4bit
+from .wide_linear8bit import WideLinear8bit
 from .wide_batchnorm_1d import WideBatchNorm1d
 from .wide_batchnorm_2d import WideBatchNorm2d
 from .wide_layernorm import WideLayerNorm
@@ -24,6 +25,7 @@ from .wide_embedding import WideEmbedding, EmbeddingStrategy
 from .wide_attention import WideAttention, AttentionStrategy
 from .wide_gru import WideGRU, GRUStrategy
 from .wide_lstm import WideLSTM, LSTMStrategy
+from .wide_sampler import WideSampler
 
 __all__ = [
     "WideConv1d", "Conv1dStrategy", "WideConv2d", "ConvStrategy", "select_conv_strategy",
@@ -33,4 +35,5 @@ __all__ = [
     "WideInstanceNorm1d", "WideInstanceNorm2d", "InstanceNormStrategy",
     "WideEmbedding", "EmbeddingStrategy", "WideAttention", "AttentionStrategy",
     "WideGRU", "GRUStrategy", "WideLSTM", "LSTMStrategy", "WideHeadNormRotary", "WideLinear4bit",
+    "WideLinear8bit", "WideSampler",
 ]

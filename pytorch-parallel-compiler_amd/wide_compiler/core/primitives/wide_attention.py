@@ -264,18 +264,34 @@ class WideAttention(nn.Module):
         return self._project_out(attn)
 
     def step(self, x: Tensor, cache: "WidePagedCache", block_table: Tensor, lengths: Tensor,
-             head_norm: Optional["WideHeadNormRotary"] = None) -> Tensor:
+             head_norm: Optional["WideHeadNormRotary"] = None, prefix: Optional[Tuple[Tensor, Tensor]] = None) -> Tensor:
         """Self-attention of one new token of every sequence, x [N, B, D]: its keys and values go to the pages of
         ``cache`` as token lengths[n, b] - 1 (int32; the new token counted), and its queries attend over all
         lengths[n, b] tokens.  A sequence of length 0 takes part in nothing.  ``head_norm`` norms and turns queries
-        and keys first, at that position."""
+        and keys first, at that position.
+
+        ``prefix``: a table int32 [N, G, M] and lengths int32 [N, G] of prefixes in ``cache`` (left there by ``prompt``), each
+        shared by B / G neighbouring sequences.  Then ``block_table`` and ``lengths`` are of the tokens behind the
+        prefix, positions count on from it and the queries attend over both, a prefix read once for all its sequences."""
         what = "WideAttention.step"
         if x.dim() != 3 or x.shape[0] != self.n or x.shape[2] != self.d_model:
             raise RuntimeError(f"{what}: x must be [N={self.n}, B, {self.d_model}], got {list(x.shape)}")
         start = lengths - 1
-        q, k, v = self._cached_heads(what, x[:, :, None], cache, start[..., None], head_norm)
+        if prefix is None:
+            q, k, v = self._cached_heads(what, x[:, :, None], cache, start[..., None], head_norm)
+            cache.write(k, v, block_table, start)
+            return self._project_out(cache.attend(q[:, :, 0], block_table, lengths).flatten(-2))
+        table, common = prefix
+        n, b = x.shape[:2]
+        if common.dim() != 2 or common.shape[0] != n or lengths.shape != x.shape[:2] or (b % common.shape[1] if common.shape[1] else b):
+            raise RuntimeError(f"{what}: {list(common.shape)} prefix lengths and {list(lengths.shape)} lengths for [N={n}, B={b}] "
+                               "sequences in groups of one size")
+        share = b // common.shape[1] if common.shape[1] else 1
+        position = start + common.repeat_interleave(share, 1)
+        q, k, v = self._cached_heads(what, x[:, :, None], cache, position[..., None], head_norm)
         cache.write(k, v, block_table, start)
-        return self._project_out(cache.attend(q[:, :, 0], block_table, lengths).flatten(-2))
+        own = lengths.masked_fill(lengths <= 0, -1)
+        return self._project_out(cache.attend_shared(q[:, :, 0], table, common, block_table, own).flatten(-2))
 
     def _fusable(self, x: Tensor, mask: Optional[Tensor], params) -> bool:
         """The conditions of wc_self_attention: bf16, head dim 32, 1 <= S <= 512, D <= 768, no

@@ -1,0 +1,182 @@
+"""Sampling (GPU) against the definition in 64 bits, row by row."""
+
+import pytest
+import torch
+
+from tests._answer import draw
+from tests._util import gen
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+INF = float("inf")
+
+
+def _logits(n, b, v, seed, dtype, spread=2.0):
+    g = gen(seed)
+    x = torch.randn(n, b, v, generator=g) * spread
+    x[..., torch.randint(0, v, (5,), generator=g)] += 6
+    return x.to(dtype)
+
+
+def _check(sampler, x, u, rules, **given):
+    with torch.no_grad():
+        got = sampler(x.to(DEV), u.to(DEV), **{k: t.to(DEV) for k, t in given.items()}).cpu()
+    assert got.shape == u.shape and got.dtype == torch.int64
+    for at in torch.cartesian_prod(*(torch.arange(s) for s in u.shape)).view(-1, u.dim()).tolist():
+        at = tuple(at)
+        rule = {k: (r[at[0]] if isinstance(r, (list, tuple)) else r) for k, r in rules.items()}
+        rule.update({k: t.expand(u.shape)[at].item() for k, t in given.items()})
+        want = draw(x[at], u[at].item(), **rule)
+        assert got[at].item() == want, (at, rule, got[at].item(), want)
+
+
+RULES = [dict(), dict(temperature=0.0), dict(temperature=0.25), dict(top_k=1), dict(top_k=7), dict(top_p=0.9), dict(top_p=0.0),
+         dict(min_p=0.05), dict(min_p=1.0), dict(temperature=1.7, top_k=50, top_p=0.8, min_p=0.01), dict(top_k=40, top_p=0.5),
+         dict(temperature=5.0, top_p=0.99), dict(temperature=30.0, top_k=3000), dict(temperature=1e-3, top_p=0.7), dict(temperature=INF, top_k=9)]
+
+
+# one logit, pieces of a vector, odd sizes, one and several pieces a thread, segments that end early
+@pytest.mark.parametrize("v", [1, 2, 7, 64, 1000, 1025, 8191, 8192, 20011, 131072, 200003])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tokens(v, dtype):
+    import wide_compiler as wc
+    n, b = 3, 2
+    x = _logits(n, b, v, v, dtype)
+    for i, rules in enumerate(RULES):
+        u = torch.rand(n, b, generator=gen(i))
+        _check(wc.WideSampler(n, **rules).to(DEV), x, u, rules)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rules", [dict(), dict(top_k=3), dict(top_k=5, top_p=0.5), dict(top_p=0.5), dict(min_p=1.0), dict(temperature=0.0)])
+def test_equal_values_go_by_their_place(rules, dtype):
+    import wide_compiler as wc
+    for v in (1, 5, 64, 3000):
+        for x in (torch.zeros(1, 4, v), torch.arange(v).flip(0).div(7, rounding_mode="floor").expand(1, 4, v).float() * 0.5,
+                  torch.randint(0, 3, (1, 4, v), generator=gen(v)).float()):
+            u = torch.tensor([[0.0, 0.3, 0.77, 1 - 2.0 ** -24]])
+            _check(wc.WideSampler(1, **rules).to(DEV), x.to(dtype), u, rules)
+
+
+def test_every_token_has_its_share():
+    """u on a grid of 1 / 64: weights 1, 2, 4, ... of a sum of 63 each get as many of the 63 grid steps."""
+    import wide_compiler as wc
+    x = torch.log(torch.tensor([4.0, 1.0, 32.0, 2.0, 16.0, 8.0])).expand(1, 63, 6)
+    u = ((torch.arange(63) + 0.5) / 63)[None]
+    with torch.no_grad():
+        got = wc.WideSampler(1).to(DEV)(x.to(DEV), u.to(DEV)).cpu()
+    assert torch.bincount(got[0], minlength=6).tolist() == [4, 1, 32, 2, 16, 8]
+    assert (got[0].diff() >= 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinities_and_nan(dtype):
+    import wide_compiler as wc
+    x = torch.randn(1, 9, 300, generator=gen(1))
+    x[0, 0] = -INF
+    x[0, 1] = float("nan")
+    x[0, 2, :299] = -INF
+    x[0, 3, ::2] = float("nan")
+    x[0, 4, [5, 90, 250]] = INF
+    x[0, 5, :] = -INF
+    x[0, 5, [3, 8]] = torch.finfo(torch.float16).min
+    x[0, 6, 1:] = torch.finfo(torch.float16).min
+    x[0, 7, :150] = -INF
+    x[0, 8, 7] = float("nan")
+    for rules in RULES:
+        _check(wc.WideSampler(1, **rules).to(DEV), x.to(dtype), torch.rand(1, 9, generator=gen(2)), rules)
+
+
+def test_the_ends_of_u():
+    import wide_compiler as wc
+    x = _logits(1, 6, 5000, 3, torch.float32)
+    x[0, :, 0] = -INF
+    x[0, :, -1] = -INF
+    u = torch.tensor([[0.0, 1 - 2.0 ** -24, 1.0, -3.0, 2.0, 1e-30]])
+    for rules in RULES:
+        _check(wc.WideSampler(1, **rules).to(DEV), x, u, rules)
+
+
+def test_values_far_apart_and_tiny():
+    """Values that differ in the last bit of fp32, of 1e30 and of 1e-40, at temperatures as extreme."""
+    import wide_compiler as wc
+    base = torch.rand(2, 3, 777, generator=gen(4))
+    for x, t in ((base * 1e30, 1e29), (base * 1e-40, 1e-40), (1e30 + base * 1e24, 1e24), (base, 1e-30), (base, 1e30), (-base * 1e38, 3e38)):
+        for rules in (dict(), dict(top_p=0.6), dict(top_k=5), dict(min_p=0.9)):
+            _check(wc.WideSampler(2, temperature=t, **rules).to(DEV), x, torch.rand(2, 3, generator=gen(5)), dict(temperature=t, **rules))
+
+
+def test_rules_of_models_and_of_rows():
+    import wide_compiler as wc
+    n, b, v = 3, 4, 700
+    x = _logits(n, b, v, 6, torch.float32)
+    u = torch.rand(n, b, generator=gen(7))
+    rules = dict(temperature=[0.5, 1.0, 0.0], top_k=[0, 20, 5], top_p=[0.9, 1.0, 0.3], min_p=[0.0, 0.1, 0.0])
+    s = wc.WideSampler(n, **rules).to(DEV)
+    _check(s, x, u, rules)
+    _check(s.to(torch.bfloat16), x, u, rules)               # the rules stay as they are
+    _check(s, x, u, rules, temperature=torch.rand(n, b, generator=gen(8)) + 0.2, top_k=torch.randint(0, 30, (b,), generator=gen(9), dtype=torch.int32))
+    _check(s, x, u, rules, top_p=torch.rand(n, 1, generator=gen(10)), min_p=torch.tensor(0.02))
+    s.set(temperature=1.5, top_k=[1, 2, 3])
+    _check(s, x, u, {**rules, "temperature": 1.5, "top_k": [1, 2, 3]})
+
+
+def test_strides_and_batches():
+    import wide_compiler as wc
+    base = torch.randn(3, 5, 2, 1001, generator=gen(11))
+    s = wc.WideSampler(2, top_p=0.8).to(DEV)
+    u = torch.rand(5, 2, 3, generator=gen(12)).permute(1, 0, 2)
+    with torch.no_grad():
+        for x in (base.permute(2, 1, 0, 3)[..., 1:], base.permute(2, 1, 0, 3)[..., ::2], base.permute(2, 1, 0, 3)[..., :900]):
+            got = s(x.to(DEV), u.to(DEV))
+            on = base.to(DEV).permute(2, 1, 0, 3)
+            view = on[..., 1:] if x.shape[-1] == 1000 else on[..., ::2] if x.shape[-1] == 501 else on[..., :900]
+            assert torch.equal(s(view, u.to(DEV)), got)
+            for i, j, k in ((0, 0, 0), (1, 4, 2), (0, 3, 1)):
+                assert got[i, j, k].item() == draw(x[i, j, k], u[i, j, k].item(), top_p=0.8)
+        t = torch.rand(2, 3, 5, generator=gen(13)).permute(0, 2, 1) + 0.5          # a rule of its own strides
+        got = s(base.permute(2, 1, 0, 3).to(DEV), u.to(DEV), temperature=t.to(DEV))
+        for i, j, k in ((0, 0, 0), (1, 4, 2), (1, 2, 1)):
+            assert got[i, j, k].item() == draw(base[k, j, i], u[i, j, k].item(), temperature=t[i, j, k].item(), top_p=0.8)
+        assert s(torch.zeros(2, 0, 9, device=DEV), torch.zeros(2, 0, device=DEV)).shape == (2, 0)
+
+
+def test_many_rows():
+    import wide_compiler as wc
+    x, u = _logits(4, 300, 515, 14, torch.bfloat16), torch.rand(4, 300, generator=gen(15))
+    _check(wc.WideSampler(4, temperature=0.9, top_p=0.95).to(DEV), x, u, dict(temperature=0.9, top_p=0.95))
+
+
+def test_a_graph_replays_with_new_numbers_and_rules():
+    import wide_compiler as wc
+    s = wc.WideSampler(2, temperature=1.0, top_p=0.9).to(DEV)
+    x, u = _logits(2, 5, 9001, 16, torch.float16).to(DEV), torch.rand(2, 5, device=DEV)
+    with torch.no_grad():
+        s(x, u)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = s(x, u)
+        for rep in range(4):
+            x.copy_(_logits(2, 5, 9001, 20 + rep, torch.float16))
+            u.copy_(torch.rand(2, 5, generator=gen(rep)))
+            if rep == 2:
+                s.set(top_k=4, min_p=0.1)
+            graph.replay()
+            torch.cuda.synchronize()
+            want = got.clone()
+            assert torch.equal(s(x, u), want)
+
+
+def test_on_another_stream():
+    import wide_compiler as wc
+    s = wc.WideSampler(1, top_k=30).to(DEV)
+    x, u = _logits(1, 3, 50001, 17, torch.float32).to(DEV), torch.rand(1, 3, device=DEV)
+    with torch.no_grad():
+        want = s(x, u)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got = s(x, u)
+        torch.cuda.synchronize()
+    assert torch.equal(got, want)
