@@ -103,7 +103,7 @@ def test_values_far_apart_and_tiny():
     import wide_compiler as wc
     base = torch.rand(2, 3, 777, generator=gen(4))
     for x, t in ((base * 1e30, 1e29), (base * 1e-40, 1e-40), (1e30 + base * 1e24, 1e24), (base, 1e-30), (base, 1e30), (-base * 1e38, 3e38)):
-        for rules in (dict(), dict(top_p=0.6), dict(top_k=5), dict(min_p=0.9)):
+        for rules in (dict(), dict(top_p=0.6), dict(top_k=5), dict(min_p=0.9), dict(top_k=200, top_p=0.7)):
             _check(wc.WideSampler(2, temperature=t, **rules).to(DEV), x, torch.rand(2, 3, generator=gen(5)), dict(temperature=t, **rules))
 
 
