@@ -37,16 +37,90 @@ typedef __attribute__((address_space(3))) i32x4 lds_i32x4;
 
 __device__ __forceinline__ i32x4 mma8(i32x4 a, i32x4 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 
-// 16 values of a row from column k on, zeros from its end on
+// 16 values of a row, as they lie
 template <typename T>
-__device__ __forceinline__ void load16(const T* x, int k, int end, T (&v)[16]) {
-  if (k + 16 <= end) {
-    __builtin_memcpy(v, x + k, sizeof v);            // at element alignment
-  } else {
+struct Piece {
+  static constexpr int N = sizeof(T), E = 16 / sizeof(T);              // vectors, values of each
+  u32x4 v[N];
+  // those of lane group g in a tile, zeros from the row's end on
+  __device__ __forceinline__ void load(const T* x, int tile, int g, int end) {
+    const int k = tile * 64 + g * 16;
+    if (tile * 64 + 64 <= end) {                      // the same for the wave
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = k + e < end ? x[k + e] : from_f32<T>(0.f);
+      for (int i = 0; i < N; ++i) __builtin_memcpy(&v[i], x + k + i * E, 16);          // at element alignment
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int at = k + i * E + q * (4 / static_cast<int>(sizeof(T)));
+          uint32_t w = 0;
+          if constexpr (sizeof(T) == 4) {
+            if (at < end) w = __builtin_bit_cast(uint32_t, x[at]);
+          } else {
+            if (at < end) w = __builtin_bit_cast(uint16_t, x[at]);
+            if (at + 1 < end) w |= static_cast<uint32_t>(__builtin_bit_cast(uint16_t, x[at + 1])) << 16;
+          }
+          v[i][q] = w;
+        }
+    }
   }
-}
+  __device__ __forceinline__ float value(int e) const {
+    const uint32_t w = v[e / E][e % E / (4 / sizeof(T))];
+    if constexpr (sizeof(T) == 4)
+      return __builtin_bit_cast(float, w);
+    else if constexpr (std::is_same<T, bf16>::value)
+      return e & 1 ? bf16_hi(w) : bf16_lo(w);
+    else
+      return static_cast<float>(__builtin_bit_cast(f16, static_cast<uint16_t>(e & 1 ? w >> 16 : w)));
+  }
+  // the larger of `top` and the largest magnitude, as bits of the type: two 16-bit ones in a register, each of its own half
+  __device__ __forceinline__ uint32_t top(uint32_t top) const {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t w = v[i][q];
+        if constexpr (sizeof(T) == 4)
+          top = std::max(top, w & 0x7fffffffu);
+        else
+          top = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, top), __builtin_bit_cast(u16x2, w & 0x7fff7fffu)));
+      }
+    return top;
+  }
+  // that as the bits of a float
+  static __device__ __forceinline__ uint32_t as_float(uint32_t top) {
+    if constexpr (sizeof(T) == 4)
+      return top;
+    else
+      return __builtin_bit_cast(uint32_t, to_f32(__builtin_bit_cast(T, static_cast<uint16_t>(std::max(top & 0xffffu, top >> 16)))));
+  }
+  static __device__ __forceinline__ u32x4 packed(const uint32_t (&code)[16], bool finite) {
+    u32x4 o;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t* c = code + 4 * q;
+      const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400u);
+      o[q] = finite ? lo | hi << 16 : 0u;
+    }
+    return o;
+  }
+  __device__ __forceinline__ u32x4 codes(float scale, float inv, bool finite) const {
+    uint32_t code[16];
+    float far = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      float off;
+      code[e] = code8(value(e), scale, inv, off);
+      far = fmaxf(far, off);
+    }
+    if (far > scale * kNearHalf)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) code[e] = code8_near_half(value(e), scale, inv);
+    return packed(code, finite);
+  }
+};
 
 // Codes and scales of 16 rows of x: lane l has row l % 16 and columns 16 (l / 16).. of every tile of its wave, which is what
 // it writes.  KEPT tiles a wave stay in registers between the search for the scale and the codes; rows longer than that
@@ -54,27 +128,23 @@ __device__ __forceinline__ void load16(const T* x, int k, int end, T (&v)[16]) {
 template <typename T, int NW, int KEPT>
 __global__ __launch_bounds__(NW * 64) void linear8_codes_kernel(Linear8 a) {
   __shared__ uint32_t tops[NW][16];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
   const uint32_t model = fdiv(blockIdx.x, a.by_mtiles);
   const int mt = blockIdx.x - model * a.by_mtiles.d;
   const uint32_t r = min(mt * 16 + j, a.m - 1), outer = fdiv(r, a.by_rows);        // past the last: the last again
   const T* x = reinterpret_cast<const T*>(a.x) + model * a.xn + outer * a.xo + (r - outer * a.by_rows.d) * a.xi;
-  T v[KEPT][16];
-  auto top16 = [](const T(&t)[16], uint32_t top) {
+  Piece<T> v[KEPT];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) top = max(top, __builtin_bit_cast(uint32_t, to_f32(t[e])) & 0x7fffffffu);
-    return top;
-  };
+  for (int i = 0; i < KEPT; ++i) v[i].load(x, wave + i * NW, g, a.k);
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < KEPT; ++i) load16(x, ((wave + i * NW) * 4 + g) * 16, a.k, v[i]);
-#pragma unroll
-  for (int i = 0; i < KEPT; ++i) top = top16(v[i], top);
+  for (int i = 0; i < KEPT; ++i) top = v[i].top(top);
   for (int t = wave + KEPT * NW; t < a.ktiles; t += NW) {
-    T u[16];
-    load16(x, (t * 4 + g) * 16, a.k, u);
-    top = top16(u, top);
+    Piece<T> u;
+    u.load(x, t, g, a.k);
+    top = u.top(top);
   }
+  top = Piece<T>::as_float(top);
   top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
   top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 32, 64)));
   if (g == 0) tops[wave][j] = top;
@@ -85,53 +155,55 @@ __global__ __launch_bounds__(NW * 64) void linear8_codes_kernel(Linear8 a) {
   const float scale = finite ? row_scale(top) : __builtin_nanf("");
   const float inv = __builtin_amdgcn_rcpf(scale);
   if (threadIdx.x < 16) a.s[static_cast<int64_t>(blockIdx.x) * 16 + j] = scale;
-  uint8_t* out = a.c + (static_cast<int64_t>(blockIdx.x) * a.ktiles) * 1024 + lane * 16;
-  auto put = [&](const T(&t)[16], int tile) {
-    uint32_t code[16];
-    float far = 0.f;
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      float off;
-      code[e] = code8(to_f32(t[e]), scale, inv, off);
-      far = fmaxf(far, off);
-    }
-    if (far > scale * kNearHalf)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) code[e] = code8_near_half(to_f32(t[e]), scale, inv);
-    u32x4 o;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const uint32_t* c = code + 4 * q;
-      const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x0c0c0400u);
-      o[q] = finite ? lo | hi << 16 : 0u;
-    }
-    *reinterpret_cast<u32x4*>(out + static_cast<int64_t>(tile) * 1024) = o;
-  };
+  u32x4* out = reinterpret_cast<u32x4*>(a.c) + static_cast<int64_t>(blockIdx.x) * a.ktiles * 64 + lane;
 #pragma unroll
   for (int i = 0; i < KEPT; ++i)
-    if (wave + i * NW < a.ktiles) put(v[i], wave + i * NW);
+    if (wave + i * NW < a.ktiles) out[static_cast<int64_t>(wave + i * NW) * 64] = v[i].codes(scale, inv, finite);
+#pragma unroll 1
   for (int t = wave + KEPT * NW; t < a.ktiles; t += NW) {
-    T u[16];
-    load16(x, (t * 4 + g) * 16, a.k, u);
-    put(u, t);
+    Piece<T> u;
+    u.load(x, t, g, a.k);
+    out[static_cast<int64_t>(t) * 64] = u.codes(scale, inv, finite);
   }
 }
 
+// Scales and bias of outputs o..o + 3
+struct Columns {
+  float scale[4], bias[4];
+};
+template <typename T>
+__device__ __forceinline__ Columns columns(const Linear8& a, uint32_t model, int o) {
+  Columns c;
+  const int64_t at = static_cast<int64_t>(model) * a.o;
+  const T* bias = reinterpret_cast<const T*>(a.bias);
+  if (a.vec) {                                        // all four or none are there
+    const int64_t i = at + (o < a.o ? o : 0);
+    T b[4];
+    __builtin_memcpy(c.scale, a.scales + i, 16);
+    if (a.bias) __builtin_memcpy(b, bias + i, sizeof b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) c.bias[e] = a.bias ? to_f32(b[e]) : 0.f;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t i = at + std::min(o + e, a.o - 1);
+      c.scale[e] = a.scales[i];
+      c.bias[e] = a.bias ? to_f32(bias[i]) : 0.f;
+    }
+  }
+  return c;
+}
+__device__ __forceinline__ float row_of_scale(const Linear8& a, uint32_t model, int r) {
+  return a.s[static_cast<int64_t>(model) * a.mtiles * 16 + std::min(r, a.m - 1)];
+}
 // outputs o..o + 3 of row r, those there are
 template <typename T>
-__device__ __forceinline__ void finish4(const Linear8& a, uint32_t model, int r, int o, i32x4 sum) {
+__device__ __forceinline__ void finish4(const Linear8& a, uint32_t model, int r, int o, i32x4 sum, float s, const Columns& c) {
   if (r >= a.m || o >= a.o) return;
-  const int64_t at = static_cast<int64_t>(model) * a.o + o;
-  const float s = a.s[static_cast<int64_t>(model) * a.mtiles * 16 + r];
   T* y = reinterpret_cast<T*>(a.y) + (static_cast<int64_t>(model) * a.m + r) * a.o + o;
-  const T* bias = reinterpret_cast<const T*>(a.bias) + at;
   T v[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const bool in = o + e < a.o;
-    const float f = static_cast<float>(sum[e]) * (s * a.scales[in ? at + e : at]);
-    v[e] = from_f32<T>(a.bias ? f + to_f32(bias[in ? e : 0]) : f);
-  }
+  for (int e = 0; e < 4; ++e) v[e] = from_f32<T>(static_cast<float>(sum[e]) * (s * c.scale[e]) + c.bias[e]);
   if (a.vec) {
     __builtin_memcpy(__builtin_assume_aligned(y, 4 * sizeof(T)), v, sizeof v);
   } else {
@@ -139,6 +211,26 @@ __device__ __forceinline__ void finish4(const Linear8& a, uint32_t model, int r,
     for (int e = 0; e < 4; ++e)
       if (o + e < a.o) y[e] = v[e];
   }
+}
+// a wave's FN x FM tiles
+template <typename T, int FN, int FM>
+__device__ __forceinline__ void finish(const Linear8& a, uint32_t model, int ot, int mt, int lane, const i32x4 (&acc)[FN][FM]) {
+  float s[FM];
+#pragma unroll
+  for (int j = 0; j < FM; ++j) s[j] = row_of_scale(a, model, (mt + j) * 16 + (lane & 15));
+#pragma unroll
+  for (int i = 0; i < FN; ++i) {
+    const int o = (ot + i) * 16 + (lane >> 4) * 4;
+    const Columns c = columns<T>(a, model, o);
+#pragma unroll
+    for (int j = 0; j < FM; ++j) finish4<T>(a, model, (mt + j) * 16 + (lane & 15), o, acc[i][j], s[j], c);
+  }
+}
+// a barrier that waits for nothing but the other waves
+__device__ __forceinline__ void bare_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // Up to 16 rows of x: a workgroup has RT tiles of output rows, its waves every NW-th tile of columns, D of them on their way.
@@ -180,7 +272,93 @@ __global__ __launch_bounds__(NW * 64) void linear8_few_kernel(Linear8 a) {
     i32x4 sum = part[0][t][lane];
 #pragma unroll
     for (int v = 1; v < NW; ++v) sum += part[v][t][lane];
-    finish4<T>(a, model, mt * 16 + (lane & 15), (ot0 + t) * 16 + (lane >> 4) * 4, sum);
+    const int r = mt * 16 + (lane & 15), o = (ot0 + t) * 16 + (lane >> 4) * 4;
+    finish4<T>(a, model, r, o, sum, row_of_scale(a, model, r), columns<T>(a, model, o));
+  }
+}
+
+// The same for so few rows of x (kFusedPieces pieces of 16 columns in all) that every workgroup finds their codes for itself,
+// in LDS, while its first weights are on their way: a launch costs more.
+constexpr int kFusedPieces = 1024;
+template <typename T, int RT, int NW, int D>
+__global__ __launch_bounds__(NW * 64) void linear8_fused_kernel(Linear8 a) {
+  constexpr int NT = NW * 64, KEPT = kFusedPieces / NT;
+  __shared__ i32x4 part[NW][RT][64];
+  __shared__ u32x4 codes[kFusedPieces];              // [row][columns / 16]
+  __shared__ uint32_t tops[16];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 15, g = lane >> 4;
+  const uint32_t model = fdiv(blockIdx.x, a.by_wg);
+  const int ot0 = (blockIdx.x - model * a.by_wg.d) * RT;
+  const i32x4* w[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t)
+    w[t] = reinterpret_cast<const i32x4*>(a.w) + (static_cast<int64_t>(model) * a.otiles + min(ot0 + t, a.otiles - 1)) * a.ktiles * 64 + lane;
+  // piece tid + i NT of x: row p / (4 ktiles), columns 16 (p % (4 ktiles))..
+  const int per = a.ktiles * 4, pieces = a.m * per;
+  Piece<T> v[KEPT];
+  int row[KEPT];
+#pragma unroll
+  for (int i = 0; i < KEPT; ++i) {
+    const int p = min(tid + i * NT, pieces - 1), c = p % per;
+    row[i] = p / per;
+    const uint32_t outer = fdiv(row[i], a.by_rows);
+    v[i].load(reinterpret_cast<const T*>(a.x) + model * a.xn + outer * a.xo + (row[i] - outer * a.by_rows.d) * a.xi, c >> 2, c & 3, a.k);
+  }
+  i32x4 acc[RT] = {}, wf[D][RT];
+  auto fetch = [&](int d, int kt) {                   // past the last: the last again
+    const int64_t at = static_cast<int64_t>(min(kt, a.ktiles - 1)) * 64;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) wf[d][t] = w[t][at];
+  };
+#pragma unroll
+  for (int d = 0; d < D; ++d) fetch(d, wave + d * NW);
+  if (tid < 16) tops[tid] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < KEPT; ++i) {
+    uint32_t top = Piece<T>::as_float(v[i].top(0));
+    if (__all(row[i] == __builtin_amdgcn_readfirstlane(row[i]))) {
+#pragma unroll
+      for (int off = 32; off; off >>= 1) top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), off, 64)));
+      if (lane == 0) atomicMax(&tops[row[i]], top);
+    } else {
+      atomicMax(&tops[row[i]], top);
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < KEPT; ++i) {
+    if (tid + i * NT >= pieces) continue;
+    const uint32_t top = tops[row[i]];
+    const bool finite = top < 0x7f800000u;
+    const float scale = finite ? row_scale(top) : __builtin_nanf("");
+    codes[tid + i * NT] = v[i].codes(scale, __builtin_amdgcn_rcpf(scale), finite);
+  }
+  __syncthreads();
+  const u32x4* mine = codes + min(j, a.m - 1) * per + g;
+#pragma unroll 1
+  for (int k0 = wave; k0 < a.ktiles; k0 += D * NW) {
+#pragma unroll
+    for (int d = 0; d < D; ++d) {
+      const int kt = k0 + d * NW;
+      if (kt < a.ktiles) {
+        const i32x4 c = __builtin_bit_cast(i32x4, mine[kt * 4]);       // lanes without a row have another's
+#pragma unroll
+        for (int t = 0; t < RT; ++t) acc[t] = mma8(wf[d][t], c, acc[t]);
+      }
+      fetch(d, kt + D * NW);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < RT; ++t) part[wave][t][lane] = acc[t];
+  __syncthreads();
+  for (int t = wave; t < RT; t += NW) {
+    i32x4 sum = part[0][t][lane];
+#pragma unroll
+    for (int e = 1; e < NW; ++e) sum += part[e][t][lane];
+    const uint32_t top = tops[min(j, a.m - 1)];
+    const int o = (ot0 + t) * 16 + g * 4;
+    finish4<T>(a, model, j, o, sum, top < 0x7f800000u ? row_scale(top) : __builtin_nanf(""), columns<T>(a, model, o));
   }
 }
 
@@ -218,7 +396,7 @@ __global__ __launch_bounds__(WM * WN * 64) void linear8_tile_kernel(Linear8 a) {
   for (int s = 0; s < stages; ++s) {
     // stage s has landed for this wave, then for all; the slot of stage s - 1 is free
     __builtin_amdgcn_s_waitcnt((((NS - 2) * PER) & 15) | ((((NS - 2) * PER) >> 4) << 14) | 0x0070 | 0x0f00);
-    __syncthreads();
+    bare_barrier();
     issue(s + NS - 1);
     const lds_char* const st = lds + (s % NS) * (PIECES * 1024) + lane * 16;
 #pragma unroll
@@ -235,11 +413,139 @@ __global__ __launch_bounds__(WM * WN * 64) void linear8_tile_kernel(Linear8 a) {
     }
   }
   __builtin_amdgcn_s_waitcnt(0x0f70);                  // no DMA outlives the workgroup
+  finish<T>(a, model, ot0 + wn, mt0 + wm, lane, acc);
+}
+
+// Tiles of 256 x 256 outputs for whole rounds of the compute units: 8 waves of 128 outputs x 64 rows each, two stages of 128 columns
+// in LDS.  A workgroup walks its tiles without a pause between them: stages of all its tiles are one line, and while one is
+// multiplied the next but one is on its way.  Within a stage the waves stream their tiles of W through four registers,
+// four groups of MFMAs ahead of their use, so that a wave seldom waits for what it reads.
+constexpr int kLargeThreads = 512, kLargeTiles = 16, kLargeStage = 4 * kLargeTiles * 1024;
+
+template <typename T>
+__global__ __launch_bounds__(kLargeThreads, 1) void linear8_large_kernel(Linear8 a, int tiles_total, int per) {
+  __shared__ __attribute__((aligned(1024))) char raw[2 * kLargeStage];       // [2][W tiles, x tiles][2 halves]
+  lds_char* const lds = (lds_char*)raw;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = (wave & 1) * 8, wm = (wave >> 1) * 4, stages = a.ktiles / 2;
+  // this workgroup's tiles: XCD x = blockIdx % 8 has a range of neighbours, which share what they read
+  const int grid = gridDim.x;
+  int first = blockIdx.x, step = grid, mine;
+  if (grid % 8 == 0) {
+    const int x = blockIdx.x & 7, lo = static_cast<int>(static_cast<int64_t>(tiles_total) * x >> 3);
+    const int hi = static_cast<int>(static_cast<int64_t>(tiles_total) * (x + 1) >> 3);
+    step = grid >> 3;
+    first = lo + (blockIdx.x >> 3);
+    mine = first < hi ? (hi - first + step - 1) / step : 0;
+  } else {
+    mine = first < tiles_total ? (tiles_total - first + step - 1) / step : 0;
+  }
+  const int total = mine * stages;
+  if (total == 0) return;
+  struct Tile {
+    uint32_t model;
+    int ot, mt;
+  };
+  auto tile_of = [&](int i) {
+    // neighbours are 8 tiles along the rows by 4 along the outputs: 32 compute units of an XCD read 12 tiles' operands
+    const uint32_t t = first + i * step, model = fdiv(t, a.by_wg), rem = t - model * a.by_wg.d;
+    const int ots = a.by_wg.d / per, band = rem / (8 * ots), high = std::min(8, per - band * 8), in = rem - band * 8 * ots;
+    return Tile{model, in / high * kLargeTiles, (band * 8 + in % high) * kLargeTiles};
+  };
+  // piece q of the wave's eight of a stage: halves q % 2 of tiles 2 wave and 2 wave + 1 of W, then of x; past the last the last
+  // again, stages too, which keeps the count of loads
+  struct Source {
+    const uint8_t* w[2];
+    const uint8_t* x[2];
+    lds_char* to;
+  };
+  auto source_of = [&](int s) {
+    const int at = s < total ? s : total - 1, i = at / stages;
+    const Tile t = tile_of(i);
+    const int64_t k = static_cast<int64_t>(at - i * stages) * 2048;
+    Source c;
 #pragma unroll
-  for (int i = 0; i < FN; ++i)
+    for (int e = 0; e < 2; ++e) {
+      const int64_t w = static_cast<int64_t>(t.model) * a.otiles + std::min(t.ot + 2 * wave + e, a.otiles - 1);
+      const int64_t x = static_cast<int64_t>(t.model) * a.mtiles + std::min(t.mt + 2 * wave + e, a.mtiles - 1);
+      c.w[e] = a.w + w * a.ktiles * 1024 + k;
+      c.x[e] = a.c + x * a.ktiles * 1024 + k;
+    }
+    c.to = lds + (s & 1) * kLargeStage + wave * 4096;
+    return c;
+  };
+  auto bring = [&](const Source& c, int q) {
+    const uint8_t* from = (q < 4 ? c.w[q >> 1 & 1] : c.x[q >> 1 & 1]) + (q & 1) * 1024 + lane * 16;
+    __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(from),
+                                     (lds_ptr_t)(c.to + (q < 4 ? 0 : kLargeStage / 2) + (q & 3) * 1024), 16, 0, 0);
+  };
+  i32x4 acc[8][4], wr[4], x0[4], x1[4];
+  auto read_w = [&](int s, int g) {
+    wr[g & 3] = *(const lds_i32x4*)(lds + (s & 1) * kLargeStage + ((wn + (g & 7)) * 2 + (g >> 3)) * 1024 + lane * 16);
+  };
+  auto read_x = [&](int s, int h, i32x4(&x)[4]) {
 #pragma unroll
-    for (int j = 0; j < FM; ++j)
-      finish4<T>(a, model, (mt0 + wm + j) * 16 + (lane & 15), (ot0 + wn + i) * 16 + (lane >> 4) * 4, acc[i][j]);
+    for (int j = 0; j < 4; ++j)
+      x[j] = *(const lds_i32x4*)(lds + (s & 1) * kLargeStage + kLargeStage / 2 + ((wm + j) * 2 + h) * 1024 + lane * 16);
+  };
+  // everything on its way has landed (and, `all` false, what was stored may still be)
+  auto landed = [&]() {
+    __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0) lgkmcnt(0)
+    bare_barrier();
+  };
+  {
+    const Source c = source_of(0);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) bring(c, q);
+  }
+  landed();
+  {
+    const Source c = source_of(1);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) bring(c, q);
+  }
+#pragma unroll
+  for (int g = 0; g < 4; ++g) read_w(0, g);
+  read_x(0, 0, x0);
+  auto stage = [&](int s, bool zero) {
+    Source c;
+#pragma unroll
+    for (int g = 0; g < 16; ++g) {
+      if (g < 14) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[g & 7][j] = mma8(wr[g & 3], g < 8 ? x0[j] : x1[j], zero && g < 8 ? i32x4{0, 0, 0, 0} : acc[g & 7][j]);
+      } else {
+        // one of the next but one stage's loads after each MFMA: back to back they stall the wave
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          acc[g & 7][j] = mma8(wr[g & 3], x1[j], acc[g & 7][j]);
+          __builtin_amdgcn_sched_barrier(0);
+          bring(c, 4 * (g - 14) + j);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      if (g == 1) read_x(s, 1, x1);
+      if (g + 4 < 16) read_w(s, g + 4);
+      if (g == 13) {
+        // every read of stage s is done and stage s + 1 has landed: its slot can take stage s + 2
+        landed();
+        read_x(s + 1, 0, x0);
+        read_w(s + 1, 0);
+        read_w(s + 1, 1);
+        c = source_of(s + 2);
+      }
+      if (g == 14) read_w(s + 1, 2);
+      if (g == 15) read_w(s + 1, 3);
+    }
+  };
+  for (int i = 0; i < mine; ++i) {
+    stage(i * stages, true);
+    for (int k = 1; k < stages; ++k) stage(i * stages + k, false);
+    const Tile t = tile_of(i);
+    finish<T>(a, t.model, t.ot + wn, t.mt + wm, lane, acc);
+  }
+  __builtin_amdgcn_s_waitcnt(0x0f70);                  // no DMA outlives the workgroup
 }
 
 template <typename T, int RT, int NW, int D>
@@ -247,6 +553,13 @@ void launch_few(Linear8 a, int64_t n, hipStream_t s) {
   const int64_t per = cdiv(a.otiles, RT);
   a.by_wg = make_fastdiv(static_cast<uint32_t>(per));
   linear8_few_kernel<T, RT, NW, D><<<dim3(static_cast<uint32_t>(n * per), static_cast<uint32_t>(a.mtiles)), NW * 64, 0, s>>>(a);
+}
+
+template <typename T, int RT, int NW, int D>
+void launch_fused(Linear8 a, int64_t n, hipStream_t s) {
+  const int64_t per = cdiv(a.otiles, RT);
+  a.by_wg = make_fastdiv(static_cast<uint32_t>(per));
+  linear8_fused_kernel<T, RT, NW, D><<<static_cast<uint32_t>(n * per), NW * 64, 0, s>>>(a);
 }
 
 template <typename T, int FM, int FN, int WM, int WN, int NS>
@@ -261,11 +574,24 @@ void launch_tile(Linear8 a, int64_t n, hipStream_t s) {
 }
 
 template <typename T>
+void launch_large(Linear8 a, int64_t n, hipStream_t s) {
+  const int64_t per = cdiv(a.mtiles, kLargeTiles), tiles = per * cdiv(a.otiles, kLargeTiles);
+  a.by_wg = make_fastdiv(static_cast<uint32_t>(tiles));
+  const int64_t grid = std::min<int64_t>(n * tiles, std::max(device_cu_count(), 8));
+  linear8_large_kernel<T><<<static_cast<uint32_t>(grid), kLargeThreads, 0, s>>>(a, static_cast<int>(n * tiles), static_cast<int>(per));
+}
+
+template <typename T>
 void launch(const Linear8& a, int64_t n, hipStream_t s) {
   const uint32_t tiles = static_cast<uint32_t>(n * a.mtiles);
-  linear8_codes_kernel<T, 16, 4><<<tiles, 1024, 0, s>>>(a);
+  if (a.m <= 16 && static_cast<int64_t>(a.m) * a.ktiles * 4 <= kFusedPieces) return launch_fused<T, 1, 4, 8>(a, n, s);
+  if (a.ktiles <= 16)
+    linear8_codes_kernel<T, 4, 4><<<tiles, 256, 0, s>>>(a);
+  else
+    linear8_codes_kernel<T, 8, 8><<<tiles, 512, 0, s>>>(a);
   if (a.mtiles == 1) return launch_few<T, 1, 4, 8>(a, n, s);
   if (a.mtiles <= 4) return launch_tile<T, 4, 2, 1, 4, 3>(a, n, s);
+  if (n * cdiv(a.mtiles, kLargeTiles) * cdiv(a.otiles, kLargeTiles) >= 256) return launch_large<T>(a, n, s);
   launch_tile<T, 4, 4, 2, 2, 2>(a, n, s);
 }
 
