@@ -14,86 +14,14 @@
 //            up their e-th values
 #include <algorithm>
 
-#include "wc_answer_abi.h"
-#include "wc_paged_attn.h"
+#include "wc_shared.h"
 
 namespace wc {
 namespace {
 
-constexpr int kTile = kPagedTile;    // tokens a wave takes at a time
-constexpr int kLeast = 8;            // tiles in a share at least, two for each of its waves
-constexpr int kTarget = 1024;        // shares of a line at most
-constexpr int kWaves = 4;
-
-// Stretches of tokens and the sequences that read them
-struct Walk {
-  PagedTable t;
-  const int32_t* lengths;            // [units]
-  float* part;                       // [parts][share][heads][dh]
-  float2* ml;                        // [parts][share][heads]: maximum and sum, -1 where there are no tokens
-  int2* parts;                       // [units]: first part and how many, where the line of all tiles is cut (budget > 0)
-  int32_t units, share, budget, most, rows;          // rows: query heads of a unit that read one key head
-  FastDiv by_tiles, by_units;        // tiles of rows; units of a model
-};
-struct Shared {
-  Walk walk[2];                      // prefixes, own tokens
-  const char *k, *v, *q;
-  const float *ks, *vs;
-  char* o;
-  int64_t qn, qb, qh;
-  int32_t heads, group, dh, row_bytes, qvec, blocks;  // blocks: workgroups of the prefixes' walk
-  FastDiv by_kvh, by_group, by_heads, by_share;
-  float scale;                       // of the scores, times log2 e
-};
-
-__device__ __forceinline__ PagedSpan span_of(const Walk& w, int unit) { return paged_span(0, w.lengths[unit], w.most); }
-
-// Where stretches are cut, the tiles of all of them count as one line, of which every workgroup (of a key head and a tile of rows)
-// has an equal share however uneven the lengths are: share w is tiles [w size, (w + 1) size), of one unit or the ends and
-// wholes of several.  What share w has of unit s is part w + s: no two are alike, a unit's parts are neighbours, and there
-// are at most shares + units of them.  Every wave finds its share from the lengths by itself.
-struct Line {
-  int size, total;
-};
-__device__ __forceinline__ Line line_of(const Walk& w, int lane) {
-  int total = 0;
-  for (int s = lane; s < w.units; s += 64) total += paged_tiles(span_of(w, s));
-#pragma unroll
-  for (int off = 32; off; off >>= 1) total += __shfl_xor(total, off, 64);
-  return Line{max((total + w.budget - 1) / w.budget, kLeast), total};
-}
-// the unit that has tile `at` of the line (at < total), and the line's tiles before it
-__device__ __forceinline__ int2 find_tile(const Walk& w, int at, int lane) {
-  int done = 0;
-  for (int s0 = 0; s0 < w.units; s0 += 64) {
-    const int s = s0 + lane, n = s < w.units ? paged_tiles(span_of(w, s)) : 0;
-    const int start = done + before(n, lane);
-    const uint64_t mine = __ballot(at >= start && at < start + n);
-    if (mine) {
-      const int l = __ffsll(static_cast<unsigned long long>(mine)) - 1;
-      return make_int2(s0 + l, __shfl(start, l, 64));
-    }
-    done = __shfl(start + n, 63, 64);
-  }
-  return make_int2(w.units, 0);
-}
-// each unit's first part and how many it has, for the kernel that joins them; and the fault of lengths that were cut
-__device__ __forceinline__ void list_parts(const Walk& w, int size, int lane) {
-  int done = 0;
-  for (int s0 = 0; s0 < w.units; s0 += 64) {
-    const int s = s0 + lane;
-    const PagedSpan span = s < w.units ? span_of(w, s) : PagedSpan{0, 0, false};
-    if (span.cut) paged_fault(w.t);
-    const int n = paged_tiles(span);
-    const int start = done + before(n, lane), w0 = start / size;
-    if (s < w.units) w.parts[s] = n ? make_int2(w0 + s, (start + n - 1) / size - w0 + 1) : make_int2(0, 0);
-    done = __shfl(start + n, 63, 64);
-  }
-}
-
 // QT: type of q and o; KT: stored type (int8_t for codes); DC: columns provided for; RT: tiles of 16 rows
 template <typename QT, typename KT, int DC, int RT>
-__device__ __forceinline__ void walk(const Shared& a, const Walk& w, uint32_t id, float* lds) {
+__device__ __forceinline__ void walk(const SharedAttn& a, const SharedWalk& w, uint32_t id, float* lds) {
   constexpr bool kF32 = std::is_same<KT, float>::value;
   constexpr bool kQ8 = std::is_same<KT, int8_t>::value;
   // fp16 has no room for a weight times a row's scale: over codes, fp16 queries go as two bf16 planes
@@ -107,7 +35,7 @@ __device__ __forceinline__ void walk(const Shared& a, const Walk& w, uint32_t id
   constexpr int NP = std::is_same<MT, f16>::value ? 2 : 3;                                      // and of P
   // fp16 weights are taken 2^14 times as large (m - 14 in their exponents), so that those far under 1 keep their bits
   constexpr float kShift = std::is_same<MT, f16>::value ? 14.f : 0.f;
-  constexpr int NW = kWaves;
+  constexpr int NW = kSharedWaves;
   typedef typename Raw<CE * ES>::type VR;
 
   const int lane0 = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -119,12 +47,12 @@ __device__ __forceinline__ void walk(const Shared& a, const Walk& w, uint32_t id
   // this workgroup's tiles: those of one unit, or a share of the line
   int unit = up, start = 0, from = 0, to = 1 << 30;
   if (w.budget > 0) {
-    const Line line = line_of(w, lane0);
-    if (id == 0 && row0 == 0 && wave == 0) list_parts(w, line.size, lane0);
+    const SharedLine line = shared_line(w, lane0);
+    if (id == 0 && row0 == 0 && wave == 0) shared_list(w, line.size, lane0);
     from = up * line.size;
     if (from >= line.total) return;
     to = min(from + line.size, line.total);
-    const int2 first = find_tile(w, from, lane0);
+    const int2 first = shared_find(w, from, lane0);
     unit = first.x;
     start = first.y;
   }
@@ -138,9 +66,9 @@ __device__ __forceinline__ void walk(const Shared& a, const Walk& w, uint32_t id
     const int tile_lo = max(from - start, 0);
     // The table's entry for token `lane % 32` of a tile, two tiles ahead of its use; nothing looks at it (and so waits for
     // it) before row_of, the pool's row of that token or -1 for none.
-    auto look = [&](int tile) { return paged_entry(w.t, unit, static_cast<uint32_t>(tile) * kTile + (lane & 31)); };
+    auto look = [&](int tile) { return paged_entry(w.t, unit, static_cast<uint32_t>(tile) * kPagedTile + (lane & 31)); };
     int row = look(tile_lo + wave), next = look(tile_lo + wave + NW);
-    const PagedSpan span = span_of(w, unit);
+    const PagedSpan span = shared_span(w, unit);
     const int hi = span.hi, tiles = paged_tiles(span), tile_hi = min(tiles, to - start);
     if (w.budget == 0 && span.cut && threadIdx.x == 0) paged_fault(w.t);
     start += tiles;
@@ -191,7 +119,7 @@ __device__ __forceinline__ void walk(const Shared& a, const Walk& w, uint32_t id
     bool any = false;
 
     auto row_of = [&](int tile, int page) {
-      const int tok = tile * kTile + (lane & 31);
+      const int tok = tile * kPagedTile + (lane & 31);
       if (tile >= tile_hi || tok >= hi) return -1;
       const int r = paged_row(w.t, page, tok, kvh);
       if (r < 0) paged_fault(w.t);
@@ -433,7 +361,7 @@ __device__ __forceinline__ void walk(const Shared& a, const Walk& w, uint32_t id
 }
 
 template <typename QT, typename KT, int DC, int RT>
-__global__ __launch_bounds__(kWaves * 64) void shared_attention_kernel(Shared a) {
+__global__ __launch_bounds__(kSharedWaves * 64) void shared_attention_kernel(SharedAttn a) {
   extern __shared__ float lds[];
   const int own = static_cast<int>(blockIdx.x) >= a.blocks;
   const uint32_t id = blockIdx.x - (own ? a.blocks : 0);
@@ -450,15 +378,15 @@ __global__ __launch_bounds__(kWaves * 64) void shared_attention_kernel(Shared a)
 // Joins the parts of one (sequence, query head): their weights first, then their outputs, four columns a thread and as
 // many parts at a time as threads remain.  VEC: rows are whole vectors.
 template <typename QT, bool VEC>
-__global__ __launch_bounds__(256) void shared_join_kernel(Shared a) {
-  constexpr int kMost = 2 * kTarget;
+__global__ __launch_bounds__(256) void shared_join_kernel(SharedAttn a) {
+  constexpr int kMost = 2 * kSharedTarget;
   __shared__ float weight[kMost], out[4 * 256], red[8];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t at = blockIdx.x, seq = fdiv(at, a.by_heads), head = at - seq * a.by_heads.d;
   const uint32_t unit = fdiv(seq, a.by_share), place = seq - unit * a.by_share.d;
-  const Walk &w0 = a.walk[0], &w1 = a.walk[1];
+  const SharedWalk &w0 = a.walk[0], &w1 = a.walk[1];
   const int2 p0 = w0.parts[unit], p1 = w1.budget > 0 ? w1.parts[seq] : make_int2(seq, 1);
-  const int n0 = min(p0.y, kTarget), n = w1.lengths[seq] < 0 ? 0 : n0 + min(p1.y, kTarget);
+  const int n0 = min(p0.y, kSharedTarget), n = w1.lengths[seq] < 0 ? 0 : n0 + min(p1.y, kSharedTarget);
   // row of part s of these: the prefix's, then the own
   auto row = [&](int s) {
     return s < n0 ? ((p0.x + s) * static_cast<int64_t>(w0.share) + place) * a.heads + head
@@ -516,7 +444,7 @@ __global__ __launch_bounds__(256) void shared_join_kernel(Shared a) {
 // How the work is spread: tiles of 16 rows that a workgroup of the prefixes' walk has, and shares of both lines (own tokens
 // 0: whole sequences)
 struct Plan {
-  int rt;
+  int stream, rt;            // rows of a workgroup of the walk through LDS, or 0: tiles of 16 rows
   int64_t budget[2], parts[2];
 };
 int tiles_of_rows(const wc_shared_attn_args& p) {
@@ -524,14 +452,15 @@ int tiles_of_rows(const wc_shared_attn_args& p) {
 }
 Plan plan_of(const wc_shared_attn_args& p) {
   Plan plan;
-  plan.rt = tiles_of_rows(p);
+  plan.stream = shared_stream_rows(p);
+  plan.rt = plan.stream ? plan.stream / 16 : tiles_of_rows(p);
   const int64_t group = p.q_heads / p.cache.heads, units = p.cache.n * (p.cache.b / p.share), seqs = p.cache.n * p.cache.b;
   const int64_t heads0 = p.cache.heads * cdiv(p.share * group, plan.rt * 16), heads1 = p.cache.heads * cdiv(group, 16);
   const int64_t target = 512;
-  plan.budget[0] = std::min<int64_t>(cdiv(target, heads0), kTarget);
+  plan.budget[0] = std::min<int64_t>(cdiv(target, heads0), kSharedTarget);
   plan.parts[0] = plan.budget[0] + units;
   const bool whole = seqs * heads1 >= 2048 || p.max_length <= 1024;
-  plan.budget[1] = whole ? 0 : std::min<int64_t>(cdiv(target, heads1), kTarget);
+  plan.budget[1] = whole ? 0 : std::min<int64_t>(cdiv(target, heads1), kSharedTarget);
   plan.parts[1] = plan.budget[1] + seqs;
   return plan;
 }
@@ -559,16 +488,16 @@ Space space_of(const wc_shared_attn_args& p, const Plan& plan) {
 }
 
 template <typename QT, typename KT, int DC, int RT>
-void launch(const Shared& a, int64_t grid, hipStream_t s) {
-  constexpr size_t lds = static_cast<size_t>(kWaves) * 16 * (DC + 2) * sizeof(float);
+void launch(const SharedAttn& a, int64_t grid, hipStream_t s) {
+  constexpr size_t lds = static_cast<size_t>(kSharedWaves) * 16 * (DC + 2) * sizeof(float);
   const auto kernel = shared_attention_kernel<QT, KT, DC, RT>;
   if (lds > 65536)
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
-  kernel<<<static_cast<uint32_t>(grid), kWaves * 64, lds, s>>>(a);
+  kernel<<<static_cast<uint32_t>(grid), kSharedWaves * 64, lds, s>>>(a);
 }
 
 template <typename QT>
-void dispatch(const Shared& a, bool q8, int rt, int64_t grid, hipStream_t s) {
+void dispatch(const SharedAttn& a, bool q8, int rt, int64_t grid, hipStream_t s) {
   auto go = [&](auto k, auto dc) {
     typedef decltype(k) KT;
     constexpr int DC = decltype(dc)::value;
@@ -647,7 +576,7 @@ extern "C" int32_t wc_shared_attention(const wc_shared_attn_args* args, void* st
   WC_REQUIRE(p.workspace && p.workspace_bytes >= space.bytes, WC_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what,
              (long long)p.workspace_bytes, (long long)space.bytes);
   WC_REQUIRE(aligned(p.workspace, 16), WC_ERR_ALIGN, "%s: workspace must be 16-byte aligned", what);
-  Shared a;
+  SharedAttn a;
   a.k = static_cast<const char*>(c.k_pages);
   a.v = static_cast<const char*>(c.v_pages);
   a.ks = c.k_scales;
@@ -674,7 +603,7 @@ extern "C" int32_t wc_shared_attention(const wc_shared_attn_args* args, void* st
   prefix.table_stride = p.prefix_stride;
   int64_t blocks[2];
   for (int i = 0; i < 2; ++i) {
-    Walk& w = a.walk[i];
+    SharedWalk& w = a.walk[i];
     w.lengths = i ? p.lengths : p.prefix_lengths;
     w.t = paged_table(i ? c : prefix, w.lengths);
     char* ws = static_cast<char*>(p.workspace);
@@ -695,7 +624,13 @@ extern "C" int32_t wc_shared_attention(const wc_shared_attn_args* args, void* st
   const hipStream_t s = as_stream(stream);
   auto go = [&](auto t) {
     typedef decltype(t) QT;
-    dispatch<QT>(a, c.bits == 8, plan.rt, blocks[0] + blocks[1], s);
+    if (plan.stream) {
+      shared_stream(a, c.dtype, c.bits == 8, plan.stream, blocks[0], s);
+      a.blocks = 0;
+      dispatch<QT>(a, c.bits == 8, 1, blocks[1], s);
+    } else {
+      dispatch<QT>(a, c.bits == 8, plan.rt, blocks[0] + blocks[1], s);
+    }
     (c.head_dim % 4 ? shared_join_kernel<QT, false> : shared_join_kernel<QT, true>)<<<static_cast<uint32_t>(seqs * p.q_heads), 256, 0, s>>>(a);
   };
   if (c.dtype == WC_F32)

@@ -52,8 +52,19 @@ def _bars(cache, big, total, planes=2.0 ** -16):
     return attend_slack(cache.dtype, big, cache.head_dim, total, v.nan_to_num(0).abs().max().item(), planes)
 
 
-def _check(made, planes=2.0 ** -16, **kw):
+def _planes(cache, q, prefix, lens):
+    """What of a weight is left out.  In 16 bits, over prefixes of more than 32 rows a key head, heads of up to 128 columns,
+    weights are rounded to the type once (over 8-bit pages bf16's, in fp16 two of them): half a step of each, so at most that of
+    the largest value in a sum whose weights add up to one."""
+    rows = lens.shape[1] // max(prefix.shape[1], 1) * (q.shape[2] // cache.n_kv_heads)
+    if cache.dtype == torch.float32 or rows <= 32 or cache.head_dim > 128 or (cache.quantized and cache.dtype == torch.float16):
+        return 2.0 ** -16
+    return HALF[cache.dtype]
+
+
+def _check(made, **kw):
     cache, q, pt, prefix, table, lens = made
+    planes = _planes(cache, q, prefix, lens)
     with torch.no_grad():
         o = cache.attend_shared(q, pt, prefix, table, lens, **kw)
     cache.index_error()
