@@ -19,9 +19,11 @@
 namespace wc {
 namespace {
 
+constexpr int kLeast = 4;            // tiles of 32 tokens in a share at least
+
 // QT: type of q and o; KT: stored type (int8_t for codes); DC: columns provided for; RT: tiles of 16 rows
 template <typename QT, typename KT, int DC, int RT>
-__device__ __forceinline__ void walk(const SharedAttn& a, const SharedWalk& w, uint32_t id, float* lds) {
+__device__ __forceinline__ void walk(const SharedAttn& a, const SharedWalk w, uint32_t id, float* lds) {
   constexpr bool kF32 = std::is_same<KT, float>::value;
   constexpr bool kQ8 = std::is_same<KT, int8_t>::value;
   // fp16 has no room for a weight times a row's scale: over codes, fp16 queries go as two bf16 planes
@@ -68,49 +70,41 @@ __device__ __forceinline__ void walk(const SharedAttn& a, const SharedWalk& w, u
     // it) before row_of, the pool's row of that token or -1 for none.
     auto look = [&](int tile) { return paged_entry(w.t, unit, static_cast<uint32_t>(tile) * kPagedTile + (lane & 31)); };
     int row = look(tile_lo + wave), next = look(tile_lo + wave + NW);
-    const PagedSpan span = shared_span(w, unit);
-    const int hi = span.hi, tiles = paged_tiles(span), tile_hi = min(tiles, to - start);
-    if (w.budget == 0 && span.cut && threadIdx.x == 0) paged_fault(w.t);
-    start += tiles;
-    if (w.budget > 0 && tile_lo >= tile_hi) continue;             // a unit without tokens
-
-    // the rows of q: row r is head r % group of sequence r / group; past the last the last again
+    // The rows of q: row r is head r % group of sequence r / group; past the last the last again, from column 0 instead of not
+    // at all, without branches that every load would wait in.  What these loads, the length and the table's entries depend on is the
+    // unit alone, so that one wait serves them all.
     constexpr int N = kF32 ? 4 : 8, NX = kF32 ? NCK : NF;
     auto column = [&](int i) {                                    // the same columns of each product as K's
       return kF32 ? (i * 4 + g) * 4 : kQ8 ? ((i / 2) * 4 + g) * 16 + (i % 2) * 8 : (i * 4 + g) * 8;
     };
     constexpr int NV = 16 / sizeof(QT);
-    u32x4 qf[RT][kF32 ? 1 : NF][NQ];
-    float q32[RT][kF32 ? NCK : 1][4];
+    u32x4 raw[RT][NX][N / NV];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       const int r = min(row0 + t * 16 + j, rows - 1);
       const uint32_t s = fdiv(r, a.by_group), h = r - s * a.by_group.d;
       const QT* q = reinterpret_cast<const QT*>(a.q) + model * a.qn + (b0 + s) * a.qb + (kvh * a.group + h) * a.qh;
 #pragma unroll
-      for (int i = 0; i < NX; ++i) {
-        QT v[N];
+      for (int i = 0; i < NX * N / NV; ++i) {
+        const int d = column(i / (N / NV)) + i % (N / NV) * NV;
+        u32x4& x = raw[t][i / (N / NV)][i % (N / NV)];
         if (a.qvec) {
-#pragma unroll
-          for (int e = 0; e < N; e += NV) {
-            const int d = column(i) + e;
-            __builtin_memcpy(v + e, __builtin_assume_aligned(q + (d < dh ? d : 0), 16), 16);
-          }
+          x = *reinterpret_cast<const u32x4*>(q + (d < dh ? d : 0));
         } else {
+          QT v[NV];
 #pragma unroll
-          for (int e = 0; e < N; ++e) v[e] = q[column(i) + e < dh ? column(i) + e : 0];
-        }
-        float x[N];
-#pragma unroll
-        for (int e = 0; e < N; ++e) x[e] = column(i) + e < dh ? to_f32(v[e]) : 0.f;
-        if constexpr (kF32) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) q32[t][i][e] = x[e];
-        } else {
-          planes<MT, NQ>(x, qf[t][i]);
+          for (int e = 0; e < NV; ++e) v[e] = q[d + e < dh ? d + e : 0];
+          __builtin_memcpy(&x, v, sizeof v);
         }
       }
     }
+    const PagedSpan span = shared_span(w, unit);
+    const int hi = span.hi, tiles = paged_tiles(span), tile_hi = min(tiles, to - start);
+    if (w.budget == 0 && span.cut && threadIdx.x == 0) paged_fault(w.t);
+    start += tiles;
+    if (w.budget > 0 && tile_lo >= tile_hi) continue;             // a unit without tokens
+    u32x4 qf[RT][kF32 ? 1 : NF][NQ];
+    float q32[RT][kF32 ? NCK : 1][4];
 
     f32x4 acc[RT][NCV][CE] = {};
     float m[RT], l[RT];
@@ -144,6 +138,22 @@ __device__ __forceinline__ void walk(const SharedAttn& a, const SharedWalk& w, u
     if (tile_lo + wave < tile_hi) {
       row = row_of(tile_lo + wave, row);
       load_k(row);
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int i = 0; i < NX; ++i) {
+          QT v[N];
+          float x[N];
+          __builtin_memcpy(v, raw[t][i], sizeof v);
+#pragma unroll
+          for (int e = 0; e < N; ++e) x[e] = column(i) + e < dh ? to_f32(v[e]) : 0.f;
+          if constexpr (kF32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q32[t][i][e] = x[e];
+          } else {
+            planes<MT, NQ>(x, qf[t][i]);
+          }
+        }
     }
     for (int tile = tile_lo + wave; tile < tile_hi; tile += NW) {
       const bool full = __all(row >= 0);
@@ -214,14 +224,6 @@ __device__ __forceinline__ void walk(const SharedAttn& a, const SharedWalk& w, u
       row = row_of(tile + NW, next);
       load_k(row);
       next = look(tile + 2 * NW);
-      if (!full) {
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
-          if (vrow[u] < 0) {
-#pragma unroll
-            for (int c = 0; c < NCV; ++c) clear(vf[u][c]);
-          }
-      }
       u32x4 pf[RT][NP];
       float p[RT][8];
 #pragma unroll
@@ -237,22 +239,32 @@ __device__ __forceinline__ void walk(const SharedAttn& a, const SharedWalk& w, u
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         top = fmaxf(top, __shfl_xor(top, 32, 64));
         const float mn = fmaxf(m[t], top), use = finite_top(mn) - kShift;
-        if (__any(mn > m[t])) {
-          const float shrink = weight2(m[t], finite_top(mn));
-          l[t] *= shrink;
-#pragma unroll
-          for (int c = 0; c < NCV; ++c)
-#pragma unroll
-            for (int e = 0; e < CE; ++e) acc[t][c][e] *= shrink;
-        }
+        const float shrink = weight2(m[t], finite_top(mn));
         m[t] = mn;
+        l[t] *= shrink;
+#pragma unroll
+        for (int c = 0; c < NCV; ++c)
+#pragma unroll
+          for (int e = 0; e < CE; ++e) acc[t][c][e] *= shrink;
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
           p[t][u] = __builtin_amdgcn_exp2f(p[t][u] - use);
-          if (!full && vrow[u] < 0) p[t][u] = 0.f;
           l[t] += p[t][u];
-          if constexpr (kQ8) p[t][u] = !full && vrow[u] < 0 ? 0.f : p[t][u] * vscale[u];
+          if constexpr (kQ8) p[t][u] *= vscale[u];
         }
+      }
+      if (!full) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+          if (vrow[u] < 0) {
+#pragma unroll
+            for (int t = 0; t < RT; ++t) p[t][u] = 0.f;
+#pragma unroll
+            for (int c = 0; c < NCV; ++c) clear(vf[u][c]);
+          }
+      }
+#pragma unroll
+      for (int t = 0; t < RT; ++t) {
         if constexpr (!kF32) {
           if constexpr (std::is_same<QT, float>::value)
             planes<MT, NP>(p[t], pf[t]);
@@ -293,9 +305,11 @@ __device__ __forceinline__ void walk(const SharedAttn& a, const SharedWalk& w, u
       }
     }
 
-    // join the waves, a tile of rows at a time: [NW][16][DC] outputs, then [NW][16] maxima and sums (a sum of -1: no tokens),
+    // Join the waves, a tile of rows at a time: [NW][16][kRow] outputs (rows 4 values apart from whole banks: with rows of DC the
+    // 16 that a wave writes at a time all meet in one bank, 10 us of 41 over 128 sequences of up to 500 tokens), then [NW][16] maxima and sums (a sum of -1: no tokens),
     // which become the weights of the waves' outputs
-    float* om = lds + NW * 16 * DC;
+    constexpr int kRow = DC + 4;
+    float* om = lds + NW * 16 * kRow;
     float* ol = om + NW * 16;
     const int64_t first = static_cast<int64_t>(w.budget > 0 ? up + unit : unit) * w.share;      // part's first (sequence, ..)
 #pragma unroll
@@ -304,16 +318,18 @@ __device__ __forceinline__ void walk(const SharedAttn& a, const SharedWalk& w, u
       l[t] += __shfl_xor(l[t], 16, 64);
       l[t] += __shfl_xor(l[t], 32, 64);
       __syncthreads();
-      float* o = lds + (wave * 16 + j) * DC;
+      if (j < rows - row0 - t * 16) {
+        float* o = lds + (wave * 16 + j) * kRow;
 #pragma unroll
-      for (int c = 0; c < NCV; ++c)
+        for (int c = 0; c < NCV; ++c)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+          for (int r = 0; r < 4; ++r)
 #pragma unroll
-          for (int e = 0; e < CE; ++e) o[(c * 16 + g * 4 + r) * CE + e] = acc[t][c][e][r];
-      if (g == 0) {
-        om[wave * 16 + j] = m[t];
-        ol[wave * 16 + j] = any ? l[t] : -1.f;
+            for (int e = 0; e < CE; ++e) o[(c * 16 + g * 4 + r) * CE + e] = acc[t][c][e][r];
+        if (g == 0) {
+          om[wave * 16 + j] = m[t];
+          ol[wave * 16 + j] = any ? l[t] : -1.f;
+        }
       }
       __syncthreads();
       auto at = [&](int h) {                         // of row h of the tile: its place among the part's (sequence, head)
@@ -344,7 +360,7 @@ __device__ __forceinline__ void walk(const SharedAttn& a, const SharedWalk& w, u
         const int h = i / (DC / 4), d = i % (DC / 4) * 4;
         f32x4 sum = {};
 #pragma unroll
-        for (int v = 0; v < NW; ++v) sum += om[v * 16 + h] * *reinterpret_cast<const f32x4*>(lds + (v * 16 + h) * DC + d);
+        for (int v = 0; v < NW; ++v) sum += om[v * 16 + h] * *reinterpret_cast<const f32x4*>(lds + (v * 16 + h) * kRow + d);
         float* y = w.part + at(h) * dh;
         if (dh % 4 == 0) {
           if (d < dh) *reinterpret_cast<f32x4*>(y + d) = sum;
@@ -366,7 +382,8 @@ __global__ __launch_bounds__(kSharedWaves * 64) void shared_attention_kernel(Sha
   const int own = static_cast<int>(blockIdx.x) >= a.blocks;
   const uint32_t id = blockIdx.x - (own ? a.blocks : 0);
   if constexpr (RT == 1) {
-    walk<QT, KT, DC, 1>(a, a.walk[own], id, lds);
+    const SharedWalk w = own ? a.walk[1] : a.walk[0];        // a copy: an index into the arguments would be followed with every use
+    walk<QT, KT, DC, 1>(a, w, id, lds);
   } else {
     if (own)
       walk<QT, KT, DC, 1>(a, a.walk[1], id, lds);
@@ -375,70 +392,76 @@ __global__ __launch_bounds__(kSharedWaves * 64) void shared_attention_kernel(Sha
   }
 }
 
-// Joins the parts of one (sequence, query head): their weights first, then their outputs, four columns a thread and as
-// many parts at a time as threads remain.  VEC: rows are whole vectors.
+// Joins the parts of a (sequence, query head), one wave for each: lane s has the weight of part s, 64 parts at a time, and
+// as many parts as columns leave lanes for are added up side by side.  VEC: rows are whole vectors.
 template <typename QT, bool VEC>
-__global__ __launch_bounds__(256) void shared_join_kernel(SharedAttn a) {
-  constexpr int kMost = 2 * kSharedTarget;
-  __shared__ float weight[kMost], out[4 * 256], red[8];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const uint32_t at = blockIdx.x, seq = fdiv(at, a.by_heads), head = at - seq * a.by_heads.d;
+__global__ __launch_bounds__(256) void shared_join_kernel(SharedAttn a, uint32_t total) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (at >= total) return;
+  const uint32_t seq = fdiv(at, a.by_heads), head = at - seq * a.by_heads.d;
   const uint32_t unit = fdiv(seq, a.by_share), place = seq - unit * a.by_share.d;
-  const SharedWalk &w0 = a.walk[0], &w1 = a.walk[1];
-  const int2 p0 = w0.parts[unit], p1 = w1.budget > 0 ? w1.parts[seq] : make_int2(seq, 1);
-  const int n0 = min(p0.y, kSharedTarget), n = w1.lengths[seq] < 0 ? 0 : n0 + min(p1.y, kSharedTarget);
+  const SharedWalk w0 = a.walk[0], w1 = a.walk[1];
+  const int2 p0 = w0.budget > 0 ? w0.parts[unit] : make_int2(unit, 1), p1 = w1.budget > 0 ? w1.parts[seq] : make_int2(seq, 1);
+  const int n0 = p0.y, n = w1.lengths[seq] < 0 ? 0 : n0 + p1.y;
   // row of part s of these: the prefix's, then the own
   auto row = [&](int s) {
     return s < n0 ? ((p0.x + s) * static_cast<int64_t>(w0.share) + place) * a.heads + head
                   : (p1.x + s - n0) * static_cast<int64_t>(a.heads) + head;
   };
-  const int quads = (a.dh + 3) / 4, rows = 256 / quads, q = tid % quads, r = tid / quads;
-  float top = -INFINITY;
-  bool some = false;
-  for (int s = tid; s < n; s += 256) {
-    const float2 x = (s < n0 ? w0.ml : w1.ml)[row(s)];
+  auto mass = [&](int s) { return s < n ? (s < n0 ? w0.ml : w1.ml)[row(s)] : make_float2(-INFINITY, -1.f); };
+  const float2 first = mass(lane);
+  float top = first.x;
+  bool some = !(first.y < 0.f);
+  for (int s = 64 + lane; s < n; s += 64) {
+    const float2 x = mass(s);
     top = fmaxf(top, x.x);
     some |= !(x.y < 0.f);
   }
 #pragma unroll
   for (int off = 32; off; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  if (lane == 0) red[wave] = top;
-  some = __syncthreads_or(some);
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  some = __any(some);
+  int lanes = 1;                                       // of a row: a power of two
+  while (lanes * 4 < a.dh) lanes *= 2;
+  const int q = lane & (lanes - 1), g = lane / lanes, groups = 64 / lanes;
   float sum = 0.f;
-  for (int s = tid; s < n; s += 256) {
-    const float2 x = (s < n0 ? w0.ml : w1.ml)[row(s)];
-    const float f = x.y < 0.f ? 0.f : weight2(x.x, finite_top(top));
-    weight[s] = f;
-    sum += x.y < 0.f ? 0.f : f * x.y;
-  }
-#pragma unroll
-  for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off, 64);
-  if (lane == 0) red[4 + wave] = sum;
-  __syncthreads();
-  sum = red[4] + red[5] + red[6] + red[7];
   f32x4 o = {};
-  if (r < rows) {
-    for (int s = r; s < n; s += rows) {
-      const float* p = (s < n0 ? w0.part : w1.part) + row(s) * a.dh + q * 4;
-      f32x4 v;
-      if constexpr (VEC) {
-        v = *reinterpret_cast<const f32x4*>(p);
-      } else {
+  for (int s0 = 0; s0 < n; s0 += 64) {
+    const float2 x = s0 ? mass(s0 + lane) : first;
+    const float f = x.y < 0.f ? 0.f : weight2(x.x, finite_top(top));       // 0 for a part without tokens, which holds zeros
+    sum += x.y < 0.f ? 0.f : f * x.y;
+    const int m = min(64, n - s0);
+    // eight outputs a lane on their way together; past the last part the last again, which is not added
+    for (int i = g; i - g < m; i += 8 * groups) {
+      f32x4 v[8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = p[q * 4 + e < a.dh ? e : 0];
+      for (int u = 0; u < 8; ++u) {
+        const int c = s0 + min(i + u * groups, m - 1);
+        const float* p = (c < n0 ? w0.part : w1.part) + row(c) * a.dh;
+        if constexpr (VEC) {
+          v[u] = *reinterpret_cast<const f32x4*>(p + (q * 4 < a.dh ? q * 4 : 0));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[u][e] = p[q * 4 + e < a.dh ? q * 4 + e : 0];
+        }
       }
-      // a part without tokens holds zeros
-      o += weight[s] * v;
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float weight = __shfl(f, min(i + u * groups, 63), 64);
+        if (i + u * groups < m) o += weight * v[u];
+      }
     }
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) out[e * 256 + tid] = o[e];
-  __syncthreads();
-  if (tid >= a.dh) return;
-  float v = 0.f;
-  for (int i = 0; i < rows; ++i) v += out[(tid & 3) * 256 + i * quads + tid / 4];
-  reinterpret_cast<QT*>(a.o)[static_cast<int64_t>(at) * a.dh + tid] = from_f32<QT>(some ? v / sum : 0.f);
+  for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  for (int off = lanes; off < 64; off *= 2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], off, 64);
+  if (g) return;
+  QT* y = reinterpret_cast<QT*>(a.o) + static_cast<int64_t>(at) * a.dh;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (q * 4 + e < a.dh) y[q * 4 + e] = from_f32<QT>(some ? o[e] / sum : 0.f);
 }
 
 // How the work is spread: tiles of 16 rows that a workgroup of the prefixes' walk has, and shares of both lines (own tokens
@@ -456,7 +479,7 @@ Plan plan_of(const wc_shared_attn_args& p) {
   plan.rt = plan.stream ? plan.stream / 16 : tiles_of_rows(p);
   const int64_t group = p.q_heads / p.cache.heads, units = p.cache.n * (p.cache.b / p.share), seqs = p.cache.n * p.cache.b;
   const int64_t heads0 = p.cache.heads * cdiv(p.share * group, plan.rt * 16), heads1 = p.cache.heads * cdiv(group, 16);
-  const int64_t target = 512;
+  const int64_t target = 512;                        // two workgroups a compute unit; of 64 rows through LDS one
   plan.budget[0] = std::min<int64_t>(cdiv(target, heads0), kSharedTarget);
   plan.parts[0] = plan.budget[0] + units;
   const bool whole = seqs * heads1 >= 2048 || p.max_length <= 1024;
@@ -489,7 +512,7 @@ Space space_of(const wc_shared_attn_args& p, const Plan& plan) {
 
 template <typename QT, typename KT, int DC, int RT>
 void launch(const SharedAttn& a, int64_t grid, hipStream_t s) {
-  constexpr size_t lds = static_cast<size_t>(kSharedWaves) * 16 * (DC + 2) * sizeof(float);
+  constexpr size_t lds = static_cast<size_t>(kSharedWaves) * 16 * (DC + 6) * sizeof(float);
   const auto kernel = shared_attention_kernel<QT, KT, DC, RT>;
   if (lds > 65536)
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds));
@@ -613,6 +636,7 @@ extern "C" int32_t wc_shared_attention(const wc_shared_attn_args* args, void* st
     w.units = static_cast<int32_t>(i ? seqs : units);
     w.share = static_cast<int32_t>(i ? 1 : p.share);
     w.budget = static_cast<int32_t>(plan.budget[i]);
+    w.least = kLeast;
     w.most = static_cast<int32_t>(most_of(p, i));
     w.rows = w.share * a.group;
     const int64_t tiles = cdiv(w.rows, i ? 16 : plan.rt * 16);
@@ -631,7 +655,8 @@ extern "C" int32_t wc_shared_attention(const wc_shared_attn_args* args, void* st
     } else {
       dispatch<QT>(a, c.bits == 8, plan.rt, blocks[0] + blocks[1], s);
     }
-    (c.head_dim % 4 ? shared_join_kernel<QT, false> : shared_join_kernel<QT, true>)<<<static_cast<uint32_t>(seqs * p.q_heads), 256, 0, s>>>(a);
+    const uint32_t total = static_cast<uint32_t>(seqs * p.q_heads);
+    (c.head_dim % 4 ? shared_join_kernel<QT, false> : shared_join_kernel<QT, true>)<<<(total + 3) / 4, 256, 0, s>>>(a, total);
   };
   if (c.dtype == WC_F32)
     go(float());

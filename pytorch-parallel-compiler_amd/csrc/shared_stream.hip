@@ -4,7 +4,7 @@
 // A workgroup of four waves has 128 rows, 32 a wave (or 64, of which two waves have the same and half of the tokens each),
 // and walks its share of a prefix in tiles of 64 tokens, K and V row-major in LDS, double-buffered: 16-bit pages come by LDS-DMA
 // issued one tile ahead, 8-bit ones through registers, as 16-bit numbers that hold the codes exactly.  Which rows of
-// the pool a tile has, the lanes find from the table two tiles ahead.  Per tile and wave, with v_mfma_f32_32x32x16:
+// the pool a tile has, the lanes find from 64 entries of the table, which they hold.  Per tile and wave, with v_mfma_f32_32x32x16:
 //   S^T = K Q^T      lane l holds row l % 32 and tokens 8 (r / 4) + 4 (l / 32) + r % 4 of each block of 32
 //   softmax          in the lane; the lane halves that share a row exchange their maxima, and O is rescaled, only in tiles where
 //                    a lane of the wave finds a new running maximum
@@ -30,6 +30,28 @@ __device__ __forceinline__ f32x16 mma32(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
+// The fragments of V^T of 16 tokens by 32 columns each, at LDS byte addresses `at` + OFF and, 8 tokens on, OFF + NEXT.  Written as
+// one block with its wait, because the compiler has the builtin wait for all loads into LDS that are on their way.
+template <int OFF, int NEXT>
+__device__ __forceinline__ void read_v(const uint32_t (&at)[2], i16x4 (&v)[2][2]) {
+  asm volatile("ds_read_b64_tr_b16 %0, %4 offset:%6\n\tds_read_b64_tr_b16 %1, %4 offset:%7\n\t"
+               "ds_read_b64_tr_b16 %2, %5 offset:%6\n\tds_read_b64_tr_b16 %3, %5 offset:%7\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1])
+               : "v"(at[0]), "v"(at[1]), "n"(OFF), "n"(OFF + NEXT) : "memory");
+}
+template <int OFF, int NEXT>
+__device__ __forceinline__ void read_v(const uint32_t (&at)[4], i16x4 (&v)[4][2]) {
+  asm volatile("ds_read_b64_tr_b16 %0, %8 offset:%12\n\tds_read_b64_tr_b16 %1, %8 offset:%13\n\t"
+               "ds_read_b64_tr_b16 %2, %9 offset:%12\n\tds_read_b64_tr_b16 %3, %9 offset:%13\n\t"
+               "ds_read_b64_tr_b16 %4, %10 offset:%12\n\tds_read_b64_tr_b16 %5, %10 offset:%13\n\t"
+               "ds_read_b64_tr_b16 %6, %11 offset:%12\n\tds_read_b64_tr_b16 %7, %11 offset:%13\n\t"
+               "s_waitcnt lgkmcnt(0)"
+               : "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]), "=&v"(v[3][0]),
+                 "=&v"(v[3][1])
+               : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(OFF), "n"(OFF + NEXT) : "memory");
+}
+
 // T: type of q and o; KT: stored type; DHP: columns provided for; RW: waves that have rows of their own
 template <typename T, typename KT, int DHP, int RW>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void shared_stream_kernel(SharedAttn a) {
@@ -41,7 +63,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
   constexpr int NKS = DHP / 16, DT = DHP / 32, TILE = kStBK * DHP;
   constexpr int TS = 4 / RW, NB = 2 / TS;            // waves that share rows; blocks of 32 tokens of a wave
   constexpr int CPR = DHP * static_cast<int>(sizeof(KT)) / 16, CH = kStBK * CPR, PIECES = 2 * CH / 256;     // 16-byte pieces of a row, of a tile; a thread's
-  __shared__ __attribute__((aligned(16))) uint16_t lds[2][2 * TILE];   // [buffer][K tile, V tile]
+  __shared__ __attribute__((aligned(16))) uint16_t lds[2][2 * TILE];           // [buffer][K tile, V tile]
   __shared__ float scales[kQ8 ? 2 : 1][2][kStBK];
   const SharedWalk& w = a.walk[0];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -62,16 +84,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
   const int2 first = shared_find(w, from, lane);
   int unit = first.x, start = first.y;
   bool clear_columns = a.row_bytes < DHP * static_cast<int>(sizeof(KT));       // those that no row has stay zero
-  // this thread's pieces of a tile: row of the tile and the column that goes to its place (16 bits), or is brought (8 bits)
-  int prow[PIECES], pcol[PIECES];
+  // This thread's pieces of a tile, those of K first: their rows are a whole number of swizzles apart, so that all of K have the same
+  // column (16 bits: that which goes to the piece's place; 8 bits: that which is brought), and all of V.
+  constexpr int kPer = CH / 256, kApart = 256 / CPR;
+  static_assert(CH % 256 == 0 && kApart % 16 == 0, "pieces of a thread are whole swizzles apart");
+  const int prow = tid / CPR;
+  const int kcol = kQ8 ? tid % CPR * 16 : k_at<DHP>(prow, tid % CPR) - prow * DHP;
+  const int vcol = kQ8 ? kcol : v_at<DHP>(prow, tid % CPR * 8) - prow * DHP;
+  const bool kin = kcol * static_cast<int>(sizeof(KT)) < a.row_bytes, vin = vcol * static_cast<int>(sizeof(KT)) < a.row_bytes;
+  const char* kp = a.k + kcol * static_cast<int>(sizeof(KT));
+  const char* vp = a.v + vcol * static_cast<int>(sizeof(KT));
+  uint32_t vat[DT];                                    // of the lane's V^T fragments in a tile, in bytes
 #pragma unroll
-  for (int u = 0; u < PIECES; ++u) {
-    const bool isv = wave * 64 + u * 256 >= CH;        // the same for all lanes of a wave
-    const int e = tid + u * 256 - (isv ? CH : 0);
-    prow[u] = e / CPR;
-    const int ch = e % CPR;
-    pcol[u] = kQ8 ? ch * 16 : (isv ? v_at<DHP>(prow[u], ch * 8) : k_at<DHP>(prow[u], ch)) - prow[u] * DHP;
-  }
+  for (int d = 0; d < DT; ++d) vat[d] = v_at<DHP>(4 * hf + ((lane & 15) >> 2), 32 * d + (lane & 16) + 4 * (lane & 3)) * 2;
   // the maximum is that of the sums, times a positive scale: the queries take the sign, or are 0
   const float c = a.scale == 0.f ? 1.f : fabsf(a.scale);
   const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u, keep = a.scale == 0.f ? 0u : ~0u;
@@ -84,7 +109,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
     const int tiles = paged_tiles(span), tile_hi = min(tiles, to - start);
     start += tiles;
     if (tile_lo >= tile_hi) continue;                 // a unit without tokens
-    const int begin = tile_lo * kPagedTile, end = min(span.hi, tile_hi * kPagedTile), n = (end - begin + kStBK - 1) / kStBK;
+    // the same for all lanes, which the compiler is told, so that what hangs on it is branches
+    const int begin = __builtin_amdgcn_readfirstlane(tile_lo * kPagedTile);
+    const int end = __builtin_amdgcn_readfirstlane(min(span.hi, tile_hi * kPagedTile)), n = (end - begin + kStBK - 1) / kStBK;
 
     // Q^T fragments (B operand of S^T): row l32 of the wave's, columns 16 k + 8 hf .. + 8
     bf16x8 qf[NKS];
@@ -112,10 +139,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
       }
     }
 
-    // the table's entry and then the pool's row of token `lane` of tile i, -1 for none
-    auto look = [&](int i) { return paged_entry(w.t, unit, static_cast<uint32_t>(begin) + i * kStBK + lane); };
-    auto row_of = [&](int i, int page) {
+    // The table's entries from block `held` on, one a lane: 64 blocks, which last for a page's length of tiles.  They have come
+    // before anything else is brought, so that no tile waits for what is on its way behind it.
+    int entries = 0, held = -64;
+    // the pool's row of token `lane` of tile i, -1 for none
+    auto row_of = [&](int i) __attribute__((always_inline)) {
       const int tok = begin + i * kStBK + lane;
+      const int block = fdiv(tok, w.t.by_page), lo = __builtin_amdgcn_readfirstlane(block);
+      if (__builtin_amdgcn_readlane(block, 63) - held >= 64) {
+        held = lo;
+        entries = paged_entry(w.t, unit, static_cast<uint32_t>(held + lane) * w.t.by_page.d);
+        asm volatile("" : "+v"(entries));
+      }
+      const int page = __shfl(entries, block - held, 64);
       if (tok >= end) return -1;
       const int r = paged_row(w.t, page, tok, kvh);
       if (r < 0) paged_fault(w.t);
@@ -123,30 +159,40 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
     };
     u32x4 raw[kQ8 ? PIECES : 1];
     float ks = 0.f, vs = 0.f;
-    // tile rows `row` (by lane) on their way into buffer `buf`; those there are none of as zeros: their scores are taken out, but 0
-    // times what is left of an earlier tile may not be 0
+    // tile rows `row` (by lane) on their way into buffer `buf`; where there are none, row 0 of the pool, so that every tile is as many
+    // loads of the wave
     auto fetch = [&](int buf, int row) {
       if constexpr (kQ8) {
         ks = row >= 0 ? a.ks[row] : 0.f;
         vs = row >= 0 ? a.vs[row] : 0.f;
       }
+      int r[kPer];
 #pragma unroll
-      for (int u = 0; u < PIECES; ++u) {
-        const bool isv = wave * 64 + u * 256 >= CH;
-        const int r = __shfl(row, prow[u], 64);
-        const char* p = (isv ? a.v : a.k) + static_cast<int64_t>(max(r, 0)) * a.row_bytes + pcol[u] * static_cast<int>(sizeof(KT));
-        const bool in = pcol[u] * static_cast<int>(sizeof(KT)) < a.row_bytes;
+      for (int u = 0; u < kPer; ++u) r[u] = __shfl(row, prow + u * kApart, 64);
+      auto bring = [&](const char* p, bool in, int first) __attribute__((always_inline)) {
         if constexpr (kQ8) {
-          raw[u] = u32x4{0, 0, 0, 0};
-          if (in && r >= 0) raw[u] = *reinterpret_cast<const u32x4*>(p);
-        } else {
-          if (in && r >= 0)
-            __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(p),
-                                             (__attribute__((address_space(3))) void*)(&lds[buf][(wave * 64 + u * 256) * 8]), 16, 0, 0);
-          else if (r < 0)
-            *reinterpret_cast<uint4*>(&lds[buf][(tid + u * 256) * 8]) = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int u = 0; u < kPer; ++u) {
+            raw[first + u] = u32x4{0, 0, 0, 0};
+            if (in && r[u] >= 0) raw[first + u] = *reinterpret_cast<const u32x4*>(p + static_cast<int64_t>(r[u]) * a.row_bytes);
+          }
+        } else if (in) {
+#pragma unroll
+          for (int u = 0; u < kPer; ++u)
+            __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(p + static_cast<int64_t>(max(r[u], 0)) * a.row_bytes),
+                                             (__attribute__((address_space(3))) void*)(&lds[buf][(wave * 64 + (first + u) * 256) * 8]), 16, 0,
+                                             0);
         }
-      }
+      };
+      bring(kp, kin, 0);
+      bring(vp, vin, kPer);
+    };
+    // Rows of a tile that has come of which there are none, as zeros: their scores are taken out, but 0 times what stands there
+    // may not be 0.
+    auto blank = [&](int buf, uint64_t valid) {
+#pragma unroll
+      for (int u = 0; u < PIECES; ++u)
+        if (!(valid >> (prow + u % kPer * kApart) & 1)) *reinterpret_cast<uint4*>(&lds[buf][(tid + u * 256) * 8]) = make_uint4(0, 0, 0, 0);
     };
     // 8 bits: the codes that have come, as numbers into LDS
     auto put = [&](int buf) {
@@ -155,8 +201,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
         if (wave == 1) scales[buf][1][lane] = vs;
 #pragma unroll
         for (int u = 0; u < PIECES; ++u) {
-          const bool isv = wave * 64 + u * 256 >= CH;
-          if (pcol[u] >= a.row_bytes) continue;
+          const bool isv = u >= kPer;
+          if (!kin) continue;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             u32x4 x;
@@ -166,7 +212,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
               const float f0 = byte_f32(v, (e & 1) * 2), f1 = byte_f32(v, (e & 1) * 2 + 1);
               x[e] = isv ? pack2<PT>(f0, f1) : pack2<T>(f0, f1);
             }
-            const int at = isv ? TILE + v_at<DHP>(prow[u], pcol[u] + h * 8) : k_at<DHP>(prow[u], pcol[u] / 8 + h);
+            const int at = isv ? TILE + v_at<DHP>(prow + (u - kPer) * kApart, kcol + h * 8) : k_at<DHP>(prow + u * kApart, kcol / 8 + h);
             *reinterpret_cast<u32x4*>(&lds[buf][at]) = x;
           }
         }
@@ -183,27 +229,31 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
     float base = 0.f, lrun = 0.f;
     bool fresh = true, any = false;
 
-    int row = row_of(0, look(0)), next = look(1);
     __syncthreads();                                   // the buffers are free
     if (clear_columns) {
       for (int e = tid; e < 2 * 2 * TILE / 8; e += 256) reinterpret_cast<uint4*>(&lds[0][0])[e] = make_uint4(0, 0, 0, 0);
       __syncthreads();
       clear_columns = TS == 2;                         // where the waves' outputs meet in the buffers, again
     }
+    int row = row_of(0);
+    uint64_t valid = __ballot(row >= 0), coming = 0;   // which of the tokens of the tile at work and of the next there are
     fetch(0, row);
-    uint64_t valid = __ballot(row >= 0);
     put(0);
-    __builtin_amdgcn_s_waitcnt(0x0070);                // vmcnt(0) lgkmcnt(0)
-    __syncthreads();
     for (int i = 0; i < n; ++i) {
-      const uint16_t* ks_ = lds[i & 1];
-      const uint16_t* vs_ = ks_ + TILE;
-      uint64_t coming = 0;
-      if (i + 1 < n) {                                 // the other buffer was last read before the previous barrier
-        row = row_of(i + 1, next);
+      const int buf = i & 1;
+      // the tile has come for this wave, then for all, and nobody is at the one before
+      __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0), lgkmcnt(0)
+      __syncthreads();
+      if (!kQ8 && valid != ~0ull) {
+        blank(buf, valid);
+        __syncthreads();
+      }
+      const uint16_t* ks_ = lds[buf];
+      const uint32_t vbase = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_i16x4*)(ks_ + TILE)));
+      if (i + 1 < n) {
+        row = row_of(i + 1);
         coming = __ballot(row >= 0);
-        fetch((i + 1) & 1, row);
-        next = look(i + 2);
+        fetch(buf ^ 1, row);
       }
       any |= valid != 0;
       f32x16 s[NB];
@@ -220,7 +270,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
         if constexpr (kQ8) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const f32x4 f = *reinterpret_cast<const f32x4*>(&scales[i & 1][0][32 * blk + q * 8 + 4 * hf]);
+            const f32x4 f = *reinterpret_cast<const f32x4*>(&scales[buf][0][32 * blk + q * 8 + 4 * hf]);
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[b][q * 4 + e] *= f[e];
           }
@@ -267,7 +317,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
           l0 += p0;
           l1 += p1;
           if constexpr (kQ8) {
-            const float* f = &scales[i & 1][1][32 * blk + (r >> 1) * 8 + 4 * hf + (r & 1) * 2];
+            const float* f = &scales[buf][1][32 * blk + (r >> 1) * 8 + 4 * hf + (r & 1) * 2];
             p0 *= f[0];
             p1 *= f[1];
           }
@@ -275,29 +325,29 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
           if constexpr (NP == 2) pk[1][r] = pack2<PT>(p0 - unpack_lo<PT>(pk[0][r]), p1 - unpack_hi<PT>(pk[0][r]));
         }
         lrun += l0 + l1;
+        // tokens 32 blk + 16 j + 8 piece + 4 hf + (0 .. 3), columns 32 d + 16 (lane / 16 % 2) + (0 .. 15)
+        uint32_t at[DT];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          bf16x8 pf[NP];
-#pragma unroll
-          for (int q = 0; q < NP; ++q)
-            pf[q] = __builtin_bit_cast(bf16x8, make_uint4(pk[q][4 * j], pk[q][4 * j + 1], pk[q][4 * j + 2], pk[q][4 * j + 3]));
+        for (int d = 0; d < DT; ++d) at[d] = vbase + vat[d] + (TS == 1 ? 0 : tw * NB * 32 * DHP * 2);
+        auto product = [&](auto J) __attribute__((always_inline)) {
+          constexpr int j = decltype(J)::value;
+          i16x4 v[DT][2];
+          if (b == 0) read_v<j * 16 * DHP * 2, 8 * DHP * 2>(at, v);
+          else read_v<(32 + j * 16) * DHP * 2, 8 * DHP * 2>(at, v);
 #pragma unroll
           for (int d = 0; d < DT; ++d) {
-            // tokens 32 blk + 16 j + 8 piece + 4 hf + (0 .. 3), columns 32 d + 16 (lane / 16 % 2) + (0 .. 15)
-            const int vr = 32 * blk + 16 * j + 4 * hf + ((lane & 15) >> 2), vc = 32 * d + (lane & 16) + 4 * (lane & 3);
-            const i16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vs_ + v_at<DHP>(vr, vc)));
-            const i16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(vs_ + v_at<DHP>(vr + 8, vc)));
-            const i16x8 vf = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            const i16x8 vf = __builtin_shufflevector(v[d][0], v[d][1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
-            for (int q = NP - 1; q >= 0; --q) oacc[d] = mma32<PT>(__builtin_bit_cast(bf16x8, vf), pf[q], oacc[d]);
+            for (int q = NP - 1; q >= 0; --q) {
+              const bf16x8 pf = __builtin_bit_cast(bf16x8, make_uint4(pk[q][4 * j], pk[q][4 * j + 1], pk[q][4 * j + 2], pk[q][4 * j + 3]));
+              oacc[d] = mma32<PT>(__builtin_bit_cast(bf16x8, vf), pf, oacc[d]);
+            }
           }
-        }
+        };
+        product(std::integral_constant<int, 0>());
+        product(std::integral_constant<int, 1>());
       }
-      if (i + 1 < n) {
-        put((i + 1) & 1);
-        __builtin_amdgcn_s_waitcnt(0x0070);
-        __syncthreads();
-      }
+      if (i + 1 < n) put(buf ^ 1);
       valid = coming;
     }
 

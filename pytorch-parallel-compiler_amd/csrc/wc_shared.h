@@ -6,7 +6,6 @@
 
 namespace wc {
 
-constexpr int kSharedLeast = 8;      // tiles in a share at least, two for each of its waves
 constexpr int kSharedTarget = 1024;  // shares of a line at most
 constexpr int kSharedWaves = 4;
 
@@ -17,7 +16,7 @@ struct SharedWalk {
   float* part;                       // [parts][share][heads][dh]
   float2* ml;                        // [parts][share][heads]: maximum and sum, -1 where there are no tokens
   int2* parts;                       // [units]: first part and how many, where the line of all tiles is cut (budget > 0)
-  int32_t units, share, budget, most, rows;          // rows: query heads of a unit that read one key head
+  int32_t units, share, budget, least, most, rows;   // least: tiles of a share at least; rows: query heads of a unit that read one key head
   FastDiv by_tiles, by_units;        // tiles of rows; units of a model
 };
 struct SharedAttn {
@@ -45,7 +44,7 @@ __device__ __forceinline__ SharedLine shared_line(const SharedWalk& w, int lane)
   for (int s = lane; s < w.units; s += 64) total += paged_tiles(shared_span(w, s));
 #pragma unroll
   for (int off = 32; off; off >>= 1) total += __shfl_xor(total, off, 64);
-  return SharedLine{max((total + w.budget - 1) / w.budget, kSharedLeast), total};
+  return SharedLine{max((total + w.budget - 1) / w.budget, w.least), total};
 }
 // the unit that has tile `at` of the line (at < total), and the line's tiles before it
 __device__ __forceinline__ int2 shared_find(const SharedWalk& w, int at, int lane) {
