@@ -257,31 +257,69 @@ struct Row {
           if (e >= skip[i] && e < v) go(value_in<T>(t[i], e), static_cast<int>(from[i]) + e);
     });
   }
-  // put(index, place) of the values within [lo, hi], places from take(how many there are): first a bit for each of a thread's 8 E
-  // values, then a turn for each bit
+  // put(index, place) of the values within [lo, hi], places from take(how many a wave has): a bit for each of a thread's 8 E values
+  // at a time, while the next are on their way, then a turn for each bit.
   template <typename G, typename F>
   __device__ __forceinline__ void select(float lo, float hi, G take, F put) const {
-    batches([&](const u32x4(&t)[8], const int64_t(&from)[8], const int(&skip)[8]) __attribute__((always_inline)) {
+    constexpr int step = kThreads * E;
+    if (v < E) {
+      const float f = static_cast<int>(threadIdx.x) < v ? to_f32(x[threadIdx.x]) : __builtin_nanf("");
+      if (f >= lo && f <= hi) put(threadIdx.x, take(1));
+      return;
+    }
+    const uint32_t last = v - E;                       // pieces over the end from there, where what is not their own is left out
+    auto load = [&](uint32_t at, u32x4(&t)[8]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) __builtin_memcpy(&t[i], x + smaller(at + i * step, last), 16);
+    };
+    const int lane = threadIdx.x & 63;
+    const uint32_t end = v, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 64 * E;
+    u32x4 t[8], next[8];
+    uint32_t first = wave;                             // of the wave: the same for its lanes
+    if (first < end) load(first + lane * E, t);
+    for (; first < end; first += 8 * step) {
+      const uint32_t at = first + lane * E;
+      if (first + 8 * step < end) load(at + 8 * step, next);
       uint64_t mine = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         uint32_t m = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-          const float x = value_in<T>(t[i], e);
-          m |= x >= lo && x <= hi ? 1u << e : 0u;
+          const float f = value_in<T>(t[i], e);
+          m |= __builtin_amdgcn_fmed3f(f, lo, hi) == f ? 1u << e : 0u;
         }
-        m &= (~0u << skip[i]) & ((1u << smaller(v, E)) - 1);
         mine |= static_cast<uint64_t>(m) << i * E;
       }
-      int at = mine ? take(__popcll(mine)) : 0;
-      while (mine) {
-        const int bit = __ffsll(static_cast<unsigned long long>(mine)) - 1, i = bit / E;
-        mine &= mine - 1;
-        const int64_t own = from[0] + static_cast<int64_t>(i) * (kThreads * E);
-        put(static_cast<int>(i ? smaller(own, static_cast<int64_t>(v - E)) : from[0]) + bit % E, at++);
+      if (first + 7 * step + 64 * E > end) {           // the wave's last: pieces that begin before their own place, or have none
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t own = at + i * step;
+          const uint32_t skip = smaller(own - smaller(own, last), static_cast<uint32_t>(E));
+          const uint64_t bits = ~0u << skip & ((1u << E) - 1);
+          mine &= bits << i * E | ~(((1ull << E) - 1) << i * E);
+        }
       }
-    });
+      if (__ballot(mine != 0)) {
+        const int n = __popcll(mine);
+        int upto = n;
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) {
+          const int up = __shfl_up(upto, off, 64);
+          if (lane >= off) upto += up;
+        }
+        int place = 0;
+        if (lane == 63) place = take(upto);
+        place = __builtin_amdgcn_readlane(place, 63) + upto - n;
+        while (mine) {
+          const int bit = __ffsll(static_cast<unsigned long long>(mine)) - 1;
+          mine &= mine - 1;
+          put(static_cast<int>(smaller(at + bit / E * step, last)) + bit % E, place++);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = next[i];
+    }
   }
 };
 
@@ -761,17 +799,15 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(Sample a) {
       if (tid == 0) s.found32[1] = 0;
       __syncthreads();
       // The values whose places are under the upper edge of b0 and from the lower edge of b1 on: places rise with values, so
-      // the last and first of them are next to the edges divided by the scale.
+      // the last and first of them are next to the edges divided by the scale.  A lane has a candidate.
       float hi = INFINITY, lo = -3.402823466e38f;
       if (b0) {
-        const float edge = bins.base - b0 + 1;
-        hi = value_of(key_of(edge / bins.scale) + 16);
-        for (int i = 0; i < 64 && bins.scaled(hi) >= edge; ++i) hi = value_of(key_of(hi) - 1);
+        const float edge = bins.base - b0 + 1, at = value_of(key_of(edge / bins.scale) + 16 - lane);
+        hi = __shfl(at, (__ffsll(static_cast<unsigned long long>(__ballot(!(bins.scaled(at) >= edge)))) + 63) & 63, 64);
       }
       if (b1 < kBins - 1) {
-        const float edge = bins.base - b1;
-        lo = value_of(key_of(edge / bins.scale) - 16);
-        for (int i = 0; i < 64 && bins.scaled(lo) < edge; ++i) lo = value_of(key_of(lo) + 1);
+        const float edge = bins.base - b1, at = value_of(key_of(edge / bins.scale) - 16 + lane);
+        lo = __shfl(at, (__ffsll(static_cast<unsigned long long>(__ballot(!(bins.scaled(at) < edge)))) + 63) & 63, 64);
       }
       row.select(lo, hi, [&](int n) { return static_cast<int>(atomicAdd(&s.found32[1], static_cast<uint32_t>(n))); },
                  [&](int i, int at) {
@@ -793,12 +829,13 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(Sample a) {
     // all but proportional to values where these differ by little, and equal ones are parted by their places.
     auto cut_list = [&](bool by_count, uint64_t above, uint64_t limit) __attribute__((always_inline)) {
       constexpr int N = kList / kThreads;
-      uint64_t v[N];
+      uint64_t v[N], by[N];                           // of each: what it counts for
       int n = listed, mine = 0;                       // of the thread: those of the part
 #pragma unroll
       for (int e = 0; e < N; ++e) {
         const int i = tid + e * kThreads;
         v[e] = i < n ? s.list[i] : 0;                // 0: none
+        by[e] = by_count || !v[e] ? 1 : w(value_of(list_key(v[e])));
       }
       while (n > kRank) {
         constexpr uint64_t none = ~static_cast<uint64_t>(0);
@@ -830,7 +867,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(Sample a) {
           part[e] = v[e] ? static_cast<int>((hi - v[e]) >> shift) : -1;
           if (v[e])
             atomicAdd(reinterpret_cast<unsigned long long*>(&s.bin_weight[part[e]]),
-                      by_count ? 1ull : static_cast<unsigned long long>(w(value_of(list_key(v[e])))));
+                      static_cast<unsigned long long>(by[e]));
         }
         __syncthreads();
         uint64_t all;
@@ -860,7 +897,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(Sample a) {
         if (v[e]) {
           const uint32_t at = atomicAdd(&s.found32[3], 1u);
           s.other[at] = v[e];
-          s.rank_weight[at] = by_count ? 1 : w(value_of(list_key(v[e])));
+          s.rank_weight[at] = by[e];
         }
       __syncthreads();
       rank_all(s.other, n, s);
