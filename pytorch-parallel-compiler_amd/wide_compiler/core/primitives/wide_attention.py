@@ -287,7 +287,7 @@ class WideAttention(nn.Module):
             raise RuntimeError(f"{what}: {list(common.shape)} prefix lengths and {list(lengths.shape)} lengths for [N={n}, B={b}] "
                                "sequences in groups of one size")
         share = b // common.shape[1] if common.shape[1] else 1
-        position = start + common.repeat_interleave(share, 1)
+        position = start + common.clamp_min(0).repeat_interleave(share, 1)
         q, k, v = self._cached_heads(what, x[:, :, None], cache, position[..., None], head_norm)
         cache.write(k, v, block_table, start)
         own = lengths.masked_fill(lengths <= 0, -1)
