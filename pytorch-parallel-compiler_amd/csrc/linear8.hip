@@ -416,18 +416,18 @@ __global__ __launch_bounds__(WM * WN * 64) void linear8_tile_kernel(Linear8 a) {
   finish<T>(a, model, ot0 + wn, mt0 + wm, lane, acc);
 }
 
-// Tiles of 256 x 256 outputs for whole rounds of the compute units: 8 waves of 128 outputs x 64 rows each, two stages of 128 columns
+// Tiles of 256 x 256 outputs for whole rounds of the compute units: 8 waves of 128 outputs x 64 rows each, four stages of 64 columns
 // in LDS.  A workgroup walks its tiles without a pause between them: stages of all its tiles are one line, and while one is
-// multiplied the next but one is on its way.  Within a stage the waves stream their tiles of W through four registers,
+// multiplied the next three are on their way.  Within a stage the waves stream their tiles of W through four registers,
 // four groups of MFMAs ahead of their use, so that a wave seldom waits for what it reads.
-constexpr int kLargeThreads = 512, kLargeTiles = 16, kLargeStage = 4 * kLargeTiles * 1024;
+constexpr int kLargeThreads = 512, kLargeTiles = 16, kLargeStage = 2 * kLargeTiles * 1024;
 
 template <typename T>
 __global__ __launch_bounds__(kLargeThreads, 1) void linear8_large_kernel(Linear8 a, int tiles_total, int per) {
-  __shared__ __attribute__((aligned(1024))) char raw[2 * kLargeStage];       // [2][W tiles, x tiles][2 halves]
+  __shared__ __attribute__((aligned(1024))) char raw[4 * kLargeStage];       // [4][W tiles, x tiles]
   lds_char* const lds = (lds_char*)raw;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wn = (wave & 1) * 8, wm = (wave >> 1) * 4, stages = a.ktiles / 2;
+  const int wn = (wave & 1) * 8, wm = (wave >> 1) * 4, stages = a.ktiles;
   // this workgroup's tiles: XCD x = blockIdx % 8 has a range of neighbours, which share what they read
   const int grid = gridDim.x;
   int first = blockIdx.x, step = grid, mine;
@@ -440,8 +440,7 @@ __global__ __launch_bounds__(kLargeThreads, 1) void linear8_large_kernel(Linear8
   } else {
     mine = first < tiles_total ? (tiles_total - first + step - 1) / step : 0;
   }
-  const int total = mine * stages;
-  if (total == 0) return;
+  if (mine == 0) return;
   struct Tile {
     uint32_t model;
     int ot, mt;
@@ -452,96 +451,94 @@ __global__ __launch_bounds__(kLargeThreads, 1) void linear8_large_kernel(Linear8
     const int ots = a.by_wg.d / per, band = rem / (8 * ots), high = std::min(8, per - band * 8), in = rem - band * 8 * ots;
     return Tile{model, in / high * kLargeTiles, (band * 8 + in % high) * kLargeTiles};
   };
-  // piece q of the wave's eight of a stage: halves q % 2 of tiles 2 wave and 2 wave + 1 of W, then of x; past the last the last
-  // again, stages too, which keeps the count of loads
-  struct Source {
-    const uint8_t* w[2];
-    const uint8_t* x[2];
-    lds_char* to;
-  };
-  auto source_of = [&](int s) {
-    const int at = s < total ? s : total - 1, i = at / stages;
+  // What comes next: tiles 2 wave and 2 wave + 1 of W, then of x; past the last stage the last again, which keeps the count of loads.
+  const uint8_t* from[4];
+  int coming = 0, left = 0, to = 0;                    // tile, its stages that are left, slot
+  auto aim = [&](int i) {
     const Tile t = tile_of(i);
-    const int64_t k = static_cast<int64_t>(at - i * stages) * 2048;
-    Source c;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const int64_t w = static_cast<int64_t>(t.model) * a.otiles + std::min(t.ot + 2 * wave + e, a.otiles - 1);
-      const int64_t x = static_cast<int64_t>(t.model) * a.mtiles + std::min(t.mt + 2 * wave + e, a.mtiles - 1);
-      c.w[e] = a.w + w * a.ktiles * 1024 + k;
-      c.x[e] = a.c + x * a.ktiles * 1024 + k;
+      from[e] = a.w + (static_cast<int64_t>(t.model) * a.otiles + std::min(t.ot + 2 * wave + e, a.otiles - 1)) * a.ktiles * 1024;
+      from[2 + e] = a.c + (static_cast<int64_t>(t.model) * a.mtiles + std::min(t.mt + 2 * wave + e, a.mtiles - 1)) * a.ktiles * 1024;
     }
-    c.to = lds + (s & 1) * kLargeStage + wave * 4096;
-    return c;
+    coming = i;
+    left = stages;
   };
-  auto bring = [&](const Source& c, int q) {
-    const uint8_t* from = (q < 4 ? c.w[q >> 1 & 1] : c.x[q >> 1 & 1]) + (q & 1) * 1024 + lane * 16;
-    __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(from),
-                                     (lds_ptr_t)(c.to + (q < 4 ? 0 : kLargeStage / 2) + (q & 3) * 1024), 16, 0, 0);
+  auto bring = [&](int q) __attribute__((always_inline)) {
+    __builtin_amdgcn_global_load_lds(reinterpret_cast<const void*>(from[q] + lane * 16),
+                                     (lds_ptr_t)(lds + to * kLargeStage + (q >> 1) * (kLargeStage / 2) + (2 * wave + (q & 1)) * 1024), 16, 0, 0);
   };
-  i32x4 acc[8][4], wr[4], x0[4], x1[4];
-  auto read_w = [&](int s, int g) {
-    wr[g & 3] = *(const lds_i32x4*)(lds + (s & 1) * kLargeStage + ((wn + (g & 7)) * 2 + (g >> 3)) * 1024 + lane * 16);
-  };
-  auto read_x = [&](int s, int h, i32x4(&x)[4]) {
+  auto next = [&]() __attribute__((always_inline)) {
+    to = (to + 1) & 3;
+    if (left > 1) {
+      --left;
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      x[j] = *(const lds_i32x4*)(lds + (s & 1) * kLargeStage + kLargeStage / 2 + ((wm + j) * 2 + h) * 1024 + lane * 16);
+      for (int e = 0; e < 4; ++e) from[e] += 1024;
+    } else if (coming + 1 < mine) {
+      aim(coming + 1);
+    }
   };
-  // everything on its way has landed (and, `all` false, what was stored may still be)
-  auto landed = [&]() {
-    __builtin_amdgcn_s_waitcnt(0x0070);              // vmcnt(0) lgkmcnt(0)
-    bare_barrier();
+  i32x4 acc[8][4], wr[4], xa[4], xb[4];
+  auto read_w = [&](int slot, int g) __attribute__((always_inline)) {
+    wr[g & 3] = *(const lds_i32x4*)(lds + slot * kLargeStage + (wn + g) * 1024 + lane * 16);
   };
-  {
-    const Source c = source_of(0);
+  auto read_x = [&](int slot, i32x4(&x)[4]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) bring(c, q);
+    for (int j = 0; j < 4; ++j) x[j] = *(const lds_i32x4*)(lds + slot * kLargeStage + kLargeStage / 2 + (wm + j) * 1024 + lane * 16);
+  };
+  aim(0);
+#pragma unroll
+  for (int s = 0; s < 3; ++s) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) bring(q);
+    next();
   }
-  landed();
-  {
-    const Source c = source_of(1);
-#pragma unroll
-    for (int q = 0; q < 8; ++q) bring(c, q);
-  }
+  bring(0);
+  bring(1);
+  __builtin_amdgcn_s_waitcnt(0x0070 | 10);             // of 14 loads the first stage's
+  bare_barrier();
 #pragma unroll
   for (int g = 0; g < 4; ++g) read_w(0, g);
-  read_x(0, 0, x0);
-  auto stage = [&](int s, bool zero) {
-    Source c;
+  read_x(0, xa);
+  // the stage in a slot; its rows of x are in x, those of the next come into y
+  auto stage = [&](int slot, const i32x4(&x)[4], i32x4(&y)[4]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int g = 0; g < 16; ++g) {
-      if (g < 14) {
+    for (int g = 0; g < 8; ++g) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          acc[g & 7][j] = mma8(wr[g & 3], g < 8 ? x0[j] : x1[j], zero && g < 8 ? i32x4{0, 0, 0, 0} : acc[g & 7][j]);
-      } else {
-        // one of the next but one stage's loads after each MFMA: back to back they stall the wave
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          acc[g & 7][j] = mma8(wr[g & 3], x1[j], acc[g & 7][j]);
+      for (int j = 0; j < 4; ++j) {
+        acc[g][j] = mma8(wr[g & 3], x[j], acc[g][j]);
+        if (j == 1 && (g < 2 || g > 5)) {              // one load at a time: back to back they stall the wave
           __builtin_amdgcn_sched_barrier(0);
-          bring(c, 4 * (g - 14) + j);
+          bring(g < 2 ? 2 + g : g - 6);
           __builtin_amdgcn_sched_barrier(0);
         }
       }
-      if (g == 1) read_x(s, 1, x1);
-      if (g + 4 < 16) read_w(s, g + 4);
-      if (g == 13) {
-        // every read of stage s is done and stage s + 1 has landed: its slot can take stage s + 2
-        landed();
-        read_x(s + 1, 0, x0);
-        read_w(s + 1, 0);
-        read_w(s + 1, 1);
-        c = source_of(s + 2);
+      if (g == 1) next();
+      if (g + 4 < 8) read_w(slot, g + 4);
+      if (g == 5) {
+        // the wave's reads of this stage are done and the next has landed, which leaves two stages of four loads on their way; then
+        // all waves': the slot can take the next but three
+        __builtin_amdgcn_s_waitcnt(0x0070 | 8);
+        bare_barrier();
+        read_x((slot + 1) & 3, y);
+        read_w((slot + 1) & 3, 0);
+        read_w((slot + 1) & 3, 1);
       }
-      if (g == 14) read_w(s + 1, 2);
-      if (g == 15) read_w(s + 1, 3);
+      if (g == 6) read_w((slot + 1) & 3, 2);
+      if (g == 7) read_w((slot + 1) & 3, 3);
     }
   };
+  int slot = 0;
   for (int i = 0; i < mine; ++i) {
-    stage(i * stages, true);
-    for (int k = 1; k < stages; ++k) stage(i * stages + k, false);
+#pragma unroll
+    for (int g = 0; g < 8; ++g)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[g][j] = i32x4{0, 0, 0, 0};
+    for (int k = 0; k < stages; k += 2) {              // of whole tiles of 128 columns
+      stage(slot, xa, xb);
+      stage(slot + 1, xb, xa);
+      slot = (slot + 2) & 3;
+    }
     const Tile t = tile_of(i);
     finish<T>(a, t.model, t.ot + wn, t.mt + wm, lane, acc);
   }

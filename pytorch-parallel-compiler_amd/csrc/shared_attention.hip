@@ -479,7 +479,7 @@ Plan plan_of(const wc_shared_attn_args& p) {
   plan.rt = plan.stream ? plan.stream / 16 : tiles_of_rows(p);
   const int64_t group = p.q_heads / p.cache.heads, units = p.cache.n * (p.cache.b / p.share), seqs = p.cache.n * p.cache.b;
   const int64_t heads0 = p.cache.heads * cdiv(p.share * group, plan.rt * 16), heads1 = p.cache.heads * cdiv(group, 16);
-  const int64_t target = 512;                        // two workgroups a compute unit; of 64 rows through LDS one
+  const int64_t target = 512;                        // two workgroups a compute unit
   plan.budget[0] = std::min<int64_t>(cdiv(target, heads0), kSharedTarget);
   plan.parts[0] = plan.budget[0] + units;
   const bool whole = seqs * heads1 >= 2048 || p.max_length <= 1024;
