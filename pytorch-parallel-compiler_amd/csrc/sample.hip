@@ -258,8 +258,8 @@ struct Row {
     });
   }
   // put(index, place) of the values within [lo, hi], places from take(how many a wave has): a bit for each of a thread's 8 E values
-  // at a time, while the next are on their way, then a turn for each bit.
-  template <typename G, typename F>
+  // at a time, while the next are on their way (AHEAD), then a turn for each bit.
+  template <bool AHEAD, typename G, typename F>
   __device__ __forceinline__ void select(float lo, float hi, G take, F put) const {
     constexpr int step = kThreads * E;
     if (v < E) {
@@ -276,10 +276,11 @@ struct Row {
     const uint32_t end = v, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) * 64 * E;
     u32x4 t[8], next[8];
     uint32_t first = wave;                             // of the wave: the same for its lanes
-    if (first < end) load(first + lane * E, t);
+    if (AHEAD && first < end) load(first + lane * E, t);
     for (; first < end; first += 8 * step) {
       const uint32_t at = first + lane * E;
-      if (first + 8 * step < end) load(at + 8 * step, next);
+      if (!AHEAD) load(at, t);
+      if (AHEAD && first + 8 * step < end) load(at + 8 * step, next);
       uint64_t mine = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -318,7 +319,7 @@ struct Row {
         }
       }
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = next[i];
+      for (int i = 0; AHEAD && i < 8; ++i) t[i] = next[i];
     }
   }
 };
@@ -531,13 +532,19 @@ __device__ __attribute__((noinline)) void draw_by_digits(Row<T> row, Weights w, 
 
 
 // A workgroup's chunk of a row: its largest value, the sum of its weights, and its bins.
+struct ChunkShared {
+  uint64_t weight[kBins], red[kChunkThreads / 64];
+  uint32_t count[kBins];
+  double table[64];
+  float tops[kChunkThreads / 64];
+};
 template <typename T>
-__global__ __launch_bounds__(kChunkThreads) void sample_chunks_kernel(Sample a) {
+__device__ __forceinline__ void sum_chunk(const Sample& a, ChunkShared& s) {
   constexpr int E = Row<T>::E, NW = kChunkThreads / 64, KEPT = 16 / E;       // 16 values a thread stay in registers
-  __shared__ uint64_t weight[kBins], red[NW];
-  __shared__ uint32_t count[kBins];
-  __shared__ double table[64];
-  __shared__ float tops[NW];
+  uint64_t *const weight = s.weight, *const red = s.red;
+  uint32_t* const count = s.count;
+  double* const table = s.table;
+  float* const tops = s.tops;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t rowi = fdiv(blockIdx.x, a.by_chunks), c = blockIdx.x - rowi * a.by_chunks.d;
   const uint32_t model = fdiv(rowi, a.by_m), r = rowi - model * a.by_m.d, outer = fdiv(r, a.by_rows);
@@ -668,6 +675,11 @@ __global__ __launch_bounds__(kChunkThreads) void sample_chunks_kernel(Sample a) 
     out.sum = sum;
   }
 }
+template <typename T>
+__global__ __launch_bounds__(kChunkThreads) void sample_chunks_kernel(Sample a) {
+  __shared__ ChunkShared s;
+  sum_chunk<T>(a, s);
+}
 
 // The rank of each of n <= kRank different values among them, from the largest down, and the sum of the weights (in
 // rank_weight) of those before it.  A wave compares 64 of them with its share of all.
@@ -692,9 +704,17 @@ __device__ void rank_all(const uint64_t* list, int n, Shared& s) {
   __syncthreads();
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_rows_kernel(Sample a) {
+// A row's token.  WHOLE: rows are one chunk each, and their workgroups sum it first, which saves a launch (one row of 2000 by top-p:
+// MEASURED).
+template <typename T, bool WHOLE>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WHOLE ? 4 : 2))) void sample_rows_kernel(Sample a) {
+  static_assert(kThreads == kChunkThreads, "one workgroup does both");
   __shared__ Shared s;
+  if constexpr (WHOLE) {
+    __shared__ ChunkShared c;
+    sum_chunk<T>(a, c);
+    __syncthreads();                                   // what is written of the chunk is there for all waves
+  }
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t model = fdiv(blockIdx.x, a.by_m), r = blockIdx.x - model * a.by_m.d, outer = fdiv(r, a.by_rows);
   const Row<T> row{reinterpret_cast<const T*>(a.x) + model * a.xn + outer * a.xo + (r - outer * a.by_rows.d) * a.xi, a.v};
@@ -809,7 +829,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(Sample a) {
         const float edge = bins.base - b1, at = value_of(key_of(edge / bins.scale) - 16 + lane);
         lo = __shfl(at, (__ffsll(static_cast<unsigned long long>(__ballot(!(bins.scaled(at) < edge)))) + 63) & 63, 64);
       }
-      row.select(lo, hi, [&](int n) { return static_cast<int>(atomicAdd(&s.found32[1], static_cast<uint32_t>(n))); },
+      row.template select<!WHOLE>(lo, hi, [&](int n) { return static_cast<int>(atomicAdd(&s.found32[1], static_cast<uint32_t>(n))); },
                  [&](int i, int at) {
                    if (at < kList) s.list[at] = i;
                  });
@@ -909,7 +929,8 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(Sample a) {
       cut_key = list_key(s.found64[1]);
       cut_last = list_index(s.found64[1]);
     };
-    const bool by_k = counts && static_cast<uint64_t>(rules.top_k) < all;
+    // Where only the values are counted, a top_k that leaves all of them cuts at the last: they are few.
+    const bool by_k = counts && (!weights || static_cast<uint64_t>(rules.top_k) < all);
     // Places are known to an eighth of a bin, and their edges exact, where they are not too far from zero; at temperatures over
     // 92 products of the smallest values round to 0, so that an edge there is far from its quotient.
     bool digits = !(fabsf(bins.base) < 0x1p20f && bins.scale >= 0.125f && bins.scale < INFINITY);
@@ -945,7 +966,7 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(Sample a) {
     };
     const bool counted = counts && !weights;       // the chunks' weights are not known: the list has to hold all
     if (by_k && !digits) {
-      const uint64_t k = rules.top_k;
+      const uint64_t k = smaller(static_cast<uint64_t>(rules.top_k), all);
       const int b = find_bin(s.above_count, k);
       digits = !bring(b) || (counted && list_from > 0);
       if (!digits) {
@@ -963,7 +984,6 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(Sample a) {
         }
       }
     }
-    if (rules.top_p < 1.f && !digits && counted && !by_k) digits = true;
     if (rules.top_p < 1.f && !digits) {
       const uint64_t limit = limit_of(sum);
       // at most the bin of top_k's cut, whose sum in the chunks' units may be a few less
@@ -982,11 +1002,11 @@ __global__ __launch_bounds__(kThreads) void sample_rows_kernel(Sample a) {
       if (b < list_from) {
         const int end = smaller(smaller(b + 3, kBins - 1), cut_bin);
         const int begin = s.above_count[end] + s.bin_count[end] <= kList ? 0 : smaller(b, end);
-        digits = (counted && begin > 0) || !gather(begin, end);
+        digits = !gather(begin, end);
         if (!digits && begin == 0 && listed <= kRank && !by_k && !(rules.top_p < 1.f)) return draw_few();
       }
     }
-    if (digits || (counted && list_from == kBins)) {
+    if (digits) {
       __syncthreads();
       return draw_by_digits(row, w, s, rules, top, u, token);
     }
@@ -1171,8 +1191,12 @@ extern "C" int32_t wc_sample(const wc_sample_args* args, void* stream) {
   const hipStream_t s = as_stream(stream);
   auto go = [&](auto t) {
     typedef decltype(t) T;
-    sample_chunks_kernel<T><<<rows * static_cast<uint32_t>(a.chunks), kChunkThreads, 0, s>>>(a);
-    sample_rows_kernel<T><<<rows, kThreads, 0, s>>>(a);
+    if (a.chunks == 1) {
+      sample_rows_kernel<T, true><<<rows, kThreads, 0, s>>>(a);
+    } else {
+      sample_chunks_kernel<T><<<rows * static_cast<uint32_t>(a.chunks), kChunkThreads, 0, s>>>(a);
+      sample_rows_kernel<T, false><<<rows, kThreads, 0, s>>>(a);
+    }
   };
   if (p.dtype == WC_F32)
     go(float());

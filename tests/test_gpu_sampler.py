@@ -180,3 +180,21 @@ def test_on_another_stream():
             got = s(x, u)
         torch.cuda.synchronize()
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("v", [185, 829, 8192, 30000])
+@pytest.mark.parametrize("top_k", [50, 464, 1024, 1100])
+def test_fewer_allowed_than_top_k(top_k, v):
+    """Rows in which all but a few logits are banned by -infinity, under and over top_k, with each other filter."""
+    import wide_compiler as wc
+    for left in (1, 3, 49, 128, 129, 463, 900, 1090):
+        if left > v:
+            continue
+        x = _logits(1, 6, v, left, torch.bfloat16)
+        kept = torch.randperm(v, generator=gen(left))[:left]
+        banned = torch.ones(v, dtype=torch.bool)
+        banned[kept] = False
+        x[..., banned] = -INF
+        for i, rest in enumerate((dict(), dict(top_p=0.9), dict(min_p=0.02), dict(top_p=0.7, min_p=0.05, temperature=1.5))):
+            rules = dict(top_k=top_k, **rest)
+            _check(wc.WideSampler(1, **rules).to(DEV), x, torch.rand(1, 6, generator=gen(i)), rules)
