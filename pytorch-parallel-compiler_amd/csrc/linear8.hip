@@ -139,10 +139,12 @@ __global__ __launch_bounds__(NW * 64) void linear8_codes_kernel(Linear8 a) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < KEPT; ++i) top = v[i].top(top);
-  for (int t = wave + KEPT * NW; t < a.ktiles; t += NW) {
-    Piece<T> u;
-    u.load(x, t, g, a.k);
-    top = u.top(top);
+  for (int t = wave + KEPT * NW; t < a.ktiles; t += 4 * NW) {       // four at a time on their way; past the last there are zeros
+    Piece<T> u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i].load(x, t + i * NW, g, a.k);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = u[i].top(top);
   }
   top = Piece<T>::as_float(top);
   top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
@@ -160,10 +162,13 @@ __global__ __launch_bounds__(NW * 64) void linear8_codes_kernel(Linear8 a) {
   for (int i = 0; i < KEPT; ++i)
     if (wave + i * NW < a.ktiles) out[static_cast<int64_t>(wave + i * NW) * 64] = v[i].codes(scale, inv, finite);
 #pragma unroll 1
-  for (int t = wave + KEPT * NW; t < a.ktiles; t += NW) {
-    Piece<T> u;
-    u.load(x, t, g, a.k);
-    out[static_cast<int64_t>(t) * 64] = u.codes(scale, inv, finite);
+  for (int t = wave + KEPT * NW; t < a.ktiles; t += 4 * NW) {
+    Piece<T> u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[i].load(x, t + i * NW, g, a.k);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (t + i * NW < a.ktiles) out[static_cast<int64_t>(t + i * NW) * 64] = u[i].codes(scale, inv, finite);
   }
 }
 
@@ -584,9 +589,15 @@ void launch(const Linear8& a, int64_t n, hipStream_t s) {
   if (a.m <= 16 && static_cast<int64_t>(a.m) * a.ktiles * 4 <= kFusedPieces) return launch_fused<T, 1, 4, 8>(a, n, s);
   if (a.ktiles <= 16)
     linear8_codes_kernel<T, 4, 4><<<tiles, 256, 0, s>>>(a);
-  else
+  else if (a.ktiles <= 64 || sizeof(T) == 4)
     linear8_codes_kernel<T, 8, 8><<<tiles, 512, 0, s>>>(a);
-  if (a.mtiles == 1) return launch_few<T, 1, 4, 8>(a, n, s);
+  else
+    linear8_codes_kernel<T, 16, 8><<<tiles, 1024, 0, s>>>(a);
+  // A workgroup for each 16 rows and outputs while all of them are at work at once, eight a compute unit: W comes from L2 for all
+  // rows but the first 16, which costs less than long walks on few units do.
+  if (a.mtiles == 1 || n * a.mtiles * a.otiles <= 2048) return launch_few<T, 1, 4, 8>(a, n, s);
+  // Where tiles are fewer than compute units, one has a unit's LDS to itself and more stages on their way.
+  if (n * cdiv(a.mtiles, 4) * cdiv(a.otiles, 8) <= 256) return launch_tile<T, 4, 2, 1, 4, 6>(a, n, s);
   if (a.mtiles <= 4) return launch_tile<T, 4, 2, 1, 4, 3>(a, n, s);
   if (n * cdiv(a.mtiles, kLargeTiles) * cdiv(a.otiles, kLargeTiles) >= 256) return launch_large<T>(a, n, s);
   launch_tile<T, 4, 4, 2, 2, 2>(a, n, s);

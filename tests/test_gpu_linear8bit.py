@@ -44,6 +44,18 @@ def test_products(n, m, k, o, dtype):
     _check(y, x, codes, scales, bias)
 
 
+# several tiles of rows by workgroups of one tile of outputs, on both sides of 2048 of them; tiles of 64 x 128 on both sides
+# of 256 of them; rows longer than 4096 and 8192 columns
+@pytest.mark.parametrize("n,m,k,o", [(2, 31, 7008, 96), (1, 48, 8200, 304), (1, 129, 4100, 416), (1, 33, 200, 10930), (1, 33, 200, 10900),
+                                     (2, 293, 700, 1004), (1, 500, 650, 4090), (1, 520, 650, 4090)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_few_tiles(n, m, k, o, dtype):
+    mod, codes, scales, bias = _module(n, k, o, dtype)
+    x = torch.randn(n, m, k, generator=gen(4)).to(DEV, dtype)
+    with torch.no_grad():
+        _check(mod(x), x, codes, scales, bias)
+
+
 def test_large_tiles_at_the_edges():
     """Rows and outputs next to the largest tile's, both ends of it ragged."""
     for m, k, o in ((2049, 512, 1025), (2304, 384, 2303)):
