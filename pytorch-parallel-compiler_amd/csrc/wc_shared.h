@@ -44,7 +44,8 @@ __device__ __forceinline__ SharedLine shared_line(const SharedWalk& w, int lane)
   for (int s = lane; s < w.units; s += 64) total += paged_tiles(shared_span(w, s));
 #pragma unroll
   for (int off = 32; off; off >>= 1) total += __shfl_xor(total, off, 64);
-  return SharedLine{max((total + w.budget - 1) / w.budget, w.least), total};
+  // `least` is for cuts of one unit: short units are not put together for it, which would walk them one after the other
+  return SharedLine{max((total + w.budget - 1) / w.budget, min(w.least, (total + w.units - 1) / max(w.units, 1))), total};
 }
 // the unit that has tile `at` of the line (at < total), and the line's tiles before it
 __device__ __forceinline__ int2 shared_find(const SharedWalk& w, int at, int lane) {
