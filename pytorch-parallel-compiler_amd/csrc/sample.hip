@@ -15,6 +15,9 @@
 // Which token comes out must not hang on the order of a sum, so weights are summed as whole numbers, of 2^-48 of the
 // largest weight (more where rows are so long that 64 bits could not hold the sum): each is the exponential in 64 bits,
 // off by 2^-46 of itself, and rounded once, to 1 at least, so that u = 0 gives the first that has a weight at all.
+//
+// Those exponentials, some 20 operations in 64 bits a value, bound the first kernel: 256 rows of 131072 in fp32, unfiltered, 39 us
+// (3.4 TB/s); with bins, an atomic in LDS a value more, 128 of 100003 in bf16 25 us (5.2e11 values a second; 8.6e11 without bins).
 #include <algorithm>
 
 #include "wc_answer_abi.h"
@@ -704,8 +707,10 @@ __device__ void rank_all(const uint64_t* list, int n, Shared& s) {
   __syncthreads();
 }
 
-// A row's token.  WHOLE: rows are one chunk each, and their workgroups sum it first, which saves a launch (one row of 2000 by top-p:
-// MEASURED).
+// A row's token.  WHOLE: rows are one chunk each, and their workgroups sum it first, which saves a launch (128 greedy rows of 1000: 6.1
+// and 5.0 us), with registers for two workgroups a unit instead of one (518 rows of 185: 49 and 38 us; 58 of 829: 25.6 and 27.1).
+// Latency bounds it: a row's bins, its list and its token are some 30 steps that wait for each other, 39 us for 128 rows of 100003 (25.6 MB,
+// of which each row is read once more to fill the list).
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WHOLE ? 4 : 2))) void sample_rows_kernel(Sample a) {
   static_assert(kThreads == kChunkThreads, "one workgroup does both");
@@ -1108,11 +1113,10 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WHOLE 
   }
 }
 
-// Values of a chunk, and chunks of a row: 16 values a thread, or 4 where that leaves compute units without a workgroup.
-int64_t chunk_of(const wc_sample_args& p) {
-  const int64_t least = mul_sat({p.n, p.m, cdiv(p.v, 8192)}) < 256 ? 2048 : 8192;
-  return std::max(least, cdiv(cdiv(p.v, kChunks), 16) * 16);
-}
+// Values of a chunk, and chunks of a row: 16 values a thread.  Smaller chunks add more bins up than they spread work (of 8192 and of 2048
+// values: 128 rows of 100003 by top-p 62 and 89 us, 256 of 131072 unfiltered 48 and 137, one row of 131072 by top-p 38 and 46; only
+// unfiltered it is 16 and 11).
+int64_t chunk_of(const wc_sample_args& p) { return std::max<int64_t>(8192, cdiv(cdiv(p.v, kChunks), 16) * 16); }
 int64_t chunks_of(const wc_sample_args& p) { return cdiv(p.v, chunk_of(p)); }
 
 int32_t check(const wc_sample_args& p, const char* what) {

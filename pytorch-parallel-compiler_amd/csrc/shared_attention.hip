@@ -5,13 +5,18 @@
 // The softmax is joined from parts that have a maximum, a sum and an output each, so a prefix is walked once for all
 // its sequences: their query heads are the rows that every K and V row meets, 16 for each tile of the matrix instructions.
 // Both walks are one kernel, of stretches of tokens with rows that read them: a prefix with the heads of its sequences,
-// and a sequence's own tokens with its heads.  A second kernel joins the parts.
+// and a sequence's own tokens with its heads.  A second kernel joins the parts.  Prefixes that more than 32 rows read in 16 bits
+// are walked by shared_stream.hip instead.
 //
 // A wave takes 32 tokens at a time, K and V straight from memory into the operands of MFMAs:
 //   scores   S [token][row] = K Q^T, lane l brings 16-byte pieces of token l % 16
 //   softmax  the accumulator has row l % 16 and tokens 4 (l / 16) + r, of two tiles of 16 tokens
 //   output   O^T [column][row] = V^T P, lane l loads those 8 tokens' rows at columns of its own, and operand e pairs
 //            up their e-th values
+//
+// Own tokens are bound by memory and by waves that wait for their sequence's rows: 128 sequences of up to 500 tokens, 8 key heads of 128
+// columns in bf16, 164 MB in 37 us (4.4 TB/s); 64 of up to 2000, 325 MB in 67 us (4.9 TB/s).  Small calls are bound by two launches and
+// four waits for memory: 2 sequences over a prefix of 300 tokens 10.2 us.
 #include <algorithm>
 
 #include "wc_shared.h"
@@ -19,7 +24,9 @@
 namespace wc {
 namespace {
 
-constexpr int kLeast = 4;            // tiles of 32 tokens in a share at least
+// Tiles of 32 tokens in a share at least (one prefix of 300 tokens, 3 x 3 of up to 1777, own tokens up to 2000: 1: 10.0, 27.9 and 42.2 us,
+// 2: 10.2, 27.9 and 38.1, 4: 10.6, 29.6 and 38.7)
+constexpr int kLeast = 2;
 
 // QT: type of q and o; KT: stored type (int8_t for codes); DC: columns provided for; RT: tiles of 16 rows
 template <typename QT, typename KT, int DC, int RT>
@@ -482,7 +489,9 @@ Plan plan_of(const wc_shared_attn_args& p) {
   const int64_t target = 512;                        // two workgroups a compute unit
   plan.budget[0] = std::min<int64_t>(cdiv(target, heads0), kSharedTarget);
   plan.parts[0] = plan.budget[0] + units;
-  const bool whole = seqs * heads1 >= 2048 || p.max_length <= 1024;
+  // Sequences stay whole where they are short, or many for their length (45 of up to 130 tokens, 2 key heads: 29.6 us, cut 34.5; 128 of
+  // up to 500, 8 key heads: 83.7 and 87.4); few long ones are cut (4 of up to 1000, 8 key heads: whole 17.5, cut 12.1).
+  const bool whole = p.max_length <= 256 || seqs * heads1 >= (p.max_length <= 1024 ? 256 : 2048);
   plan.budget[1] = whole ? 0 : std::min<int64_t>(cdiv(target, heads1), kSharedTarget);
   plan.parts[1] = plan.budget[1] + seqs;
   return plan;

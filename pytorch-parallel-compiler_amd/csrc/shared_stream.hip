@@ -12,6 +12,10 @@
 // A row's K scale multiplies its scores, its V scale its weights.  The weights enter the products rounded to 16 bits, half a step
 // of 2^-8 (bf16) or 2^-11 (fp16) of each, as in attention over a prompt; their sum is fp32.  fp16 over 8-bit pages takes
 // them as two bf16 numbers, because fp16 has no room for a weight times a scale.
+//
+// 64 rows are bound by memory and the waits for each tile: 4 x 2 prefixes of up to 6000 tokens, 8 key heads of 128 columns, 147 MB in
+// 42 us (3.5 TB/s; four buffers and one workgroup a unit 49).  128 rows are
+// bound by the matrix and vector pipes in turn: one prefix of 65536 tokens, 256 rows a key head, 110 us, 6.2e14 operations a second.
 #include "wc_attn.h"
 #include "wc_shared.h"
 
@@ -412,6 +416,8 @@ void launch(const SharedAttn& a, int rows, int64_t grid, hipStream_t s) {
 
 }  // namespace
 
+// Up to 32 rows the walk without LDS reads a prefix once as well and needs no barriers; from there on it reads it again for every 32
+// (64 rows: 86.0 us for the whole call of the case above, and 83.7 through LDS; 256 rows: 386 and 176).
 int shared_stream_rows(const wc_shared_attn_args& p) {
   const int64_t rows = p.share * (p.q_heads / p.cache.heads);
   if (p.cache.dtype == WC_F32 || p.cache.head_dim > 128 || rows <= 32) return 0;
