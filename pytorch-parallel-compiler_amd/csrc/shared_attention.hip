@@ -313,7 +313,8 @@ __device__ __forceinline__ void walk(const SharedAttn& a, const SharedWalk w, ui
     }
 
     // Join the waves, a tile of rows at a time: [NW][16][kRow] outputs (rows 4 values apart from whole banks: with rows of DC the
-    // 16 that a wave writes at a time all meet in one bank, 10 us of 41 over 128 sequences of up to 500 tokens), then [NW][16] maxima and sums (a sum of -1: no tokens),
+    // 16 that a wave writes at a time all meet in one bank, 10 us of 41 over 128 sequences of up to 500 tokens), then [NW][16] maxima and
+    // sums (a sum of -1: no tokens),
     // which become the weights of the waves' outputs
     constexpr int kRow = DC + 4;
     float* om = lds + NW * 16 * kRow;
