@@ -594,12 +594,24 @@ template <typename T>
 void launch(const Linear8& a, int64_t n, hipStream_t s) {
   const uint32_t tiles = static_cast<uint32_t>(n * a.mtiles);
   if (a.m <= 16 && static_cast<int64_t>(a.m) * a.ktiles * 4 <= kFusedPieces) return launch_fused<T, 1, 4, 8>(a, n, s);
-  if (a.ktiles <= 16)
-    linear8_codes_kernel<T, 4, 4><<<tiles, 256, 0, s>>>(a);
+  auto codes = [&](auto nw, auto kept) {
+    constexpr int NW = decltype(nw)::value;
+    linear8_codes_kernel<T, NW, decltype(kept)::value><<<tiles, NW * 64, 0, s>>>(a);
+  };
+  typedef std::integral_constant<int, 1> One;
+  typedef std::integral_constant<int, 4> Four;
+  typedef std::integral_constant<int, 8> Eight;
+  typedef std::integral_constant<int, 16> Sixteen;
+  if (tiles < 256 && a.ktiles <= 16)
+    codes(Sixteen(), One());
+  else if (tiles < 256 && a.ktiles <= 64)
+    codes(Sixteen(), Four());
+  else if (a.ktiles <= 16)
+    codes(Four(), Four());
   else if (a.ktiles <= 64 || sizeof(T) == 4)
-    linear8_codes_kernel<T, 8, 8><<<tiles, 512, 0, s>>>(a);
+    codes(Eight(), Eight());
   else
-    linear8_codes_kernel<T, 16, 8><<<tiles, 1024, 0, s>>>(a);
+    codes(Sixteen(), Eight());
   // A workgroup for each 16 rows and outputs while all of them are at work at once, eight a compute unit: W comes from L2 for all
   // rows but the first 16, which costs less than long walks on few units do (129 rows [7280 -> 416], two models: 51 us by tiles of 64 x 128,
   // 30 so; 128 rows [4096 -> 4096], 2048 of them: 36.6 and 32.4; 293 rows [6832 -> 1004], 2394 of them: 50 and 64).
