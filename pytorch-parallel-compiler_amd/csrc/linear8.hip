@@ -123,10 +123,10 @@ struct Piece {
 };
 
 // Codes and scales of 16 rows of x: lane l has row l % 16 and columns 16 (l / 16).. of every tile of its wave, which is what
-// it writes.  KEPT tiles a wave stay in registers between the search for the scale and the codes; rows longer than that
-// are read a second time (129 rows of 7280 in bf16, of 4096 columns kept and of 8192: 70 and 64 us for the whole product).  Memory and the
-// three phases that all workgroups are in at once bound it: 2 x 4096 rows of 4096, 100 MB, 30 us (3.3 TB/s).
-template <typename T, int NW, int KEPT>
+// it writes.  S workgroups share the codes of 16 rows, of which each looks for the scale by itself.  KEPT of its tiles a wave stay in
+// registers until the scale is known; more are read a second time.  Memory and the three phases that all workgroups are in at
+// once bound it: 2 x 4096 rows of 4096, 100 MB, 30 us (3.3 TB/s).
+template <typename T, int NW, int KEPT, int S>
 __global__ __launch_bounds__(NW * 64) void linear8_codes_kernel(Linear8 a) {
   __shared__ uint32_t tops[NW][16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), j = lane & 15, g = lane >> 4;
@@ -134,18 +134,34 @@ __global__ __launch_bounds__(NW * 64) void linear8_codes_kernel(Linear8 a) {
   const int mt = blockIdx.x - model * a.by_mtiles.d;
   const uint32_t r = min(mt * 16 + j, a.m - 1), outer = fdiv(r, a.by_rows);        // past the last: the last again
   const T* x = reinterpret_cast<const T*>(a.x) + model * a.xn + outer * a.xo + (r - outer * a.by_rows.d) * a.xi;
+  const int share = S == 1 ? 0 : blockIdx.y;
+  auto own = [&](int i) { return (i * S + share) * NW + wave; };         // the workgroup's tiles, of the wave
   Piece<T> v[KEPT];
 #pragma unroll
-  for (int i = 0; i < KEPT; ++i) v[i].load(x, wave + i * NW, g, a.k);
+  for (int i = 0; i < KEPT; ++i) v[i].load(x, own(i), g, a.k);
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < KEPT; ++i) top = v[i].top(top);
-  for (int t = wave + KEPT * NW; t < a.ktiles; t += 4 * NW) {       // four at a time on their way; past the last there are zeros
+  // the others' and those behind the kept, four at a time on their way; past the last there are zeros
+  if constexpr (S > 1) {
+    const int others = (a.ktiles + NW * S - 1) / (NW * S) * (S - 1);
+    for (int i0 = 0; i0 < others; i0 += 4) {
+      Piece<T> u[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = i0 + e, round = i / (S - 1), s = i - round * (S - 1);
+        u[e].load(x, (round * S + s + (s >= share)) * NW + wave, g, a.k);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = u[e].top(top);
+    }
+  }
+  for (int i = KEPT; own(i) < a.ktiles; i += 4) {
     Piece<T> u[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i].load(x, t + i * NW, g, a.k);
+    for (int e = 0; e < 4; ++e) u[e].load(x, own(i + e), g, a.k);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = u[i].top(top);
+    for (int e = 0; e < 4; ++e) top = u[e].top(top);
   }
   top = Piece<T>::as_float(top);
   top = max(top, static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), 16, 64)));
@@ -157,19 +173,19 @@ __global__ __launch_bounds__(NW * 64) void linear8_codes_kernel(Linear8 a) {
   const bool finite = top < 0x7f800000u;
   const float scale = finite ? row_scale(top) : __builtin_nanf("");
   const float inv = __builtin_amdgcn_rcpf(scale);
-  if (threadIdx.x < 16) a.s[static_cast<int64_t>(blockIdx.x) * 16 + j] = scale;
+  if (share == 0 && threadIdx.x < 16) a.s[static_cast<int64_t>(blockIdx.x) * 16 + j] = scale;
   u32x4* out = reinterpret_cast<u32x4*>(a.c) + static_cast<int64_t>(blockIdx.x) * a.ktiles * 64 + lane;
 #pragma unroll
   for (int i = 0; i < KEPT; ++i)
-    if (wave + i * NW < a.ktiles) out[static_cast<int64_t>(wave + i * NW) * 64] = v[i].codes(scale, inv, finite);
+    if (own(i) < a.ktiles) out[static_cast<int64_t>(own(i)) * 64] = v[i].codes(scale, inv, finite);
 #pragma unroll 1
-  for (int t = wave + KEPT * NW; t < a.ktiles; t += 4 * NW) {
+  for (int i = KEPT; own(i) < a.ktiles; i += 4) {
     Piece<T> u[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i].load(x, t + i * NW, g, a.k);
+    for (int e = 0; e < 4; ++e) u[e].load(x, own(i + e), g, a.k);
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (t + i * NW < a.ktiles) out[static_cast<int64_t>(t + i * NW) * 64] = u[i].codes(scale, inv, finite);
+    for (int e = 0; e < 4; ++e)
+      if (own(i + e) < a.ktiles) out[static_cast<int64_t>(own(i + e)) * 64] = u[e].codes(scale, inv, finite);
   }
 }
 
@@ -371,7 +387,7 @@ __global__ __launch_bounds__(NW * 64) void linear8_fused_kernel(Linear8 a) {
 }
 
 // Tiles of BM x BN outputs through LDS: WM x WN waves of FM x FN tiles each, NS stages of 128 columns in a ring, brought by DMA.  Eight
-// models' 64 rows [2048 -> 8192]: 40 us with the codes, 3.6 TB/s of W.
+// models' 64 rows [2048 -> 8192]: 30 us, 4.8 TB/s.
 template <typename T, int FM, int FN, int WM, int WN, int NS>
 __global__ __launch_bounds__(WM * WN * 64) void linear8_tile_kernel(Linear8 a) {
   constexpr int NW = WM * WN, TM = FM * WM, TN = FN * WN, PIECES = (TM + TN) * 2, PER = PIECES / NW;
@@ -594,27 +610,25 @@ template <typename T>
 void launch(const Linear8& a, int64_t n, hipStream_t s) {
   const uint32_t tiles = static_cast<uint32_t>(n * a.mtiles);
   if (a.m <= 16 && static_cast<int64_t>(a.m) * a.ktiles * 4 <= kFusedPieces) return launch_fused<T, 1, 4, 8>(a, n, s);
-  auto codes = [&](auto nw, auto kept) {
-    constexpr int NW = decltype(nw)::value;
-    linear8_codes_kernel<T, NW, decltype(kept)::value><<<tiles, NW * 64, 0, s>>>(a);
-  };
-  typedef std::integral_constant<int, 1> One;
-  typedef std::integral_constant<int, 4> Four;
-  typedef std::integral_constant<int, 8> Eight;
-  typedef std::integral_constant<int, 16> Sixteen;
+  // Where rows' tiles are fewer than compute units, more waves have them (256 rows [1024 -> 1024], eight models: by four waves 21.8 us for
+  // the whole product, by 16 18.0), and of longer rows four workgroups, each with a quarter of the codes (64 rows [4096 -> 4096]: by
+  // one of eight waves 26.0, by four 19.7; 129 rows [7280 -> 416], two models: 29.9 and 23.4).
   if (tiles < 256 && a.ktiles <= 16)
-    codes(Sixteen(), One());
-  else if (tiles < 256 && a.ktiles <= 64)
-    codes(Sixteen(), Four());
+    linear8_codes_kernel<T, 16, 1, 1><<<tiles, 1024, 0, s>>>(a);
+  else if (tiles < 256 && a.ktiles <= 32)
+    linear8_codes_kernel<T, 8, 1, 4><<<dim3(tiles, 4), 512, 0, s>>>(a);
+  else if (tiles < 256)
+    linear8_codes_kernel<T, 8, 4, 4><<<dim3(tiles, 4), 512, 0, s>>>(a);
   else if (a.ktiles <= 16)
-    codes(Four(), Four());
+    linear8_codes_kernel<T, 4, 4, 1><<<tiles, 256, 0, s>>>(a);
   else if (a.ktiles <= 64 || sizeof(T) == 4)
-    codes(Eight(), Eight());
-  else
-    codes(Sixteen(), Eight());
+    linear8_codes_kernel<T, 8, 8, 1><<<tiles, 512, 0, s>>>(a);
+  else if constexpr (sizeof(T) != 4)
+    linear8_codes_kernel<T, 16, 8, 1><<<tiles, 1024, 0, s>>>(a);
   // A workgroup for each 16 rows and outputs while all of them are at work at once, eight a compute unit: W comes from L2 for all
-  // rows but the first 16, which costs less than long walks on few units do (129 rows [7280 -> 416], two models: 51 us by tiles of 64 x 128,
-  // 30 so; 128 rows [4096 -> 4096], 2048 of them: 36.6 and 32.4; 293 rows [6832 -> 1004], 2394 of them: 50 and 64).
+  // rows but the first 16, which costs less than long walks on few units do (129 rows [7280 -> 416], two models, codes
+  // included: 51 us by tiles of 64 x 128, 30 so; 128 rows [4096 -> 4096], 2048 of them: 36.6 and 32.4; 293 rows [6832 -> 1004], 2394
+  // of them: 50 and 64).
   if (a.mtiles == 1 || n * a.mtiles * a.otiles <= 2048) return launch_few<T, 1, 4, 8>(a, n, s);
   // Where tiles are fewer than compute units, one has a unit's LDS to itself and more stages on their way (293 rows [6832 -> 1004], two
   // models: by tiles of 128 x 128 in two stages 62 us, so 50).

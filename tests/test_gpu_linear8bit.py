@@ -56,6 +56,19 @@ def test_few_tiles(n, m, k, o, dtype):
         _check(mod(x), x, codes, scales, bias)
 
 
+# codes of as many rows as there are compute units of 16, of lengths that registers hold and longer ones
+@pytest.mark.parametrize("k", [200, 1100, 2100, 4200, 8300])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_rows_of_any_length(k, dtype):
+    mod, codes, scales, bias = _module(2, k, 40, dtype)
+    x = torch.randn(2, 2100, k, generator=gen(5)).to(DEV, dtype)
+    x[1, 2050, k - 1] = 1000.0                               # a row's largest in its last column
+    with torch.no_grad():
+        _check(mod(x), x, codes, scales, bias)
+        # the same rows, their codes found by several workgroups
+        assert torch.equal(mod(x[:, 2040:2060]), mod(x)[:, 2040:2060])
+
+
 def test_large_tiles_at_the_edges():
     """Rows and outputs next to the largest tile's, both ends of it ragged."""
     for m, k, o in ((2049, 512, 1025), (2304, 384, 2303)):
