@@ -634,8 +634,9 @@ void launch(const Linear8& a, int64_t n, hipStream_t s) {
   // models: by tiles of 128 x 128 in two stages 62 us, so 50).
   if (n * cdiv(a.mtiles, 4) * cdiv(a.otiles, 8) <= 256) return launch_tile<T, 4, 2, 1, 4, 6>(a, n, s);
   if (a.mtiles <= 4) return launch_tile<T, 4, 2, 1, 4, 3>(a, n, s);
-  // whole rounds of the units by the largest tiles, which else leave most of them idle
-  if (n * cdiv(a.mtiles, kLargeTiles) * cdiv(a.otiles, kLargeTiles) >= 256) return launch_large<T>(a, n, s);
+  // The largest tiles where few units are left without one (2 models' 1280 rows [2048 -> 4096], 160 of them: 45.9 us, by tiles of 128 x 128
+  // 55.7; 2048 rows [4096 -> 4096], 128 of them: 67.8 and 61.5)
+  if (n * cdiv(a.mtiles, kLargeTiles) * cdiv(a.otiles, kLargeTiles) >= 150) return launch_large<T>(a, n, s);
   launch_tile<T, 4, 4, 2, 2, 2>(a, n, s);
 }
 

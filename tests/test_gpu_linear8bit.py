@@ -78,6 +78,16 @@ def test_large_tiles_at_the_edges():
             _check(mod(x), x, codes, scales, bias)
 
 
+# as many of the largest tiles as there are compute units, fewer and more, both ends ragged; a stage or two of columns, and many
+@pytest.mark.parametrize("n,m,k,o", [(8, 1040, 65, 1030), (8, 1040, 700, 1030), (8, 2049, 128, 1025), (8, 2049, 390, 1025), (1, 3000, 1000, 3300)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rounds_of_large_tiles(n, m, k, o, dtype):
+    mod, codes, scales, bias = _module(n, k, o, dtype)
+    x = torch.randn(n, m, k, generator=gen(6)).to(DEV, dtype)
+    with torch.no_grad():
+        _check(mod(x), x, codes, scales, bias)
+
+
 def test_the_largest_sums():
     """All codes 127, as many columns as are allowed: 2 114 060 288 < 2^31, whatever order it is summed in."""
     import wide_compiler as wc
