@@ -64,6 +64,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
   constexpr int NP = kQ8 && std::is_same<T, f16>::value ? 2 : 1;
   // fp16 weights are taken 2^14 times as large, so that those far under 1 keep their bits (and as the other walk takes them)
   constexpr float kShift = std::is_same<PT, f16>::value ? 14.f : 0.f;
+  // A row's base stays while its scores are no more than this above it: weights are then up to 2^8 (fp16: 2^15 with their shift), and
+  // most tiles rescale nothing.
+  constexpr float kOver = std::is_same<PT, f16>::value ? 1.f : 8.f;
   constexpr int NKS = DHP / 16, DT = DHP / 32, TILE = kStBK * DHP;
   constexpr int TS = 4 / RW, NB = 2 / TS;            // waves that share rows; blocks of 32 tokens of a wave
   constexpr int CPR = DHP * static_cast<int>(sizeof(KT)) / 16, CH = kStBK * CPR, PIECES = 2 * CH / 256;     // 16-byte pieces of a row, of a tile; a thread's
@@ -298,7 +301,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
                                                  __builtin_fmaxf(__builtin_fmaxf(m3, m4), s[b][15])));
       }
       bm *= c;
-      if (__builtin_amdgcn_ballot_w64(fresh || bm > base) != 0) {
+      if (__builtin_amdgcn_ballot_w64(fresh || bm > base + kOver) != 0) {
         bm = __builtin_fmaxf(bm, __shfl_xor(bm, 32, 64));
         const bool higher = (fresh || bm > base) && bm > -INFINITY;
         const float nbase = higher ? bm : base;
