@@ -7,7 +7,7 @@
 // the pool a tile has, the lanes find from 64 entries of the table, which they hold.  Per tile and wave, with v_mfma_f32_32x32x16:
 //   S^T = K Q^T      lane l holds row l % 32 and tokens 8 (r / 4) + 4 (l / 32) + r % 4 of each block of 32
 //   softmax          in the lane; the lane halves that share a row exchange their maxima, and O is rescaled, only in tiles where
-//                    a lane of the wave finds a new running maximum
+//                    a lane of the wave finds a score well over the row's base
 //   O^T += V^T P^T   P^T is the S^T register block itself, V^T through ds_read_b64_tr_b16
 // A row's K scale multiplies its scores, its V scale its weights.  The weights enter the products rounded to 16 bits, half a step
 // of 2^-8 (bf16) or 2^-11 (fp16) of each, as in attention over a prompt; their sum is fp32.  fp16 over 8-bit pages takes
@@ -15,7 +15,8 @@
 //
 // 64 rows are bound by memory and the waits for each tile: 4 x 2 prefixes of up to 6000 tokens, 8 key heads of 128 columns, 147 MB in
 // 42 us (3.5 TB/s; four buffers and one workgroup a unit 49).  128 rows are
-// bound by the matrix and vector pipes in turn: one prefix of 65536 tokens, 256 rows a key head, 110 us, 6.2e14 operations a second.
+// bound by the matrix and vector pipes in turn: one prefix of 65536 tokens, 256 rows a key head, 105 us, 6.5e14 operations a second (110 with outputs
+// rescaled for every new maximum).
 #include "wc_attn.h"
 #include "wc_shared.h"
 
@@ -420,7 +421,7 @@ void launch(const SharedAttn& a, int rows, int64_t grid, hipStream_t s) {
 }  // namespace
 
 // Up to 32 rows the walk without LDS reads a prefix once as well and needs no barriers; from there on it reads it again for every 32
-// (64 rows: 86.0 us for the whole call of the case above, and 83.7 through LDS; 256 rows: 386 and 176).
+// (64 rows: 86.0 us for the whole call of the case above, and 83.7 through LDS; 256 rows: 386 and 169).
 int shared_stream_rows(const wc_shared_attn_args& p) {
   const int64_t rows = p.share * (p.q_heads / p.cache.heads);
   if (p.cache.dtype == WC_F32 || p.cache.head_dim > 128 || rows <= 32) return 0;

@@ -232,3 +232,18 @@ def test_equals_attention_of_each_sequence():
         with torch.no_grad():
             one = cache.attend(q[:, b:b + 1], both.contiguous(), lens[:, b:b + 1] + p)
         assert (one - o[:, b:b + 1]).abs().max() <= 2.0 ** -20
+
+
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 0), (torch.float16, 0), (torch.bfloat16, 8), (torch.float16, 8), (torch.float32, 0)])
+@pytest.mark.parametrize("rise", [0.02, 0.3, 5.0, -5.0, 12.0])
+def test_scores_that_rise_along_the_tokens(rise, dtype, bits):
+    """Scores that grow from the first token of a prefix to the last, by steps from a part of a weight's power of two a tile to
+    many, and that fall: what is kept of earlier tokens is scaled in some tiles and not in others."""
+    made = _make([[700, 333]], [[3] * 24], 8, 2, 64, 16, dtype, bits)
+    cache, q, pt, prefix, table, lens = made
+    g = gen(9)
+    k = torch.randn(1, 2, 700, 2, 64, generator=g) * 0.1 + torch.linspace(0, rise, 700)[:, None, None]
+    v = torch.randn(1, 2, 700, 2, 64, generator=g)
+    cache.write(k.to(DEV, dtype), v.to(DEV, dtype), pt, torch.zeros_like(prefix), prefix)
+    q.copy_((torch.randn(q.shape, generator=g) * 0.1 + 1).to(DEV, dtype))
+    _check(made)
