@@ -542,7 +542,7 @@ struct ChunkShared {
   float tops[kChunkThreads / 64];
 };
 template <typename T>
-__device__ __forceinline__ void sum_chunk(const Sample& a, ChunkShared& s) {
+__device__ __forceinline__ void sum_chunk(const Sample& a, ChunkShared& s, ChunkSums& out) {
   constexpr int E = Row<T>::E, NW = kChunkThreads / 64, KEPT = 16 / E;       // 16 values a thread stay in registers
   uint64_t *const weight = s.weight, *const red = s.red;
   uint32_t* const count = s.count;
@@ -586,7 +586,6 @@ __device__ __forceinline__ void sum_chunk(const Sample& a, ChunkShared& s) {
   __syncthreads();
 #pragma unroll
   for (int v = 0; v < NW; ++v) top = fmaxf(top, tops[v]);
-  ChunkSums& out = a.sums[blockIdx.x];
   const Weights w(table, top, rules.t, a.fraction);
   if (tid == 0) {
     out.top = key_of(top);
@@ -681,7 +680,7 @@ __device__ __forceinline__ void sum_chunk(const Sample& a, ChunkShared& s) {
 template <typename T>
 __global__ __launch_bounds__(kChunkThreads) void sample_chunks_kernel(Sample a) {
   __shared__ ChunkShared s;
-  sum_chunk<T>(a, s);
+  sum_chunk<T>(a, s, a.sums[blockIdx.x]);
 }
 
 // The rank of each of n <= kRank different values among them, from the largest down, and the sum of the weights (in
@@ -708,22 +707,26 @@ __device__ void rank_all(const uint64_t* list, int n, Shared& s) {
 }
 
 // A row's token.  WHOLE: rows are one chunk each, and their workgroups sum it first, which saves a launch (128 greedy rows of 1000: 6.1
-// and 5.0 us), with registers for two workgroups a unit instead of one (518 rows of 185: 49 and 38 us; 58 of 829: 25.6 and 27.1).
+// and 5.0 us), with registers for two workgroups a unit instead of one (518 rows of 185: 49 and 37 us; 58 of 829: 25.6 and 29).
 // Latency bounds it: a row's bins, its list and its token are some 30 steps that wait for each other, 39 us for 128 rows of 100003 (25.6 MB,
 // of which each row is read once more to fill the list).
 template <typename T, bool WHOLE>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WHOLE ? 4 : 2))) void sample_rows_kernel(Sample a) {
   static_assert(kThreads == kChunkThreads, "one workgroup does both");
   __shared__ Shared s;
+  __shared__ ChunkSums whole;
   if constexpr (WHOLE) {
     __shared__ ChunkShared c;
-    sum_chunk<T>(a, c);
-    __syncthreads();                                   // what is written of the chunk is there for all waves
+    sum_chunk<T>(a, c, whole);
+    __syncthreads();
   }
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t model = fdiv(blockIdx.x, a.by_m), r = blockIdx.x - model * a.by_m.d, outer = fdiv(r, a.by_rows);
   const Row<T> row{reinterpret_cast<const T*>(a.x) + model * a.xn + outer * a.xo + (r - outer * a.by_rows.d) * a.xi, a.v};
-  const ChunkSums* chunks = a.sums + static_cast<int64_t>(blockIdx.x) * a.chunks;
+  const ChunkSums* const chunks = [&]() __attribute__((always_inline)) -> const ChunkSums* {
+    if constexpr (WHOLE) return &whole;
+    else return a.sums + static_cast<int64_t>(blockIdx.x) * a.chunks;
+  }();
   // every wave: lane c has chunk c
   const bool mine = lane < a.chunks;
   const ChunkSums& my = chunks[mine ? lane : 0];
@@ -1138,7 +1141,8 @@ extern "C" int64_t wc_sample_workspace_bytes(const wc_sample_args* args) {
     return -1;
   }
   if (check(*args, "wc_sample")) return -1;
-  return args->n * args->m * chunks_of(*args) * static_cast<int64_t>(sizeof(ChunkSums));
+  const int64_t chunks = chunks_of(*args);             // rows of one have their sums in LDS
+  return chunks > 1 ? args->n * args->m * chunks * static_cast<int64_t>(sizeof(ChunkSums)) : 0;
 }
 
 extern "C" int32_t wc_sample(const wc_sample_args* args, void* stream) {
@@ -1178,7 +1182,7 @@ extern "C" int32_t wc_sample(const wc_sample_args* args, void* stream) {
   a.mm = p.min_p_stride_m;
   a.v = static_cast<int32_t>(p.v);
   const int64_t need = wc_sample_workspace_bytes(args);
-  WC_REQUIRE(p.workspace && p.workspace_bytes >= need, WC_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what,
+  WC_REQUIRE(need == 0 || (p.workspace && p.workspace_bytes >= need), WC_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what,
              (long long)p.workspace_bytes, (long long)need);
   WC_REQUIRE(aligned(p.workspace, 16), WC_ERR_ALIGN, "%s: workspace must be 16-byte aligned", what);
   a.sums = static_cast<ChunkSums*>(p.workspace);
