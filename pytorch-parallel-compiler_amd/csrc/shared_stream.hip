@@ -9,14 +9,14 @@
 //   softmax          in the lane; the lane halves that share a row exchange their maxima, and O is rescaled, only in tiles where
 //                    a lane of the wave finds a score well over the row's base
 //   O^T += V^T P^T   P^T is the S^T register block itself, V^T through ds_read_b64_tr_b16
-// A row's K scale multiplies its scores, its V scale its weights.  The weights enter the products rounded to 16 bits, half a step
-// of 2^-8 (bf16) or 2^-11 (fp16) of each, as in attention over a prompt; their sum is fp32.  fp16 over 8-bit pages takes
-// them as two bf16 numbers, because fp16 has no room for a weight times a scale.
+// A row's K scale multiplies its scores, its V scale its weights.  The weights enter the products as two numbers of 16 bits each, off by at
+// most 2^-16 of a weight (bf16; fp16 2^-21), so that a row's result does not hang on how many others share its prefix; over 8-bit
+// pages as bf16 ones, because fp16 has no room for a weight times a scale.  Their sum is fp32.
 //
 // 64 rows are bound by memory and the waits for each tile: 4 x 2 prefixes of up to 6000 tokens, 8 key heads of 128 columns, 147 MB in
 // 42 us (3.5 TB/s; four buffers and one workgroup a unit 49).  128 rows are
-// bound by the matrix and vector pipes in turn: one prefix of 65536 tokens, 256 rows a key head, 105 us, 6.5e14 operations a second (110 with outputs
-// rescaled for every new maximum).
+// bound by the matrix and vector pipes in turn: one prefix of 65536 tokens, 256 rows a key head, 132 us for 1.03e11 operations,
+// which a large product does in 82 (weights rounded to 16 bits once: 105 us for 6.9e10; the 64 rows above take 42 us either way).
 #include "wc_attn.h"
 #include "wc_shared.h"
 
@@ -62,7 +62,7 @@ template <typename T, typename KT, int DHP, int RW>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void shared_stream_kernel(SharedAttn a) {
   constexpr bool kQ8 = std::is_same<KT, int8_t>::value;
   typedef typename std::conditional<kQ8, bf16, T>::type PT;            // of P and V
-  constexpr int NP = kQ8 && std::is_same<T, f16>::value ? 2 : 1;
+  constexpr int NP = 2;                                                // numbers of a weight
   // fp16 weights are taken 2^14 times as large, so that those far under 1 keep their bits (and as the other walk takes them)
   constexpr float kShift = std::is_same<PT, f16>::value ? 14.f : 0.f;
   // A row's base stays while its scores are no more than this above it: weights are then up to 2^8 (fp16: 2^15 with their shift), and
@@ -316,44 +316,44 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void s
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const int blk = TS == 1 ? b : tw * NB + b;
-        uint32_t pk[NP][8];
-        float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][2 * r], c, kShift - base));
-          float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][2 * r + 1], c, kShift - base));
-          l0 += p0;
-          l1 += p1;
-          if constexpr (kQ8) {
-            const float* f = &scales[buf][1][32 * blk + (r >> 1) * 8 + 4 * hf + (r & 1) * 2];
-            p0 *= f[0];
-            p1 *= f[1];
-          }
-          pk[0][r] = pack2<PT>(p0, p1);
-          if constexpr (NP == 2) pk[1][r] = pack2<PT>(p0 - unpack_lo<PT>(pk[0][r]), p1 - unpack_hi<PT>(pk[0][r]));
-        }
-        lrun += l0 + l1;
         // tokens 32 blk + 16 j + 8 piece + 4 hf + (0 .. 3), columns 32 d + 16 (lane / 16 % 2) + (0 .. 15)
         uint32_t at[DT];
 #pragma unroll
         for (int d = 0; d < DT; ++d) at[d] = vbase + vat[d] + (TS == 1 ? 0 : tw * NB * 32 * DHP * 2);
-        auto product = [&](auto J) __attribute__((always_inline)) {
+        float l0 = 0.f, l1 = 0.f;
+        auto half = [&](auto J) __attribute__((always_inline)) {
           constexpr int j = decltype(J)::value;
+          float p[8];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * j + 2 * r], c, kShift - base));
+            float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * j + 2 * r + 1], c, kShift - base));
+            l0 += p0;
+            l1 += p1;
+            if constexpr (kQ8) {
+              const float* f = &scales[buf][1][32 * blk + (2 * j + (r >> 1)) * 8 + 4 * hf + (r & 1) * 2];
+              p0 *= f[0];
+              p1 *= f[1];
+            }
+            p[2 * r] = p0;
+            p[2 * r + 1] = p1;
+          }
+          u32x4 pf[NP];
+          weight_planes<PT, NP>(p, pf);
           i16x4 v[DT][2];
           if (b == 0) read_v<j * 16 * DHP * 2, 8 * DHP * 2>(at, v);
           else read_v<(32 + j * 16) * DHP * 2, 8 * DHP * 2>(at, v);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const i16x8 vf = __builtin_shufflevector(v[d][0], v[d][1], 0, 1, 2, 3, 4, 5, 6, 7);
+          for (int q = NP - 1; q >= 0; --q)
 #pragma unroll
-            for (int q = NP - 1; q >= 0; --q) {
-              const bf16x8 pf = __builtin_bit_cast(bf16x8, make_uint4(pk[q][4 * j], pk[q][4 * j + 1], pk[q][4 * j + 2], pk[q][4 * j + 3]));
-              oacc[d] = mma32<PT>(__builtin_bit_cast(bf16x8, vf), pf, oacc[d]);
+            for (int d = 0; d < DT; ++d) {
+              const i16x8 vf = __builtin_shufflevector(v[d][0], v[d][1], 0, 1, 2, 3, 4, 5, 6, 7);
+              oacc[d] = mma32<PT>(__builtin_bit_cast(bf16x8, vf), __builtin_bit_cast(bf16x8, pf[q]), oacc[d]);
             }
-          }
         };
-        product(std::integral_constant<int, 0>());
-        product(std::integral_constant<int, 1>());
+        half(std::integral_constant<int, 0>());
+        half(std::integral_constant<int, 1>());
+        lrun += l0 + l1;
       }
       if (i + 1 < n) put(buf ^ 1);
       valid = coming;
@@ -421,7 +421,7 @@ void launch(const SharedAttn& a, int rows, int64_t grid, hipStream_t s) {
 }  // namespace
 
 // Up to 32 rows the walk without LDS reads a prefix once as well and needs no barriers; from there on it reads it again for every 32
-// (64 rows: 86.0 us for the whole call of the case above, and 83.7 through LDS; 256 rows: 386 and 169).
+// (64 rows: 86.0 us for the whole call of the case above, and 84.7 through LDS; 256 rows: 386 and 188).
 int shared_stream_rows(const wc_shared_attn_args& p) {
   const int64_t rows = p.share * (p.q_heads / p.cache.heads);
   if (p.cache.dtype == WC_F32 || p.cache.head_dim > 128 || rows <= 32) return 0;

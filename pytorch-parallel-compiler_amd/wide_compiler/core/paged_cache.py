@@ -243,10 +243,8 @@ class WidePagedCache:
         the tokens behind the prefix that a sequence has of its own, 0 for none.  A sequence of negative length takes
         part in nothing and gets zeros, as does one without any token.  The pages of a prefix are read once for all its
         sequences, where ``attend`` reads them for each.  ``max_prefix`` and ``max_length`` bound the lengths (default: what
-        the tables can name); tight bounds split short ones less.  In 16 bits with heads of up to
-        128 columns, where more than 32 query heads (those of all its sequences) share a key head of a prefix, the weights enter
-        the products with it rounded to the type once, as over a prompt; elsewhere, and for fp16 over 8-bit pages, they
-        enter as two or more numbers of 16 bits (off by at most 2^-16 of a weight)."""
+        the tables can name); tight bounds split short ones less.  In 16 bits the weights enter
+        the products as two or more numbers (off by at most 2^-16 of a weight), however many sequences share a prefix."""
         if torch.compiler.is_compiling():
             return _serve.uncompiled(self.attend_shared, q, prefix_table, prefix_lengths, block_table, lengths, scale,
                                      max_prefix, max_length)

@@ -247,3 +247,29 @@ def test_scores_that_rise_along_the_tokens(rise, dtype, bits):
     cache.write(k.to(DEV, dtype), v.to(DEV, dtype), pt, torch.zeros_like(prefix), prefix)
     q.copy_((torch.randn(q.shape, generator=g) * 0.1 + 1).to(DEV, dtype))
     _check(made)
+
+
+@pytest.mark.parametrize("dh", [32, 64, 80, 128])
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 0), (torch.bfloat16, 8), (torch.float16, 0), (torch.float16, 8)])
+def test_weights_keep_their_bits_however_many_share_a_prefix(dtype, bits, dh):
+    """From 1 query head to 256 to a key head, weights enter the products off by at most 2^-16 of themselves."""
+    for prefix, lens, hq, hkv in (([[130]], [[1]], 1, 1), ([[130]], [[5] * 32], 1, 1), ([[130]], [[5] * 33], 1, 1), ([[40, 300]], [[3] * 32], 8, 2),
+                                  ([[70]], [[2] * 65], 1, 1), ([[1000]], [[0] * 64], 4, 1)):
+        cache, q, pt, prefix, table, lens = _make(prefix, lens, hq, hkv, dh, 16, dtype, bits)
+        with torch.no_grad():
+            o = cache.attend_shared(q, pt, prefix, table, lens)
+        cache.index_error()
+        ref, big = shared(q, *_values(cache), pt, prefix, table, lens)
+        within(o, ref, HALF[dtype] + 2.0 ** -23, _bars(cache, big, int(prefix.max()) + int(lens.max())))
+
+
+def test_a_row_hangs_little_on_how_many_share_its_prefix():
+    """The same query among 1, 32, 33 and 70 sequences of a prefix: fp32 sums in other orders, weights off by 2^-16, and the result's own
+    rounding are all that may differ."""
+    cache, q, pt, prefix, table, lens = _make([[200]], [[4] * 70], 1, 1, 64, 16, torch.bfloat16, 0)
+    k, v = _values(cache)
+    ref, big = shared(q, k, v, pt, prefix, table, lens)
+    with torch.no_grad():
+        for share in (1, 32, 33, 70):
+            o = cache.attend_shared(q[:, :share].contiguous(), pt, prefix, table[:, :share].contiguous(), lens[:, :share].contiguous())
+            within(o, ref[:, :share], HALF[torch.bfloat16] + 2.0 ** -23, _bars(cache, big, 204))
