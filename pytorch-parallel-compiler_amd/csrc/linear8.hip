@@ -122,6 +122,12 @@ struct Piece {
   }
 };
 
+// What the sums of a row are multiplied by, whose largest magnitude as the bits of a float is `top`: its scale, NaN where it is not
+// finite, and 1 where all is zero, as good there and a usual number
+__device__ __forceinline__ float factor(uint32_t top) {
+  return top >= 0x7f800000u ? __builtin_nanf("") : top == 0 ? 1.f : row_scale(top);
+}
+
 // Codes and scales of 16 rows of x: lane l has row l % 16 and columns 16 (l / 16).. of every tile of its wave, which is what
 // it writes.  S workgroups share the codes of 16 rows, of which each looks for the scale by itself.  KEPT of its tiles a wave stay in
 // registers until the scale is known; more are read a second time.  Memory and the three phases that all workgroups are in at
@@ -173,7 +179,7 @@ __global__ __launch_bounds__(NW * 64) void linear8_codes_kernel(Linear8 a) {
   const bool finite = top < 0x7f800000u;
   const float scale = finite ? row_scale(top) : __builtin_nanf("");
   const float inv = __builtin_amdgcn_rcpf(scale);
-  if (share == 0 && threadIdx.x < 16) a.s[static_cast<int64_t>(blockIdx.x) * 16 + j] = scale;
+  if (share == 0 && threadIdx.x < 16) a.s[static_cast<int64_t>(blockIdx.x) * 16 + j] = factor(top);
   u32x4* out = reinterpret_cast<u32x4*>(a.c) + static_cast<int64_t>(blockIdx.x) * a.ktiles * 64 + lane;
 #pragma unroll
   for (int i = 0; i < KEPT; ++i)
@@ -218,14 +224,37 @@ __device__ __forceinline__ Columns columns(const Linear8& a, uint32_t model, int
 __device__ __forceinline__ float row_of_scale(const Linear8& a, uint32_t model, int r) {
   return a.s[static_cast<int64_t>(model) * a.mtiles * 16 + std::min(r, a.m - 1)];
 }
-// outputs o..o + 3 of row r, those there are
+// Scales whose products with each other are normal numbers, whichever they are
+__device__ __forceinline__ bool usual(float s) { return fabsf(s) >= 0x1p-63f && fabsf(s) <= 0x1p63f; }
+__device__ __forceinline__ bool usual(const Columns& c) {
+  bool all = true;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) all &= usual(c.scale[e]) || c.scale[e] == 0.f;
+  return all;
+}
+// sum s scale + bias where the scales' product may be too small or too large for fp32 though the result is not: what does not
+// fit their product's exponent goes to the sum.
+__device__ __forceinline__ float scaled_far(int sum, float s, float scale, float bias) {
+  const int e = __builtin_amdgcn_frexp_expf(s) + __builtin_amdgcn_frexp_expf(scale), near = min(max(e, -120), 120);
+  const float f = __builtin_amdgcn_ldexpf(__builtin_amdgcn_frexp_mantf(s) * __builtin_amdgcn_frexp_mantf(scale), near);
+  return fmaf(__builtin_amdgcn_ldexpf(static_cast<float>(sum), e - near), f, bias);
+}
+// outputs o..o + 3 of row r, those there are; near: all scales of the wave are usual
 template <typename T>
-__device__ __forceinline__ void finish4(const Linear8& a, uint32_t model, int r, int o, i32x4 sum, float s, const Columns& c) {
+__device__ __forceinline__ void finish4(const Linear8& a, uint32_t model, int r, int o, i32x4 sum, float s, const Columns& c, bool near) {
+  float f[4];
+  if (near) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = static_cast<float>(sum[e]) * (s * c.scale[e]) + c.bias[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = scaled_far(sum[e], s, c.scale[e], c.bias[e]);
+  }
   if (r >= a.m || o >= a.o) return;
   T* y = reinterpret_cast<T*>(a.y) + (static_cast<int64_t>(model) * a.m + r) * a.o + o;
   T v[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = from_f32<T>(static_cast<float>(sum[e]) * (s * c.scale[e]) + c.bias[e]);
+  for (int e = 0; e < 4; ++e) v[e] = from_f32<T>(f[e]);
   if (a.vec) {
     __builtin_memcpy(__builtin_assume_aligned(y, 4 * sizeof(T)), v, sizeof v);
   } else {
@@ -238,14 +267,19 @@ __device__ __forceinline__ void finish4(const Linear8& a, uint32_t model, int r,
 template <typename T, int FN, int FM>
 __device__ __forceinline__ void finish(const Linear8& a, uint32_t model, int ot, int mt, int lane, const i32x4 (&acc)[FN][FM]) {
   float s[FM];
+  bool rows = true;
 #pragma unroll
-  for (int j = 0; j < FM; ++j) s[j] = row_of_scale(a, model, (mt + j) * 16 + (lane & 15));
+  for (int j = 0; j < FM; ++j) {
+    s[j] = row_of_scale(a, model, (mt + j) * 16 + (lane & 15));
+    rows &= usual(s[j]);
+  }
 #pragma unroll
   for (int i = 0; i < FN; ++i) {
     const int o = (ot + i) * 16 + (lane >> 4) * 4;
     const Columns c = columns<T>(a, model, o);
+    const bool near = __all(rows && usual(c));
 #pragma unroll
-    for (int j = 0; j < FM; ++j) finish4<T>(a, model, (mt + j) * 16 + (lane & 15), o, acc[i][j], s[j], c);
+    for (int j = 0; j < FM; ++j) finish4<T>(a, model, (mt + j) * 16 + (lane & 15), o, acc[i][j], s[j], c, near);
   }
 }
 // a barrier that waits for nothing but the other waves
@@ -296,7 +330,9 @@ __global__ __launch_bounds__(NW * 64) void linear8_few_kernel(Linear8 a) {
 #pragma unroll
     for (int v = 1; v < NW; ++v) sum += part[v][t][lane];
     const int r = mt * 16 + (lane & 15), o = (ot0 + t) * 16 + (lane >> 4) * 4;
-    finish4<T>(a, model, r, o, sum, row_of_scale(a, model, r), columns<T>(a, model, o));
+    const float scale = row_of_scale(a, model, r);
+    const Columns c = columns<T>(a, model, o);
+    finish4<T>(a, model, r, o, sum, scale, c, __all(usual(scale) && usual(c)));
   }
 }
 
@@ -382,7 +418,9 @@ __global__ __launch_bounds__(NW * 64) void linear8_fused_kernel(Linear8 a) {
     for (int e = 1; e < NW; ++e) sum += part[e][t][lane];
     const uint32_t top = tops[min(j, a.m - 1)];
     const int o = (ot0 + t) * 16 + g * 4;
-    finish4<T>(a, model, j, o, sum, top < 0x7f800000u ? row_scale(top) : __builtin_nanf(""), columns<T>(a, model, o));
+    const float scale = factor(top);
+    const Columns c = columns<T>(a, model, o);
+    finish4<T>(a, model, j, o, sum, scale, c, __all(usual(scale) && usual(c)));
   }
 }
 

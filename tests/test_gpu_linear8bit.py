@@ -221,3 +221,38 @@ def test_gradients_are_refused():
     mod, *_ = _module(1, 16, 8, torch.float32)
     with pytest.raises(RuntimeError):
         mod(torch.zeros(1, 2, 16, device=DEV, requires_grad=True))
+
+
+# a row, few rows, tiles of 64 x 128 in six stages and in three, of 128 x 128, the largest
+@pytest.mark.parametrize("n,m,k,o", [(2, 3, 200, 52), (2, 40, 200, 50), (1, 300, 130, 2100), (8, 60, 70, 4099), (8, 200, 70, 2100), (8, 1040, 65, 1030)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_and_scales_of_any_size(n, m, k, o, dtype):
+    """Rows of 1e-38 to 1e38 against scales of 1e-40 to 1e38: the scales' product may be far under or over fp32's range where
+    the result is not.  The same roundings as elsewhere: the sum's, the scales' product's, theirs with it and the result's."""
+    import wide_compiler as wc
+    g = gen(7)
+    codes = torch.randint(-127, 128, (n, o, k), generator=g, dtype=torch.int8).to(DEV)
+    scales = torch.logspace(-40, 38, o, dtype=torch.float64).float().expand(n, o)[:, torch.randperm(o, generator=g)].contiguous().to(DEV)
+    scales[:, 0], scales[:, 1] = 0.0, -3e-6
+    x = torch.randn(n, m, k, generator=g).clamp(-3, 3).double() * torch.logspace(-38, 38, m, dtype=torch.float64)[torch.randperm(m, generator=g)][:, None]
+    x[:, 1] = 0
+    x = x.clamp(-3e38, 3e38).to(DEV, dtype)
+    mod = wc.WideLinear8bit.from_codes(codes, scales)
+    with torch.no_grad():
+        y = mod(x)
+    _check(y, x, codes, scales, None)
+    assert (y[:, 1] == 0).all() and (y[..., 0] == 0).all()
+
+
+def test_small_rows_of_usual_weights():
+    """Rows of 1e-36 and 1e-37 of weights of 3e-4: outputs are normal numbers, right to the roundings of 1."""
+    mod, codes, scales, bias = _module(2, 256, 64, torch.float32, bias=False)
+    import wide_compiler as wc
+    scales = scales * 1e-3
+    mod = wc.WideLinear8bit.from_codes(codes, scales)
+    for m in (2, 20, 600):
+        base = torch.randn(2, m, 256, generator=gen(m)).to(DEV)
+        for size in (1.0, 1e-34, 1e-35, 1e-36, 1e-37):
+            x = base * size
+            with torch.no_grad():
+                _check(mod(x), x, codes, scales, None)
