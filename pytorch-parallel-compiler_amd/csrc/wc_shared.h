@@ -39,13 +39,19 @@ __device__ __forceinline__ PagedSpan shared_span(const SharedWalk& w, int unit) 
 struct SharedLine {
   int size, total;
 };
+// Tiles of a share, one at least, where there are none at all too: units' first shares are counted by dividing by it.  `least` is for
+// cuts of one unit: short units are not put together for it, which would walk them one after the other.
+__host__ __device__ inline int shared_size(int total, int budget, int least, int units) {
+  const int equal = (total + budget - 1) / budget, low = (total + units - 1) / (units > 1 ? units : 1);
+  const int size = least < low ? least : low;
+  return size > equal ? size : equal > 1 ? equal : 1;
+}
 __device__ __forceinline__ SharedLine shared_line(const SharedWalk& w, int lane) {
   int total = 0;
   for (int s = lane; s < w.units; s += 64) total += paged_tiles(shared_span(w, s));
 #pragma unroll
   for (int off = 32; off; off >>= 1) total += __shfl_xor(total, off, 64);
-  // `least` is for cuts of one unit: short units are not put together for it, which would walk them one after the other
-  return SharedLine{max((total + w.budget - 1) / w.budget, min(w.least, (total + w.units - 1) / max(w.units, 1))), total};
+  return SharedLine{shared_size(total, w.budget, w.least, w.units), total};
 }
 // the unit that has tile `at` of the line (at < total), and the line's tiles before it
 __device__ __forceinline__ int2 shared_find(const SharedWalk& w, int at, int lane) {

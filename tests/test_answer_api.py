@@ -5,6 +5,7 @@ import ctypes
 import hashlib
 import os
 import re
+import shutil
 import subprocess
 import sys
 
@@ -330,3 +331,57 @@ def test_answer_host_side_clean_under_sanitizers():
     assert r.returncode == 0, r.stderr[-6000:]
     assert "runtime error" not in r.stderr and "AddressSanitizer" not in r.stderr, r.stderr[-6000:]
     assert "no sanitizer report" in r.stdout
+
+
+LINE = r"""
+#include <cstdint>
+#include <cstdio>
+#include <vector>
+
+#include "wc_shared.h"
+
+// Units' tiles as one line in shares of shared_size tiles: units of none at all too, every tile in one share, no more shares
+// than the budget, no two parts alike.
+int main() {
+  using namespace wc;
+  uint32_t seed = 20261208;
+  auto below = [&](int n) { return static_cast<int>((seed = seed * 1664525u + 1013904223u) >> 8) % n; };
+  int none = 0;
+  for (int it = 0; it < 50000; ++it) {
+    const int units = 1 + below(below(2) ? 6 : 200), budget = 1 + below(below(2) ? 8 : 512), least = 1 + below(4), top = below(3) ? 1 + below(300) : 1;
+    std::vector<int> tiles(units);
+    int total = 0;
+    for (int& t : tiles) total += t = below(top);
+    const int size = shared_size(total, budget, least, units);
+    if (size < 1) return 1;
+    none += total == 0;
+    if (total && (total - 1) / size + 1 > budget) return 2;
+    std::vector<char> used(budget + units, 0);
+    int start = 0;
+    for (int s = 0; s < units; start += tiles[s++]) {
+      const int first = start / size;
+      for (int w = first; tiles[s] && w <= (start + tiles[s] - 1) / size; ++w) {
+        if (w + s >= budget + units || used[w + s]) return 3;
+        used[w + s] = 1;
+      }
+    }
+  }
+  printf("%d lines without tiles\n", none);
+  return none > 100 ? 0 : 4;
+}
+"""
+
+
+def test_shares_of_a_line_of_tiles(tmp_path):
+    """How shared attention cuts its line of tiles, on the host, under the sanitizer that stops at a division by zero."""
+    hipcc = next((h for h in ("/opt/rocm/bin/hipcc", "hipcc") if shutil.which(h)), None)
+    if hipcc is None:
+        pytest.skip("no hipcc")
+    src, exe = tmp_path / "line.cpp", tmp_path / "line"
+    src.write_text(LINE)
+    r = subprocess.run([hipcc, "-x", "hip", "--offload-host-only", "-std=c++17", "-O1", "-w", "-Xarch_host", "-fsanitize=undefined", "-Xarch_host",
+                        "-fno-sanitize-recover=undefined", "-I", os.path.join(PKG, "csrc"), "-I", os.path.join(ROOT, "include"), str(src),
+                        "-o", str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-4000:]
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, (r.returncode, r.stdout, r.stderr[-2000:])

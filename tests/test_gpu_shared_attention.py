@@ -273,3 +273,13 @@ def test_a_row_hangs_little_on_how_many_share_its_prefix():
         for share in (1, 32, 33, 70):
             o = cache.attend_shared(q[:, :share].contiguous(), pt, prefix, table[:, :share].contiguous(), lens[:, :share].contiguous())
             within(o, ref[:, :share], HALF[torch.bfloat16] + 2.0 ** -23, _bars(cache, big, 204))
+
+
+@pytest.mark.parametrize("dtype,bits", [(torch.bfloat16, 0), (torch.bfloat16, 8), (torch.float32, 0)])
+@pytest.mark.parametrize("share", [3, 40])
+def test_no_tokens_at_all(share, dtype, bits):
+    """Prefixes without a token, own pages without one, and both, where the bounds allow long ones that would be cut."""
+    for prefix, own in ((0, 0), (0, 9), (70, 0), (-1, -1), (70, -1)):
+        made = _make([[prefix, prefix]], [[own] * 2 * share], 2, 1, 64, 16, dtype, bits)
+        _check(made, max_prefix=5000, max_length=1000)
+        _check(made, max_prefix=5000, max_length=200)
