@@ -198,3 +198,25 @@ def test_fewer_allowed_than_top_k(top_k, v):
         for i, rest in enumerate((dict(), dict(top_p=0.9), dict(min_p=0.02), dict(top_p=0.7, min_p=0.05, temperature=1.5))):
             rules = dict(top_k=top_k, **rest)
             _check(wc.WideSampler(1, **rules).to(DEV), x, torch.rand(1, 6, generator=gen(i)), rules)
+
+
+@pytest.mark.parametrize("v", [200, 8192, 9001, 70001])
+@pytest.mark.parametrize("min_p", [1e-3, 1e-6, 2.0 ** -33, 1e-12, 1e-15, 2.0 ** -70, 1e-38, 1e-45])
+def test_a_small_min_p_filters_what_it_says(v, min_p):
+    """Values either side of min_p's border, a part of it and powers of two apart, the lower ones at the lowest places, which
+    u = 0 gives if they are kept: with each other filter, and at temperatures that are taken over the digits of the values."""
+    import wide_compiler as wc
+    g = gen(v)
+    border = -torch.log(torch.tensor(min_p, dtype=torch.float32).double()).item()
+    for t in (1.0, 0.6, 40.0, 200.0):
+        off = torch.cat([-torch.logspace(1.5, -4, 40), torch.logspace(-4, 1.5, 40)])     # from far below the border up to far above it
+        x = -border * t + torch.randn(1, 8, v, generator=g).double() * 0.01 - 50 * t
+        x[..., 3:83] = -border * t + off.double() * t
+        x[..., v // 2:v // 2 + 3] = 0.0
+        x = (x.clamp_max(0.0) + 3.0).float()
+        u = torch.tensor([[0.0, 1e-30, 2.0 ** -39, 1e-9, 0.2, 0.5, 0.99, 1 - 2.0 ** -24]])
+        for rest in (dict(), dict(top_k=60), dict(top_k=4, top_p=0.999999), dict(top_p=0.9999999)):
+            rules = dict(temperature=t, min_p=min_p, **rest)
+            _check(wc.WideSampler(1, **rules).to(DEV), x[:, :1], u[:, :1], rules)
+            if min_p >= 2.0 ** -33:                          # weights of many units: the sums, too, are those in 64 bits
+                _check(wc.WideSampler(1, **rules).to(DEV), x, u, rules)
