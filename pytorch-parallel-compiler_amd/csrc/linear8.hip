@@ -13,6 +13,7 @@
 
 #include "wc_answer_abi.h"
 #include "wc_codes.h"
+#include "wc_linear8.h"
 
 namespace wc {
 namespace {
@@ -339,7 +340,6 @@ __global__ __launch_bounds__(NW * 64) void linear8_few_kernel(Linear8 a) {
 // The same for so few rows of x (kFusedPieces pieces of 16 columns in all) that every workgroup finds their codes for itself,
 // in LDS, while its first weights are on their way: a launch costs more (four models' [4096 -> 4096], one row: 13.7 us, 4.9 TB/s; with
 // a launch for the codes 21.0; four rows 16.9 and 23.2).
-constexpr int kFusedPieces = 1024;
 template <typename T, int RT, int NW, int D>
 __global__ __launch_bounds__(NW * 64) void linear8_fused_kernel(Linear8 a) {
   constexpr int NT = NW * 64, KEPT = kFusedPieces / NT;
@@ -486,7 +486,7 @@ __global__ __launch_bounds__(WM * WN * 64) void linear8_tile_kernel(Linear8 a) {
 // 2.1e15 operations a second.  LDS bounds it: a stage is 1024 cycles of MFMAs, and as many to write its 32 KB and read 96 KB out of
 // it at 128 bytes a cycle.  (Two stages of 128 columns took 137 us; four waves of 128 x 128, which read a third less, 161 us, as
 // one wave a SIMD hides nothing and 256 accumulators leave too few registers.)
-constexpr int kLargeThreads = 512, kLargeTiles = 16, kLargeStage = 2 * kLargeTiles * 1024;
+constexpr int kLargeThreads = 512, kLargeStage = 2 * kLargeTiles * 1024;
 
 template <typename T>
 __global__ __launch_bounds__(kLargeThreads, 1) void linear8_large_kernel(Linear8 a, int tiles_total, int per) {
@@ -647,7 +647,8 @@ void launch_large(Linear8 a, int64_t n, hipStream_t s) {
 template <typename T>
 void launch(const Linear8& a, int64_t n, hipStream_t s) {
   const uint32_t tiles = static_cast<uint32_t>(n * a.mtiles);
-  if (a.m <= 16 && static_cast<int64_t>(a.m) * a.ktiles * 4 <= kFusedPieces) return launch_fused<T, 1, 4, 8>(a, n, s);
+  const Linear8Form form = linear8_form(n, a.m, a.mtiles, a.otiles, a.ktiles);
+  if (form == Linear8Form::fused) return launch_fused<T, 1, 4, 8>(a, n, s);
   // Where rows' tiles are fewer than compute units, more waves have them (256 rows [1024 -> 1024], eight models: by four waves 21.8 us for
   // the whole product, by 16 18.0), and of longer rows four workgroups, each with a quarter of the codes (64 rows [4096 -> 4096]: by
   // one of eight waves 26.0, by four 19.7; 129 rows [7280 -> 416], two models: 29.9 and 23.4).
@@ -663,19 +664,13 @@ void launch(const Linear8& a, int64_t n, hipStream_t s) {
     linear8_codes_kernel<T, 8, 8, 1><<<tiles, 512, 0, s>>>(a);
   else if constexpr (sizeof(T) != 4)
     linear8_codes_kernel<T, 16, 8, 1><<<tiles, 1024, 0, s>>>(a);
-  // A workgroup for each 16 rows and outputs while all of them are at work at once, eight a compute unit: W comes from L2 for all
-  // rows but the first 16, which costs less than long walks on few units do (129 rows [7280 -> 416], two models, codes
-  // included: 51 us by tiles of 64 x 128, 30 so; 128 rows [4096 -> 4096], 2048 of them: 36.6 and 32.4; 293 rows [6832 -> 1004], 2394
-  // of them: 50 and 64).
-  if (a.mtiles == 1 || n * a.mtiles * a.otiles <= 2048) return launch_few<T, 1, 4, 8>(a, n, s);
-  // Where tiles are fewer than compute units, one has a unit's LDS to itself and more stages on their way (293 rows [6832 -> 1004], two
-  // models: by tiles of 128 x 128 in two stages 62 us, so 50).
-  if (n * cdiv(a.mtiles, 4) * cdiv(a.otiles, 8) <= 256) return launch_tile<T, 4, 2, 1, 4, 6>(a, n, s);
-  if (a.mtiles <= 4) return launch_tile<T, 4, 2, 1, 4, 3>(a, n, s);
-  // The largest tiles where few units are left without one (2 models' 1280 rows [2048 -> 4096], 160 of them: 45.9 us, by tiles of 128 x 128
-  // 55.7; 2048 rows [4096 -> 4096], 128 of them: 67.8 and 61.5)
-  if (n * cdiv(a.mtiles, kLargeTiles) * cdiv(a.otiles, kLargeTiles) >= 150) return launch_large<T>(a, n, s);
-  launch_tile<T, 4, 4, 2, 2, 2>(a, n, s);
+  switch (form) {
+    case Linear8Form::few: return launch_few<T, 1, 4, 8>(a, n, s);
+    case Linear8Form::ring6: return launch_tile<T, 4, 2, 1, 4, 6>(a, n, s);
+    case Linear8Form::ring3: return launch_tile<T, 4, 2, 1, 4, 3>(a, n, s);
+    case Linear8Form::large: return launch_large<T>(a, n, s);
+    default: return launch_tile<T, 4, 4, 2, 2, 2>(a, n, s);
+  }
 }
 
 int32_t check(const wc_linear8_args& p, const char* what) {

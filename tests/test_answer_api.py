@@ -385,3 +385,33 @@ def test_shares_of_a_line_of_tiles(tmp_path):
     assert r.returncode == 0, r.stderr[-4000:]
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, (r.returncode, r.stdout, r.stderr[-2000:])
+
+
+FORM = r"""
+#include <cstdio>
+#include <cstdlib>
+
+#include "wc_linear8.h"
+
+int main(int argc, char** argv) {
+  const char* names[] = {"fused", "few", "ring6", "ring3", "large", "tiles"};
+  auto tiles = [](long x, long of) { return (x + of - 1) / of; };
+  for (int i = 1; i + 3 < argc; i += 4) {
+    const long n = atol(argv[i]), m = atol(argv[i + 1]), k = atol(argv[i + 2]), o = atol(argv[i + 3]);
+    puts(names[static_cast<int>(wc::linear8_form(n, m, tiles(m, 16), tiles(o, 16), tiles(k, 128) * 2))]);
+  }
+}
+"""
+
+
+def test_the_tests_of_8_bit_products_reach_every_kernel(tmp_path):
+    from tests.test_gpu_linear8bit import FORMS
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no g++")
+    src, exe = tmp_path / "form.cpp", tmp_path / "form"
+    src.write_text(FORM)
+    subprocess.run([gxx, "-std=c++17", "-I", os.path.join(PKG, "csrc"), str(src), "-o", str(exe)], check=True, timeout=120)
+    shapes = [(form, shape) for form, each in FORMS.items() for shape in each]
+    r = subprocess.run([str(exe), *(str(x) for _, shape in shapes for x in shape)], capture_output=True, text=True, timeout=60)
+    assert r.stdout.split() == [form for form, _ in shapes], list(zip(r.stdout.split(), shapes))

@@ -246,8 +246,8 @@ def test_rows_and_scales_of_any_size(n, m, k, o, dtype):
 
 def test_small_rows_of_usual_weights():
     """Rows of 1e-36 and 1e-37 of weights of 3e-4: outputs are normal numbers, right to the roundings of 1."""
-    mod, codes, scales, bias = _module(2, 256, 64, torch.float32, bias=False)
     import wide_compiler as wc
+    _, codes, scales, _ = _module(2, 256, 64, torch.float32, bias=False)
     scales = scales * 1e-3
     mod = wc.WideLinear8bit.from_codes(codes, scales)
     for m in (2, 20, 600):
@@ -256,3 +256,31 @@ def test_small_rows_of_usual_weights():
             x = base * size
             with torch.no_grad():
                 _check(mod(x), x, codes, scales, None)
+
+
+# (models, rows, columns, outputs) by the kernel that makes them (test_answer_api.py checks that it does): ragged rows and outputs,
+# columns of one stage, of two and of several times the ring
+FORMS = {
+    "fused": [(3, 16, 960, 100), (2, 1, 1024, 17), (1, 3, 5000, 33)],
+    "few": [(2, 16, 1100, 200), (1, 129, 700, 416), (3, 17, 65, 33)],
+    "ring6": [(1, 300, 130, 2100), (2, 293, 900, 1004), (1, 40, 2000, 16400)],
+    "ring3": [(8, 64, 2048, 4104), (9, 33, 200, 3800), (16, 49, 65, 2100), (11, 17, 130, 3000), (10, 60, 450, 3334)],
+    "large": [(4, 2049, 512, 1025), (2, 2304, 384, 2303), (10, 257, 65, 2049)],
+    "tiles": [(1, 2049, 512, 1025), (8, 200, 70, 2100), (3, 500, 300, 2100)],
+}
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_every_kernel(form, dtype):
+    for n, m, k, o in FORMS[form]:
+        mod, codes, scales, bias = _module(n, k, o, dtype, seed=o)
+        x = torch.randn(n, m, k, generator=gen(8)).to(DEV, dtype)
+        x[:, m - 1, k - 1] = 9.0                             # the last row's largest in its last column
+        with torch.no_grad():
+            y = mod(x)
+        _check(y, x, codes, scales, bias)
+        # the same bits from a few of the rows
+        at = torch.tensor([0, m // 2, m - 1], device=DEV)
+        with torch.no_grad():
+            assert torch.equal(mod(x[:, at].contiguous()), y[:, at])
