@@ -33,7 +33,7 @@ from typing import List, Optional, Tuple, Union
 import torch
 from torch import Tensor, nn
 
-from ... import _hip
+from ... import _hip, _serve
 from .._layout import rows_or_contiguous
 
 
@@ -286,6 +286,11 @@ class WideAttention(nn.Module):
         if common.dim() != 2 or common.shape[0] != n or lengths.shape != x.shape[:2] or (b % common.shape[1] if common.shape[1] else b):
             raise RuntimeError(f"{what}: {list(common.shape)} prefix lengths and {list(lengths.shape)} lengths for [N={n}, B={b}] "
                                "sequences in groups of one size")
+        # what attend_shared would refuse once the cache is written
+        if table.dim() != 3 or table.dtype != torch.int32 or common.dtype != torch.int32 or table.shape[:2] != common.shape:
+            raise RuntimeError(f"{what}: prefix must be a table int32 [N={n}, G, M] and lengths int32 [N={n}, G], got {table.dtype} "
+                               f"{list(table.shape)} and {common.dtype} {list(common.shape)}")
+        _serve.same_device(what, x, table, common)
         share = b // common.shape[1] if common.shape[1] else 1
         position = start + common.clamp_min(0).repeat_interleave(share, 1)
         q, k, v = self._cached_heads(what, x[:, :, None], cache, position[..., None], head_norm)

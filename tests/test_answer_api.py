@@ -415,3 +415,22 @@ def test_the_tests_of_8_bit_products_reach_every_kernel(tmp_path):
     shapes = [(form, shape) for form, each in FORMS.items() for shape in each]
     r = subprocess.run([str(exe), *(str(x) for _, shape in shapes for x in shape)], capture_output=True, text=True, timeout=60)
     assert r.stdout.split() == [form for form, _ in shapes], list(zip(r.stdout.split(), shapes))
+
+
+def test_step_refuses_a_prefix_before_it_writes(anywhere, monkeypatch):
+    import wide_compiler as wc
+
+    def reached(*args, **kw):
+        raise AssertionError("projected or written")
+    attn = wc.WideAttention(2, 128, 2).requires_grad_(False)
+    monkeypatch.setattr(attn, "_cached_heads", reached)
+    pages = torch.zeros(5, 2, 16, 64)
+    cache = wc.WidePagedCache.from_pages(pages, pages)
+    monkeypatch.setattr(cache, "write", reached)
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(AssertionError, match="projected"):
+        attn.step(torch.zeros(2, 4, 128), cache, i(2, 4, 1), i(2, 4), prefix=(i(2, 2, 4), i(2, 2)))
+    for prefix in ((i(2, 2, 4).long(), i(2, 2)), (i(2, 2, 4), i(2, 2).long()), (i(2, 2), i(2, 2)), (i(2, 1, 4), i(2, 2)), (i(1, 2, 4), i(2, 2)),
+                   (torch.zeros(2, 2, 4, dtype=torch.int32, device="meta"), i(2, 2))):
+        with pytest.raises(RuntimeError, match="WideAttention.step"):
+            attn.step(torch.zeros(2, 4, 128), cache, i(2, 4, 1), i(2, 4), prefix=prefix)
