@@ -46,7 +46,9 @@ class WideSampler(nn.Module):
         self._plans = _serve.Plans()
 
     def set(self, temperature=None, top_k=None, top_p=None, min_p=None) -> None:
-        """New rules, in place: a number for all models or one of each; None leaves a rule as it is."""
+        """New rules, in place: a number for all models or one of each; None leaves a rule as it is.  Where one is refused, all stay
+        as they were."""
+        new = []
         for i, (name, rule) in enumerate(zip(_RULES, (temperature, top_k, top_p, min_p))):
             if rule is None:
                 continue
@@ -55,12 +57,14 @@ class WideSampler(nn.Module):
             values = list(values) if isinstance(values, (list, tuple)) else [values] * self.n
             if len(values) != self.n:
                 raise ValueError(f"WideSampler: {name} must be a number or {self.n} of them, got {len(values)}")
-            if whole and any(int(v) != v or not 0 <= v < 2 ** 31 for v in values):
+            if whole and any(not 0 <= v < 2 ** 31 or int(v) != v for v in values):
                 raise ValueError(f"WideSampler: top_k must be whole numbers from 0 on, got {rule}")
             if not whole and any(math.isnan(v) or v < 0 for v in values):
                 raise ValueError(f"WideSampler: {name} must not be negative, got {rule}")
             t = torch.tensor(values, dtype=torch.int32 if whole else torch.float32)
-            self.rules[:, i].copy_(t if whole else t.view(torch.int32))
+            new.append((i, t if whole else t.view(torch.int32)))
+        for i, t in new:
+            self.rules[:, i].copy_(t)
 
     def forward(self, logits: Tensor, u: Tensor, temperature: Optional[Tensor] = None, top_k: Optional[Tensor] = None,
                 top_p: Optional[Tensor] = None, min_p: Optional[Tensor] = None) -> Tensor:

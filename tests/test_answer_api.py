@@ -434,3 +434,16 @@ def test_step_refuses_a_prefix_before_it_writes(anywhere, monkeypatch):
                    (torch.zeros(2, 2, 4, dtype=torch.int32, device="meta"), i(2, 2))):
         with pytest.raises(RuntimeError, match="WideAttention.step"):
             attn.step(torch.zeros(2, 4, 128), cache, i(2, 4, 1), i(2, 4), prefix=prefix)
+
+
+def test_sampler_rules_change_all_or_not_at_all():
+    import wide_compiler as wc
+    s = wc.WideSampler(2, temperature=0.7, top_k=5, top_p=0.9)
+    before = s.rules.clone()
+    for kw in (dict(temperature=2.0, top_k=-1), dict(temperature=1.0, top_p=[0.5, 0.5, 0.5]), dict(top_k=3, min_p=float("nan")),
+               dict(top_k=float("inf")), dict(temperature=0.1, top_k=float("nan")), dict(top_p=0.1, min_p=-1.0)):
+        with pytest.raises(ValueError):
+            s.set(**kw)
+        assert torch.equal(s.rules, before), kw
+    s.set(temperature=float("inf"), top_k=[2 ** 31 - 1, 0])
+    assert s.rules[:, 1].tolist() == [2 ** 31 - 1, 0]
