@@ -87,7 +87,7 @@ class WideSampler(nn.Module):
         if not rules.is_contiguous():
             rules = rules.contiguous()
         if copies:
-            given = tuple(t.expand(u.shape).reshape(self.n, -1) if t is not None and i in copies else t
+            given = tuple(t.expand(u.shape).contiguous() if t is not None and i in copies else t
                           for i, t in enumerate(given))
         tokens = torch.empty(u.shape, dtype=torch.int64, device=u.device)
         if tokens.numel():
@@ -123,7 +123,7 @@ class WideSampler(nn.Module):
                 strides += [wide.stride(0), dims[-1][1] if dims else 0]
             else:
                 copies.append(i)
-                strides += [u[0].numel(), 1]
+                strides += [math.prod(u.shape[1:]), 1]
         _serve.same_device(what, logits, u, rules, *given)
         dense, rows = rows_or_contiguous(logits)
         sizes = (_hip.dtype_code(logits.dtype, what), self.n, rows.rows, logits.shape[-1])

@@ -447,3 +447,14 @@ def test_sampler_rules_change_all_or_not_at_all():
         assert torch.equal(s.rules, before), kw
     s.set(temperature=float("inf"), top_k=[2 ** 31 - 1, 0])
     assert s.rules[:, 1].tolist() == [2 ** 31 - 1, 0]
+
+
+def test_sampler_takes_an_empty_batch_with_rules_of_any_strides(anywhere):
+    """Rules that a call copies, because a model's rows reach them by more than one stride, over batches without a row."""
+    import wide_compiler as wc
+    s = wc.WideSampler(2)
+    for shape in ((2, 0, 5), (2, 5, 0), (2, 0)):
+        for t in (torch.ones(()), torch.ones(shape[-1]), torch.ones(2, *[1] * (len(shape) - 1))):
+            assert s(torch.zeros(*shape, 9), torch.zeros(shape), temperature=t).shape == shape
+    none = wc.WideSampler(0)
+    assert none(torch.zeros(0, 3, 5, 9), torch.zeros(0, 3, 5), top_p=torch.ones(3, 1)).shape == (0, 3, 5)
