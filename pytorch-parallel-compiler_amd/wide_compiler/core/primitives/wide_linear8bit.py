@@ -25,6 +25,8 @@ from torch import Tensor, nn
 from ... import _answer, _hip, _serve
 from .._layout import rows_or_contiguous
 
+_MOST = float.fromhex("0x1.020406p121")          # the largest scale: 127 of the next one round to infinity in fp32
+
 
 class WideLinear8bit(nn.Module):
     def __init__(self, n: int, in_features: int, out_features: int, bias: bool = True, dtype: torch.dtype = torch.float32):
@@ -128,7 +130,8 @@ class WideLinear8bit(nn.Module):
 
     @classmethod
     def from_modules(cls, modules: List[nn.Linear]) -> "WideLinear8bit":
-        """Quantises N nn.Linear: scale = max |w| / 127 of each output's weights, code = w / scale to the nearest."""
+        """Quantises N nn.Linear: scale = max |w| / 127 of each output's weights (a step less for fp32's largest value), code =
+        w / scale to the nearest."""
         t = modules[0]
         form = lambda m: (tuple(m.weight.shape), m.weight.dtype, m.weight.device,  # noqa: E731
                           None if m.bias is None else (m.bias.dtype, m.bias.device))
@@ -139,7 +142,9 @@ class WideLinear8bit(nn.Module):
         with torch.no_grad():
             for i, m in enumerate(modules):
                 w = m.weight.double()
-                s = (w.abs().amax(-1) / 127).clamp_min(2.0 ** -126).float()
+                top = w.abs().amax(-1)
+                s = (top / 127).clamp_min(2.0 ** -126).float()
+                s = torch.where(torch.isfinite(top), s.clamp_max(_MOST), s)
                 wide._pack(i, torch.round(w / s.double()[:, None]).clamp(-127, 127).to(torch.int8))
                 wide._set_scales(i, s)
                 if m.bias is not None:

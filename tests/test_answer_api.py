@@ -458,3 +458,16 @@ def test_sampler_takes_an_empty_batch_with_rules_of_any_strides(anywhere):
             assert s(torch.zeros(*shape, 9), torch.zeros(shape), temperature=t).shape == shape
     none = wc.WideSampler(0)
     assert none(torch.zeros(0, 3, 5, 9), torch.zeros(0, 3, 5), top_p=torch.ones(3, 1)).shape == (0, 3, 5)
+
+
+def test_linear8_keeps_the_largest_weight_finite():
+    """fp32's largest value comes back as 127 of the largest scale whose 127 fp32 holds, a step of the scale less."""
+    import wide_compiler as wc
+    mod = torch.nn.Linear(5, 3)
+    with torch.no_grad():
+        mod.weight[1] = torch.finfo(torch.float32).max
+        mod.weight[2, 0] = -torch.finfo(torch.float32).max
+    back = wc.WideLinear8bit.from_modules([mod]).dequantize()[0]
+    assert torch.isfinite(back).all()
+    w = mod.weight.double()
+    assert not ((back.double() - w).abs() > w.abs().amax(-1, keepdim=True) / 127 * (0.5 + 2.0 ** -15)).any()
