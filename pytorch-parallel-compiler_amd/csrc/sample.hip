@@ -6,11 +6,17 @@
 // The filters all keep the first of one order, so a kept set is a cut: a value, all above it, and those equal to it up to an
 // index.  A row of logits is cut into chunks.  The first kernel has a workgroup for each chunk, which brings it into
 // registers, finds its largest value, sums its weights and, where something is filtered, counts and sums them in bins: an
-// eighth of a power of two of the weight each, so a bin holds few values and what lies above it is known without
+// eighth of a power of two of the weight each, so a bin holds a small part of the values and what lies above it is known without
 // looking again.  The second has a workgroup for each row: it adds the chunks' bins up, finds the bin in which the cut falls,
 // gathers what the bin holds (or all that may be kept, where that is little), finds the cut there, then the chunk that
-// holds the token by the sums, and the token in the chunk.  Rows with more in one bin than a list holds (thousands of
-// equal logits, as a rule) are cut on the values' bits, digit by digit, over the whole row.
+// holds the token by the sums, and the token in the chunk.
+//
+// A bin may hold more than a list: of rows as vocabularies' heads give them, of 131072 logits and more at a temperature of 1, the bin of
+// top_p = 0.95 does (4400 values of 262144).  For top-p such a bin is parted by its values' bits in one more look at the row, and
+// what is above the part with the cut goes to the chunks' sums; for min-p, whose least value is known, all that is kept does
+// (128 rows of 200003 in bf16, top_p = 0.95: at a temperature of 0.7, where the bin fits, 89 us; of 1.0 134, over the digits of the
+// whole row 1276).  What is left is cut on the values' bits, digit by digit, over the whole row: thousands of equal values at the cut, a
+// top_k whose bin does not fit, and rows of one chunk, which are short (64 of 8000 with all values in a few bins: 33 us, spread 29).
 //
 // Which token comes out must not hang on the order of a sum, so weights are summed as whole numbers, of 2^-48 of the
 // largest weight (more where rows are so long that 64 bits could not hold the sum): each is the exponential in 64 bits,
@@ -78,7 +84,7 @@ constexpr Powers powers() {
 __constant__ const Powers kPowers = powers();
 
 // Weights as whole numbers: 2^(y + fraction), y = x log2(e) / t - floor, with 2^(i/64) from a table and the rest, at most
-// 2^-7 of a power, from the first terms of its series, whose next is under 2^-58.  `floor` is a whole number next to the
+// 2^-7 of a power, from the first terms of its series, whose next is under 2^-54.  `floor` is a whole number next to the
 // largest value's x log2(e) / t, by which sums of different ones can be brought together; y is at most 2^-12, whatever t is,
 // because it is counted from the largest value down.
 constexpr uint64_t kMagic = 0x4330000000000000;      // 2^52 as a float of 64 bits: its last bits are a whole number added to it
@@ -442,6 +448,65 @@ __device__ __forceinline__ uint32_t least_key(const Weights& w, uint32_t top, do
   return hi;
 }
 
+// Of the values with keys [klo, khi], which are more than a list holds, those next to the place where weights summed from the top
+// and from `above` on reach the limit: into s.list, the sum above them into s.found64[0] and the weights between them and khi that
+// min_p keeps into s.chunk_sum, by their chunks.  How many are listed, or -1 where more than a list holds are equal.
+template <typename T>
+__device__ __forceinline__ int part_bin(Row<T> row, Weights w, Shared& s, uint32_t klo, uint32_t khi, uint32_t least, uint64_t above, uint64_t limit,
+                                        FastDiv by_chunk) {
+  const int tid = threadIdx.x;
+  const auto none = [](int) { return 0; };
+  uint32_t lo = klo, hi = khi;
+  for (;;) {
+    const uint32_t width = hi - lo;
+    const int shift = larger(0, 32 - __clz(width | 1) - kDigitBits);          // parts of 2^shift keys, at most kDigits
+    __syncthreads();
+    for (int i = tid; i < kDigits; i += kThreads) {
+      s.weight[i] = 0;
+      s.count[i] = 0;
+    }
+    if (tid == 0) s.found32[0] = 0, s.found64[0] = above;
+    __syncthreads();
+    row.template select<false>(value_of(lo), value_of(hi), none, [&](int i, int) {
+      const float x = to_f32(row.x[i]);
+      const uint32_t k = key_of(x);
+      if (k < lo || k > hi) return;                    // a zero of the other sign
+      atomicAdd(&s.count[(k - lo) >> shift], 1u);
+      atomicAdd(reinterpret_cast<unsigned long long*>(&s.weight[(k - lo) >> shift]), static_cast<unsigned long long>(w(x)));
+    });
+    __syncthreads();
+    // parts from the top, two a thread: the first that reaches the limit; where rounding leaves that behind all, the last that has any
+    const int d1 = kDigits - 1 - 2 * tid, d0 = d1 - 1;
+    const uint64_t v1 = s.weight[d1], v0 = s.weight[d0];
+    uint64_t total;
+    const uint64_t had1 = above + before64(v1 + v0, s, total), had0 = had1 + v1;
+    if (v1 && had1 < limit && (had0 >= limit || had0 == above + total)) s.found32[0] = d1, s.found64[0] = had1;
+    if (v0 && had0 < limit && (had0 + v0 >= limit || had0 + v0 == above + total)) s.found32[0] = d0, s.found64[0] = had0;
+    __syncthreads();
+    const uint32_t part = s.found32[0], n = s.count[part];
+    above = s.found64[0];
+    lo += part << shift;
+    hi = smaller(hi, lo + ((1u << shift) - 1));
+    if (n <= kList) break;
+    if (shift == 0) return -1;
+  }
+  __syncthreads();
+  if (tid == 0) s.found32[1] = 0;
+  if (tid < kChunks) s.chunk_sum[tid] = 0;
+  __syncthreads();
+  row.template select<false>(value_of(lo), value_of(khi), none, [&](int i, int) {
+    const float x = to_f32(row.x[i]);
+    const uint32_t k = key_of(x);
+    if (k < lo || k > khi) return;
+    if (k <= hi)
+      s.list[atomicAdd(&s.found32[1], 1u)] = static_cast<uint64_t>(k) << 32 | ~static_cast<uint32_t>(i);
+    else if (k >= least)
+      atomicAdd(reinterpret_cast<unsigned long long*>(&s.chunk_sum[fdiv(static_cast<uint32_t>(i), by_chunk)]), static_cast<unsigned long long>(w(x)));
+  });
+  __syncthreads();
+  return static_cast<int>(s.found32[1]);
+}
+
 // The draw by the digits of keys, over the whole row.
 template <typename T>
 __device__ __attribute__((noinline)) void draw_by_digits(Row<T> row, Weights w, Shared& s, Rules rules, uint32_t top, uint32_t least, float u,
@@ -766,6 +831,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WHOLE 
   // the kept: keys above cut_key, and those that are it up to index cut_last
   uint32_t cut_key = kNever, cut_last = 0;
   int list_from = kBins, listed = 0;             // all of the bins before list_from are kept, and what of the list is
+  bool parted = false;                           // and what is above the list in its bin, in the chunks' sums already
   bool filter = rules.filter(a.v);
   // what min_p keeps: keys from `least` on, of weights of 2^power of the largest or more
   const uint32_t least = rules.min_p > 0.f ? least_key(w, top, power) : kNever + 1;
@@ -828,14 +894,11 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WHOLE 
         if (lo + step < kBins && above[lo + step] < limit) lo += step;
       return lo;
     };
-    // the values of bins [b0, b1] into the list; whether they fit
-    auto gather = [&](int b0, int b1) __attribute__((always_inline)) {
-      __syncthreads();
-      if (tid == 0) s.found32[1] = 0;
-      __syncthreads();
-      // The values whose places are under the upper edge of b0 and from the lower edge of b1 on: places rise with values, so
-      // the last and first of them are next to the edges divided by the scale.  A lane has a candidate.
-      float hi = INFINITY, lo = -3.402823466e38f;
+    // The values of bins [b0, b1], whose places are under the upper edge of b0 and from the lower edge of b1 on: places rise with values,
+    // so the last and first of them are next to the edges divided by the scale.  A lane has a candidate.
+    auto edges = [&](int b0, int b1, float& lo, float& hi) __attribute__((always_inline)) {
+      hi = INFINITY;
+      lo = -3.402823466e38f;
       if (b0) {
         const float edge = bins.base - b0 + 1, at = value_of(key_of(edge / bins.scale) + 16 - lane);
         hi = __shfl(at, (__ffsll(static_cast<unsigned long long>(__ballot(!(bins.scaled(at) >= edge)))) + 63) & 63, 64);
@@ -844,6 +907,14 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WHOLE 
         const float edge = bins.base - b1, at = value_of(key_of(edge / bins.scale) - 16 + lane);
         lo = __shfl(at, (__ffsll(static_cast<unsigned long long>(__ballot(!(bins.scaled(at) < edge)))) + 63) & 63, 64);
       }
+    };
+    // the values of bins [b0, b1] into the list; whether they fit
+    auto gather = [&](int b0, int b1) __attribute__((always_inline)) {
+      float lo, hi;
+      edges(b0, b1, lo, hi);
+      __syncthreads();
+      if (tid == 0) s.found32[1] = 0;
+      __syncthreads();
       row.template select<!WHOLE>(lo, hi, [&](int n) { return static_cast<int>(atomicAdd(&s.found32[1], static_cast<uint32_t>(n))); },
                  [&](int i, int at) {
                    if (at < kList) s.list[at] = i;
@@ -1003,11 +1074,27 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WHOLE 
       const uint64_t limit = limit_of(sum);
       // at most the bin of top_k's cut, whose sum in the chunks' units may be a few less
       const int b = list_from == 0 ? 0 : smaller(find_bin(s.above_weight, limit), cut_bin);
-      if (b < list_from) digits = !bring(b);
+      uint64_t above = 0;
+      if (b < list_from) {
+        // how many there are is known to a factor of 2^(11/8): a bin that cannot fit is not tried
+        digits = (!WHOLE && s.bin_count[b] > kList * 2.6f) || !bring(b);
+        if constexpr (!WHOLE) {
+          if (digits) {
+            float lo, hi;
+            edges(b, b, lo, hi);
+            listed = part_bin(row, w, s, key_of(lo), smaller(key_of(hi), top), least, s.above_weight[b], limit, a.by_chunk);
+            list_from = b;
+            above = s.found64[0];
+            parted = true;
+            digits = listed < 0;
+          }
+        }
+      }
       if (!digits) {
-        if (!by_k && list_from == 0 && listed <= kRank) return draw_few();
+        if (!by_k && !parted && list_from == 0 && listed <= kRank) return draw_few();
         if (list_from) cut_bin = b;
-        cut_list(false, list_from ? s.above_weight[list_from] : 0, limit);
+        if (!parted && list_from) above = s.above_weight[list_from];
+        cut_list(false, above, limit);
       }
     }
     if (rules.min_p > 0.f && !digits) {
@@ -1018,7 +1105,27 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WHOLE 
         const int end = smaller(smaller(b + 3, kBins - 1), cut_bin);
         const int begin = s.above_count[end] + s.bin_count[end] <= kList ? 0 : smaller(b, end);
         digits = !gather(begin, end);
-        if (!digits && begin == 0 && listed <= kRank && !by_k && !(rules.top_p < 1.f)) return draw_few();
+        parted = false;
+        if constexpr (!WHOLE) {
+          if (digits) {                                // more than a list holds: what is kept of them goes to the chunks' sums at once
+            float lo, hi;
+            edges(begin, end, lo, hi);
+            __syncthreads();
+            if (tid < kChunks) s.chunk_sum[tid] = 0;
+            __syncthreads();
+            row.template select<false>(value_of(least), hi, [](int) { return 0; }, [&](int i, int) {
+              const float x = to_f32(row.x[i]);
+              if (kept(key_of(x), static_cast<uint32_t>(i)))
+                atomicAdd(reinterpret_cast<unsigned long long*>(&s.chunk_sum[fdiv(static_cast<uint32_t>(i), a.by_chunk)]),
+                          static_cast<unsigned long long>(w(x)));
+            });
+            listed = 0;
+            list_from = begin;
+            parted = true;
+            digits = false;
+          }
+        }
+        if (!digits && !parted && begin == 0 && listed <= kRank && !by_k && !(rules.top_p < 1.f)) return draw_few();
       }
     }
     if (digits) {
@@ -1044,7 +1151,7 @@ __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(WHOLE 
       uint64_t sum = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum += s.other[tid * 8 + i];
-      s.chunk_sum[tid] = sum;
+      s.chunk_sum[tid] = parted ? s.chunk_sum[tid] + sum : sum;
     }
     __syncthreads();
     if (list_from > 0)

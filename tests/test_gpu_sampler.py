@@ -220,3 +220,76 @@ def test_a_small_min_p_filters_what_it_says(v, min_p):
             _check(wc.WideSampler(1, **rules).to(DEV), x[:, :1], u[:, :1], rules)
             if min_p >= 2.0 ** -33:                          # weights of many units: the sums, too, are those in 64 bits
                 _check(wc.WideSampler(1, **rules).to(DEV), x, u, rules)
+
+
+def _crowded(kind, b, v, seed, dtype):
+    """Rows of which one bin of weights next to the cut holds more values than a workgroup lists."""
+    g = gen(seed)
+    if kind == "wide":                                       # a large vocabulary's usual spread
+        x = torch.randn(1, b, v, generator=g) * 2
+        x[..., torch.randint(0, v, (20,), generator=g)] += 6
+    elif kind == "flat":                                     # all in a bin or two, the largest among them
+        x = 3 + torch.randn(1, b, v, generator=g) * 1e-3
+    elif kind == "dense":                                    # a third of them next to each other within a part of the bin
+        x = torch.randn(1, b, v, generator=g)
+        x[..., ::3] = 0.5 + torch.randn(1, b, (v + 2) // 3, generator=g) * 1e-6
+        x[..., 5] = 3.0
+    elif kind == "zeros":                                    # small values of both signs about zero, zeros of both signs among them
+        x = torch.randn(1, b, v, generator=g) * 1e-3
+        x[..., ::7], x[..., 1::7] = 0.0, -0.0
+        x[..., 11] = 2.0
+    else:                                                    # far below: the last bin holds nearly all
+        x = torch.randn(1, b, v, generator=g) - 60
+        x[..., 9] = 0.0
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("kind,v", [("wide", 131072), ("wide", 262144), ("flat", 8000), ("flat", 20011), ("dense", 8192), ("dense", 70001), ("zeros", 8191),
+                                    ("zeros", 40009), ("far", 8000), ("far", 30000)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_more_values_in_a_bin_than_a_list_holds(kind, v, dtype):
+    import wide_compiler as wc
+    b = 5
+    x = _crowded(kind, b, v, v, dtype)
+    for i, rules in enumerate((dict(top_p=0.95), dict(top_p=0.5), dict(top_p=0.999), dict(top_p=1e-3), dict(temperature=1.5, top_p=0.9),
+                               dict(temperature=4.0, top_p=0.3), dict(top_p=0.95, min_p=0.02), dict(top_p=0.99, min_p=1e-4, temperature=2.0),
+                               dict(top_p=0.9, top_k=5000), dict(top_p=0.95, top_k=3000, min_p=1e-3), dict(top_p=0.97, min_p=0.9),
+                               dict(temperature=0.01, top_p=0.95), dict(min_p=0.9), dict(min_p=0.01, temperature=4.0), dict(min_p=1e-5),
+                               dict(min_p=1e-26), dict(min_p=1e-3, top_p=0.9999), dict(min_p=0.999, top_k=4000), dict(min_p=1e-4, top_k=20000))):
+        u = torch.rand(1, b, generator=gen(i))
+        u[0, 0], u[0, 1] = 0.0, 1 - 2.0 ** -24
+        _check(wc.WideSampler(1, **rules).to(DEV), x, u, rules)
+
+
+def test_more_equal_values_than_a_list_holds():
+    import wide_compiler as wc
+    x = torch.randint(0, 8, (1, 4, 100003), generator=gen(1)).float() * 0.3
+    x[0, 2:] = torch.randint(0, 60, (2, 100003), generator=gen(2)).float() * 0.03
+    u = torch.tensor([[0.0, 0.37, 0.81, 1 - 2.0 ** -24]])
+    for dtype in DTYPES:
+        for rules in (dict(top_p=0.5), dict(top_p=0.95), dict(top_p=0.7, min_p=0.3), dict(top_p=0.8, top_k=4000), dict(temperature=2.0, top_p=0.99)):
+            _check(wc.WideSampler(1, **rules).to(DEV), x.to(dtype), u, rules)
+
+
+def test_usual_rows_take_no_longer_than_their_neighbours():
+    """Top-p over a large vocabulary takes about as long whether the cut's bin of weights holds a thousand values (temperature
+    0.7) or several (1.0 and 1.5)."""
+    import wide_compiler as wc
+    x = _crowded("wide", 64, 200003, 3, torch.bfloat16).to(DEV)
+    u = torch.rand(1, 64, generator=gen(4)).to(DEV)
+
+    def time(t):
+        s = wc.WideSampler(1, temperature=t, top_p=0.95).to(DEV)
+        at = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+        times = []
+        with torch.no_grad():
+            for _ in range(9):
+                at[0].record()
+                for _ in range(5):
+                    s(x, u)
+                at[1].record()
+                torch.cuda.synchronize()
+                times.append(at[0].elapsed_time(at[1]))
+        return sorted(times)[4]
+    base = time(0.7)
+    assert time(1.0) < 4 * base and time(1.5) < 4 * base, (base, time(1.0), time(1.5))
