@@ -88,7 +88,8 @@ int32_t wc_linear8(const wc_linear8_args* args, void* stream);
  * the order is always kept.  NaN logits count as -infinity, which is never drawn; where there is +infinity, only it is.  A row
  * without a logit above -infinity gets -1.  u outside [0, 1) is taken as the nearest in it, under 2^-40 as 0.  Weights are
  * summed as whole numbers of 2^-w of the largest, w = min(48, 63 - log2 of the row's length, rounded up), of which each above
- * 2^-1075 has one at least, so results do not depend on any order.
+ * 2^-1075 has one at least; rows of more than 8192 logits in stretches, each in units of its own largest weight, whose sums have one
+ * of the row's units at least.  So results do not depend on any order.  min_p is compared with the weights themselves.
  */
 typedef struct wc_sample_args {
   int32_t dtype;                  /* of the logits */

@@ -20,9 +20,10 @@
 //
 // Which token comes out must not hang on the order of a sum, so weights are summed as whole numbers, of 2^-48 of the
 // largest weight (more where rows are so long that 64 bits could not hold the sum): each is the exponential in 64 bits,
-// off by 2^-46 of itself, and rounded once, to 1 at least, so that u = 0 gives the first that has a weight at all.
+// off by 2^-46 of itself, and rounded once, to 1 at least, so that u = 0 gives the first that has a weight at all.  A chunk's are of its
+// own largest, and its sums are brought to the row's units by a shift, to 1 at least.
 //
-// Those exponentials, some 20 operations in 64 bits a value, bound the first kernel: 256 rows of 131072 in fp32, unfiltered, 39 us
+// Those exponentials, some 20 operations in 64 bits a value and as many others, bound the first kernel by instructions: 256 rows of 131072 in fp32, unfiltered, 39 us
 // (3.4 TB/s); with bins, an atomic in LDS a value more, 128 of 100003 in bf16 25 us (5.2e11 values a second; 8.6e11 without bins).
 #include <algorithm>
 
@@ -780,7 +781,8 @@ __device__ void rank_all(const uint64_t* list, int n, Shared& s) {
 }
 
 // A row's token.  WHOLE: rows are one chunk each, and their workgroups sum it first, which saves a launch (128 greedy rows of 1000: 6.1
-// and 5.0 us), with registers for two workgroups a unit instead of one (518 rows of 185: 49 and 37 us; 58 of 829: 25.6 and 29).
+// and 4.9 us), with registers for two workgroups a unit instead of one, at the price of some in scratch memory (fp32 7, fp16 16, bf16
+// 75 of them: 518 rows of 185 in bf16 by top-k and top-p 33.6 us, by one workgroup 40.5; 58 of 829 by top-p and min-p 16.5 and 14.6).
 // Latency bounds it: a row's bins, its list and its token are some 30 steps that wait for each other, 39 us for 128 rows of 100003 (25.6 MB,
 // of which each row is read once more to fill the list).
 template <typename T, bool WHOLE>

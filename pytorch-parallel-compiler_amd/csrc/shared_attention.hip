@@ -487,7 +487,9 @@ Plan plan_of(const wc_shared_attn_args& p) {
   plan.rt = plan.stream ? plan.stream / 16 : tiles_of_rows(p);
   const int64_t group = p.q_heads / p.cache.heads, units = p.cache.n * (p.cache.b / p.share), seqs = p.cache.n * p.cache.b;
   const int64_t heads0 = p.cache.heads * cdiv(p.share * group, plan.rt * 16), heads1 = p.cache.heads * cdiv(group, 16);
-  const int64_t target = 512;                        // two workgroups a compute unit
+  // Workgroups of one round where a unit holds two, as it does in 16 bits of up to 128 columns (up to 256 registers; fewer of 64 columns, where it
+  // would hold three).  fp32 of 128 columns and all of more than 128 (259 to 512 registers) take two rounds of one.
+  const int64_t target = 512;
   plan.budget[0] = std::min<int64_t>(cdiv(target, heads0), kSharedTarget);
   plan.parts[0] = plan.budget[0] + units;
   // Sequences stay whole where they are short, or many for their length (45 of up to 130 tokens, 2 key heads: 29.6 us, cut 34.5; 128 of

@@ -15,7 +15,8 @@ that broadcast to ``u`` (float32, int32 for top_k).  temperature <= 0 takes the 
 of lowest index; top_k <= 0, top_p >= 1 and min_p <= 0 filter nothing, and the most likely token is always kept.  NaN
 logits count as -infinity, which is never drawn; +infinity leaves nothing else.  A row without a logit above -infinity gives
 -1.  Weights are summed exactly, as whole numbers of 2^-48 of the largest (2^-46 at 131072 logits, a bit less for every
-doubling), of which each that 64 bits hold has one at least, so what is drawn hangs on its row alone.  ``u`` outside [0, 1)
+doubling), of which each that 64 bits hold has one at least (of more than 8192 logits: each stretch of them, whose own sum is
+in units of its own largest weight), so what is drawn hangs on its row alone.  ``u`` outside [0, 1)
 counts as the nearest in it, under 2^-40 as 0.
 
 The rules are read on the GPU: a captured graph replays with what they hold then.  The reference has no counterpart.
